@@ -209,7 +209,6 @@ def prepare(case, seed):
         return t
     if op == "prefill":
         lens = _split(c["T"], c["B"])
-        t["max_len"] = max(lens)
         t["offsets"] = _int32([sum(lens[:b]) for b in range(c["B"] + 1)])
         return t
     if op == "append":
@@ -374,7 +373,7 @@ def run(t):
         window = c["window"] or None
         if c["op"] == "prefill":
             return sink_window_attention(t["q"], t["k"], t["v"], window=window, sinks=c["sinks"],
-                                         offsets=t["offsets"], max_len=t["max_len"])
+                                         offsets=t["offsets"])
         o = sink_window_attention(t["q"], t["k"], t["v"], window=window, sinks=c["sinks"])
         dq, dk, dv = torch.autograd.grad(o, (t["q"], t["k"], t["v"]), t["do"])
         return {"o": o.detach(), "dq": dq, "dk": dk, "dv": dv}
