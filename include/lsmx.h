@@ -437,6 +437,47 @@ int lsmx_gemm_mx_promote(const uint8_t *a, int64_t lda, const float *a_scale, in
                          int op_fmt, void *c, int c_dtype, int64_t ldc, int64_t M, int64_t N, int64_t K,
                          const uint64_t *flag, uint64_t epoch, void *stream);
 
+/* ------------------------------------------------------------- attention
+ * Causal attention with a sliding window and sinks, the operator between the
+ * linears of a block (the reference's train.py:46-52 calls
+ * F.scaled_dot_product_attention there; windows and sinks are an extension):
+ *
+ *   query i of n queries over m keys has position p = i + m - n and sees key j
+ *   when 0 <= j <= p and (window == 0, or j > p - window, or j < sinks);
+ *   o_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys it sees, 0 where
+ *   it sees none.
+ *
+ * heads % kv_heads == 0; query head h reads key head h / (heads / kv_heads).
+ * Sequences are dense (offsets NULL: batch of them, q_len queries and k_len
+ * keys each) or packed one after another along the token axis (offsets
+ * [batch + 1] in device memory, tokens offsets[b] .. offsets[b+1]-1 belong to
+ * sequence b; q_len == k_len == all tokens, the sequence strides are unused;
+ * tokens of no sequence see nothing).  offsets must ascend. */
+typedef struct {
+    const void *q, *k, *v; /* LSMX_BF16 | LSMX_F16, unit stride along head_dim */
+    void *o;               /* the same type                                     */
+    float *lse;            /* log2(sum_j exp(scale q . k_j)), -inf for a row that
+                              sees nothing: [batch, heads, q_len] or, packed,
+                              [heads, tokens]; may be NULL forward              */
+    int dtype;
+    int64_t batch, q_len, k_len, heads, kv_heads;
+    int64_t head_dim;       /* a multiple of 8, at most 128                      */
+    int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3]; /* sequence, token,
+                              head; multiples of 8, 16-byte aligned bases       */
+    const int32_t *offsets;
+    int64_t window, sinks;  /* window 0: none                                    */
+    float scale;            /* finite, > 0                                       */
+} lsmx_attention;
+
+int lsmx_attention_fwd(const lsmx_attention *a, void *stream);
+
+/* Gradients, given o and lse of the forward call and d_o (strides do_stride):
+ * dq, dk, dv are contiguous [.., token, head, head_dim] of the inputs' type.
+ * ws: lsmx_attention_workspace(a) bytes, 16-byte aligned, no initial contents. */
+int64_t lsmx_attention_workspace(const lsmx_attention *a);
+int lsmx_attention_bwd(const lsmx_attention *a, const void *d_o, const int64_t *do_stride, void *dq, void *dk,
+                       void *dv, void *ws, int64_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -68,9 +68,12 @@ SIGNATURES = {
     "lsmx_scale_to_e8m0_batch": [_vp, _int, _vp, _u64, _vp],
     "lsmx_gemm_mx_promote": [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _int, _vp, _int, _i64, _i64,
                              _i64, _i64, _vp, _u64, _vp],
+    "lsmx_attention_fwd": [_vp, _vp],
+    "lsmx_attention_workspace": [_vp],
+    "lsmx_attention_bwd": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
 }
 
-RET_I64 = ("lsmx_gemm_bf16f4_workspace",)
+RET_I64 = ("lsmx_gemm_bf16f4_workspace", "lsmx_attention_workspace")
 
 
 class QItem(ctypes.Structure):
@@ -90,6 +93,14 @@ class E8m0Item(ctypes.Structure):
     """lsmx_e8m0_item of include/lsmx.h."""
     _fields_ = [("s", _vp), ("rows", _i64), ("cols", _i64), ("lds", _i64), ("layout", _int), ("out", _vp),
                 ("ldo", _i64)]
+
+
+class Attention(ctypes.Structure):
+    """lsmx_attention of include/lsmx.h."""
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("o", _vp), ("lse", _vp), ("dtype", _int), ("batch", _i64),
+                ("q_len", _i64), ("k_len", _i64), ("heads", _i64), ("kv_heads", _i64), ("head_dim", _i64),
+                ("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("v_stride", _i64 * 3), ("o_stride", _i64 * 3),
+                ("offsets", _vp), ("window", _i64), ("sinks", _i64), ("scale", ctypes.c_float)]
 
 
 # Epochs for lsmx_scale_to_e8m0_batch's flag: unique within the process and

@@ -7,6 +7,7 @@
 #include <atomic>
 #include <mutex>
 
+#include "lsmx_attn.h"
 #include "lsmx_internal.h"
 
 namespace {
@@ -743,6 +744,90 @@ int lsmx_gemm_wonly_f4(const void *a, int a_dtype, int64_t lda, const uint8_t *w
                        int64_t M, int64_t N, int64_t K, void *stream) {
     return w4_common("lsmx_gemm_wonly_f4", a, nullptr, a_dtype, lda, w_pk, ldw, w_scale, ld_sw, scale_fmt, c, nullptr,
                      c_dtype, ldc, M, N, K, stream);
+}
+
+// The argument checks of the attention entry points; fills the kernels' form.
+static int attn_args(const char *fn, const lsmx_attention *a, bool bwd, lsmx::AttnArgs *out) {
+    if (!a) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (a->dtype != LSMX_BF16 && a->dtype != LSMX_F16) return fail(LSMX_ERR_DTYPE, "%s: dtype must be bf16 or fp16", fn);
+    if (a->batch < 0 || a->q_len < 0 || a->k_len < 0 || a->heads < 0) return fail(LSMX_ERR_SHAPE, "%s: negative size", fn);
+    if (a->kv_heads < 1 || a->heads % a->kv_heads || a->heads < 1)
+        return fail(LSMX_ERR_SHAPE, "%s: heads=%lld must be a positive multiple of kv_heads=%lld", fn,
+                    (long long)a->heads, (long long)a->kv_heads);
+    if (a->head_dim < 8 || a->head_dim > 128 || a->head_dim % 8)
+        return fail(LSMX_ERR_SHAPE, "%s: head_dim=%lld must be a multiple of 8, 8 to 128", fn, (long long)a->head_dim);
+    if (a->offsets && a->q_len != a->k_len) return fail(LSMX_ERR_SHAPE, "%s: packed sequences need q_len == k_len", fn);
+    if (a->window < 0 || a->sinks < 0) return fail(LSMX_ERR_ARG, "%s: negative window or sinks", fn);
+    if (!(a->scale > 0.f) || !(a->scale <= 3.0e38f)) return fail(LSMX_ERR_ARG, "%s: scale must be positive and finite", fn);
+    // positions, rows (tokens x heads of one key head) and work items are int32
+    const int64_t lim = (int64_t)1 << 30, group = a->heads / a->kv_heads;
+    const int64_t many = a->offsets ? 1 : a->batch;
+    if (a->q_len >= lim || a->k_len >= lim || a->batch >= lim || a->kv_heads >= lim || group >= lim ||
+        a->q_len * group >= lim || (a->q_len * group / 64 + 1) * many >= lim || (a->k_len / 64 + 1) * many >= lim ||
+        ((a->q_len * group / 64 + 1) * many + a->batch + 2) * a->kv_heads >= lim ||
+        ((a->k_len / 64 + 1) * many + a->batch + 2) * a->kv_heads >= lim)
+        return fail(LSMX_ERR_SHAPE, "%s: too many tokens or heads", fn);
+    const bool nq = a->batch && a->q_len, nk = a->batch && a->k_len;
+    if ((nq || a->offsets) && a->q_len && (!a->q || !a->o)) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if ((nk || a->offsets) && a->k_len && (!a->k || !a->v)) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (bwd && nq && !a->lse) return fail(LSMX_ERR_ARG, "%s: null lse", fn);
+    if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->o, 16) || !aligned(a->lse, 4) ||
+        !aligned(a->offsets, 4))
+        return fail(LSMX_ERR_ALIGN, "%s: operands must be 16-byte aligned", fn);
+    for (int i = 0; i < 3; ++i)
+        if (a->q_stride[i] % 8 || a->k_stride[i] % 8 || a->v_stride[i] % 8 || a->o_stride[i] % 8)
+            return fail(LSMX_ERR_ALIGN, "%s: strides must be multiples of 8 elements", fn);
+    lsmx::AttnArgs &g = *out;
+    g = lsmx::AttnArgs{};
+    g.q = a->q, g.k = a->k, g.v = a->v, g.o = a->o, g.lse = a->lse;
+    g.batch = (int)a->batch, g.heads = (int)a->heads, g.kv_heads = (int)a->kv_heads, g.group = (int)group;
+    g.dim = (int)a->head_dim, g.q_len = (int)a->q_len, g.k_len = (int)a->k_len;
+    const bool packed = a->offsets != nullptr;
+    g.q_b = packed ? 0 : a->q_stride[0], g.q_t = a->q_stride[1], g.q_h = a->q_stride[2];
+    g.k_b = packed ? 0 : a->k_stride[0], g.k_t = a->k_stride[1], g.k_h = a->k_stride[2];
+    g.v_b = packed ? 0 : a->v_stride[0], g.v_t = a->v_stride[1], g.v_h = a->v_stride[2];
+    g.o_b = packed ? 0 : a->o_stride[0], g.o_t = a->o_stride[1], g.o_h = a->o_stride[2];
+    g.lse_h = a->q_len, g.lse_b = packed ? 0 : a->heads * a->q_len;
+    g.offsets = a->offsets, g.tokens = (int)a->q_len;
+    g.window = (int)(a->window < lim ? a->window : lim), g.sinks = g.window ? (int)(a->sinks < lim ? a->sinks : lim) : 0;
+    g.scale = a->scale, g.c = a->scale * 1.4426950408889634f;
+    g.by_group = lsmx::fast_div((uint32_t)group);
+    return LSMX_OK;
+}
+
+int lsmx_attention_fwd(const lsmx_attention *a, void *stream) {
+    const char *fn = "lsmx_attention_fwd";
+    lsmx::AttnArgs g;
+    if (int r = attn_args(fn, a, false, &g)) return r;
+    if (int r = device_guard()) return r;
+    if (!g.q_len || (!g.batch && !g.offsets)) return LSMX_OK;
+    return launched(lsmx::launch_attn_fwd(g, a->dtype, (hipStream_t)stream), fn);
+}
+
+int64_t lsmx_attention_workspace(const lsmx_attention *a) {
+    lsmx::AttnArgs g;
+    if (attn_args("lsmx_attention_workspace", a, false, &g)) return 0;
+    return lsmx::attn_bwd_workspace(g);
+}
+
+int lsmx_attention_bwd(const lsmx_attention *a, const void *d_o, const int64_t *do_stride, void *dq, void *dk,
+                       void *dv, void *ws, int64_t ws_bytes, void *stream) {
+    const char *fn = "lsmx_attention_bwd";
+    lsmx::AttnArgs g;
+    if (int r = attn_args(fn, a, true, &g)) return r;
+    if (!do_stride) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    const bool nq = g.q_len && (g.batch || g.offsets), nk = g.k_len && (g.batch || g.offsets);
+    if ((nq && (!d_o || !dq)) || (nk && (!dk || !dv)) || ((nq || nk) && !ws)) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (!aligned(d_o, 16) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16) || !aligned(ws, 16))
+        return fail(LSMX_ERR_ALIGN, "%s: operands must be 16-byte aligned", fn);
+    for (int i = 0; i < 3; ++i)
+        if (do_stride[i] % 8) return fail(LSMX_ERR_ALIGN, "%s: strides must be multiples of 8 elements", fn);
+    if (ws_bytes < lsmx::attn_bwd_workspace(g)) return fail(LSMX_ERR_ARG, "%s: workspace too small", fn);
+    if (int r = device_guard()) return r;
+    if (!nq && !nk) return LSMX_OK;
+    g.d_o = d_o, g.do_b = g.offsets ? 0 : do_stride[0], g.do_t = do_stride[1], g.do_h = do_stride[2];
+    g.dq = dq, g.dk = dk, g.dv = dv, g.delta = (float *)ws;
+    return launched(lsmx::launch_attn_bwd(g, a->dtype, (hipStream_t)stream), fn);
 }
 
 }  // extern "C"
