@@ -478,6 +478,61 @@ int64_t lsmx_attention_workspace(const lsmx_attention *a);
 int lsmx_attention_bwd(const lsmx_attention *a, const void *d_o, const int64_t *do_stride, void *dq, void *dk,
                        void *dv, void *ws, int64_t ws_bytes, void *stream);
 
+/* ------------------------------------------------- attention over a cache
+ * A paged MXFP4 key-value cache (an extension: the reference trains only).
+ * A page holds `page` tokens of every key head; a token's key (value) of one
+ * head is head_dim E2M1 codes, two per byte, and head_dim / 32 E8M0 scales,
+ * the bytes lsmx_quantize_mxfp4 makes of it (fp4.py:57-72).  Sequence b has
+ * lengths[b] tokens, token j in page table[b][j / page], slot j % page.
+ * table and lengths are device memory; an id outside the pool is never
+ * followed (its tokens are hidden, and not written), a length is cut to the
+ * table's capacity.  Buffers 16-byte aligned. */
+typedef struct {
+    uint8_t *k_codes, *k_scale; /* [pages, kv_heads, page, head_dim / 2], [.., head_dim / 32] */
+    uint8_t *v_codes, *v_scale;
+    int64_t pages, page;        /* page: a power of two, 16 to 1024 */
+    int64_t kv_heads, head_dim; /* head_dim 64 or 128               */
+    const int32_t *table;       /* [batch, max_pages]               */
+    const int32_t *lengths;     /* [batch]                          */
+    int64_t batch, max_pages;
+} lsmx_kv_cache;
+
+/* Writes new tokens: k, v (LSMX_BF16 | LSMX_F16) [tokens, kv_heads, head_dim]
+ * with strides {token, head} (multiples of 8).  Sequence b's n_b tokens,
+ * offsets[b] .. offsets[b+1]-1 or (offsets NULL) per_seq for each, become its
+ * positions lengths[b] - n_b .. lengths[b] - 1: lengths already counts them.
+ * Positions below 0 or past the table are not written.  k_out, v_out (both
+ * or neither): the values now held, bf16 [tokens, kv_heads, head_dim], exact. */
+int lsmx_kv_append(const lsmx_kv_cache *c, const void *k, const int64_t *k_stride, const void *v,
+                   const int64_t *v_stride, int dtype, int64_t tokens, int64_t per_seq, const int32_t *offsets,
+                   void *k_out, void *v_out, void *stream);
+
+/* Attention of the newest q_len tokens of every sequence over its cache: the
+ * query i of sequence b has position lengths[b] - q_len + i; visibility and
+ * softmax as for lsmx_attention_fwd.  q [batch, q_len, heads, head_dim] with
+ * strides {sequence, token, head}; o contiguous, of q's type (LSMX_BF16 |
+ * LSMX_F16).  weights (NULL, or fp32 [batch, kv_heads, w_len], w_len >= page
+ * max_pages): weights[b, h, j] += the softmax weights of key j, summed over
+ * the q_len tokens and the heads that share key head h.
+ * ws: lsmx_kv_attend_workspace bytes, 16-byte aligned, no initial contents. */
+int64_t lsmx_kv_attend_workspace(const lsmx_kv_cache *c, int64_t q_len, int64_t heads, int64_t window, int64_t sinks,
+                                 int weights);
+int lsmx_kv_attend(const lsmx_kv_cache *c, const void *q, const int64_t *q_stride, int dtype, int64_t q_len,
+                   int64_t heads, int64_t window, int64_t sinks, float scale, void *o, float *weights, int64_t w_len,
+                   void *ws, int64_t ws_bytes, void *stream);
+
+/* Cuts every sequence and key head to at most `keep` tokens: the first
+ * `sinks`, the last `recent`, and of the others those with the largest
+ * weights [batch, kv_heads, w_len] (ties: the lower position; -0 equals 0; a
+ * NaN is above all), in their order (sinks + recent <= keep).  They are
+ * copied to positions 0, 1, .. of the pages out_table [batch, out_max_pages]
+ * of the same pool, which must not be pages of `table`.  index
+ * [batch, kv_heads, keep]: the positions they had, -1 past the last;
+ * new_weights: their weights, 0 past the last; new_lengths [batch]. */
+int lsmx_kv_evict(const lsmx_kv_cache *c, const float *weights, int64_t w_len, int64_t keep, int64_t sinks,
+                  int64_t recent, const int32_t *out_table, int64_t out_max_pages, int32_t *index,
+                  float *new_weights, int32_t *new_lengths, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -71,9 +71,14 @@ SIGNATURES = {
     "lsmx_attention_fwd": [_vp, _vp],
     "lsmx_attention_workspace": [_vp],
     "lsmx_attention_bwd": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "lsmx_kv_append": [_vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _vp, _vp, _vp, _vp],
+    "lsmx_kv_attend_workspace": [_vp, _i64, _i64, _i64, _i64, _int],
+    "lsmx_kv_attend": [_vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, ctypes.c_float, _vp, _vp, _i64, _vp, _i64, _vp],
+    "lsmx_kv_evict": [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp],
 }
 
-RET_I64 = ("lsmx_gemm_bf16f4_workspace", "lsmx_attention_workspace")
+RET_I64 = ("lsmx_gemm_bf16f4_workspace", "lsmx_attention_workspace",
+           "lsmx_kv_attend_workspace")
 
 
 class QItem(ctypes.Structure):
@@ -101,6 +106,13 @@ class Attention(ctypes.Structure):
                 ("q_len", _i64), ("k_len", _i64), ("heads", _i64), ("kv_heads", _i64), ("head_dim", _i64),
                 ("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("v_stride", _i64 * 3), ("o_stride", _i64 * 3),
                 ("offsets", _vp), ("window", _i64), ("sinks", _i64), ("scale", ctypes.c_float)]
+
+
+class KVCache(ctypes.Structure):
+    """lsmx_kv_cache of include/lsmx.h."""
+    _fields_ = [("k_codes", _vp), ("k_scale", _vp), ("v_codes", _vp), ("v_scale", _vp), ("pages", _i64), ("page", _i64),
+                ("kv_heads", _i64), ("head_dim", _i64), ("table", _vp), ("lengths", _vp), ("batch", _i64),
+                ("max_pages", _i64)]
 
 
 # Epochs for lsmx_scale_to_e8m0_batch's flag: unique within the process and

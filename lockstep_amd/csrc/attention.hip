@@ -26,6 +26,13 @@ constexpr int kBN = 64;   // keys of a tile
 template <typename T, int DP>
 struct DenseKV {
     static constexpr int NC = DP / 8, NU = kBN * NC / 256;
+    static constexpr bool kHoles = false;
+    typedef AttnArgs Args;
+    LSMX_DEV static const AttnArgs &attn(const Args &a) { return a; }
+    LSMX_DEV static bool find(const Args &a, int t, Seq &s) {
+        // the last tile of a sequence first: under a causal mask it is the longest
+        return find_tile(a, a.tiles - 1 - t, kBM, a.group, a.q_len, s);
+    }
     const T *k, *v;
     int64_t k_t, v_t;
     int k_len, dim;
@@ -55,19 +62,87 @@ struct DenseKV {
     }
 };
 
-template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_fwd_kernel(AttnArgs a) {
-    constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16;
+// Keys and values of a paged MXFP4 cache, expanded to bf16 on their way into
+// LDS (exact).  A thread takes a quarter of one key's and one value's vector.
+template <int DP>
+struct PagedKV {
+    static constexpr int NC = DP / 8, NW = DP / 32;  // words of codes of a thread
+    static constexpr bool kHoles = true;
+    typedef AttendArgs Args;
+    typedef __bf16 T;
+    const Pool *p;
+    int b, h, k_len, row, part;
+    uint32_t kr[NW], vr[NW];
+    uint32_t ke, ve;
+    bool in;
+
+    LSMX_DEV static const AttnArgs &attn(const Args &a) { return a.a; }
+    LSMX_DEV static bool find(const Args &x, int t, Seq &s) {
+        const AttnArgs &a = x.a;
+        const int per = (a.q_len * a.group + kBM - 1) / kBM;
+        t = a.tiles - 1 - t;
+        s.b = t / per;
+        s.tile = t - s.b * per;
+        s.q_len = a.q_len;
+        s.k_len = x.p.length(s.b);
+        s.shift = s.k_len - s.q_len;
+        s.q0 = s.k0 = 0;
+        return true;
+    }
+    LSMX_DEV void init(const Args &a, const Seq &s, int hkv) {
+        p = &a.p, b = s.b, h = hkv, k_len = s.k_len, row = threadIdx.x >> 2, part = threadIdx.x & 3;
+    }
+    LSMX_DEV void load(int j0) {
+        const int j = j0 + row, pg = j < k_len ? p->page_of(b, j) : -1;
+        in = pg >= 0;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) kr[i] = vr[i] = 0;
+        ke = ve = 0;
+        if (in) {
+            const int64_t v = p->vec(pg, h, j);
+            const uint8_t *kp = p->kc + v * (DP / 2) + part * (DP / 8), *vp = p->vc + v * (DP / 2) + part * (DP / 8);
+            if constexpr (NW == 4) {
+                *(u32x4 *)kr = *(const u32x4 *)kp;
+                *(u32x4 *)vr = *(const u32x4 *)vp;
+            } else {
+                *(u32x2 *)kr = *(const u32x2 *)kp;
+                *(u32x2 *)vr = *(const u32x2 *)vp;
+            }
+            const int blk = part * (DP / 32) / 4;
+            ke = p->ks[v * (DP / 32) + blk];
+            ve = p->vs[v * (DP / 32) + blk];
+        }
+    }
+    LSMX_DEV void store(T *sk, T *sv) {
+        const float ksc = e8m0_to_f32(ke), vsc = e8m0_to_f32(ve);
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            const int c = swz<NC>(row, part * NW + i);
+            *(bf16x8 *)(sk + row * DP + c * 8) = fp4x8_to_bf16(kr[i], ksc);
+            *(bf16x8 *)(sv + row * DP + c * 8) = fp4x8_to_bf16(vr[i], vsc);
+        }
+    }
+};
+
+// TQ: type of q and o; T: type of the products' operands.  fp16 rows against
+// a cache (whose values need bf16's exponents) enter as two bf16 terms, and
+// so do their probabilities.
+template <typename TQ, typename T, int DP, typename KV>
+__global__ __launch_bounds__(256) void attn_fwd_kernel(typename KV::Args args) {
+    constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, NT = sizeof(TQ) == sizeof(T) && __is_same(TQ, T) ? 1 : 2;
     typedef typename Vec<T>::x8 X8;
     typedef typename Vec<T>::x4 X4;
+    typedef typename Vec<TQ>::x8 Q8;
+    typedef typename Vec<TQ>::x4 Q4;
     __shared__ T sk[kBN * DP], sv[kBN * DP];
+    __shared__ int s_in[KV::kHoles ? kBN : 1];
 
+    const AttnArgs &a = KV::attn(args);
     const int item = xcd_item(blockIdx.x, a.per);
     if (item >= a.tiles * a.kv_heads) return;
     const int hkv = item / a.tiles;
     Seq s;
-    // the last tile of a sequence first: under a causal mask it is the longest
-    if (!find_tile(a, a.tiles - 1 - item % a.tiles, kBM, a.group, a.q_len, s)) return;
+    if (!KV::find(args, item % a.tiles, s)) return;
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
     const int row0 = s.tile * kBM, rows = s.q_len * a.group;
@@ -76,7 +151,7 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(AttnArgs a) {
     // this lane's rows: wrow and wrow + 16
     int pos[2];
     int64_t o_at[2], l_at[2];
-    X8 qf[2][NS];
+    X8 qf[NT][2][NS];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const int row = wrow + 16 * t;
@@ -85,11 +160,15 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(AttnArgs a) {
         pos[t] = in ? tok + s.shift : -1;
         o_at[t] = in ? s.b * a.o_b + (s.q0 + tok) * a.o_t + h * a.o_h : -1;
         l_at[t] = s.b * a.lse_b + h * a.lse_h + s.q0 + tok;
-        const T *qp = (const T *)a.q + s.b * a.q_b + (s.q0 + tok) * a.q_t + h * a.q_h;
+        const TQ *qp = (const TQ *)a.q + s.b * a.q_b + (s.q0 + tok) * a.q_t + h * a.q_h;
 #pragma unroll
         for (int st = 0; st < NS; ++st) {
             const int c = st * 4 + g;
-            qf[t][st] = in && c * 8 < a.dim ? *(const X8 *)(qp + c * 8) : X8{};
+            const Q8 x = in && c * 8 < a.dim ? *(const Q8 *)(qp + c * 8) : Q8{};
+            if constexpr (NT == 1)
+                qf[0][t][st] = x;
+            else
+                split(x, qf[0][t][st], qf[1][t][st]);
         }
     }
 
@@ -107,13 +186,17 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(AttnArgs a) {
     auto next = [&](int t) { return t + 1 < t_sink ? t + 1 : max(t + 1, t_lo); };
     int t = t_sink > 0 ? 0 : t_lo;
 
-    DenseKV<T, DP> kv;
-    kv.init(a, s, hkv);
+    KV kv;
+    kv.init(args, s, hkv);
     if (t < t_hi) kv.load(t * kBN);
     while (t < t_hi) {
         const int j0 = t * kBN, tn = next(t);
         __syncthreads();
         kv.store(sk, sv);
+        if (KV::kHoles) {
+            if constexpr (KV::kHoles)
+                if (kv.part == 0) s_in[kv.row] = kv.in;
+        }
         __syncthreads();
         if (tn < t_hi) kv.load(tn * kBN);
 
@@ -125,24 +208,31 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(AttnArgs a) {
 #pragma unroll
             for (int x = 0; x < NS; ++x) {
                 const X8 kf = *(const X8 *)(sk + j * DP + swz<NC>(j, x * 4 + g) * 8);
-                st[kt][0] = mfma(kf, qf[0][x], st[kt][0]);
-                st[kt][1] = mfma(kf, qf[1][x], st[kt][1]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    st[kt][0] = mfma(kf, qf[n][0][x], st[kt][0]);
+                    st[kt][1] = mfma(kf, qf[n][1][x], st[kt][1]);
+                }
             }
         }
-        const bool full = j0 + kBN - 1 <= pmin && (!a.window || j0 > pmax - a.window || j0 + kBN - 1 < a.sinks);
+        bool full = j0 + kBN - 1 <= pmin && (!a.window || j0 > pmax - a.window || j0 + kBN - 1 < a.sinks);
+        if constexpr (KV::kHoles) full = full & __all(s_in[lane]);
         if (!full) {
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int j = j0 + kt * 16 + g * 4 + i;
+                    bool in = true;
+                    if constexpr (KV::kHoles) in = s_in[kt * 16 + g * 4 + i];
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        st[kt][x][i] = sees(j, pos[x], window_low(pos[x], a.window), a.sinks) ? st[kt][x][i] : -INFINITY;
+                        const bool see = in & sees(j, pos[x], window_low(pos[x], a.window), a.sinks);
+                        st[kt][x][i] = see ? st[kt][x][i] : -INFINITY;
                     }
                 }
         }
-        X8 pf[2][2];  // [pair of key tiles][row]
+        X8 pf[NT][2][2];  // [term][pair of key tiles][row]
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             float mx = m[x];
@@ -165,7 +255,9 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(AttnArgs a) {
                     sum += p;
                     // the probabilities are the product's operand in the
                     // inputs' type; their sum is of the unrounded ones
-                    pf[kt >> 1][x][(kt & 1) * 4 + i] = (T)p;
+                    pf[0][kt >> 1][x][(kt & 1) * 4 + i] = (T)p;
+                    if constexpr (NT == 2)
+                        pf[1][kt >> 1][x][(kt & 1) * 4 + i] = (T)(p - (float)pf[0][kt >> 1][x][(kt & 1) * 4 + i]);
                 }
             l[x] = l[x] * alpha + sum;
 #pragma unroll
@@ -180,8 +272,11 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(AttnArgs a) {
                 const X4 v0 = read_tr<T>(sv + j * DP + swz<NC>(j, c) * 8 + e);
                 const X4 v1 = read_tr<T>(sv + (j + 16) * DP + swz<NC>(j + 16, c) * 8 + e);
                 const X8 vf = join<X4, X8>(v0, v1);
-                o[d][0] = mfma(vf, pf[u][0], o[d][0]);
-                o[d][1] = mfma(vf, pf[u][1], o[d][1]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    o[d][0] = mfma(vf, pf[n][u][0], o[d][0]);
+                    o[d][1] = mfma(vf, pf[n][u][1], o[d][1]);
+                }
             }
         }
         t = tn;
@@ -193,13 +288,13 @@ __global__ __launch_bounds__(256) void attn_fwd_kernel(AttnArgs a) {
         sum += __shfl_xor(sum, 32);
         const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
         if (o_at[x] < 0) continue;
-        T *op = (T *)a.o + o_at[x];
+        TQ *op = (TQ *)a.o + o_at[x];
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            X4 w;
+            Q4 w;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = (T)(o[d][x][i] * inv);
-            if (d * 16 + g * 4 < a.dim) *(X4 *)(op + d * 16 + g * 4) = w;
+            for (int i = 0; i < 4; ++i) w[i] = (TQ)(o[d][x][i] * inv);
+            if (d * 16 + g * 4 < a.dim) *(Q4 *)(op + d * 16 + g * 4) = w;
         }
         if (a.lse && g == 0) a.lse[l_at[x]] = sum > 0.f ? m[x] * a.c + __log2f(sum) : sum != sum ? sum : -INFINITY;
     }
@@ -209,13 +304,30 @@ template <typename T>
 hipError_t fwd(const AttnArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)a.per * 8);
     if (a.dim <= 64)
-        attn_fwd_kernel<T, 64><<<grid, 256, 0, s>>>(a);
+        attn_fwd_kernel<T, T, 64, DenseKV<T, 64>><<<grid, 256, 0, s>>>(a);
     else
-        attn_fwd_kernel<T, 128><<<grid, 256, 0, s>>>(a);
+        attn_fwd_kernel<T, T, 128, DenseKV<T, 128>><<<grid, 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t chunk(const AttendArgs &x, hipStream_t s) {
+    const dim3 grid((unsigned)x.a.per * 8);
+    if (x.p.dim == 64)
+        attn_fwd_kernel<T, __bf16, 64, PagedKV<64>><<<grid, 256, 0, s>>>(x);
+    else
+        attn_fwd_kernel<T, __bf16, 128, PagedKV<128>><<<grid, 256, 0, s>>>(x);
     return hipGetLastError();
 }
 
 }  // namespace
+
+hipError_t launch_kv_chunk(const AttendArgs &in, int dtype, hipStream_t s) {
+    AttendArgs x = in;
+    x.a.tiles = (int)(((int64_t)x.a.q_len * x.a.group + kBM - 1) / kBM) * x.a.batch;
+    x.a.per = (int)(((int64_t)x.a.tiles * x.a.kv_heads + 7) / 8);
+    return dtype == LSMX_BF16 ? chunk<__bf16>(x, s) : chunk<_Float16>(x, s);
+}
 
 hipError_t launch_attn_fwd(const AttnArgs &in, int dtype, hipStream_t s) {
     AttnArgs a = in;

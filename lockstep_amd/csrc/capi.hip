@@ -830,4 +830,171 @@ int lsmx_attention_bwd(const lsmx_attention *a, const void *d_o, const int64_t *
     return launched(lsmx::launch_attn_bwd(g, a->dtype, (hipStream_t)stream), fn);
 }
 
+// The checks of a cache description; fills the kernels' form.
+static int kv_pool(const char *fn, const lsmx_kv_cache *c, lsmx::Pool *p) {
+    if (!c) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    const int64_t lim = (int64_t)1 << 30;
+    if (c->pages < 0 || c->batch < 0 || c->max_pages < 0 || c->kv_heads < 1)
+        return fail(LSMX_ERR_SHAPE, "%s: negative size or no heads", fn);
+    if (c->page < 16 || c->page > 1024 || (c->page & (c->page - 1)))
+        return fail(LSMX_ERR_SHAPE, "%s: page=%lld must be a power of two, 16 to 1024", fn, (long long)c->page);
+    if (c->head_dim != 64 && c->head_dim != 128)
+        return fail(LSMX_ERR_SHAPE, "%s: head_dim=%lld must be 64 or 128", fn, (long long)c->head_dim);
+    if (c->pages >= lim || c->kv_heads >= lim || c->batch >= lim || c->max_pages * c->page >= lim ||
+        c->batch * c->kv_heads >= lim)
+        return fail(LSMX_ERR_SHAPE, "%s: too many pages, sequences or heads", fn);
+    if (c->pages && (!c->k_codes || !c->k_scale || !c->v_codes || !c->v_scale))
+        return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (c->batch && (!c->lengths || (c->max_pages && !c->table))) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (!aligned(c->k_codes, 16) || !aligned(c->k_scale, 16) || !aligned(c->v_codes, 16) || !aligned(c->v_scale, 16) ||
+        !aligned(c->table, 4) || !aligned(c->lengths, 4))
+        return fail(LSMX_ERR_ALIGN, "%s: cache buffers must be 16-byte aligned", fn);
+    int shift = 0;
+    while ((1 << shift) < c->page) ++shift;
+    *p = lsmx::Pool{c->k_codes, c->k_scale, c->v_codes, c->v_scale, c->table, c->lengths, (int)c->pages,
+                    (int)c->kv_heads, (int)c->head_dim, (int)c->page, shift, (int)c->max_pages};
+    return LSMX_OK;
+}
+
+int lsmx_kv_append(const lsmx_kv_cache *c, const void *k, const int64_t *k_stride, const void *v,
+                   const int64_t *v_stride, int dtype, int64_t tokens, int64_t per_seq, const int32_t *offsets,
+                   void *k_out, void *v_out, void *stream) {
+    const char *fn = "lsmx_kv_append";
+    lsmx::AppendArgs a{};
+    if (int r = kv_pool(fn, c, &a.p)) return r;
+    if (dtype != LSMX_BF16 && dtype != LSMX_F16) return fail(LSMX_ERR_DTYPE, "%s: dtype must be bf16 or fp16", fn);
+    const int64_t lim = (int64_t)1 << 30;
+    if (tokens < 0 || tokens >= lim || per_seq < 0) return fail(LSMX_ERR_SHAPE, "%s: bad number of tokens", fn);
+    if (!offsets && tokens != per_seq * c->batch)
+        return fail(LSMX_ERR_SHAPE, "%s: tokens=%lld is not per_seq=%lld for each of %lld sequences", fn,
+                    (long long)tokens, (long long)per_seq, (long long)c->batch);
+    if (!k_stride || !v_stride || (tokens && (!k || !v)) || !k_out != !v_out) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (!aligned(k, 16) || !aligned(v, 16) || !aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(offsets, 4) ||
+        k_stride[0] % 8 || k_stride[1] % 8 || v_stride[0] % 8 || v_stride[1] % 8)
+        return fail(LSMX_ERR_ALIGN, "%s: k and v must be 16-byte aligned, with strides that are multiples of 8", fn);
+    if (int r = device_guard()) return r;
+    if (!tokens) return LSMX_OK;
+    a.k = k, a.v = v, a.k_t = k_stride[0], a.k_h = k_stride[1], a.v_t = v_stride[0], a.v_h = v_stride[1];
+    a.batch = (int)c->batch, a.tokens = (int)tokens, a.per_seq = (int)per_seq, a.offsets = offsets;
+    a.by_seq = lsmx::fast_div(offsets ? 1 : (uint32_t)per_seq);
+    a.k_out = k_out, a.v_out = v_out;
+    return launched(lsmx::launch_kv_append(a, dtype, (hipStream_t)stream), fn);
+}
+
+// What the keys of one call's rows span at most, whatever the lengths.
+static int64_t kv_span(const lsmx_kv_cache *c, int64_t q_len, int64_t window, int64_t sinks) {
+    const int64_t cap = c->max_pages * c->page;
+    return window && window < cap && q_len + window + sinks < cap ? q_len + window + sinks : cap;
+}
+
+// Splits, and the workspace: partial rows of the splits, then the rows' lse
+// where weights are asked for.
+struct KvPlan {
+    int splits;
+    int64_t part, part_m, lse, bytes;
+};
+static KvPlan kv_plan(const lsmx_kv_cache *c, int64_t q_len, int64_t heads, int64_t window, int64_t sinks, bool weights) {
+    KvPlan p{};
+    const int64_t rows = q_len * (heads / c->kv_heads), bh = c->batch * c->kv_heads;
+    p.splits = bh && rows ? lsmx::kv_attend_splits((int)c->batch, (int)c->kv_heads, (int)rows, kv_span(c, q_len, window, sinks)) : 1;
+    const auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+    if (p.splits > 1) {
+        p.part_m = up(bh * p.splits * rows * c->head_dim * 4);
+        p.bytes = p.part_m + up(bh * p.splits * rows * 8);
+    }
+    p.lse = p.bytes;
+    if (weights) p.bytes += up(bh * rows * 4);
+    return p;
+}
+
+static int kv_attend_check(const char *fn, const lsmx_kv_cache *c, int64_t q_len, int64_t heads, int64_t window,
+                           int64_t sinks, lsmx::Pool *p) {
+    if (int r = kv_pool(fn, c, p)) return r;
+    if (heads < 1 || heads % c->kv_heads)
+        return fail(LSMX_ERR_SHAPE, "%s: heads=%lld must be a positive multiple of kv_heads=%lld", fn, (long long)heads,
+                    (long long)c->kv_heads);
+    if (window < 0 || sinks < 0) return fail(LSMX_ERR_ARG, "%s: negative window or sinks", fn);
+    const int64_t lim = (int64_t)1 << 30, rows = q_len * (heads / c->kv_heads), bh = c->batch * c->kv_heads;
+    if (q_len < 0 || q_len >= lim || heads >= lim || rows >= lim || (bh && (rows + 256) * bh >= lim) ||
+        bh * (c->max_pages * c->page / 64 + 1) >= lim)
+        return fail(LSMX_ERR_SHAPE, "%s: too many tokens, sequences or heads", fn);
+    return LSMX_OK;
+}
+
+int64_t lsmx_kv_attend_workspace(const lsmx_kv_cache *c, int64_t q_len, int64_t heads, int64_t window, int64_t sinks,
+                                 int weights) {
+    lsmx::Pool p;
+    if (kv_attend_check("lsmx_kv_attend_workspace", c, q_len, heads, window, sinks, &p)) return 0;
+    return kv_plan(c, q_len, heads, window, sinks, weights != 0).bytes;
+}
+
+int lsmx_kv_attend(const lsmx_kv_cache *c, const void *q, const int64_t *q_stride, int dtype, int64_t q_len,
+                   int64_t heads, int64_t window, int64_t sinks, float scale, void *o, float *weights, int64_t w_len,
+                   void *ws, int64_t ws_bytes, void *stream) {
+    const char *fn = "lsmx_kv_attend";
+    lsmx::AttendArgs x{};
+    if (int r = kv_attend_check(fn, c, q_len, heads, window, sinks, &x.p)) return r;
+    if (dtype != LSMX_BF16 && dtype != LSMX_F16) return fail(LSMX_ERR_DTYPE, "%s: dtype must be bf16 or fp16", fn);
+    if (!(scale > 0.f) || !(scale <= 3.0e38f)) return fail(LSMX_ERR_ARG, "%s: scale must be positive and finite", fn);
+    if (!q_stride || (q_len && c->batch && (!q || !o))) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (weights && w_len < c->max_pages * c->page)
+        return fail(LSMX_ERR_SHAPE, "%s: weights are %lld wide, the table spans %lld tokens", fn, (long long)w_len,
+                    (long long)(c->max_pages * c->page));
+    if (!aligned(q, 16) || !aligned(o, 16) || !aligned(weights, 4) || !aligned(ws, 16) || q_stride[0] % 8 ||
+        q_stride[1] % 8 || q_stride[2] % 8)
+        return fail(LSMX_ERR_ALIGN, "%s: q and o must be 16-byte aligned, with strides that are multiples of 8", fn);
+    const KvPlan plan = kv_plan(c, q_len, heads, window, sinks, weights != nullptr);
+    if (plan.bytes && (!ws || ws_bytes < plan.bytes)) return fail(LSMX_ERR_ARG, "%s: workspace too small", fn);
+    if (int r = device_guard()) return r;
+    if (!c->batch || !q_len) return LSMX_OK;
+    const int64_t lim = (int64_t)1 << 30;
+    lsmx::AttnArgs &a = x.a;
+    a.q = q, a.o = o, a.lse = weights ? (float *)((uint8_t *)ws + plan.lse) : nullptr;
+    a.batch = (int)c->batch, a.heads = (int)heads, a.kv_heads = (int)c->kv_heads, a.group = (int)(heads / c->kv_heads);
+    a.dim = (int)c->head_dim, a.q_len = (int)q_len;
+    a.q_b = q_stride[0], a.q_t = q_stride[1], a.q_h = q_stride[2];
+    a.o_h = c->head_dim, a.o_t = heads * c->head_dim, a.o_b = q_len * a.o_t;
+    a.lse_h = q_len, a.lse_b = heads * q_len;
+    a.window = (int)(window < lim ? window : lim), a.sinks = window ? (int)(sinks < lim ? sinks : lim) : 0;
+    a.scale = scale, a.c = scale * 1.4426950408889634f, a.by_group = lsmx::fast_div((uint32_t)a.group);
+    x.weights = weights, x.w_len = w_len, x.splits = plan.splits;
+    x.part = (float *)ws, x.part_m = (float *)((uint8_t *)ws + plan.part_m);
+    // calls of several host threads on one stream may share a workspace: the
+    // launches of one stay together
+    static std::mutex mu;
+    std::lock_guard<std::mutex> lk(mu);
+    if (int r = launched(lsmx::launch_kv_attend(x, dtype, (hipStream_t)stream), fn)) return r;
+    return weights ? launched(lsmx::launch_kv_weights(x, dtype, (hipStream_t)stream), fn) : LSMX_OK;
+}
+
+int lsmx_kv_evict(const lsmx_kv_cache *c, const float *weights, int64_t w_len, int64_t keep, int64_t sinks,
+                  int64_t recent, const int32_t *out_table, int64_t out_max_pages, int32_t *index,
+                  float *new_weights, int32_t *new_lengths, void *stream) {
+    const char *fn = "lsmx_kv_evict";
+    lsmx::EvictArgs a{};
+    if (int r = kv_pool(fn, c, &a.p)) return r;
+    const int64_t lim = (int64_t)1 << 30;
+    if (keep < 1 || keep >= lim || sinks < 0 || recent < 0 || sinks + recent > keep)
+        return fail(LSMX_ERR_ARG, "%s: needs 1 <= keep and sinks + recent <= keep", fn);
+    if (out_max_pages < 0 || out_max_pages * c->page >= lim) return fail(LSMX_ERR_SHAPE, "%s: bad out_max_pages", fn);
+    const int64_t cap = c->max_pages * c->page, most = keep < cap ? keep : cap;
+    if (out_max_pages * c->page < most)
+        return fail(LSMX_ERR_SHAPE, "%s: out_table holds %lld tokens, %lld may stay", fn,
+                    (long long)(out_max_pages * c->page), (long long)most);
+    if (w_len < cap) return fail(LSMX_ERR_SHAPE, "%s: weights are %lld wide, the table spans %lld tokens", fn,
+                                 (long long)w_len, (long long)cap);
+    if (c->batch * c->kv_heads * (keep / 16 + 1) >= lim) return fail(LSMX_ERR_SHAPE, "%s: too many sequences or heads", fn);
+    if (c->batch && ((cap && !weights) || (out_max_pages && !out_table) || !index || !new_weights || !new_lengths))
+        return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (!aligned(weights, 4) || !aligned(out_table, 4) || !aligned(index, 4) || !aligned(new_weights, 4) ||
+        !aligned(new_lengths, 4))
+        return fail(LSMX_ERR_ALIGN, "%s: misaligned pointer", fn);
+    if (int r = device_guard()) return r;
+    if (!c->batch) return LSMX_OK;
+    a.out_table = out_table, a.out_max_pages = (int)out_max_pages, a.weights = weights, a.w_len = w_len;
+    a.batch = (int)c->batch, a.keep = (int)keep, a.sinks = (int)sinks, a.recent = (int)recent;
+    a.index = index, a.new_lengths = new_lengths, a.new_weights = new_weights;
+    return launched(lsmx::launch_kv_evict(a, (hipStream_t)stream), fn);
+}
+
 }  // extern "C"

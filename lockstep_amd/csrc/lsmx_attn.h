@@ -164,6 +164,88 @@ LSMX_DEV bool find_tile(const AttnArgs &a, int t, int size, int mult, int len, S
     return false;
 }
 
+// A paged MXFP4 cache: pool of pages [pages][kv_heads][page][..], codes D / 2
+// and E8M0 scales D / 32 bytes per vector; block tables and lengths of the
+// sequences.  A page id outside the pool and a position past the table are
+// never followed: their keys are hidden.
+struct Pool {
+    uint8_t *kc, *ks, *vc, *vs;
+    const int32_t *table, *lengths;
+    int pages, kv_heads, dim, page, page_shift, max_pages;
+
+    LSMX_DEV int length(int b) const { return min(max(lengths[b], 0), max_pages << page_shift); }
+    // the page of position j of sequence b, or -1
+    LSMX_DEV int page_of(int b, int j) const {
+        const int p = table[(int64_t)b * max_pages + (j >> page_shift)];
+        return (uint32_t)p < (uint32_t)pages ? p : -1;
+    }
+    // vector index (in units of one token's head vector) of position j in page p
+    LSMX_DEV int64_t vec(int p, int h, int j) const {
+        return (((int64_t)p * kv_heads + h) << page_shift) + (j & (page - 1));
+    }
+};
+
+// Attention of the newest q_len tokens of every sequence over the cache.
+struct AttendArgs {
+    AttnArgs a;  // q, o, lse, strides, mask and scale; k_len and the rest unused
+    Pool p;
+    float *weights;       // [batch, kv_heads, w_len], or null
+    int64_t w_len;
+    int splits;           // decode: workgroups per sequence and key head
+    float *part, *part_m; // decode: [batch kv_heads splits rows][DP] and [..][2]
+};
+
+struct AppendArgs {
+    const void *k, *v;
+    int64_t k_t, k_h, v_t, v_h;  // strides, in elements
+    Pool p;
+    int batch, tokens, per_seq;  // per_seq: tokens of each sequence, packed with offsets: 0
+    const int32_t *offsets;
+    FastDiv by_seq;
+    void *k_out, *v_out;         // bf16 values [tokens, kv_heads, dim], or null
+};
+
+struct EvictArgs {
+    Pool p;
+    const int32_t *out_table;
+    int out_max_pages;
+    const float *weights;
+    int64_t w_len;
+    int batch, keep, sinks, recent;
+    int32_t *index, *new_lengths;
+    float *new_weights;
+};
+
+// The 8 elements of four bytes of codes, times 2^e of their block.
+LSMX_DEV bf16x8 fp4x8_to_bf16(uint32_t w, float sc) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3);
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// An fp16 vector as the sum of two bf16 ones, exact: 8 + 3 significant bits,
+// and bf16's exponents cover fp16's subnormals.
+LSMX_DEV void split(f16x8 x, bf16x8 &hi, bf16x8 &lo) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float f = (float)x[i];
+        hi[i] = (__bf16)f;
+        // an infinity or NaN stays in the first term alone
+        const float d = f - (float)hi[i];
+        lo[i] = (__bf16)(d == d ? d : 0.f);
+    }
+}
+
+// Rows (tokens x heads of a key head) up to which the keys of a sequence are
+// split over workgroups; more rows run in tiles of 128.
+constexpr int kDecodeRows = 64;
+hipError_t launch_kv_append(const AppendArgs &a, int dtype, hipStream_t s);
+int kv_attend_splits(int batch, int kv_heads, int rows, int64_t keys);
+hipError_t launch_kv_attend(const AttendArgs &a, int dtype, hipStream_t s);
+hipError_t launch_kv_chunk(const AttendArgs &a, int dtype, hipStream_t s);
+hipError_t launch_kv_weights(const AttendArgs &a, int dtype, hipStream_t s);
+hipError_t launch_kv_evict(const EvictArgs &a, hipStream_t s);
+
 hipError_t launch_attn_fwd(const AttnArgs &a, int dtype, hipStream_t s);
 int64_t attn_bwd_workspace(const AttnArgs &a);
 hipError_t launch_attn_bwd(const AttnArgs &a, int dtype, hipStream_t s);
