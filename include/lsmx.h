@@ -463,7 +463,8 @@ typedef struct {
     int64_t batch, q_len, k_len, heads, kv_heads;
     int64_t head_dim;       /* a multiple of 8, at most 128                      */
     int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3]; /* sequence, token,
-                              head; multiples of 8, 16-byte aligned bases       */
+                              head; multiples of 8, token strides below 2^23;
+                              16-byte aligned bases                             */
     const int32_t *offsets;
     int64_t window, sinks;  /* window 0: none                                    */
     float scale;            /* finite, > 0                                       */

@@ -59,7 +59,7 @@ def _args(q, k, v, o, lse, offsets, window, sinks, scale):
 
 
 def _forward(q, k, v, offsets, window, sinks, scale):
-    q, k, v = rows16(q), rows16(k), rows16(v)
+    q, k, v = (rows16(t) if t.stride(-3) < 2 ** 23 else t.contiguous() for t in (q, k, v))
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lead = q.shape[:1] if offsets is None else ()
     lse = torch.empty((*lead, q.shape[-2], q.shape[-3]), dtype=torch.float32, device=q.device)
@@ -82,7 +82,7 @@ class _SinkWindowAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o, _):
         q, k, v, o, lse, *offsets = ctx.saved_tensors
-        d_o = rows16(d_o.to(q.dtype))
+        d_o = rows16(d_o.to(q.dtype)) if d_o.stride(-3) < 2 ** 23 else d_o.contiguous()
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         if q.numel() or k.numel():
             a = _args(q, k, v, o, lse, offsets[0] if offsets else None, *ctx.mask)

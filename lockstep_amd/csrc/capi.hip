@@ -777,6 +777,10 @@ static int attn_args(const char *fn, const lsmx_attention *a, bool bwd, lsmx::At
     for (int i = 0; i < 3; ++i)
         if (a->q_stride[i] % 8 || a->k_stride[i] % 8 || a->v_stride[i] % 8 || a->o_stride[i] % 8)
             return fail(LSMX_ERR_ALIGN, "%s: strides must be multiples of 8 elements", fn);
+    // offsets within a tile are 32-bit
+    if (a->q_stride[1] < 0 || a->k_stride[1] < 0 || a->v_stride[1] < 0 || a->q_stride[1] >= 1 << 23 ||
+        a->k_stride[1] >= 1 << 23 || a->v_stride[1] >= 1 << 23)
+        return fail(LSMX_ERR_SHAPE, "%s: token strides must be below 2^23", fn);
     lsmx::AttnArgs &g = *out;
     g = lsmx::AttnArgs{};
     g.q = a->q, g.k = a->k, g.v = a->v, g.o = a->o, g.lse = a->lse;
