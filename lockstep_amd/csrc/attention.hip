@@ -22,9 +22,14 @@ namespace {
 
 constexpr int kBN = 64;  // keys of a tile
 
-// Waits for a wave's own direct-to-LDS loads (issued in inline assembly, which
-// the compiler does not count).
-LSMX_DEV void wait_dma() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Waits for a wave's own direct-to-LDS loads, which are issued in inline
+// assembly and not counted by the compiler.  It sees this wait, so that it
+// puts no wait for the rows' loads into the loop, where that would be one for
+// the tile in flight.
+LSMX_DEV void wait_dma() {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    asm volatile("" ::: "memory");
+}
 
 // Keys and values as they lie in memory, loaded straight into LDS: lane l of
 // a load fills 16-byte position l, so the swizzle is in the addresses.  The
@@ -38,8 +43,6 @@ struct DenseKV {
     const T *k, *v;
     int64_t k_t, v_t;
     int k_len;
-    uint32_t row, chunk;  // of lane's first load; the others are NW * 64 / NC rows on
-    bool in;
 
     LSMX_DEV static const AttnArgs &attn(const Args &a) { return a; }
     LSMX_DEV static bool find(const Args &a, int t, int size, Seq &s) {
@@ -51,35 +54,36 @@ struct DenseKV {
         v = (const T *)a.v + s.b * a.v_b + s.k0 * a.v_t + hkv * a.v_h;
         k_t = a.k_t, v_t = a.v_t, k_len = s.k_len;
     }
-    LSMX_DEV void fetch(int j0, T *sk, T *sv, int dim) {
-        const v4i_rsrc rk = buf_rsrc(k + j0 * k_t, 0x7FFFFFFF), rv = buf_rsrc(v + j0 * v_t, 0x7FFFFFFF);
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-        const uint32_t bk = lds_u32(sk), bv = lds_u32(sv);
+    LSMX_DEV void fetch(const T *x, int64_t x_t, int j0, T *to, int dim) {
+        const v4i_rsrc rs = buf_rsrc(x + j0 * x_t, 0x7FFFFFFF);
+        const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+        const uint32_t lds = lds_u32(to);
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
             const int at = (u * NW + wave) * 64, j = (at + lane) / NC, c = swz<NC>(j, lane % NC);
             const bool ok = j0 + j < k_len && c * 8 < dim;
-            dma_x4(ok ? (uint32_t)(j * (int)k_t + c * 8) * 2 : 0x80000000u, rk, bk + at * 16);
-            dma_x4(ok ? (uint32_t)(j * (int)v_t + c * 8) * 2 : 0x80000000u, rv, bv + at * 16);
+            dma_x4(ok ? (uint32_t)(j * (int)x_t + c * 8) * 2 : 0x80000000u, rs, lds + at * 16);
         }
     }
-    LSMX_DEV void land(T *, T *, int *) { wait_dma(); }
+    LSMX_DEV void fetch_k(int j0, T *to, int dim) { fetch(k, k_t, j0, to, dim); }
+    LSMX_DEV void fetch_v(int j0, T *to, int dim) { fetch(v, v_t, j0, to, dim); }
+    LSMX_DEV void land_k(T *, int *) { wait_dma(); }
+    LSMX_DEV void land_v(T *) { wait_dma(); }
 };
 
 // Keys and values of a paged MXFP4 cache, expanded to bf16 on their way into
-// LDS (exact).  Four threads take a key's vector, and (the same four of 4
-// waves, the next of 8) a value's.
-template <int DP, int NW>
+// LDS (exact).  Four of the 256 threads take a key's vector, and a value's.
+template <int DP>
 struct PagedKV {
     static constexpr int NC = DP / 8, NQ = DP / 32;  // words of codes of a thread
-    static constexpr bool kHoles = true, kBoth = NW == 4;
+    static constexpr bool kHoles = true;
     typedef AttendArgs Args;
     typedef __bf16 T;
     const Pool *p;
     int b, h, k_len, row, part;
     uint32_t kr[NQ], vr[NQ];
     uint32_t ke, ve;
-    bool in, is_v;
+    bool in;
 
     LSMX_DEV static const AttnArgs &attn(const Args &a) { return a.a; }
     LSMX_DEV static bool find(const Args &x, int t, int size, Seq &s) {
@@ -95,52 +99,58 @@ struct PagedKV {
         return true;
     }
     LSMX_DEV void init(const Args &a, const Seq &s, int hkv) {
-        p = &a.p, b = s.b, h = hkv, k_len = s.k_len;
-        row = (threadIdx.x & 255) >> 2, part = threadIdx.x & 3, is_v = threadIdx.x >= 256;
+        p = &a.p, b = s.b, h = hkv, k_len = s.k_len, row = threadIdx.x >> 2, part = threadIdx.x & 3;
     }
-    LSMX_DEV static void codes(uint32_t (&w)[NQ], const uint8_t *c) {
-        if constexpr (NQ == 4)
-            *(u32x4 *)w = *(const u32x4 *)c;
-        else
-            *(u32x2 *)w = *(const u32x2 *)c;
-    }
-    LSMX_DEV void fetch(int j0, T *, T *, int) {
-        const int j = j0 + row, pg = j < k_len ? p->page_of(b, j) : -1;
-        in = pg >= 0;
+    // the thread's part of vector j: its codes, its block's scale; whether j is held
+    LSMX_DEV bool load(const uint8_t *codes, const uint8_t *scale, int j, uint32_t (&w)[NQ], uint32_t &e) {
+        const int pg = j < k_len ? p->page_of(b, j) : -1;
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) kr[i] = vr[i] = 0;
-        ke = ve = 0;
-        if (in) {
+        for (int i = 0; i < NQ; ++i) w[i] = 0;
+        e = 0;
+        if (pg >= 0) {
             const int64_t v = p->vec(pg, h, j);
-            const int blk = part * (DP / 32) / 4;
-            codes(kr, (is_v ? p->vc : p->kc) + v * (DP / 2) + part * (DP / 8));
-            ke = (is_v ? p->vs : p->ks)[v * (DP / 32) + blk];
-            if constexpr (kBoth) {
-                codes(vr, p->vc + v * (DP / 2) + part * (DP / 8));
-                ve = p->vs[v * (DP / 32) + blk];
-            }
+            const uint8_t *c = codes + v * (DP / 2) + part * (DP / 8);
+            if constexpr (NQ == 4)
+                *(u32x4 *)w = *(const u32x4 *)c;
+            else
+                *(u32x2 *)w = *(const u32x2 *)c;
+            e = scale[v * (DP / 32) + part * (DP / 32) / 4];
         }
+        return pg >= 0;
     }
-    LSMX_DEV void land(T *sk, T *sv, int *s_in) {
-        const float ksc = e8m0_to_f32(ke), vsc = e8m0_to_f32(ve);
-        T *first = is_v ? sv : sk;
+    LSMX_DEV void store(T *to, const uint32_t (&w)[NQ], uint32_t e) {
+        const float sc = e8m0_to_f32(e);
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-            const int c = swz<NC>(row, part * NQ + i);
-            *(bf16x8 *)(first + row * DP + c * 8) = fp4x8_to_bf16(kr[i], ksc);
-            if constexpr (kBoth) *(bf16x8 *)(sv + row * DP + c * 8) = fp4x8_to_bf16(vr[i], vsc);
-        }
-        if (part == 0 && !is_v) s_in[row] = in;
+        for (int i = 0; i < NQ; ++i) *(bf16x8 *)(to + row * DP + swz<NC>(row, part * NQ + i) * 8) = fp4x8_to_bf16(w[i], sc);
     }
+    LSMX_DEV void fetch_k(int j0, T *, int) { in = load(p->kc, p->ks, j0 + row, kr, ke); }
+    LSMX_DEV void fetch_v(int j0, T *, int) { load(p->vc, p->vs, j0 + row, vr, ve); }
+    LSMX_DEV void land_k(T *to, int *s_in) {
+        store(to, kr, ke);
+        if (part == 0) s_in[row] = in;
+    }
+    LSMX_DEV void land_v(T *to) { store(to, vr, ve); }
 };
 
 // NW waves of RT x 16 rows.  TQ: type of q and o; T: type of the products'
 // operands.  fp16 rows against a cache (whose values need bf16's exponents)
 // enter as two bf16 terms, and so do their probabilities.
+//
+// The loop is pipelined over two key tiles: the scores of the next tile are
+// products that do not wait for anything, and stand between the exponentials
+// of this one, which are as much work for the vector unit as both products
+// are for the matrix unit.
+//
+// Bound by the vector unit (exponentials, sums and conversions: 52% of its
+// cycles at head 128, 66% at 64, with the matrix unit at 34% and 32%), so that
+// waves per SIMD count: 2 at head 128, 3 at 64 (registers allow it only while
+// a step is 32 keys).  2 x 4096 tokens, 32/8 heads of 128, window 1024: 184 us
+// = 656 TFLOP/s of the visible pairs; 16384 tokens of 8/1 heads of 64 through a
+// window of 4096: 227 us.
 template <typename TQ, typename T, int DP, int RT, int NW, typename KV>
-__global__ __launch_bounds__(NW * 64, 2) void attn_fwd_kernel(typename KV::Args args) {
+__global__ __launch_bounds__(NW * 64, KV::kHoles ? (DP == 64 ? 2 : 1) : (DP == 64 ? 3 : 2)) void attn_fwd_kernel(typename KV::Args args) {
     constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, NT = __is_same(TQ, T) ? 1 : 2, BM = NW * RT * 16;
-    // a row's maximum is followed only when it grows by this factor 2^8: the
+    // a row's maximum is followed only when it grows by a factor of 2^8: the
     // probabilities stay below 2^8 and O is rescaled a few times per row
     constexpr float kLazy = 8.f;
     typedef typename Vec<T>::x8 X8;
@@ -157,7 +167,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_fwd_kernel(typename KV::Args 
     Seq s;
     if (!KV::find(args, item % a.tiles, BM, s)) return;
 
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
     const int row0 = s.tile * BM, rows = s.q_len * a.group, wrow0 = row0 + wave * RT * 16;
 
     // the keys that some row of the tile sees: the sinks, then [lo, hi)
@@ -167,14 +177,19 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_fwd_kernel(typename KV::Args 
     const int t_sink = (min(a.sinks, hi) + kBN - 1) / kBN, t_hi = hi > 0 ? (hi + kBN - 1) / kBN : 0;
     const int t_lo = lo / kBN;
     auto next = [&](int t) { return t + 1 < t_sink ? t + 1 : max(t + 1, t_lo); };
-    int t = t_sink > 0 ? 0 : t_lo, buf = 0;
-    // and those of this wave's rows
+    int t = t_sink > 0 ? 0 : t_lo, tn = next(t);
+    // and the positions of this wave's rows
     const int wmin = div_by(min(wrow0, rows - 1), a.by_group) + s.shift;
-    const int wmax = wrow0 < rows ? div_by(min(wrow0 + RT * 16, rows) - 1, a.by_group) + s.shift : -1;
+    const int wmax = div_by(min(wrow0 + RT * 16, rows) - 1, a.by_group) + s.shift;
 
     KV kv;
     kv.init(args, s, hkv);
-    if (t < t_hi) kv.fetch(t * kBN, sk[0], sv[0], a.dim);
+    if (t < t_hi) {
+        kv.fetch_k(t * kBN, sk[0], a.dim);
+        kv.fetch_v(t * kBN, sv[0], a.dim);
+        kv.land_k(sk[0], s_in[0]);
+        kv.land_v(sv[0]);
+    }
 
     // this lane's rows: wrow0 + r + 16 x
     int pos[RT], low[RT];
@@ -198,127 +213,152 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_fwd_kernel(typename KV::Args 
         }
     }
 
-    f32x4 o[ND][RT];
-    float m[RT], l[RT];
+    f32x4 o[ND][RT], st[2][RT];
+    // of each row: maximum, its limit, times c; sum over this lane's keys
+    float m[RT], limit[RT], mc[RT], l[RT];
 #pragma unroll
     for (int x = 0; x < RT; ++x) {
-        m[x] = -INFINITY, l[x] = 0.f;
+        m[x] = limit[x] = -INFINITY, mc[x] = l[x] = 0.f;
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d][x] = f32x4{0, 0, 0, 0};
     }
     const float lazy = kLazy / a.c;
 
-    if (t < t_hi) kv.land(sk[0], sv[0], s_in[0]);
-    __syncthreads();
-    while (t < t_hi) {
-        const int j0 = t * kBN, tn = next(t);
-        if (tn < t_hi) kv.fetch(tn * kBN, sk[buf ^ 1], sv[buf ^ 1], a.dim);
-        // hidden from every row of the wave: nothing to do
-        const bool none = j0 > wmax || (a.window && j0 + kBN - 1 <= wmin - a.window && j0 >= a.sinks);
-        if (!none) {
-            const T *ck = sk[buf], *cv = sv[buf];
-            f32x4 st[4][RT];
+    // scores of 32 keys from row j0 of a tile on
+    auto scores = [&](const T *ck, int j0, f32x4 (&z)[2][RT]) {
 #pragma unroll
-            for (int kt = 0; kt < 4; ++kt) {
-                const int j = kt * 16 + r;
+        for (int kt = 0; kt < 2; ++kt) {
+            const int j = j0 + kt * 16 + r;
 #pragma unroll
-                for (int x = 0; x < RT; ++x) st[kt][x] = f32x4{0, 0, 0, 0};
+            for (int x = 0; x < RT; ++x) z[kt][x] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int y = 0; y < NS; ++y) {
-                    const X8 kf = *(const X8 *)(ck + j * DP + swz<NC>(j, y * 4 + g) * 8);
+            for (int y = 0; y < NS; ++y) {
+                const X8 kf = *(const X8 *)(ck + j * DP + swz<NC>(j, y * 4 + g) * 8);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int x = 0; x < RT; ++x) st[kt][x] = mfma(kf, qf[n][x][y], st[kt][x]);
-                }
-            }
-            bool full = j0 + kBN - 1 <= wmin && (!a.window || j0 > wmax - a.window || j0 + kBN - 1 < a.sinks);
-            if constexpr (KV::kHoles) full = full & __all(s_in[buf][lane]);
-            if (!full) {
-#pragma unroll
-                for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int j = j0 + kt * 16 + g * 4 + i;
-                        bool in = true;
-                        if constexpr (KV::kHoles) in = s_in[buf][kt * 16 + g * 4 + i];
-#pragma unroll
-                        for (int x = 0; x < RT; ++x) {
-                            const bool see = in & sees(j, pos[x], low[x], a.sinks);
-                            st[kt][x][i] = see ? st[kt][x][i] : -INFINITY;
-                        }
-                    }
-            }
-            float mx[RT];
-            bool grow = false;
-#pragma unroll
-            for (int x = 0; x < RT; ++x) {
-                mx[x] = st[0][x][0];
-#pragma unroll
-                for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) mx[x] = fmaxf(mx[x], st[kt][x][i]);
-                mx[x] = fmaxf(mx[x], __shfl_xor(mx[x], 16));
-                mx[x] = fmaxf(mx[x], __shfl_xor(mx[x], 32));
-                grow = grow | (mx[x] > m[x] + lazy);
-            }
-            if (__any(grow)) {
-#pragma unroll
-                for (int x = 0; x < RT; ++x) {
-                    const float top = fmaxf(m[x], mx[x]);
-                    // a row that has seen nothing keeps -inf and its zeros
-                    const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[x] - top) * a.c);
-                    m[x] = top;
-                    l[x] *= alpha;
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) o[d][x] *= alpha;
-                }
-            }
-            X8 pf[NT][2][RT];  // [term][pair of key tiles][row]
-#pragma unroll
-            for (int x = 0; x < RT; ++x) {
-                const float mc = m[x] == -INFINITY ? 0.f : m[x] * a.c;
-                float sum = 0.f;
-#pragma unroll
-                for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kt][x][i], a.c, -mc));
-                        sum += p;
-                        // the probabilities are the product's operand in the
-                        // inputs' type; their sum is of the unrounded ones
-                        pf[0][kt >> 1][x][(kt & 1) * 4 + i] = (T)p;
-                        if constexpr (NT == 2)
-                            pf[1][kt >> 1][x][(kt & 1) * 4 + i] = (T)(p - (float)pf[0][kt >> 1][x][(kt & 1) * 4 + i]);
-                    }
-                l[x] += sum;
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int j = u * 32 + g * 4 + (r >> 2);
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    const int c = d * 2 + ((r & 3) >> 1), e = (r & 1) * 4;
-                    const X4 v0 = read_tr<T>(cv + j * DP + swz<NC>(j, c) * 8 + e);
-                    const X4 v1 = read_tr<T>(cv + (j + 16) * DP + swz<NC>(j + 16, c) * 8 + e);
-                    const X8 vf = join<X4, X8>(v0, v1);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int x = 0; x < RT; ++x) o[d][x] = mfma(vf, pf[n][u][x], o[d][x]);
-                }
+                    for (int x = 0; x < RT; ++x) z[kt][x] = mfma(kf, qf[n][x][y], z[kt][x]);
             }
         }
-        buf ^= 1;
-        if (tn < t_hi) kv.land(sk[buf], sv[buf], s_in[buf]);
-        __syncthreads();
-        t = tn;
+    };
+    // those that a row does not see, to -inf
+    auto hide = [&](int j0, const int *held, f32x4 (&z)[2][RT]) {
+        bool full = j0 + 31 <= wmin && (!a.window || j0 > wmax - a.window || j0 + 31 < a.sinks);
+        if constexpr (KV::kHoles) full = full & __all(held[lane & 31]);
+        if (full) return;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = j0 + kt * 16 + g * 4 + i;
+                bool in = true;
+                if constexpr (KV::kHoles) in = held[kt * 16 + g * 4 + i];
+#pragma unroll
+                for (int x = 0; x < RT; ++x) {
+                    const bool see = in & sees(j, pos[x], low[x], a.sinks);
+                    z[kt][x][i] = see ? z[kt][x][i] : -INFINITY;
+                }
+            }
+    };
+    // 32 keys whose scores are in st, with their values from row jv of cv on;
+    // the scores of the 32 from row jk of ck on, if there are more, take their place
+    auto step = [&](auto more, const T *ck, int jk, const T *cv, int jv) {
+        constexpr bool kMore = decltype(more)::value;
+        float mx[RT];
+        bool grow = false;
+#pragma unroll
+        for (int x = 0; x < RT; ++x) {
+            mx[x] = fmaxf(fmaxf(st[0][x][0], st[0][x][1]), st[0][x][2]);
+            mx[x] = fmaxf(fmaxf(mx[x], st[0][x][3]), st[1][x][0]);
+            mx[x] = fmaxf(fmaxf(mx[x], st[1][x][1]), st[1][x][2]);
+            mx[x] = fmaxf(mx[x], st[1][x][3]);
+            grow = grow | (mx[x] > limit[x]);
+        }
+        // the row's maximum over its 4 lanes is only needed when it grows
+        if (__any(grow)) {
+#pragma unroll
+            for (int x = 0; x < RT; ++x) {
+                const float top = fmaxf(m[x], max_rows(mx[x]));
+                // a row that has seen nothing keeps -inf and its zeros
+                const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[x] - top) * a.c);
+                m[x] = top;
+                limit[x] = top + lazy;
+                mc[x] = top == -INFINITY ? 0.f : top * a.c;
+                l[x] *= alpha;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[d][x] *= alpha;
+            }
+        }
+        X8 vf[ND];
+        const int j = jv + g * 4 + (r >> 2);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            const int c = d * 2 + ((r & 3) >> 1), e = (r & 1) * 4;
+            vf[d] = join<X4, X8>(read_tr<T>(cv + j * DP + swz<NC>(j, c) * 8 + e),
+                                 read_tr<T>(cv + (j + 16) * DP + swz<NC>(j + 16, c) * 8 + e));
+        }
+        f32x4 zn[2][RT];
+        if constexpr (kMore) scores(ck, jk, zn);
+        X8 pf[NT][RT];
+#pragma unroll
+        for (int x = 0; x < RT; ++x) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kt][x][i], a.c, -mc[x]));
+                    l[x] += p;
+                    // the probabilities are the product's operand in the
+                    // inputs' type; their sum is of the unrounded ones
+                    pf[0][x][kt * 4 + i] = (T)p;
+                    if constexpr (NT == 2) pf[1][x][kt * 4 + i] = (T)(p - (float)pf[0][x][kt * 4 + i]);
+                }
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int x = 0; x < RT; ++x) o[d][x] = mfma(vf[d], pf[n][x], o[d][x]);
+        if constexpr (kMore) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int x = 0; x < RT; ++x) st[kt][x] = zn[kt][x];
+        }
+    };
+
+    wait_dma();
+    __syncthreads();
+    if (t < t_hi) {
+        scores(sk[0], 0, st);
+        hide(t * kBN, s_in[0], st);
+    }
+    int n = 0;  // tile t is in buffer n
+    while (t < t_hi) {
+        const bool more = tn < t_hi;
+        if (more) {
+            kv.fetch_k(tn * kBN, sk[n ^ 1], a.dim);
+            kv.fetch_v(tn * kBN, sv[n ^ 1], a.dim);
+        }
+        step(BoolC<true>{}, sk[n], 32, sv[n], 0);
+        hide(t * kBN + 32, s_in[n] + (KV::kHoles ? 32 : 0), st);
+        if (more) {
+            kv.land_k(sk[n ^ 1], s_in[n ^ 1]);
+            kv.land_v(sv[n ^ 1]);
+            __syncthreads();
+            step(BoolC<true>{}, sk[n ^ 1], 0, sv[n], 32);
+            hide(tn * kBN, s_in[n ^ 1], st);
+            __syncthreads();
+        } else {
+            step(BoolC<false>{}, sk[0], 0, sv[n], 32);
+        }
+        n ^= 1, t = tn, tn = next(tn);
     }
 
 #pragma unroll
     for (int x = 0; x < RT; ++x) {
-        float sum = l[x] + __shfl_xor(l[x], 16);
-        sum += __shfl_xor(sum, 32);
+        const float sum = sum_rows(l[x]);
         const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
         const int row = wrow0 + r + 16 * x;
         if (row >= rows) continue;
@@ -346,34 +386,20 @@ void tiles_of(AttnArgs &a, int rows) {
     a.per = (int)(((int64_t)a.tiles * a.kv_heads + 7) / 8);
 }
 
-// 8 waves share the keys in LDS where their tiles still give each CU two
-// workgroups' worth of rows; else 4 waves.
-bool wide(const AttnArgs &a, int rows8) {
-    const int64_t rows = (int64_t)(a.offsets ? a.tokens : a.q_len) * a.group * (a.offsets ? 1 : a.batch);
-    return rows * a.kv_heads >= (int64_t)512 * rows8;
-}
-
+// Workgroups of 4 waves: two or three of them on a CU run out of step, and one's
+// products fall into another's exponentials.  (8 waves that share their tiles
+// were in step: 201 against 179 us at 2 x 4096 tokens, 32/8 heads of 128.)
 template <typename T, int DP, int RT>
 hipError_t fwd(AttnArgs a, hipStream_t s) {
-    if (wide(a, 8 * RT * 16)) {
-        tiles_of(a, 8 * RT * 16);
-        attn_fwd_kernel<T, T, DP, RT, 8, DenseKV<T, DP, 8>><<<(unsigned)a.per * 8, 512, 0, s>>>(a);
-    } else {
-        tiles_of(a, 4 * RT * 16);
-        attn_fwd_kernel<T, T, DP, RT, 4, DenseKV<T, DP, 4>><<<(unsigned)a.per * 8, 256, 0, s>>>(a);
-    }
+    tiles_of(a, 4 * RT * 16);
+    attn_fwd_kernel<T, T, DP, RT, 4, DenseKV<T, DP, 4>><<<(unsigned)a.per * 8, 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
 template <typename T, int DP>
 hipError_t chunk(AttendArgs x, hipStream_t s) {
-    if (wide(x.a, 256)) {
-        tiles_of(x.a, 256);
-        attn_fwd_kernel<T, __bf16, DP, 2, 8, PagedKV<DP, 8>><<<(unsigned)x.a.per * 8, 512, 0, s>>>(x);
-    } else {
-        tiles_of(x.a, 128);
-        attn_fwd_kernel<T, __bf16, DP, 2, 4, PagedKV<DP, 4>><<<(unsigned)x.a.per * 8, 256, 0, s>>>(x);
-    }
+    tiles_of(x.a, 128);
+    attn_fwd_kernel<T, __bf16, DP, 2, 4, PagedKV<DP>><<<(unsigned)x.a.per * 8, 256, 0, s>>>(x);
     return hipGetLastError();
 }
 

@@ -67,6 +67,23 @@ LSMX_DEV X8 join(X4 a, X4 b) {
 LSMX_DEV bool sees(int j, int pos, int low, int sinks) { return (j <= pos) & ((j > low) | (j < sinks)); }
 LSMX_DEV int window_low(int pos, int window) { return window ? pos - window : -1; }
 
+// max and sum over the 4 lanes 16 apart that share a row, by register swaps
+// between 16-lane rows (two VALU operations; a shuffle goes through LDS).
+LSMX_DEV float max_rows(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(x), false, false);
+    x = fmaxf(u2f(a[0]), u2f(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
+    return fmaxf(u2f(b[0]), u2f(b[1]));
+}
+LSMX_DEV float sum_rows(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(x), false, false);
+    x = u2f(a[0]) + u2f(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
+    return u2f(b[0]) + u2f(b[1]);
+}
+LSMX_DEV int lane_of(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+LSMX_DEV int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // n / d for n < 2^31 by multiplication: m = ceil(2^(31 + L) / d), L = ceil(log2 d),
 // sh = L - 1 (d = 1: n itself).
 struct FastDiv {
@@ -120,6 +137,7 @@ struct Seq {
 // belong to two more sequences that see nothing (k_len 0).
 // Returns false past the last tile.
 LSMX_DEV bool find_tile(const AttnArgs &a, int t, int size, int mult, int len, Seq &s) {
+    t = uniform(t);
     if (!a.offsets) {
         const int per = (len * mult + size - 1) / size;
         s.b = t / per;
@@ -150,16 +168,16 @@ LSMX_DEV bool find_tile(const AttnArgs &a, int t, int size, int mult, int len, S
         const uint64_t hit = __ballot(before + upto > t);
         if (hit) {
             const int w = __ffsll((unsigned long long)hit) - 1;
-            s.tile = t - before - (__shfl(upto, w) - __shfl(n, w));
-            s.q_len = __shfl(own, w);
-            s.q0 = s.k0 = __shfl(lo, w);
+            s.tile = t - before - (lane_of(upto, w) - lane_of(n, w));
+            s.q_len = lane_of(own, w);
+            s.q0 = s.k0 = lane_of(lo, w);
             const int idx = first + w;
             s.b = 0;
             s.k_len = idx >= 1 && idx <= a.batch ? s.q_len : 0;
             s.shift = s.k_len ? 0 : -s.q_len;  // dead sequence: positions below 0
             return true;
         }
-        before += __shfl(upto, 63);
+        before += lane_of(upto, 63);
     }
     return false;
 }
@@ -173,7 +191,9 @@ struct Pool {
     const int32_t *table, *lengths;
     int pages, kv_heads, dim, page, page_shift, max_pages;
 
-    LSMX_DEV int length(int b) const { return min(max(lengths[b], 0), max_pages << page_shift); }
+    LSMX_DEV int length(int b) const {
+        return __builtin_amdgcn_readfirstlane(min(max(lengths[b], 0), max_pages << page_shift));
+    }
     // the page of position j of sequence b, or -1
     LSMX_DEV int page_of(int b, int j) const {
         const int p = table[(int64_t)b * max_pages + (j >> page_shift)];
