@@ -456,6 +456,9 @@ int lsmx_gemm_mx_promote(const uint8_t *a, int64_t lda, const float *a_scale, in
 typedef struct {
     const void *q, *k, *v; /* LSMX_BF16 | LSMX_F16, unit stride along head_dim */
     void *o;               /* the same type                                     */
+    void *o_rest;          /* o as computed less o as rounded, in the same type
+                              and layout: written by the forward call unless
+                              NULL, read by the backward call                   */
     float *lse;            /* log2(sum_j exp(scale q . k_j)), -inf for a row that
                               sees nothing: [batch, heads, q_len] or, packed,
                               [heads, tokens]; may be NULL forward              */
@@ -463,7 +466,7 @@ typedef struct {
     int64_t batch, q_len, k_len, heads, kv_heads;
     int64_t head_dim;       /* a multiple of 8, at most 128                      */
     int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3]; /* sequence, token,
-                              head; multiples of 8, token strides below 2^23;
+                              head; multiples of 8, token strides below 2^22;
                               16-byte aligned bases                             */
     const int32_t *offsets;
     int64_t window, sinks;  /* window 0: none                                    */

@@ -102,7 +102,8 @@ class E8m0Item(ctypes.Structure):
 
 class Attention(ctypes.Structure):
     """lsmx_attention of include/lsmx.h."""
-    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("o", _vp), ("lse", _vp), ("dtype", _int), ("batch", _i64),
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("o", _vp), ("o_rest", _vp), ("lse", _vp),
+                ("dtype", _int), ("batch", _i64),
                 ("q_len", _i64), ("k_len", _i64), ("heads", _i64), ("kv_heads", _i64), ("head_dim", _i64),
                 ("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("v_stride", _i64 * 3), ("o_stride", _i64 * 3),
                 ("offsets", _vp), ("window", _i64), ("sinks", _i64), ("scale", ctypes.c_float)]

@@ -50,30 +50,40 @@ def _strides(t: torch.Tensor):
     return (ctypes.c_int64 * 3)(*([0] * (3 - len(s)) + s))
 
 
-def _args(q, k, v, o, lse, offsets, window, sinks, scale):
+def _args(q, k, v, o, rest, lse, offsets, window, sinks, scale):
     packed = offsets is not None
-    return C.Attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), C.dtype_code(q.dtype),
-                       offsets.numel() - 1 if packed else q.shape[0], q.shape[-3], k.shape[-3], q.shape[-2],
+    return C.Attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), rest.data_ptr() if rest is not None else None,
+                       lse.data_ptr(), C.dtype_code(q.dtype), offsets.numel() - 1 if packed else q.shape[0], q.shape[-3], k.shape[-3], q.shape[-2],
                        k.shape[-2], q.shape[-1], _strides(q), _strides(k), _strides(v), _strides(o),
                        offsets.data_ptr() if packed else None, window, sinks, scale)
 
 
-def _forward(q, k, v, offsets, window, sinks, scale):
-    q, k, v = (rows16(t) if t.stride(-3) < 2 ** 23 else t.contiguous() for t in (q, k, v))
+def _in_reach(t: torch.Tensor, group: int) -> torch.Tensor:
+    """rows16(t), its tokens and the heads of a group within the kernels' 32-bit
+    offsets."""
+    t = rows16(t)
+    far = (t.shape[-3] > 1 and t.stride(-3) >= 2 ** 22) or (t.shape[-2] > 1 and t.stride(-2) * group >= 2 ** 29)
+    return t.contiguous() if far else t
+
+
+def _forward(q, k, v, offsets, window, sinks, scale, grad):
+    group = q.shape[-2] // k.shape[-2]
+    q, k, v = _in_reach(q, group), _in_reach(k, 1), _in_reach(v, 1)
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lead = q.shape[:1] if offsets is None else ()
     lse = torch.empty((*lead, q.shape[-2], q.shape[-3]), dtype=torch.float32, device=q.device)
+    rest = torch.empty_like(o) if grad else None
     if q.numel():
-        a = _args(q, k, v, o, lse, offsets, window, sinks, scale)
+        a = _args(q, k, v, o, rest, lse, offsets, window, sinks, scale)
         C.call("lsmx_attention_fwd", ctypes.addressof(a), C.stream_of(q))
-    return q, k, v, o, lse
+    return q, k, v, o, rest, lse
 
 
 class _SinkWindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, offsets, window, sinks, scale):
-        q, k, v, o, lse = _forward(q, k, v, offsets, window, sinks, scale)
-        ctx.save_for_backward(q, k, v, o, lse, *(() if offsets is None else (offsets,)))
+        q, k, v, o, rest, lse = _forward(q, k, v, offsets, window, sinks, scale, True)
+        ctx.save_for_backward(q, k, v, o, rest, lse, *(() if offsets is None else (offsets,)))
         ctx.mask = window, sinks, scale
         ctx.mark_non_differentiable(lse)
         return o, lse
@@ -81,11 +91,11 @@ class _SinkWindowAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o, _):
-        q, k, v, o, lse, *offsets = ctx.saved_tensors
-        d_o = rows16(d_o.to(q.dtype)) if d_o.stride(-3) < 2 ** 23 else d_o.contiguous()
+        q, k, v, o, rest, lse, *offsets = ctx.saved_tensors
+        d_o = _in_reach(d_o.to(q.dtype), q.shape[-2] // k.shape[-2])
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         if q.numel() or k.numel():
-            a = _args(q, k, v, o, lse, offsets[0] if offsets else None, *ctx.mask)
+            a = _args(q, k, v, o, rest, lse, offsets[0] if offsets else None, *ctx.mask)
             n = C.load().lsmx_attention_workspace(ctypes.addressof(a))
             ws = torch.empty(n, dtype=torch.uint8, device=q.device)
             st = _strides(d_o)
@@ -134,5 +144,5 @@ def sink_window_attention(q, k, v, *, window=None, sinks=0, scale=None, offsets=
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         o, lse = _SinkWindowAttention.apply(q, k, v, offsets, window, sinks, scale)
     else:
-        *_, o, lse = _forward(q, k, v, offsets, window, sinks, scale)
+        *_, o, _, lse = _forward(q, k, v, offsets, window, sinks, scale, False)
     return (o, lse * math.log(2.0)) if return_lse else o

@@ -363,13 +363,20 @@ __global__ __launch_bounds__(NW * 64, KV::kHoles ? (DP == 64 ? 2 : 1) : (DP == 6
         const int row = wrow0 + r + 16 * x;
         if (row >= rows) continue;
         const int tok = div_by(row, a.by_group), h = hkv * a.group + row - tok * a.group;
-        TQ *op = (TQ *)a.o + s.b * a.o_b + (s.q0 + tok) * a.o_t + h * a.o_h;
+        const int64_t o_at = s.b * a.o_b + (s.q0 + tok) * a.o_t + h * a.o_h;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            Q4 w;
+            Q4 w, rest;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = (TQ)(o[d][x][i] * inv);
-            if (d * 16 + g * 4 < a.dim) *(Q4 *)(op + d * 16 + g * 4) = w;
+            for (int i = 0; i < 4; ++i) {
+                const float f = o[d][x][i] * inv;
+                w[i] = (TQ)f;
+                rest[i] = (TQ)(f - (float)w[i]);
+            }
+            if (d * 16 + g * 4 < a.dim) {
+                *(Q4 *)((TQ *)a.o + o_at + d * 16 + g * 4) = w;
+                if (a.o_lo) *(Q4 *)((TQ *)a.o_lo + o_at + d * 16 + g * 4) = rest;
+            }
         }
         if (a.lse && g == 0)
             a.lse[s.b * a.lse_b + h * a.lse_h + s.q0 + tok] =

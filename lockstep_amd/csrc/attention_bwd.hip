@@ -8,7 +8,17 @@
 // owns rows and runs over their keys (dQ), the other owns keys and runs over
 // the rows of all heads that share them (dK, dV).  Both recompute S and dP:
 // seven products where one kernel with shared accumulators would take five.
+//
+// The sinks are seen by every row: their keys would keep one workgroup busy
+// with the whole sequence while the others have a window of it.  So the rows
+// past the window of the sinks' tile are taken in chunks by a kernel of their
+// own first, 16 sinks at a time, and the owner of the sinks adds the chunks'
+// fp32 sums, in their order, before it rounds.
+//
+// Layouts as in the forward kernel: S^T = K Q^T feeds dQ^T += K^T dS^T without a
+// lane crossing, and S = Q K^T feeds dV^T += dO^T P and dK^T += Q^T dS.
 #include "lsmx_attn.h"
+#include "lsmx_dma.h"
 
 namespace lsmx {
 namespace {
@@ -17,89 +27,71 @@ constexpr int kBM = 128;  // dQ: rows of a workgroup
 constexpr int kBN = 64;   // dQ: keys of a tile
 constexpr int kKM = 128;  // dK, dV: keys of a workgroup
 constexpr int kKN = 64;   // dK, dV: rows of a tile
+constexpr int kFar = 128; // far rows: rows of a tile
 
-// delta of every row: 16 lanes per row.
+// fp16 holds 2^-24 to 65504, and gradients are often small: P enters its
+// product times 2^10, and dS times a power of two of its own row (dQ) or key
+// (dK) that is chosen when a value passes kTop and brings the largest so far
+// to 2^10; the sums so far are rescaled, as the softmax does.  bf16 needs
+// neither.
 template <typename T>
-__global__ __launch_bounds__(256) void attn_delta_kernel(AttnArgs a) {
-    typedef typename Vec<T>::x8 X8;
-    const int64_t tokens = a.offsets ? a.tokens : (int64_t)a.batch * a.q_len;
-    const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const int r = threadIdx.x & 15;
-    if (row >= tokens * a.heads) return;
-    const int64_t tok = row / a.heads;
-    const int h = (int)(row - tok * a.heads);
-    const int b = a.offsets ? 0 : (int)(tok / a.q_len);
-    const int64_t t = a.offsets ? tok : tok - (int64_t)b * a.q_len;
-    float sum = 0.f;
-    if (r * 8 < a.dim) {
-        const X8 x = *(const X8 *)((const T *)a.d_o + b * a.do_b + t * a.do_t + h * a.do_h + r * 8);
-        const X8 y = *(const X8 *)((const T *)a.o + b * a.o_b + t * a.o_t + h * a.o_h + r * 8);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf((float)x[i], (float)y[i], sum);
-    }
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor(sum, d);
-    if (r == 0) a.delta[b * a.lse_b + h * a.lse_h + t] = sum;
-}
-
-// Stages 64 rows of two tensors (strides per key row, or per token and head).
-template <typename T, int DP>
-struct Stage {
-    static constexpr int NC = DP / 8, NU = 64 * NC / 256;
-    u32x4 x[NU], y[NU];
-    LSMX_DEV void store(T *sx, T *sy) {
-#pragma unroll
-        for (int u = 0; u < NU; ++u) {
-            const int id = threadIdx.x + 256 * u, j = id / NC, c = id % NC;
-            *(u32x4 *)(sx + j * DP + swz<NC>(j, c) * 8) = x[u];
-            *(u32x4 *)(sy + j * DP + swz<NC>(j, c) * 8) = y[u];
-        }
+struct Range {
+    static constexpr bool on = __is_same(T, _Float16);
+    static constexpr float kTop = 32768.f, kP = on ? 10.f : 0.f;
+    // the power of two that brings x > 0 into [2^10, 2^11); 1 for inf and NaN,
+    // and no more than 2^100
+    LSMX_DEV static float scale_for(float x) {
+        const int e = (int)((f2u(x) >> 23) & 255) - 127;
+        return e >= 128 ? 1.f : __builtin_amdgcn_ldexpf(1.f, min(10 - e, 100));
     }
 };
 
+// 64 rows of one tensor straight into LDS, by the four waves of a workgroup;
+// offset(row, chunk) is the byte offset in rs of 16-byte chunk `chunk`, or
+// one past its end for zeros.
+template <typename T, int DP, typename F>
+LSMX_DEV void fetch_rows(v4i_rsrc rs, T *to, int rows, F offset) {
+    constexpr int NC = DP / 8;
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t lds = lds_u32(to);
+#pragma unroll
+    for (int u = 0; u < rows * NC / 256; ++u) {
+        const int at = (u * 4 + wave) * 64, j = (at + lane) / NC, c = swz<NC>(j, lane % NC);
+        dma_x4(offset(j, c), rs, lds + at * 16);
+    }
+}
+constexpr uint32_t kZeros = 0x80000000u;
+
+LSMX_DEV void wait_dma() {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0), seen by the compiler
+    asm volatile("" ::: "memory");
+}
+
+// Operand of 8 contraction rows 4g.., 16 + 4g.. of a tile from row j0 on, at
+// columns 16 d + r.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_dq_kernel(AttnArgs a) {
+LSMX_DEV typename Vec<T>::x8 columns(const T *t, int j0, int d, int g, int r) {
+    constexpr int NC = DP / 8;
+    const int j = j0 + g * 4 + (r >> 2), c = d * 2 + ((r & 3) >> 1), e = (r & 1) * 4;
+    return join<typename Vec<T>::x4, typename Vec<T>::x8>(read_tr<T>(t + j * DP + swz<NC>(j, c) * 8 + e),
+                                                          read_tr<T>(t + (j + 16) * DP + swz<NC>(j + 16, c) * 8 + e));
+}
+
+// ------------------------------------------------------------------ dQ, delta
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16;
     typedef typename Vec<T>::x8 X8;
     typedef typename Vec<T>::x4 X4;
-    __shared__ T sk[kBN * DP], sv[kBN * DP];
+    __shared__ __attribute__((aligned(16))) T sk[2][kBN * DP], sv[2][kBN * DP];
 
     const int item = xcd_item(blockIdx.x, a.per);
     if (item >= a.tiles * a.kv_heads) return;
     const int hkv = item / a.tiles;
     Seq s;
     if (!find_tile(a, a.tiles - 1 - item % a.tiles, kBM, a.group, a.q_len, s)) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
-    const int row0 = s.tile * kBM, rows = s.q_len * a.group;
-
-    int pos[2];
-    int64_t q_at[2];
-    float lse[2], delta[2];
-    X8 qf[2][NS], of[2][NS];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int row = row0 + wave * 32 + r + 16 * t;
-        const bool in = row < rows;
-        const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
-        pos[t] = in ? tok + s.shift : -1;
-        const int64_t l_at = s.b * a.lse_b + h * a.lse_h + s.q0 + tok;
-        lse[t] = in ? a.lse[l_at] : 0.f;
-        delta[t] = in ? a.delta[l_at] : 0.f;
-        const int64_t token = (a.offsets ? s.q0 : (int64_t)s.b * a.q_len) + tok;
-        q_at[t] = in ? (token * a.heads + h) * a.dim : -1;
-        const T *qp = (const T *)a.q + s.b * a.q_b + (s.q0 + tok) * a.q_t + h * a.q_h;
-        const T *op = (const T *)a.d_o + s.b * a.do_b + (s.q0 + tok) * a.do_t + h * a.do_h;
-#pragma unroll
-        for (int x = 0; x < NS; ++x) {
-            const int c = x * 4 + g;
-            const bool ok = in && c * 8 < a.dim;
-            qf[t][x] = ok ? *(const X8 *)(qp + c * 8) : X8{};
-            of[t][x] = ok ? *(const X8 *)(op + c * 8) : X8{};
-        }
-    }
-    f32x4 dq[ND][2];
-#pragma unroll
-    for (int d = 0; d < ND; ++d) dq[d][0] = dq[d][1] = f32x4{0, 0, 0, 0};
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
+    const int row0 = s.tile * kBM, rows = s.q_len * a.group, wrow0 = row0 + wave * 32;
 
     const int pmin = div_by(row0, a.by_group) + s.shift;
     const int pmax = div_by(min(row0 + kBM, rows) - 1, a.by_group) + s.shift;
@@ -107,213 +99,452 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(AttnArgs a) {
     const int t_sink = (min(a.sinks, hi) + kBN - 1) / kBN, t_hi = hi > 0 ? (hi + kBN - 1) / kBN : 0;
     const int t_lo = lo / kBN;
     auto next = [&](int t) { return t + 1 < t_sink ? t + 1 : max(t + 1, t_lo); };
-    int t = t_sink > 0 ? 0 : t_lo;
+    int t = t_sink > 0 ? 0 : t_lo, n = 0;
+    const int wmin = div_by(min(wrow0, rows - 1), a.by_group) + s.shift;
+    const int wmax = wrow0 < rows ? div_by(min(wrow0 + 32, rows) - 1, a.by_group) + s.shift : -1;
 
     const T *kp = (const T *)a.k + s.b * a.k_b + s.k0 * a.k_t + hkv * a.k_h;
     const T *vp = (const T *)a.v + s.b * a.v_b + s.k0 * a.v_t + hkv * a.v_h;
-    Stage<T, DP> kv;
-    auto load = [&](int j0) {
-#pragma unroll
-        for (int u = 0; u < Stage<T, DP>::NU; ++u) {
-            const int id = threadIdx.x + 256 * u, j = j0 + id / NC, c = id % NC;
-            const bool in = j < s.k_len && c * 8 < a.dim;
-            kv.x[u] = in ? *(const u32x4 *)(kp + j * a.k_t + c * 8) : u32x4{0, 0, 0, 0};
-            kv.y[u] = in ? *(const u32x4 *)(vp + j * a.v_t + c * 8) : u32x4{0, 0, 0, 0};
-        }
+    auto fetch = [&](int j0, int to) {
+        const auto at = [&](int64_t x_t) {
+            return [=](int j, int c) {
+                return j0 + j < s.k_len && c * 8 < a.dim ? (uint32_t)(j * (int)x_t + c * 8) * 2 : kZeros;
+            };
+        };
+        fetch_rows<T, DP>(buf_rsrc(kp + j0 * a.k_t, 0x7FFFFFFF), sk[to], kBN, at(a.k_t));
+        fetch_rows<T, DP>(buf_rsrc(vp + j0 * a.v_t, 0x7FFFFFFF), sv[to], kBN, at(a.v_t));
     };
-    if (t < t_hi) load(t * kBN);
+    if (t < t_hi) fetch(t * kBN, 0);
+
+    int pos[2], low[2];
+    int64_t q_at[2];
+    float lse[2], delta[2], mul[2] = {0.f, 0.f}, limit[2] = {0.f, 0.f};
+    X8 qf[2][NS], of[2][NS];
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+        const int row = wrow0 + r + 16 * y;
+        const bool in = row < rows;
+        const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
+        pos[y] = in ? tok + s.shift : -1;
+        low[y] = window_low(pos[y], a.window);
+        const int64_t l_at = s.b * a.lse_b + h * a.lse_h + s.q0 + tok;
+        const int64_t token = (a.offsets ? s.q0 : (int64_t)s.b * a.q_len) + tok;
+        q_at[y] = in ? (token * a.heads + h) * a.dim : -1;
+        const T *qp = (const T *)a.q + s.b * a.q_b + (s.q0 + tok) * a.q_t + h * a.q_h;
+        const T *dp = (const T *)a.d_o + s.b * a.do_b + (s.q0 + tok) * a.do_t + h * a.do_h;
+        const int64_t o_at = s.b * a.o_b + (s.q0 + tok) * a.o_t + h * a.o_h;
+        lse[y] = in ? a.lse[l_at] : 0.f;
+        // delta from o as the forward had it: its rounded value and the rest
+        float sum = 0.f;
+#pragma unroll
+        for (int x = 0; x < NS; ++x) {
+            const int c = x * 4 + g;
+            const bool ok = in && c * 8 < a.dim;
+            qf[y][x] = ok ? *(const X8 *)(qp + c * 8) : X8{};
+            of[y][x] = ok ? *(const X8 *)(dp + c * 8) : X8{};
+            const X8 hi8 = ok ? *(const X8 *)((const T *)a.o + o_at + c * 8) : X8{};
+            const X8 lo8 = ok ? *(const X8 *)((const T *)a.o_lo + o_at + c * 8) : X8{};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum = __builtin_fmaf((float)of[y][x][i], (float)hi8[i] + (float)lo8[i], sum);
+        }
+        delta[y] = sum_rows(sum);
+        if (in && g == 0) a.delta[l_at] = delta[y];
+    }
+    f32x4 dq[ND][2];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) dq[d][0] = dq[d][1] = f32x4{0, 0, 0, 0};
+
+    wait_dma();
+    __syncthreads();
     while (t < t_hi) {
         const int j0 = t * kBN, tn = next(t);
-        __syncthreads();
-        kv.store(sk, sv);
-        __syncthreads();
-        if (tn < t_hi) load(tn * kBN);
-        const bool full = j0 + kBN - 1 <= pmin && (!a.window || j0 > pmax - a.window || j0 + kBN - 1 < a.sinks);
+        if (tn < t_hi) fetch(tn * kBN, n ^ 1);
+        const T *ck = sk[n], *cv = sv[n];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            X8 df[2];
+            const int ju = j0 + u * 32;
+            if (ju > wmax || (a.window && ju + 31 <= wmin - a.window && ju >= a.sinks)) continue;
+            const bool full = ju + 31 <= wmin && (!a.window || ju > wmax - a.window || ju + 31 < a.sinks);
+            f32x4 st[2][2], dp[2][2];  // [16 keys][16 rows]
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-                const int kt = u * 2 + w, j = kt * 16 + r;
-                f32x4 st[2], dp[2];
-                st[0] = st[1] = dp[0] = dp[1] = f32x4{0, 0, 0, 0};
+                const int j = u * 32 + w * 16 + r;
+                st[w][0] = st[w][1] = dp[w][0] = dp[w][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int x = 0; x < NS; ++x) {
-                    const X8 kf = *(const X8 *)(sk + j * DP + swz<NC>(j, x * 4 + g) * 8);
-                    const X8 vf = *(const X8 *)(sv + j * DP + swz<NC>(j, x * 4 + g) * 8);
+                    const X8 kf = *(const X8 *)(ck + j * DP + swz<NC>(j, x * 4 + g) * 8);
+                    const X8 vf = *(const X8 *)(cv + j * DP + swz<NC>(j, x * 4 + g) * 8);
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
-                        st[y] = mfma(kf, qf[y][x], st[y]);
-                        dp[y] = mfma(vf, of[y][x], dp[y]);
+                        st[w][y] = mfma(kf, qf[y][x], st[w][y]);
+                        dp[w][y] = mfma(vf, of[y][x], dp[w][y]);
                     }
                 }
-#pragma unroll
-                for (int y = 0; y < 2; ++y)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int jj = j0 + kt * 16 + g * 4 + i;
-                        const float ds = __builtin_amdgcn_exp2f(__builtin_fmaf(st[y][i], a.c, -lse[y])) * (dp[y][i] - delta[y]);
-                        const bool in = full | sees(jj, pos[y], window_low(pos[y], a.window), a.sinks);
-                        df[y][w * 4 + i] = (T)(in ? ds : 0.f);
-                    }
             }
-            const int j = u * 32 + g * 4 + (r >> 2);
+            bool grow = false;
+            float top[2] = {0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        float ds = __builtin_amdgcn_exp2f(__builtin_fmaf(st[w][y][i], a.c, -lse[y])) *
+                                   (dp[w][y][i] - delta[y]);
+                        if (!full) {
+                            const int j = ju + w * 16 + g * 4 + i;
+                            ds = sees(j, pos[y], low[y], a.sinks) ? ds : 0.f;
+                        }
+                        st[w][y][i] = ds;
+                        if constexpr (Range<T>::on) top[y] = fmaxf(top[y], __builtin_fabsf(ds));
+                    }
+            if constexpr (Range<T>::on) {
+                grow = (top[0] > limit[0]) | (top[1] > limit[1]);
+                if (__any(grow)) {
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const float most = max_rows(top[y]);
+                        if (most > limit[y]) {
+                            const float m = Range<T>::scale_for(most), f = mul[y] == 0.f ? 0.f : m / mul[y];
+                            mul[y] = m, limit[y] = Range<T>::kTop / m;
+#pragma unroll
+                            for (int d = 0; d < ND; ++d) dq[d][y] *= f;
+                        }
+                    }
+                }
+            }
+            X8 df[2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        df[y][w * 4 + i] = (T)(Range<T>::on ? st[w][y][i] * mul[y] : st[w][y][i]);
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
-                const int c = d * 2 + ((r & 3) >> 1), e = (r & 1) * 4;
-                const X8 kf = join<X4, X8>(read_tr<T>(sk + j * DP + swz<NC>(j, c) * 8 + e),
-                                           read_tr<T>(sk + (j + 16) * DP + swz<NC>(j + 16, c) * 8 + e));
+                const X8 kf = columns<T, DP>(ck, u * 32, d, g, r);
                 dq[d][0] = mfma(kf, df[0], dq[d][0]);
                 dq[d][1] = mfma(kf, df[1], dq[d][1]);
             }
         }
-        t = tn;
+        n ^= 1, t = tn;
+        wait_dma();
+        __syncthreads();
     }
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
         if (q_at[y] < 0) continue;
         T *p = (T *)a.dq + q_at[y];
+        const float f = !Range<T>::on ? a.scale : mul[y] == 0.f ? 0.f : a.scale / mul[y];
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             X4 w;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = (T)(dq[d][y][i] * a.scale);
+            for (int i = 0; i < 4; ++i) w[i] = (T)(dq[d][y][i] * f);
             if (d * 16 + g * 4 < a.dim) *(X4 *)(p + d * 16 + g * 4) = w;
         }
     }
 }
 
+// ------------------------------------------------------------------ dK, dV
+// The rows of a (sequence, key head) from row0 on, gathered into LDS: q and dO,
+// and each row's lse, delta and position.
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_dkv_kernel(AttnArgs a) {
-    constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16;
+struct Rows {
+    const AttnArgs &a;
+    const Seq &s;
+    int hkv, end;
+    LSMX_DEV void fetch(int row0, T *sq, T *so, int count) {
+        const int tok0 = uniform(div_by(row0, a.by_group)), last = end, dim = a.dim;
+        const FastDiv by = a.by_group;
+        auto at = [=](int64_t x_t, int64_t x_h) {
+            return [=](int j, int c) {
+                const int row = row0 + j, tok = div_by(row, by);
+                return row < last && c * 8 < dim
+                           ? (uint32_t)((tok - tok0) * (int)x_t + (row - tok * (int)by.d) * (int)x_h + c * 8) * 2
+                           : kZeros;
+            };
+        };
+        const T *q = (const T *)a.q + s.b * a.q_b + (s.q0 + tok0) * a.q_t + hkv * a.group * a.q_h;
+        const T *d = (const T *)a.d_o + s.b * a.do_b + (s.q0 + tok0) * a.do_t + hkv * a.group * a.do_h;
+        fetch_rows<T, DP>(buf_rsrc(q, 0x7FFFFFFF), sq, count, at(a.q_t, a.q_h));
+        fetch_rows<T, DP>(buf_rsrc(d, 0x7FFFFFFF), so, count, at(a.do_t, a.do_h));
+    }
+    LSMX_DEV void stats(int row, float &lse, float &delta, int &pos) {
+        const bool in = row < end;
+        const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
+        const int64_t at = s.b * a.lse_b + h * a.lse_h + s.q0 + tok;
+        lse = in ? a.lse[at] - Range<T>::kP : 0.f;
+        delta = in ? a.delta[at] : 0.f;
+        pos = in ? tok + s.shift : -1;
+    }
+};
+
+// 32 rows from row j0 of an LDS tile on against NK x 16 keys in registers.
+template <typename T, int DP, int NK>
+struct KeySums {
+    static constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16;
+    typedef typename Vec<T>::x8 X8;
+    X8 kf[NK][NS], vf[NK][NS];
+    f32x4 dk[ND][NK], dv[ND][NK];
+    float mul[NK], limit[NK];
+
+    LSMX_DEV void init() {
+#pragma unroll
+        for (int y = 0; y < NK; ++y) {
+            mul[y] = limit[y] = 0.f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) dk[d][y] = dv[d][y] = f32x4{0, 0, 0, 0};
+        }
+    }
+    // see(y, position): whether key y of the lane is seen from there
+    template <typename F>
+    LSMX_DEV void add(const T *sq, const T *so, const float *s_lse, const float *s_delta, const int *s_pos, int j0,
+                      float c, bool full, int g, int r, F see) {
+        X8 pf[NK], df[NK];
+        f32x4 pr[2][NK], ds[2][NK];
+        float top[NK];
+#pragma unroll
+        for (int y = 0; y < NK; ++y) top[y] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const int j = j0 + w * 16 + r;
+#pragma unroll
+            for (int y = 0; y < NK; ++y) pr[w][y] = ds[w][y] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int x = 0; x < NS; ++x) {
+                const X8 qf = *(const X8 *)(sq + j * DP + swz<NC>(j, x * 4 + g) * 8);
+                const X8 of = *(const X8 *)(so + j * DP + swz<NC>(j, x * 4 + g) * 8);
+#pragma unroll
+                for (int y = 0; y < NK; ++y) {
+                    pr[w][y] = mfma(qf, kf[y][x], pr[w][y]);
+                    ds[w][y] = mfma(of, vf[y][x], ds[w][y]);
+                }
+            }
+            const f32x4 lse = *(const f32x4 *)(s_lse + j0 + w * 16 + g * 4);
+            const f32x4 delta = *(const f32x4 *)(s_delta + j0 + w * 16 + g * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int y = 0; y < NK; ++y) {
+                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(pr[w][y][i], c, -lse[i]));
+                    float d = p * (ds[w][y][i] - delta[i]);
+                    if (!full) {
+                        const bool in = see(y, s_pos[j0 + w * 16 + g * 4 + i]);
+                        p = in ? p : 0.f;
+                        d = in ? d : 0.f;
+                    }
+                    pf[y][w * 4 + i] = (T)p;
+                    if constexpr (Range<T>::on) {
+                        ds[w][y][i] = d;
+                        top[y] = fmaxf(top[y], __builtin_fabsf(d));
+                    } else {
+                        df[y][w * 4 + i] = (T)d;
+                    }
+                }
+        }
+        if constexpr (Range<T>::on) {
+            bool grow = false;
+#pragma unroll
+            for (int y = 0; y < NK; ++y) grow = grow | (top[y] > limit[y]);
+            if (__any(grow)) {
+#pragma unroll
+                for (int y = 0; y < NK; ++y) {
+                    const float most = max_rows(top[y]);
+                    if (most > limit[y]) {
+                        const float m = Range<T>::scale_for(most), f = mul[y] == 0.f ? 0.f : m / mul[y];
+                        mul[y] = m, limit[y] = Range<T>::kTop / m;
+#pragma unroll
+                        for (int d = 0; d < ND; ++d) dk[d][y] *= f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int y = 0; y < NK; ++y)
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) df[y][w * 4 + i] = (T)(ds[w][y][i] * mul[y]);
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            const X8 of = columns<T, DP>(so, j0, d, g, r), qf = columns<T, DP>(sq, j0, d, g, r);
+#pragma unroll
+            for (int y = 0; y < NK; ++y) {
+                dv[d][y] = mfma(of, pf[y], dv[d][y]);
+                dk[d][y] = mfma(qf, df[y], dk[d][y]);
+            }
+        }
+    }
+    // the sums in their own units
+    LSMX_DEV float k_unit(int y) const {
+        const float p = Range<T>::on ? 1.f / 1024.f : 1.f;
+        return !Range<T>::on ? 1.f : mul[y] == 0.f ? 0.f : p / mul[y];
+    }
+    LSMX_DEV static float v_unit() { return Range<T>::on ? 1.f / 1024.f : 1.f; }
+};
+
+// The first token past the window of the key tile that holds key j.
+LSMX_DEV int far_token(const AttnArgs &a, const Seq &s, int j, int keys) {
+    return min(j / kKM * kKM + kKM, keys) - 1 + a.window - s.shift;
+}
+
+// Far rows: one chunk of rows, 16 sinks; the 4 waves take 32 rows each of a
+// tile of 128 and are joined in LDS.  part: [16 sinks][key head][chunk][dK, dV][16][DP].
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_far_kernel(AttnArgs a) {
+    constexpr int ND = DP / 16, NS = DP / 32;
+    typedef typename Vec<T>::x8 X8;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * kFar * DP * 2];
+    __shared__ __attribute__((aligned(16))) float s_lse[kFar], s_delta[kFar];
+    __shared__ int s_pos[kFar];
+    T *sq = (T *)smem, *so = sq + kFar * DP;
+
+    const int slots = a.tiles, slot = uniform(blockIdx.x % slots), rest = uniform(blockIdx.x / slots);
+    const int hkv = rest % a.kv_heads, group = rest / a.kv_heads;
+    Seq s;
+    if (!find_tile(a, slot, a.chunk, a.group, a.q_len, s)) return;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
+    const int keys = a.offsets ? s.q_len : s.k_len, rows = s.q_len * a.group, key = group * 16 + r;
+    if (group * 16 >= keys) return;
+    const int first = max(far_token(a, s, group * 16, keys), 0);
+    if (first >= s.q_len) return;
+    const int row_lo = max(s.tile * a.chunk, first * a.group), row_hi = min((s.tile + 1) * a.chunk, rows);
+    if (row_lo >= row_hi) return;
+
+    KeySums<T, DP, 1> sums;
+    sums.init();
+    const T *kp = (const T *)a.k + s.b * a.k_b + (s.k0 + key) * a.k_t + hkv * a.k_h;
+    const T *vp = (const T *)a.v + s.b * a.v_b + (s.k0 + key) * a.v_t + hkv * a.v_h;
+#pragma unroll
+    for (int x = 0; x < NS; ++x) {
+        const int c = x * 4 + g;
+        const bool ok = key < keys && c * 8 < a.dim;
+        sums.kf[0][x] = ok ? *(const X8 *)(kp + c * 8) : X8{};
+        sums.vf[0][x] = ok ? *(const X8 *)(vp + c * 8) : X8{};
+    }
+    Rows<T, DP> in{a, s, hkv, row_hi};
+    const bool sink = key < min(a.sinks, keys);
+    for (int row0 = row_lo; row0 < row_hi; row0 += kFar) {
+        __syncthreads();
+        in.fetch(row0, sq, so, kFar);
+        if (threadIdx.x < kFar) in.stats(row0 + threadIdx.x, s_lse[threadIdx.x], s_delta[threadIdx.x], s_pos[threadIdx.x]);
+        wait_dma();
+        __syncthreads();
+        sums.add(sq, so, s_lse, s_delta, s_pos, wave * 32, a.c, false, g, r, [&](int, int pos) { return sink & (pos >= 0); });
+    }
+    // join the waves: dK, then dV
+    float *w_out = (float *)smem;  // [4][16][DP]
+    float *part = a.part + ((int64_t)(group * a.kv_heads + hkv) * slots + slot) * 2 * 16 * DP;
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        const float f = v ? sums.v_unit() : sums.k_unit(0);
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+            *(f32x4 *)(w_out + (wave * 16 + r) * DP + d * 16 + g * 4) = (v ? sums.dv[d][0] : sums.dk[d][0]) * f;
+        __syncthreads();
+        for (int i = threadIdx.x * 4; i < 16 * DP; i += 1024) {
+            f32x4 x = *(f32x4 *)(w_out + i);
+#pragma unroll
+            for (int w = 1; w < 4; ++w) x += *(f32x4 *)(w_out + w * 16 * DP + i);
+            *(f32x4 *)(part + v * 16 * DP + i) = x;
+        }
+    }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
+    constexpr int NS = DP / 32, ND = DP / 16;
     typedef typename Vec<T>::x8 X8;
     typedef typename Vec<T>::x4 X4;
-    __shared__ T sq[kKN * DP], so[kKN * DP];
-    __shared__ float s_lse[kKN], s_delta[kKN];
-    __shared__ int s_pos[kKN];
+    __shared__ __attribute__((aligned(16))) T sq[2][kKN * DP], so[2][kKN * DP];
+    __shared__ __attribute__((aligned(16))) float s_lse[2][kKN], s_delta[2][kKN];
+    __shared__ int s_pos[2][kKN];
 
     const int item = xcd_item(blockIdx.x, a.per);
     if (item >= a.tiles * a.kv_heads) return;
     const int hkv = item / a.tiles;
     Seq s;
     if (!find_tile(a, item % a.tiles, kKM, 1, a.k_len, s)) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
     const int keys = a.offsets ? s.q_len : s.k_len;  // of a dead sequence too
-    const int key0 = s.tile * kKM;
+    const int key0 = s.tile * kKM, key1 = min(key0 + kKM, keys) - 1;
 
-    X8 kf[2][NS], vf[2][NS];
+    // the rows that see some key of the tile, but for the far rows of sinks
+    const int tok_lo = max(0, key0 - s.shift);
+    int tok_hi = s.q_len;
+    if (a.window && (a.chunk || key0 >= a.sinks)) tok_hi = min(tok_hi, key1 + a.window - s.shift);
+    const int row_lo = tok_lo * a.group, row_hi = max(tok_hi, 0) * a.group;
+    Rows<T, DP> in{a, s, hkv, row_hi};
+    if (row_lo < row_hi) {
+        in.fetch(row_lo, sq[0], so[0], kKN);
+        if (threadIdx.x < kKN) in.stats(row_lo + threadIdx.x, s_lse[0][threadIdx.x], s_delta[0][threadIdx.x], s_pos[0][threadIdx.x]);
+    }
+
+    KeySums<T, DP, 2> sums;
+    sums.init();
     int key[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        key[t] = key0 + wave * 32 + t * 16 + r;
-        const T *kp = (const T *)a.k + s.b * a.k_b + (s.k0 + key[t]) * a.k_t + hkv * a.k_h;
-        const T *vp = (const T *)a.v + s.b * a.v_b + (s.k0 + key[t]) * a.v_t + hkv * a.v_h;
+    for (int y = 0; y < 2; ++y) {
+        key[y] = key0 + wave * 32 + y * 16 + r;
+        const T *kp = (const T *)a.k + s.b * a.k_b + (s.k0 + key[y]) * a.k_t + hkv * a.k_h;
+        const T *vp = (const T *)a.v + s.b * a.v_b + (s.k0 + key[y]) * a.v_t + hkv * a.v_h;
 #pragma unroll
         for (int x = 0; x < NS; ++x) {
             const int c = x * 4 + g;
-            const bool ok = key[t] < keys && c * 8 < a.dim;
-            kf[t][x] = ok ? *(const X8 *)(kp + c * 8) : X8{};
-            vf[t][x] = ok ? *(const X8 *)(vp + c * 8) : X8{};
+            const bool ok = key[y] < keys && c * 8 < a.dim;
+            sums.kf[y][x] = ok ? *(const X8 *)(kp + c * 8) : X8{};
+            sums.vf[y][x] = ok ? *(const X8 *)(vp + c * 8) : X8{};
         }
     }
-    f32x4 dk[ND][2], dv[ND][2];
-#pragma unroll
-    for (int d = 0; d < ND; ++d) dk[d][0] = dk[d][1] = dv[d][0] = dv[d][1] = f32x4{0, 0, 0, 0};
-
-    // the rows that see some key of the tile
-    const int key1 = min(key0 + kKM, keys) - 1;
-    const int tok_lo = max(0, key0 - s.shift);
-    int tok_hi = s.q_len;
-    if (a.window && key0 >= a.sinks) tok_hi = min(tok_hi, key1 + a.window - s.shift);
-    const int row_lo = tok_lo * a.group, row_hi = max(tok_hi, 0) * a.group;
-
-    Stage<T, DP> qo;
-    float lse_r = 0.f, delta_r = 0.f;
-    int pos_r = -1;
-    auto load = [&](int row0) {
-#pragma unroll
-        for (int u = 0; u < Stage<T, DP>::NU; ++u) {
-            const int id = threadIdx.x + 256 * u, row = row0 + id / NC, c = id % NC;
-            const bool in = row < row_hi;
-            const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
-            const bool ok = in && c * 8 < a.dim;
-            qo.x[u] = ok ? *(const u32x4 *)((const T *)a.q + s.b * a.q_b + (s.q0 + tok) * a.q_t + h * a.q_h + c * 8)
-                         : u32x4{0, 0, 0, 0};
-            qo.y[u] = ok ? *(const u32x4 *)((const T *)a.d_o + s.b * a.do_b + (s.q0 + tok) * a.do_t + h * a.do_h + c * 8)
-                         : u32x4{0, 0, 0, 0};
+    const int wkey0 = key0 + wave * 32, wkey1 = wkey0 + 31;
+    wait_dma();
+    __syncthreads();
+    int n = 0;
+    for (int row0 = row_lo; row0 < row_hi; row0 += kKN, n ^= 1) {
+        const bool more = row0 + kKN < row_hi;
+        float lse = 0.f, delta = 0.f;
+        int pos = -1;
+        if (more) {
+            if (threadIdx.x < kKN) in.stats(row0 + kKN + threadIdx.x, lse, delta, pos);
+            in.fetch(row0 + kKN, sq[n ^ 1], so[n ^ 1], kKN);
         }
-        if (threadIdx.x < kKN) {
-            const int row = row0 + threadIdx.x;
-            const bool in = row < row_hi;
-            const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
-            const int64_t l_at = s.b * a.lse_b + h * a.lse_h + s.q0 + tok;
-            lse_r = in ? a.lse[l_at] : 0.f;
-            delta_r = in ? a.delta[l_at] : 0.f;
-            pos_r = in ? tok + s.shift : -1;
-        }
-    };
-    if (row_lo < row_hi) load(row_lo);
-    for (int row0 = row_lo; row0 < row_hi; row0 += kKN) {
-        __syncthreads();
-        qo.store(sq, so);
-        if (threadIdx.x < kKN) s_lse[threadIdx.x] = lse_r, s_delta[threadIdx.x] = delta_r, s_pos[threadIdx.x] = pos_r;
-        __syncthreads();
-        if (row0 + kKN < row_hi) load(row0 + kKN);
-        const int pmin = div_by(row0, a.by_group) + s.shift;
-        const int pmax = div_by(min(row0 + kKN, row_hi) - 1, a.by_group) + s.shift;
-        const bool full = row0 + kKN <= row_hi && key1 == key0 + kKM - 1 && key1 <= pmin &&
-                          (!a.window || key0 > pmax - a.window || key1 < a.sinks);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            X8 pf[2], df[2];
+            const int ru = row0 + u * 32;
+            const int pmin = div_by(ru, a.by_group) + s.shift, pmax = div_by(min(ru + 32, row_hi) - 1, a.by_group) + s.shift;
+            // hidden from every row, or seen by each
+            if (ru >= row_hi || wkey0 > pmax || wkey0 > key1 || (a.window && wkey1 <= pmin - a.window && wkey0 >= a.sinks)) continue;
+            const bool full = ru + 32 <= row_hi && wkey1 <= key1 && wkey1 <= pmin &&
+                              (!a.window || wkey0 > pmax - a.window || wkey1 < a.sinks);
+            sums.add(sq[n], so[n], s_lse[n], s_delta[n], s_pos[n], u * 32, a.c, full, g, r,
+                     [&](int y, int p) { return sees(key[y], p, window_low(p, a.window), a.sinks); });
+        }
+        wait_dma();
+        if (more && threadIdx.x < kKN) s_lse[n ^ 1][threadIdx.x] = lse, s_delta[n ^ 1][threadIdx.x] = delta, s_pos[n ^ 1][threadIdx.x] = pos;
+        __syncthreads();
+    }
+
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const int rt = u * 2 + w, j = rt * 16 + r;
-                f32x4 st[2], dp[2];
-                st[0] = st[1] = dp[0] = dp[1] = f32x4{0, 0, 0, 0};
+    for (int y = 0; y < 2; ++y) {
+        const float fk = sums.k_unit(y), fv = sums.v_unit();
 #pragma unroll
-                for (int x = 0; x < NS; ++x) {
-                    const X8 qf = *(const X8 *)(sq + j * DP + swz<NC>(j, x * 4 + g) * 8);
-                    const X8 of = *(const X8 *)(so + j * DP + swz<NC>(j, x * 4 + g) * 8);
+        for (int d = 0; d < ND; ++d) sums.dk[d][y] *= fk, sums.dv[d][y] *= fv;
+        const int group = (wkey0 + y * 16) / 16;
+        if (a.chunk && wkey0 + y * 16 < min(a.sinks, keys)) {
+            const int first = max(far_token(a, s, wkey0, keys), 0) * a.group, rows = s.q_len * a.group;
+            const int slot0 = first_tile(a, s, a.chunk, a.group);
+            for (int c = first / a.chunk; c * a.chunk < rows && first < rows; ++c) {
+                const float *part = a.part + ((int64_t)(group * a.kv_heads + hkv) * a.far_slots + slot0 + c) * 2 * 16 * DP + r * DP + g * 4;
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        st[y] = mfma(qf, kf[y][x], st[y]);
-                        dp[y] = mfma(of, vf[y][x], dp[y]);
-                    }
-                }
-                const f32x4 lse = *(const f32x4 *)(s_lse + rt * 16 + g * 4);
-                const f32x4 delta = *(const f32x4 *)(s_delta + rt * 16 + g * 4);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int p = full ? 0 : s_pos[rt * 16 + g * 4 + i];
-#pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(st[y][i], a.c, -lse[i]));
-                        const float ds = pr * (dp[y][i] - delta[i]);
-                        const bool in = full | sees(key[y], p, window_low(p, a.window), a.sinks);
-                        pf[y][w * 4 + i] = (T)(in ? pr : 0.f);
-                        df[y][w * 4 + i] = (T)(in ? ds : 0.f);
-                    }
-                }
-            }
-            const int j = u * 32 + g * 4 + (r >> 2);
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                const int c = d * 2 + ((r & 3) >> 1), e = (r & 1) * 4;
-                const X8 of = join<X4, X8>(read_tr<T>(so + j * DP + swz<NC>(j, c) * 8 + e),
-                                           read_tr<T>(so + (j + 16) * DP + swz<NC>(j + 16, c) * 8 + e));
-                const X8 qf = join<X4, X8>(read_tr<T>(sq + j * DP + swz<NC>(j, c) * 8 + e),
-                                           read_tr<T>(sq + (j + 16) * DP + swz<NC>(j + 16, c) * 8 + e));
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    dv[d][y] = mfma(of, pf[y], dv[d][y]);
-                    dk[d][y] = mfma(qf, df[y], dk[d][y]);
+                for (int d = 0; d < ND; ++d) {
+                    sums.dk[d][y] += *(const f32x4 *)(part + d * 16);
+                    sums.dv[d][y] += *(const f32x4 *)(part + 16 * DP + d * 16);
                 }
             }
         }
-    }
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
         if (key[y] >= keys) continue;
         const int64_t at = (((a.offsets ? s.k0 : (int64_t)s.b * a.k_len) + key[y]) * a.kv_heads + hkv) * a.dim;
 #pragma unroll
@@ -321,8 +552,8 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(AttnArgs a) {
             X4 wk, wv;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                wk[i] = (T)(dk[d][y][i] * a.scale);
-                wv[i] = (T)dv[d][y][i];
+                wk[i] = (T)(sums.dk[d][y][i] * a.scale);
+                wv[i] = (T)sums.dv[d][y][i];
             }
             if (d * 16 + g * 4 < a.dim) {
                 *(X4 *)((T *)a.dk + at + d * 16 + g * 4) = wk;
@@ -332,15 +563,47 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(AttnArgs a) {
     }
 }
 
+// The far rows' chunks: enough of them to spread a sequence over 64 workgroups,
+// none below 512 rows.  Past 256 sinks their tiles are no exception any more,
+// and take all rows themselves.
+struct Far {
+    int chunk, slots, groups;
+    int64_t bytes;
+};
+Far far_plan(const AttnArgs &a) {
+    Far f{};
+    if (!a.window || !a.sinks || a.sinks > 256) return f;
+    const int64_t rows = (int64_t)(a.offsets ? a.tokens : a.q_len) * a.group;
+    if (rows <= (int64_t)a.window * a.group) return f;
+    f.chunk = (int)((rows / 64 + 127) / 128 * 128);
+    if (f.chunk < 512) f.chunk = 512;
+    f.slots = (int)((rows + f.chunk - 1) / f.chunk);
+    f.slots = a.offsets ? f.slots + a.batch + 2 : f.slots * a.batch;
+    f.groups = (a.sinks + 15) / 16;
+    f.bytes = (int64_t)f.groups * a.kv_heads * f.slots * 2 * 16 * (a.dim <= 64 ? 64 : 128) * 4;
+    return f;
+}
+int64_t delta_bytes(const AttnArgs &a) {
+    const int64_t rows = (a.offsets ? (int64_t)a.tokens : (int64_t)a.batch * a.q_len) * a.heads;
+    return (4 * rows + 255) / 256 * 256;
+}
+
 template <typename T, int DP>
 hipError_t bwd(const AttnArgs &in, hipStream_t s) {
     AttnArgs a = in;
-    const int64_t rows = (a.offsets ? (int64_t)a.tokens : (int64_t)a.batch * a.q_len) * a.heads;
-    if (rows) attn_delta_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, s>>>(a);
+    const Far far = far_plan(a);
+    a.part = (float *)((uint8_t *)a.delta + delta_bytes(a));
     const int pad = a.offsets ? a.batch + 2 : 0, many = a.offsets ? 1 : a.batch;
-    a.tiles = (int)(((int64_t)(a.offsets ? a.tokens : a.q_len) * a.group + kBM - 1) / kBM) * many + pad;
-    a.per = (int)(((int64_t)a.tiles * a.kv_heads + 7) / 8);
-    if (rows) attn_dq_kernel<T, DP><<<(unsigned)a.per * 8, 256, 0, s>>>(a);
+    const int tokens = a.offsets ? a.tokens : a.q_len;
+    if (tokens) {
+        a.tiles = (int)(((int64_t)tokens * a.group + kBM - 1) / kBM) * many + pad;
+        a.per = (int)(((int64_t)a.tiles * a.kv_heads + 7) / 8);
+        attn_dq_kernel<T, DP><<<(unsigned)a.per * 8, 256, 0, s>>>(a);
+        if (far.chunk) {
+            a.chunk = far.chunk, a.tiles = a.far_slots = far.slots;
+            attn_far_kernel<T, DP><<<(unsigned)far.slots * a.kv_heads * far.groups, 256, 0, s>>>(a);
+        }
+    }
     a.tiles = ((a.offsets ? a.tokens : a.k_len) + kKM - 1) / kKM * many + pad;
     a.per = (int)(((int64_t)a.tiles * a.kv_heads + 7) / 8);
     if (a.tiles) attn_dkv_kernel<T, DP><<<(unsigned)a.per * 8, 256, 0, s>>>(a);
@@ -349,10 +612,7 @@ hipError_t bwd(const AttnArgs &in, hipStream_t s) {
 
 }  // namespace
 
-int64_t attn_bwd_workspace(const AttnArgs &a) {
-    const int64_t rows = (a.offsets ? (int64_t)a.tokens : (int64_t)a.batch * a.q_len) * a.heads;
-    return (4 * rows + 255) / 256 * 256 + 256;
-}
+int64_t attn_bwd_workspace(const AttnArgs &a) { return delta_bytes(a) + far_plan(a).bytes + 256; }
 
 hipError_t launch_attn_bwd(const AttnArgs &a, int dtype, hipStream_t s) {
     if (dtype == LSMX_BF16) return a.dim <= 64 ? bwd<__bf16, 64>(a, s) : bwd<__bf16, 128>(a, s);

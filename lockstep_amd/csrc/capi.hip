@@ -770,20 +770,24 @@ static int attn_args(const char *fn, const lsmx_attention *a, bool bwd, lsmx::At
     const bool nq = a->batch && a->q_len, nk = a->batch && a->k_len;
     if ((nq || a->offsets) && a->q_len && (!a->q || !a->o)) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
     if ((nk || a->offsets) && a->k_len && (!a->k || !a->v)) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
-    if (bwd && nq && !a->lse) return fail(LSMX_ERR_ARG, "%s: null lse", fn);
-    if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->o, 16) || !aligned(a->lse, 4) ||
-        !aligned(a->offsets, 4))
+    if (bwd && nq && (!a->lse || !a->o_rest)) return fail(LSMX_ERR_ARG, "%s: null lse or o_rest", fn);
+    if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->o, 16) || !aligned(a->o_rest, 16) ||
+        !aligned(a->lse, 4) || !aligned(a->offsets, 4))
         return fail(LSMX_ERR_ALIGN, "%s: operands must be 16-byte aligned", fn);
     for (int i = 0; i < 3; ++i)
         if (a->q_stride[i] % 8 || a->k_stride[i] % 8 || a->v_stride[i] % 8 || a->o_stride[i] % 8)
             return fail(LSMX_ERR_ALIGN, "%s: strides must be multiples of 8 elements", fn);
     // offsets within a tile are 32-bit
-    if (a->q_stride[1] < 0 || a->k_stride[1] < 0 || a->v_stride[1] < 0 || a->q_stride[1] >= 1 << 23 ||
-        a->k_stride[1] >= 1 << 23 || a->v_stride[1] >= 1 << 23)
-        return fail(LSMX_ERR_SHAPE, "%s: token strides must be below 2^23", fn);
+    if (a->q_stride[1] < 0 || a->k_stride[1] < 0 || a->v_stride[1] < 0 || a->q_stride[1] >= 1 << 22 ||
+        a->k_stride[1] >= 1 << 22 || a->v_stride[1] >= 1 << 22)
+        return fail(LSMX_ERR_SHAPE, "%s: token strides must be below 2^22", fn);
+    if (a->q_stride[2] < 0 || a->k_stride[2] < 0 || a->v_stride[2] < 0)
+        return fail(LSMX_ERR_SHAPE, "%s: negative head stride", fn);
+    if (bwd && (group * a->q_stride[2] >= 1 << 29))
+        return fail(LSMX_ERR_SHAPE, "%s: the heads of a group must span less than 2^29 elements", fn);
     lsmx::AttnArgs &g = *out;
     g = lsmx::AttnArgs{};
-    g.q = a->q, g.k = a->k, g.v = a->v, g.o = a->o, g.lse = a->lse;
+    g.q = a->q, g.k = a->k, g.v = a->v, g.o = a->o, g.o_lo = a->o_rest, g.lse = a->lse;
     g.batch = (int)a->batch, g.heads = (int)a->heads, g.kv_heads = (int)a->kv_heads, g.group = (int)group;
     g.dim = (int)a->head_dim, g.q_len = (int)a->q_len, g.k_len = (int)a->k_len;
     const bool packed = a->offsets != nullptr;
@@ -826,6 +830,8 @@ int lsmx_attention_bwd(const lsmx_attention *a, const void *d_o, const int64_t *
         return fail(LSMX_ERR_ALIGN, "%s: operands must be 16-byte aligned", fn);
     for (int i = 0; i < 3; ++i)
         if (do_stride[i] % 8) return fail(LSMX_ERR_ALIGN, "%s: strides must be multiples of 8 elements", fn);
+    if (do_stride[1] < 0 || do_stride[1] >= 1 << 22 || do_stride[2] < 0 || g.group * do_stride[2] >= 1 << 29)
+        return fail(LSMX_ERR_SHAPE, "%s: do_stride out of range", fn);
     if (ws_bytes < lsmx::attn_bwd_workspace(g)) return fail(LSMX_ERR_ARG, "%s: workspace too small", fn);
     if (int r = device_guard()) return r;
     if (!nq && !nk) return LSMX_OK;

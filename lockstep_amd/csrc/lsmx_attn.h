@@ -121,8 +121,9 @@ struct AttnArgs {
     float *delta;
     void *dq, *dk, *dv;  // contiguous, laid out as q, k, v
     float scale;
-    float *part;         // partial gradients of the sink keys
-    int sink_tiles, splits;
+    void *o_lo;          // o as computed less o as rounded, laid out as o (forward: null to leave out)
+    float *part;         // far rows' partial gradients of the sinks
+    int chunk, far_slots;  // rows of a chunk (0: no far rows apart), chunks of all sequences
 };
 
 // One sequence of a packed or dense batch.
@@ -130,6 +131,7 @@ struct Seq {
     int b, q_len, k_len, shift;  // query token t has position t + shift
     int64_t q0, k0;              // first token (packed: in the token axis, else 0)
     int tile;
+    int idx;                     // packed: its place in the order of tiles
 };
 
 // The sequence and tile of work tile t, tiles of `size` rows with `mult` rows
@@ -171,7 +173,7 @@ LSMX_DEV bool find_tile(const AttnArgs &a, int t, int size, int mult, int len, S
             s.tile = t - before - (lane_of(upto, w) - lane_of(n, w));
             s.q_len = lane_of(own, w);
             s.q0 = s.k0 = lane_of(lo, w);
-            const int idx = first + w;
+            const int idx = s.idx = first + w;
             s.b = 0;
             s.k_len = idx >= 1 && idx <= a.batch ? s.q_len : 0;
             s.shift = s.k_len ? 0 : -s.q_len;  // dead sequence: positions below 0
@@ -259,6 +261,22 @@ LSMX_DEV void split(f16x8 x, bf16x8 &hi, bf16x8 &lo) {
 // Rows (tokens x heads of a key head) up to which the keys of a sequence are
 // split over workgroups; more rows run in tiles of 128.
 constexpr int kDecodeRows = 64;
+// The number of the first tile (as find_tile counts them) of sequence s.
+LSMX_DEV int first_tile(const AttnArgs &a, const Seq &s, int size, int mult) {
+    if (!a.offsets) return s.b * ((a.q_len * mult + size - 1) / size);
+    const int lane = threadIdx.x & 63;
+    int n = 0;
+    for (int first = 0; first <= s.idx; first += 64) {
+        const int i = first + lane;
+        if (i < s.idx) {
+            const int lo = i == 0 ? 0 : min(max(a.offsets[i - 1], 0), a.tokens), hi = min(max(a.offsets[i], 0), a.tokens);
+            n += (int)(((int64_t)max(hi - lo, 0) * mult + size - 1) / size);
+        }
+    }
+    for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
+    return uniform(n);
+}
+
 hipError_t launch_kv_append(const AppendArgs &a, int dtype, hipStream_t s);
 int kv_attend_splits(int batch, int kv_heads, int rows, int64_t keys);
 hipError_t launch_kv_attend(const AttendArgs &a, int dtype, hipStream_t s);
