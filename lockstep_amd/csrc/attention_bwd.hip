@@ -160,11 +160,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
         const int j0 = t * kBN, tn = next(t);
         if (tn < t_hi) fetch(tn * kBN, n ^ 1);
         const T *ck = sk[n], *cv = sv[n];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        auto half = [&](auto all, int u) {
             const int ju = j0 + u * 32;
-            if (ju > wmax || (a.window && ju + 31 <= wmin - a.window && ju >= a.sinks)) continue;
-            const bool full = ju + 31 <= wmin && (!a.window || ju > wmax - a.window || ju + 31 < a.sinks);
             f32x4 st[2][2], dp[2][2];  // [16 keys][16 rows]
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
@@ -191,7 +188,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
                     for (int y = 0; y < 2; ++y) {
                         float ds = __builtin_amdgcn_exp2f(__builtin_fmaf(st[w][y][i], a.c, -lse[y])) *
                                    (dp[w][y][i] - delta[y]);
-                        if (!full) {
+                        if constexpr (!decltype(all)::value) {
                             const int j = ju + w * 16 + g * 4 + i;
                             ds = sees(j, pos[y], low[y], a.sinks) ? ds : 0.f;
                         }
@@ -227,6 +224,16 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
                 dq[d][0] = mfma(kf, df[0], dq[d][0]);
                 dq[d][1] = mfma(kf, df[1], dq[d][1]);
             }
+        };
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int ju = j0 + u * 32;
+            // hidden from every row, or seen by each
+            if (ju > wmax || (a.window && ju + 31 <= wmin - a.window && ju >= a.sinks)) continue;
+            if (ju + 31 <= wmin && (!a.window || ju > wmax - a.window || ju + 31 < a.sinks))
+                half(BoolC<true>{}, u);
+            else
+                half(BoolC<false>{}, u);
         }
         n ^= 1, t = tn;
         wait_dma();
@@ -289,19 +296,22 @@ struct KeySums {
     X8 kf[NK][NS], vf[NK][NS];
     f32x4 dk[ND][NK], dv[ND][NK];
     float mul[NK], limit[NK];
+    // position p sees key y of the lane when 0 <= p - key <= span
+    int key[NK];
+    uint32_t span[NK];
 
-    LSMX_DEV void init() {
+    LSMX_DEV void init(const AttnArgs &a, int key0) {
 #pragma unroll
         for (int y = 0; y < NK; ++y) {
+            key[y] = key0 + y * 16;
+            span[y] = a.window && key[y] >= a.sinks ? a.window - 1 : 0x7FFFFFFF;
             mul[y] = limit[y] = 0.f;
 #pragma unroll
             for (int d = 0; d < ND; ++d) dk[d][y] = dv[d][y] = f32x4{0, 0, 0, 0};
         }
     }
-    // see(y, position): whether key y of the lane is seen from there
-    template <typename F>
     LSMX_DEV void add(const T *sq, const T *so, const float *s_lse, const float *s_delta, const int *s_pos, int j0,
-                      float c, bool full, int g, int r, F see) {
+                      float c, int g, int r) {
         X8 pf[NK], df[NK];
         f32x4 pr[2][NK], ds[2][NK];
         float top[NK];
@@ -324,17 +334,18 @@ struct KeySums {
             }
             const f32x4 lse = *(const f32x4 *)(s_lse + j0 + w * 16 + g * 4);
             const f32x4 delta = *(const f32x4 *)(s_delta + j0 + w * 16 + g * 4);
+            const i32x4 pos = *(const i32x4 *)(s_pos + j0 + w * 16 + g * 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int y = 0; y < NK; ++y) {
-                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(pr[w][y][i], c, -lse[i]));
-                    float d = p * (ds[w][y][i] - delta[i]);
-                    if (!full) {
-                        const bool in = see(y, s_pos[j0 + w * 16 + g * 4 + i]);
-                        p = in ? p : 0.f;
-                        d = in ? d : 0.f;
-                    }
+                    // three operations an element: cheaper than a second form
+                    // of the loop for tiles without hidden pairs, whose copies
+                    // of the sums do not fit the registers
+                    const bool in = (uint32_t)(pos[i] - key[y]) <= span[y];
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(pr[w][y][i], c, -lse[i]));
+                    const float p = in ? e : 0.f;
+                    const float d = p * (ds[w][y][i] - delta[i]);
                     pf[y][w * 4 + i] = (T)p;
                     if constexpr (Range<T>::on) {
                         ds[w][y][i] = d;
@@ -398,7 +409,7 @@ __global__ __launch_bounds__(256) void attn_far_kernel(AttnArgs a) {
     typedef typename Vec<T>::x8 X8;
     __shared__ __attribute__((aligned(16))) uint8_t smem[2 * kFar * DP * 2];
     __shared__ __attribute__((aligned(16))) float s_lse[kFar], s_delta[kFar];
-    __shared__ int s_pos[kFar];
+    __shared__ __attribute__((aligned(16))) int s_pos[kFar];
     T *sq = (T *)smem, *so = sq + kFar * DP;
 
     const int slots = a.tiles, slot = uniform(blockIdx.x % slots), rest = uniform(blockIdx.x / slots);
@@ -414,7 +425,7 @@ __global__ __launch_bounds__(256) void attn_far_kernel(AttnArgs a) {
     if (row_lo >= row_hi) return;
 
     KeySums<T, DP, 1> sums;
-    sums.init();
+    sums.init(a, key);
     const T *kp = (const T *)a.k + s.b * a.k_b + (s.k0 + key) * a.k_t + hkv * a.k_h;
     const T *vp = (const T *)a.v + s.b * a.v_b + (s.k0 + key) * a.v_t + hkv * a.v_h;
 #pragma unroll
@@ -425,14 +436,14 @@ __global__ __launch_bounds__(256) void attn_far_kernel(AttnArgs a) {
         sums.vf[0][x] = ok ? *(const X8 *)(vp + c * 8) : X8{};
     }
     Rows<T, DP> in{a, s, hkv, row_hi};
-    const bool sink = key < min(a.sinks, keys);
     for (int row0 = row_lo; row0 < row_hi; row0 += kFar) {
         __syncthreads();
         in.fetch(row0, sq, so, kFar);
         if (threadIdx.x < kFar) in.stats(row0 + threadIdx.x, s_lse[threadIdx.x], s_delta[threadIdx.x], s_pos[threadIdx.x]);
         wait_dma();
         __syncthreads();
-        sums.add(sq, so, s_lse, s_delta, s_pos, wave * 32, a.c, false, g, r, [&](int, int pos) { return sink & (pos >= 0); });
+        // rows past their window see none but the sinks
+        sums.add(sq, so, s_lse, s_delta, s_pos, wave * 32, a.c, g, r);
     }
     // join the waves: dK, then dV
     float *w_out = (float *)smem;  // [4][16][DP]
@@ -454,14 +465,16 @@ __global__ __launch_bounds__(256) void attn_far_kernel(AttnArgs a) {
     }
 }
 
+// 320 registers at head 128: one wave per SIMD (held to 256, the spills took
+// 1350 us against 484 at 2 x 4096 tokens, 32/8 heads, window 1024).
 template <typename T, int DP>
-__global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attn_dkv_kernel(AttnArgs a) {
     constexpr int NS = DP / 32, ND = DP / 16;
     typedef typename Vec<T>::x8 X8;
     typedef typename Vec<T>::x4 X4;
     __shared__ __attribute__((aligned(16))) T sq[2][kKN * DP], so[2][kKN * DP];
     __shared__ __attribute__((aligned(16))) float s_lse[2][kKN], s_delta[2][kKN];
-    __shared__ int s_pos[2][kKN];
+    __shared__ __attribute__((aligned(16))) int s_pos[2][kKN];
 
     const int item = xcd_item(blockIdx.x, a.per);
     if (item >= a.tiles * a.kv_heads) return;
@@ -484,11 +497,10 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
     }
 
     KeySums<T, DP, 2> sums;
-    sums.init();
-    int key[2];
+    sums.init(a, key0 + wave * 32 + r);
+    const int(&key)[2] = sums.key;
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
-        key[y] = key0 + wave * 32 + y * 16 + r;
         const T *kp = (const T *)a.k + s.b * a.k_b + (s.k0 + key[y]) * a.k_t + hkv * a.k_h;
         const T *vp = (const T *)a.v + s.b * a.v_b + (s.k0 + key[y]) * a.v_t + hkv * a.v_h;
 #pragma unroll
@@ -511,16 +523,12 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
             if (threadIdx.x < kKN) in.stats(row0 + kKN + threadIdx.x, lse, delta, pos);
             in.fetch(row0 + kKN, sq[n ^ 1], so[n ^ 1], kKN);
         }
+        // hidden from every row
+        const int pmin = div_by(row0, a.by_group) + s.shift, pmax = div_by(min(row0 + kKN, row_hi) - 1, a.by_group) + s.shift;
+        const bool none = wkey0 > pmax || wkey0 > key1 || (a.window && wkey1 <= pmin - a.window && wkey0 >= a.sinks);
+        if (!none) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int ru = row0 + u * 32;
-            const int pmin = div_by(ru, a.by_group) + s.shift, pmax = div_by(min(ru + 32, row_hi) - 1, a.by_group) + s.shift;
-            // hidden from every row, or seen by each
-            if (ru >= row_hi || wkey0 > pmax || wkey0 > key1 || (a.window && wkey1 <= pmin - a.window && wkey0 >= a.sinks)) continue;
-            const bool full = ru + 32 <= row_hi && wkey1 <= key1 && wkey1 <= pmin &&
-                              (!a.window || wkey0 > pmax - a.window || wkey1 < a.sinks);
-            sums.add(sq[n], so[n], s_lse[n], s_delta[n], s_pos[n], u * 32, a.c, full, g, r,
-                     [&](int y, int p) { return sees(key[y], p, window_low(p, a.window), a.sinks); });
+            for (int u = 0; u < 2; ++u) sums.add(sq[n], so[n], s_lse[n], s_delta[n], s_pos[n], u * 32, a.c, g, r);
         }
         wait_dma();
         if (more && threadIdx.x < kKN) s_lse[n ^ 1][threadIdx.x] = lse, s_delta[n ^ 1][threadIdx.x] = delta, s_pos[n ^ 1][threadIdx.x] = pos;

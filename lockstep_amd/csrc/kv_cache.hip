@@ -98,17 +98,42 @@ struct Codes {
     static constexpr int NW = DP / 32;
     uint32_t w[NW];
     uint32_t e;
-    LSMX_DEV void load(const uint8_t *codes, const uint8_t *scale, int64_t v, int g, bool in) {
+    // base: the first key's codes and scales (the same for the whole wave)
+    LSMX_DEV void load(const uint8_t *codes, const uint8_t *scale, int g, int r, bool in) {
 #pragma unroll
         for (int i = 0; i < NW; ++i) w[i] = 0;
         e = 0;
         if (in) {
-            const uint8_t *c = codes + v * (DP / 2) + g * (DP / 8);
+            const uint8_t *c = codes + r * (DP / 2) + g * (DP / 8);
             if constexpr (NW == 4)
                 *(u32x4 *)w = *(const u32x4 *)c;
             else
                 *(u32x2 *)w = *(const u32x2 *)c;
-            e = scale[v * (DP / 32) + g * (DP / 32) / 4];
+            e = scale[r * (DP / 32) + g * (DP / 32) / 4];
+        }
+    }
+};
+
+// 32 keys of a sequence and key head from position j0 on: two groups of 16,
+// each within one page.
+template <int DP, bool VALUES>
+struct Keys {
+    int j0, pg[2];  // pages, or -1
+    Codes<DP> k[2], v[2];
+    LSMX_DEV void find(const Pool &p, int b, int j, int len) {
+        j0 = j;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) pg[t] = j + t * 16 < len ? p.page_of(b, j + t * 16) : -1;
+    }
+    LSMX_DEV void load(const Pool &p, int h, int g, int r, int len) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            pg[t] = uniform(pg[t]);
+            const int j = j0 + t * 16;
+            const int64_t vec = p.vec(max(pg[t], 0), h, j);
+            const bool in = pg[t] >= 0 && j + r < len;
+            k[t].load(p.kc + vec * (DP / 2), p.ks + vec * (DP / 32), g, r, in);
+            if constexpr (VALUES) v[t].load(p.vc + vec * (DP / 2), p.vs + vec * (DP / 32), g, r, in);
         }
     }
 };
@@ -130,28 +155,55 @@ LSMX_DEV void load_rows(const AttnArgs &a, int b, int hkv, int row, int g, bool 
     }
 }
 
+// The scores of 16 keys, lane 16g + r holding keys 4g..4g+3 of row r; the
+// lane's part of each vector is contracted as it lies in memory.
+template <int DP, int RT, int NT>
+LSMX_DEV void scores(const Codes<DP> &k, const bf16x8 (&q)[RT][NT][DP / 32], f32x4 (&st)[RT]) {
+    const float sc = e8m0_to_f32(k.e);
+#pragma unroll
+    for (int y = 0; y < RT; ++y) st[y] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < DP / 32; ++s) {
+        const bf16x8 kf = fp4x8_to_bf16(k.w[s], sc);
+#pragma unroll
+        for (int y = 0; y < RT; ++y)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) st[y] = mfma(kf, q[y][n][s], st[y]);
+    }
+}
+
 // One workgroup: one sequence and key head, RT x 16 rows, a share of the keys;
-// its 4 waves take tiles of 32 keys in turn and are joined at the end.
+// its 4 waves take tiles of 32 keys in turn and are joined at the end.  A wave
+// has the next tile's codes in flight while it works on one, and the page
+// numbers of the tile after that.
 template <typename TQ, int DP, int RT>
 __global__ __launch_bounds__(256) void kv_decode_kernel(AttendArgs x) {
     constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, NT = __is_same(TQ, __bf16) ? 1 : 2;
-    __shared__ __attribute__((aligned(16))) uint8_t smem[4 * 32 * DP * 2];  // values of a wave's tile; then 16 x DP fp32 of a wave
+    __shared__ __attribute__((aligned(16))) uint8_t smem[4 * 32 * DP * 2];  // values of a wave's tile; then 16 x DP / 2 fp32 of a wave
     __shared__ float s_m[4][16], s_l[4][16];
     const AttnArgs &a = x.a;
     const Pool &p = x.p;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
     const int bh = blockIdx.x / x.splits, sp = blockIdx.x - bh * x.splits, b = bh / a.kv_heads, hkv = bh - b * a.kv_heads;
     const int rows = a.q_len * a.group;
     const Tiles tiles(x, b);
     const int i0 = (int)((int64_t)tiles.n * sp / x.splits), i1 = (int)((int64_t)tiles.n * (sp + 1) / x.splits);
 
+    Keys<DP, true> cur, nxt;
+    int i = i0 + wave;
+    if (i < i1) {
+        cur.find(p, b, tiles[i] * 32, tiles.len);
+        cur.load(p, hkv, g, r, tiles.len);
+        if (i + 4 < i1) nxt.find(p, b, tiles[i + 4] * 32, tiles.len);
+    }
     bf16x8 q[RT][NT][NS];
-    int pos[RT];
+    int pos[RT], low[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const int row = t * 16 + r;
         load_rows<TQ, DP, NT>(a, b, hkv, row, g, row < rows, q[t]);
         pos[t] = row < rows ? div_by(row, a.by_group) + tiles.len - a.q_len : -1;
+        low[t] = window_low(pos[t], a.window);
     }
     f32x4 o[ND][RT];
     float m[RT], l[RT];
@@ -164,82 +216,71 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(AttendArgs x) {
     __bf16 *sv = (__bf16 *)smem + wave * 32 * DP;
     const int pfirst = tiles.len - a.q_len;
 
-    for (int i = i0 + wave; i < i1; i += 4) {
-        const int j0 = tiles[i] * 32;
-        Codes<DP> k[2], v[2];
-        bool in[2];
+    for (; i < i1; i += 4) {
+        int j2 = 0, pg2[2] = {-1, -1};
+        if (i + 4 < i1) nxt.load(p, hkv, g, r, tiles.len);
+        if (i + 8 < i1) {
+            j2 = tiles[i + 8] * 32;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int j = j0 + t * 16 + r, pg = j < tiles.len ? p.page_of(b, j) : -1;
-            in[t] = pg >= 0;
-            const int64_t vec = p.vec(max(pg, 0), hkv, j);
-            k[t].load(p.kc, p.ks, vec, g, in[t]);
-            v[t].load(p.vc, p.vs, vec, g, in[t]);
+            for (int t = 0; t < 2; ++t) pg2[t] = j2 + t * 16 < tiles.len ? p.page_of(b, j2 + t * 16) : -1;
         }
+        const int j0 = cur.j0;
         f32x4 st[2][RT];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const float ksc = e8m0_to_f32(k[t].e), vsc = e8m0_to_f32(v[t].e);
-#pragma unroll
-            for (int y = 0; y < RT; ++y) st[t][y] = f32x4{0, 0, 0, 0};
+            scores<DP, RT, NT>(cur.k[t], q, st[t]);
+            const float vsc = e8m0_to_f32(cur.v[t].e);
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
-                const bf16x8 kf = fp4x8_to_bf16(k[t].w[s], ksc);
-#pragma unroll
-                for (int y = 0; y < RT; ++y)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) st[t][y] = mfma(kf, q[y][n][s], st[t][y]);
                 const int row = t * 16 + r, c = g * NS + s;
-                *(bf16x8 *)(sv + row * DP + swz<NC>(row, c) * 8) = fp4x8_to_bf16(v[t].w[s], vsc);
+                *(bf16x8 *)(sv + row * DP + swz<NC>(row, c) * 8) = fp4x8_to_bf16(cur.v[t].w[s], vsc);
             }
         }
         // hidden keys: past a row's position, outside its window, or in no page
-        const bool full = j0 + 31 <= pfirst && __all(in[0] & in[1]) && (!a.window || j0 > tiles.len - 1 - a.window || j0 + 31 < a.sinks);
+        const bool full = j0 + 31 <= pfirst && (cur.pg[0] | cur.pg[1]) >= 0 &&
+                          (!a.window || j0 > tiles.len - 1 - a.window || j0 + 31 < a.sinks);
         if (!full) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const uint64_t ok = __ballot(in[t]);
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int j = j0 + t * 16 + g * 4 + e;
-                    const bool held = (ok >> (g * 4 + e)) & 1;
 #pragma unroll
-                    for (int y = 0; y < RT; ++y)
-                        st[t][y][e] = (held & sees(j, pos[y], window_low(pos[y], a.window), a.sinks)) ? st[t][y][e] : -INFINITY;
+                    for (int y = 0; y < RT; ++y) {
+                        const bool see = (cur.pg[t] >= 0) & sees(j, pos[y], low[y], a.sinks);
+                        st[t][y][e] = see ? st[t][y][e] : -INFINITY;
+                    }
                 }
-            }
         }
         bf16x8 pf[RT][NT];
 #pragma unroll
         for (int y = 0; y < RT; ++y) {
-            float mx = m[y];
+            float mx = st[0][y][0];
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mx = fmaxf(mx, st[t][y][e]);
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float mc = mx == -INFINITY ? 0.f : mx * a.c;
-            const float alpha = __builtin_amdgcn_exp2f(m[y] * a.c - mc);
-            m[y] = mx;
-            float sum = 0.f;
+            if (__any(mx > m[y])) {
+                const float top = fmaxf(m[y], max_rows(mx));
+                const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[y] - top) * a.c);
+                m[y] = top;
+                l[y] *= alpha;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[d][y] *= alpha;
+            }
+            const float mc = m[y] == -INFINITY ? 0.f : m[y] * a.c;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][y][e], a.c, -mc));
-                    sum += w;
+                    l[y] += w;
                     pf[y][0][t * 4 + e] = (__bf16)w;
                     if constexpr (NT == 2) pf[y][1][t * 4 + e] = (__bf16)(w - (float)pf[y][0][t * 4 + e]);
                 }
-            l[y] = l[y] * alpha + sum;
-#pragma unroll
-            for (int d = 0; d < ND; ++d) o[d][y] *= alpha;
         }
-        // the wave's own LDS region: its writes above, its reads here
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+        // the wave's own LDS region: its writes above, its reads here, in order
+        asm volatile("" ::: "memory");
         const int row = g * 4 + (r >> 2);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
@@ -251,9 +292,9 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(AttendArgs x) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) o[d][y] = mfma(vf, pf[y][n], o[d][y]);
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+        asm volatile("" ::: "memory");
+        cur = nxt;
+        nxt.j0 = j2, nxt.pg[0] = pg2[0], nxt.pg[1] = pg2[1];
     }
 
     // join the waves, 16 rows at a time
@@ -261,8 +302,7 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(AttendArgs x) {
     constexpr int HD = DP / 2;
 #pragma unroll
     for (int y = 0; y < RT; ++y) {
-        float sum = l[y] + __shfl_xor(l[y], 16);
-        sum += __shfl_xor(sum, 32);
+        const float sum = sum_rows(l[y]);
         __syncthreads();
         if (g == 0) s_m[wave][r] = m[y], s_l[wave][r] = sum;
 #pragma unroll
@@ -307,91 +347,213 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(AttendArgs x) {
     }
 }
 
-// Joins the shares of one row: one wave per row.
+// Joins the shares of one row: 16 threads over the vector, 16 over the shares.
 template <typename TQ, int DP>
-__global__ __launch_bounds__(64) void kv_join_kernel(AttendArgs x) {
+__global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs x) {
+    constexpr int NE = DP / 16;
+    __shared__ float s_top[4], s_tot[16], s_acc[16][DP + 4];
     const AttnArgs &a = x.a;
-    const int rows = a.q_len * a.group, lane = threadIdx.x;
+    const int rows = a.q_len * a.group, lane = threadIdx.x & 63, part = threadIdx.x >> 4, c = (threadIdx.x & 15) * NE;
     const int row = blockIdx.x % rows, bh = blockIdx.x / rows, b = bh / a.kv_heads, hkv = bh - b * a.kv_heads;
     const int64_t at0 = (int64_t)bh * x.splits * rows + row;
     float top = -INFINITY;
-    for (int s = lane; s < x.splits; s += 64) top = fmaxf(top, x.part_m[(at0 + (int64_t)s * rows) * 2]);
+    for (int s = threadIdx.x; s < x.splits; s += 256) top = fmaxf(top, x.part_m[(at0 + (int64_t)s * rows) * 2]);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if (lane == 0) s_top[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
     const float mc = top == -INFINITY ? 0.f : top * a.c;
-    float tot = 0.f, acc[DP / 64];
+    float tot = 0.f, acc[NE];
 #pragma unroll
-    for (int e = 0; e < DP / 64; ++e) acc[e] = 0.f;
-    for (int s = 0; s < x.splits; ++s) {
+    for (int e = 0; e < NE; ++e) acc[e] = 0.f;
+#pragma unroll 4
+    for (int s = part; s < x.splits; s += 16) {
         const int64_t at = at0 + (int64_t)s * rows;
         const float f = __builtin_amdgcn_exp2f(x.part_m[at * 2] * a.c - mc);
-        tot += x.part_m[at * 2 + 1] * f;
+        tot = __builtin_fmaf(x.part_m[at * 2 + 1], f, tot);
 #pragma unroll
-        for (int e = 0; e < DP / 64; ++e) acc[e] += x.part[at * DP + lane * (DP / 64) + e] * f;
+        for (int e = 0; e < NE; e += 4) {
+            const f32x4 w = *(const f32x4 *)(x.part + at * DP + c + e);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[e + k] = __builtin_fmaf(w[k], f, acc[e + k]);
+        }
     }
-    const int tok = div_by(row, a.by_group), h = hkv * a.group + row - tok * a.group;
-    TQ *op = (TQ *)a.o + b * a.o_b + tok * a.o_t + h * a.o_h + lane * (DP / 64);
-    const float inv = tot > 0.f || tot != tot ? 1.f / tot : 0.f;
 #pragma unroll
-    for (int e = 0; e < DP / 64; ++e) op[e] = (TQ)(acc[e] * inv);
-    if (a.lse && lane == 0)
+    for (int e = 0; e < NE; ++e) s_acc[part][c + e] = acc[e];
+    if (c == 0) s_tot[part] = tot;
+    __syncthreads();
+    if (threadIdx.x >= DP) return;
+    float sum = 0.f;
+    tot = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += s_acc[i][threadIdx.x], tot += s_tot[i];
+    const int tok = div_by(row, a.by_group), h = hkv * a.group + row - tok * a.group;
+    const float inv = tot > 0.f || tot != tot ? 1.f / tot : 0.f;
+    ((TQ *)a.o)[b * a.o_b + tok * a.o_t + h * a.o_h + threadIdx.x] = (TQ)(sum * inv);
+    if (a.lse && threadIdx.x == 0)
         a.lse[b * a.lse_b + h * a.lse_h + tok] = tot > 0.f ? mc + __log2f(tot) : tot != tot ? tot : -INFINITY;
 }
 
 // ------------------------------------------------------------------ weights
 // weights[b, h, j] += sum over the rows of exp(s_ij - lse_i), the scores
-// recomputed from the keys' codes.  A wave owns 16 keys and runs over the rows
-// in tiles of 16: one owner and one order for every sum.
-template <typename TQ, int DP>
+// recomputed from the keys' codes: 68 bytes a key at head 128, where scores
+// kept by the first pass would be 8 bytes a key and row.  Each sum has one owner and
+// one order.
+//
+// Few rows: their q stays in registers, and the waves run over the keys as in
+// kv_decode_kernel.
+LSMX_DEV float sum_16(float x) {  // over the 16 lanes of a row of lanes
+    x += u2f(__builtin_amdgcn_update_dpp(0, f2u(x), 0xB1, 0xF, 0xF, true));   // quad_perm 1,0,3,2
+    x += u2f(__builtin_amdgcn_update_dpp(0, f2u(x), 0x4E, 0xF, 0xF, true));   // quad_perm 2,3,0,1
+    x += u2f(__builtin_amdgcn_update_dpp(0, f2u(x), 0x141, 0xF, 0xF, true));  // row_half_mirror
+    x += u2f(__builtin_amdgcn_update_dpp(0, f2u(x), 0x140, 0xF, 0xF, true));  // row_mirror
+    return x;
+}
+template <typename TQ, int DP, int RT>
 __global__ __launch_bounds__(256) void kv_weights_kernel(AttendArgs x) {
     constexpr int NS = DP / 32, NT = __is_same(TQ, __bf16) ? 1 : 2;
     const AttnArgs &a = x.a;
     const Pool &p = x.p;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
+    const int bh = blockIdx.x / x.splits, sp = blockIdx.x - bh * x.splits, b = bh / a.kv_heads, hkv = bh - b * a.kv_heads;
+    const int rows = a.q_len * a.group;
+    const Tiles tiles(x, b);
+    const int i0 = (int)((int64_t)tiles.n * sp / x.splits), i1 = (int)((int64_t)tiles.n * (sp + 1) / x.splits);
+    Keys<DP, false> cur, nxt;
+    int i = i0 + wave;
+    if (i >= i1) return;
+    cur.find(p, b, tiles[i] * 32, tiles.len);
+    cur.load(p, hkv, g, r, tiles.len);
+    if (i + 4 < i1) nxt.find(p, b, tiles[i + 4] * 32, tiles.len);
+    bf16x8 q[RT][NT][NS];
+    int pos[RT], low[RT];
+    float lse[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int row = t * 16 + r;
+        const bool in = row < rows;
+        load_rows<TQ, DP, NT>(a, b, hkv, row, g, in, q[t]);
+        const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
+        pos[t] = in ? tok + tiles.len - a.q_len : -1;
+        low[t] = window_low(pos[t], a.window);
+        lse[t] = a.lse[b * a.lse_b + h * a.lse_h + tok];
+    }
+    float *w = x.weights + (int64_t)bh * x.w_len;
+    for (; i < i1; i += 4) {
+        int j2 = 0, pg2[2] = {-1, -1};
+        const int j0 = cur.j0;
+        // lane r < 8 keeps the sums of key 16 (r / 4) + 4g + r % 4
+        const int mine = j0 + (r >> 2) * 16 + g * 4 + (r & 3);
+        const bool held = r < 8 && mine < tiles.len && (r < 4 ? cur.pg[0] : cur.pg[1]) >= 0;
+        float before = held ? w[mine] : 0.f;
+        if (i + 4 < i1) nxt.load(p, hkv, g, r, tiles.len);
+        if (i + 8 < i1) {
+            j2 = tiles[i + 8] * 32;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) pg2[t] = j2 + t * 16 < tiles.len ? p.page_of(b, j2 + t * 16) : -1;
+        }
+        float own = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x4 st[RT], sum{0, 0, 0, 0};
+            scores<DP, RT, NT>(cur.k[t], q, st);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                for (int y = 0; y < RT; ++y) {
+                    const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(st[y][e], a.c, -lse[y]));
+                    sum[e] += sees(j0 + t * 16 + g * 4 + e, pos[y], low[y], a.sinks) ? v : 0.f;
+                }
+                const float all = sum_16(sum[e]);
+                own = r == t * 4 + e ? all : own;
+            }
+        }
+        if (held) w[mine] = before + own;
+        cur = nxt;
+        nxt.j0 = j2, nxt.pg[0] = pg2[0], nxt.pg[1] = pg2[1];
+    }
+}
+
+// Many rows: a workgroup owns 64 keys, whose operands stay in registers, and
+// its waves take tiles of 16 rows in turn; their sums are joined in LDS.
+template <typename TQ, int DP>
+__global__ __launch_bounds__(256) void kv_weights_rows_kernel(AttendArgs x) {
+    constexpr int NS = DP / 32, NT = __is_same(TQ, __bf16) ? 1 : 2;
+    __shared__ __attribute__((aligned(16))) float s_sum[4][64];
+    const AttnArgs &a = x.a;
+    const Pool &p = x.p;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
     const int per = ((p.max_pages << p.page_shift) + 63) / 64;
     const int bh = blockIdx.x / per, b = bh / a.kv_heads, hkv = bh - b * a.kv_heads;
-    const int len = p.length(b), rows = a.q_len * a.group, first = len - a.q_len;
-    const int j0 = ((blockIdx.x - bh * per) * 4 + wave) * 16;
+    const int len = p.length(b), first = len - a.q_len, j0 = (blockIdx.x - bh * per) * 64;
     if (j0 >= len) return;
-    const int j = j0 + r, pg = j < len ? p.page_of(b, j) : -1;
-    Codes<DP> k;
-    k.load(p.kc, p.ks, p.vec(max(pg, 0), hkv, j), g, pg >= 0);
-    const uint64_t ok = __ballot(pg >= 0);
-    bf16x8 kf[NS];
-#pragma unroll
-    for (int s = 0; s < NS; ++s) kf[s] = fp4x8_to_bf16(k.w[s], e8m0_to_f32(k.e));
     // the rows that see some key of the tile
     const int tok_lo = max(0, j0 - first);
     int tok_hi = a.q_len;
-    if (a.window && j0 >= a.sinks) tok_hi = min(tok_hi, min(j0 + 15, len - 1) + a.window - first);
+    if (a.window && j0 >= a.sinks) tok_hi = min(tok_hi, min(j0 + 63, len - 1) + a.window - first);
     if (tok_lo >= tok_hi) return;
-    f32x4 sum{0, 0, 0, 0};
-    for (int r0 = tok_lo * a.group; r0 < tok_hi * a.group; r0 += 16) {
-        const int row = r0 + r;
-        const bool in = row < rows;
+    bf16x8 kf[4][NS];
+    int pg[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const int j = j0 + t * 16;
+        pg[t] = uniform(j < len ? p.page_of(b, j) : -1);
+        const int64_t vec = p.vec(max(pg[t], 0), hkv, j);
+        Codes<DP> k;
+        k.load(p.kc + vec * (DP / 2), p.ks + vec * (DP / 32), g, r, pg[t] >= 0 && j + r < len);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) kf[t][s] = fp4x8_to_bf16(k.w[s], e8m0_to_f32(k.e));
+    }
+    f32x4 sum[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) sum[t] = f32x4{0, 0, 0, 0};
+    const int row_hi = tok_hi * a.group;
+    struct Row {
         bf16x8 q[NT][NS];
-        load_rows<TQ, DP, NT>(a, b, hkv, row, g, in, q);
+        float lse;
+        int pos;
+    };
+    auto load = [&](int r0, Row &w) {
+        const int row = r0 + r;
+        const bool in = row < row_hi;
+        load_rows<TQ, DP, NT>(a, b, hkv, row, g, in, w.q);
         const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
-        const int pos = in ? tok + first : -1;
-        const float lse = a.lse[b * a.lse_b + h * a.lse_h + tok];
-        f32x4 st{0, 0, 0, 0};
+        w.lse = a.lse[b * a.lse_b + h * a.lse_h + tok];
+        w.pos = in ? tok + first : -1;
+    };
+    Row cur, nxt;
+    int r0 = tok_lo * a.group + wave * 16;
+    if (r0 < row_hi) load(r0, cur);
+    for (; r0 < row_hi; r0 += 64) {
+        if (r0 + 64 < row_hi) load(r0 + 64, nxt);
+        const int low = window_low(cur.pos, a.window);
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
+        for (int t = 0; t < 4; ++t) {
+            f32x4 st{0, 0, 0, 0};
 #pragma unroll
-            for (int n = 0; n < NT; ++n) st = mfma(kf[s], q[n][s], st);
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) st = mfma(kf[t][s], cur.q[n][s], st);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(st[e], a.c, -cur.lse));
+                sum[t][e] += sees(j0 + t * 16 + g * 4 + e, cur.pos, low, a.sinks) ? v : 0.f;
+            }
+        }
+        cur = nxt;
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const bool see = sees(j0 + g * 4 + e, pos, window_low(pos, a.window), a.sinks);
-            sum[e] += see ? __builtin_amdgcn_exp2f(__builtin_fmaf(st[e], a.c, -lse)) : 0.f;
+            const float all = sum_16(sum[t][e]);
+            if (r == 0) s_sum[wave][t * 16 + g * 4 + e] = pg[t] >= 0 ? all : 0.f;
         }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) sum[e] += __shfl_xor(sum[e], d);
-        const int at = j0 + g * 4 + e;
-        if (r == e && at < len && ((ok >> (g * 4 + e)) & 1)) x.weights[(int64_t)bh * x.w_len + at] += sum[e];
-    }
+    __syncthreads();
+    const int at = j0 + threadIdx.x;
+    if (threadIdx.x < 64 && at < len)
+        x.weights[(int64_t)bh * x.w_len + at] += s_sum[0][threadIdx.x] + s_sum[1][threadIdx.x] + s_sum[2][threadIdx.x] + s_sum[3][threadIdx.x];
 }
 
 // ------------------------------------------------------------------ eviction
@@ -509,15 +671,22 @@ hipError_t attend(const AttendArgs &x, hipStream_t s) {
         kv_decode_kernel<TQ, DP, 2><<<grid, 256, 0, s>>>(x);
     else
         kv_decode_kernel<TQ, DP, 4><<<grid, 256, 0, s>>>(x);
-    if (x.splits > 1) kv_join_kernel<TQ, DP><<<(unsigned)(rows * bh), 64, 0, s>>>(x);
+    if (x.splits > 1) kv_join_kernel<TQ, DP><<<(unsigned)(rows * bh), 256, 0, s>>>(x);
     return hipGetLastError();
 }
 
 template <typename TQ, int DP>
-hipError_t weights(const AttendArgs &x, hipStream_t s) {
-    const int keys = x.p.max_pages << x.p.page_shift;
-    const dim3 grid((unsigned)((keys + 63) / 64) * x.a.batch * x.a.kv_heads);
-    kv_weights_kernel<TQ, DP><<<grid, 256, 0, s>>>(x);
+hipError_t weights(AttendArgs x, hipStream_t s) {
+    const int rows = x.a.q_len * x.a.group, bh = x.a.batch * x.a.kv_heads;
+    const dim3 grid((unsigned)x.splits * bh);
+    if (rows <= 16)
+        kv_weights_kernel<TQ, DP, 1><<<grid, 256, 0, s>>>(x);
+    else if (rows <= 32)
+        kv_weights_kernel<TQ, DP, 2><<<grid, 256, 0, s>>>(x);
+    else if (rows <= kDecodeRows)
+        kv_weights_kernel<TQ, DP, 4><<<grid, 256, 0, s>>>(x);
+    else
+        kv_weights_rows_kernel<TQ, DP><<<(unsigned)(((x.p.max_pages << x.p.page_shift) + 63) / 64) * bh, 256, 0, s>>>(x);
     return hipGetLastError();
 }
 
