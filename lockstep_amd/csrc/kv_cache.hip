@@ -84,7 +84,7 @@ struct Tiles {
     LSMX_DEV Tiles(const AttendArgs &x, int b) {
         len = x.p.length(b);
         const int first = len - x.a.q_len;  // position of the first row
-        const int hi = (len + 31) / 32;
+        const int hi = x.p.pages ? (len + 31) / 32 : 0;
         sink = min(hi, (x.a.sinks + 31) / 32);
         lo = x.a.window ? max(sink, max(0, first - x.a.window + 1) / 32) : sink;
         n = sink + max(0, hi - lo);
@@ -98,43 +98,60 @@ struct Codes {
     static constexpr int NW = DP / 32;
     uint32_t w[NW];
     uint32_t e;
-    // base: the first key's codes and scales (the same for the whole wave)
-    LSMX_DEV void load(const uint8_t *codes, const uint8_t *scale, int g, int r, bool in) {
+    // codes, scale: of the first key (the same for the whole wave)
+    LSMX_DEV void load(const uint8_t *codes, const uint8_t *scale, int g, int r) {
+        const uint8_t *c = codes + r * (DP / 2) + g * (DP / 8);
+        if constexpr (NW == 4)
+            *(u32x4 *)w = *(const u32x4 *)c;
+        else
+            *(u32x2 *)w = *(const u32x2 *)c;
+        e = scale[r * (DP / 32) + g * (DP / 32) / 4];
+    }
+    LSMX_DEV void drop() {
 #pragma unroll
         for (int i = 0; i < NW; ++i) w[i] = 0;
         e = 0;
-        if (in) {
-            const uint8_t *c = codes + r * (DP / 2) + g * (DP / 8);
-            if constexpr (NW == 4)
-                *(u32x4 *)w = *(const u32x4 *)c;
-            else
-                *(u32x2 *)w = *(const u32x2 *)c;
-            e = scale[r * (DP / 32) + g * (DP / 32) / 4];
-        }
     }
 };
 
 // 32 keys of a sequence and key head from position j0 on: two groups of 16,
-// each within one page.
+// each within one page.  Every slot of a page can be read, so that the loads
+// stand outside all branches; what lies in no page is read from the pool's
+// first one, and hidden.
 template <int DP, bool VALUES>
 struct Keys {
     int j0, pg[2];  // pages, or -1
     Codes<DP> k[2], v[2];
-    LSMX_DEV void find(const Pool &p, int b, int j, int len) {
-        j0 = j;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) pg[t] = j + t * 16 < len ? p.page_of(b, j + t * 16) : -1;
-    }
-    LSMX_DEV void load(const Pool &p, int h, int g, int r, int len) {
+    LSMX_DEV void load(const Pool &p, int h, int g, int r) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            pg[t] = uniform(pg[t]);
-            const int j = j0 + t * 16;
-            const int64_t vec = p.vec(max(pg[t], 0), h, j);
-            const bool in = pg[t] >= 0 && j + r < len;
-            k[t].load(p.kc + vec * (DP / 2), p.ks + vec * (DP / 32), g, r, in);
-            if constexpr (VALUES) v[t].load(p.vc + vec * (DP / 2), p.vs + vec * (DP / 32), g, r, in);
+            const int64_t vec = p.vec(max(pg[t], 0), h, j0 + t * 16);
+            k[t].load(p.kc + vec * (DP / 2), p.ks + vec * (DP / 32), g, r);
+            if constexpr (VALUES) v[t].load(p.vc + vec * (DP / 2), p.vs + vec * (DP / 32), g, r);
         }
+    }
+};
+
+// The tiles i0 + wave, i0 + wave + 4, .. of one wave, and their pages: 64 page
+// numbers at a time, one of each lane, so that a tile's pages are at hand
+// without a load of their own.
+struct Walk {
+    const Pool &p;
+    const Tiles &tiles;
+    int b, end, first, pages;  // first: the tile whose pages lanes 0 and 1 hold
+    LSMX_DEV Walk(const Pool &pool, const Tiles &t, int seq, int i, int i1) : p(pool), tiles(t), b(seq), end(i1) { fill(i); }
+    LSMX_DEV void fill(int i) {
+        const int lane = threadIdx.x & 63, mine = i + 4 * (lane >> 1), j = tiles[mine] * 32 + (lane & 1) * 16;
+        first = i;
+        pages = mine < end && j < tiles.len ? p.page_of(b, j) : -1;
+    }
+    template <typename K>
+    LSMX_DEV void find(int i, K &keys) {
+        if (i - first >= 128) fill(i);
+        const int at = (i - first) >> 1;
+        keys.j0 = tiles[i] * 32;
+        keys.pg[0] = lane_of(pages, at);
+        keys.pg[1] = lane_of(pages, at + 1);
     }
 };
 
@@ -191,10 +208,10 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(AttendArgs x) {
 
     Keys<DP, true> cur, nxt;
     int i = i0 + wave;
+    Walk walk(p, tiles, b, i, i1);
     if (i < i1) {
-        cur.find(p, b, tiles[i] * 32, tiles.len);
-        cur.load(p, hkv, g, r, tiles.len);
-        if (i + 4 < i1) nxt.find(p, b, tiles[i + 4] * 32, tiles.len);
+        walk.find(i, cur);
+        cur.load(p, hkv, g, r);
     }
     bf16x8 q[RT][NT][NS];
     int pos[RT], low[RT];
@@ -217,14 +234,20 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(AttendArgs x) {
     const int pfirst = tiles.len - a.q_len;
 
     for (; i < i1; i += 4) {
-        int j2 = 0, pg2[2] = {-1, -1};
-        if (i + 4 < i1) nxt.load(p, hkv, g, r, tiles.len);
-        if (i + 8 < i1) {
-            j2 = tiles[i + 8] * 32;
-#pragma unroll
-            for (int t = 0; t < 2; ++t) pg2[t] = j2 + t * 16 < tiles.len ? p.page_of(b, j2 + t * 16) : -1;
-        }
+        // after the last tile this one again, from the cache: the loads of all
+        // rounds are alike, and the wait is for the round before
+        walk.find(i + 4 < i1 ? i + 4 : i, nxt);
+        nxt.load(p, hkv, g, r);
         const int j0 = cur.j0;
+        // hidden keys: past a row's position, outside its window, or in no page
+        const bool full = j0 + 31 <= pfirst && (cur.pg[0] | cur.pg[1]) >= 0 &&
+                          (!a.window || j0 > tiles.len - 1 - a.window || j0 + 31 < a.sinks);
+        if (!full) {
+            // what is in no row's sight must not reach a product as a NaN
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                if (cur.pg[t] < 0 || j0 + t * 16 + r >= tiles.len) cur.v[t].drop();
+        }
         f32x4 st[2][RT];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -236,9 +259,6 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(AttendArgs x) {
                 *(bf16x8 *)(sv + row * DP + swz<NC>(row, c) * 8) = fp4x8_to_bf16(cur.v[t].w[s], vsc);
             }
         }
-        // hidden keys: past a row's position, outside its window, or in no page
-        const bool full = j0 + 31 <= pfirst && (cur.pg[0] | cur.pg[1]) >= 0 &&
-                          (!a.window || j0 > tiles.len - 1 - a.window || j0 + 31 < a.sinks);
         if (!full) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -294,7 +314,6 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(AttendArgs x) {
         }
         asm volatile("" ::: "memory");
         cur = nxt;
-        nxt.j0 = j2, nxt.pg[0] = pg2[0], nxt.pg[1] = pg2[1];
     }
 
     // join the waves, 16 rows at a time
@@ -423,9 +442,9 @@ __global__ __launch_bounds__(256) void kv_weights_kernel(AttendArgs x) {
     Keys<DP, false> cur, nxt;
     int i = i0 + wave;
     if (i >= i1) return;
-    cur.find(p, b, tiles[i] * 32, tiles.len);
-    cur.load(p, hkv, g, r, tiles.len);
-    if (i + 4 < i1) nxt.find(p, b, tiles[i + 4] * 32, tiles.len);
+    Walk walk(p, tiles, b, i, i1);
+    walk.find(i, cur);
+    cur.load(p, hkv, g, r);
     bf16x8 q[RT][NT][NS];
     int pos[RT], low[RT];
     float lse[RT];
@@ -441,18 +460,15 @@ __global__ __launch_bounds__(256) void kv_weights_kernel(AttendArgs x) {
     }
     float *w = x.weights + (int64_t)bh * x.w_len;
     for (; i < i1; i += 4) {
-        int j2 = 0, pg2[2] = {-1, -1};
         const int j0 = cur.j0;
         // lane r < 8 keeps the sums of key 16 (r / 4) + 4g + r % 4
         const int mine = j0 + (r >> 2) * 16 + g * 4 + (r & 3);
         const bool held = r < 8 && mine < tiles.len && (r < 4 ? cur.pg[0] : cur.pg[1]) >= 0;
         float before = held ? w[mine] : 0.f;
-        if (i + 4 < i1) nxt.load(p, hkv, g, r, tiles.len);
-        if (i + 8 < i1) {
-            j2 = tiles[i + 8] * 32;
-#pragma unroll
-            for (int t = 0; t < 2; ++t) pg2[t] = j2 + t * 16 < tiles.len ? p.page_of(b, j2 + t * 16) : -1;
-        }
+        // after the last tile this one again, from the cache: the loads of all
+        // rounds are alike, and the wait is for the round before
+        walk.find(i + 4 < i1 ? i + 4 : i, nxt);
+        nxt.load(p, hkv, g, r);
         float own = 0.f;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -471,7 +487,6 @@ __global__ __launch_bounds__(256) void kv_weights_kernel(AttendArgs x) {
         }
         if (held) w[mine] = before + own;
         cur = nxt;
-        nxt.j0 = j2, nxt.pg[0] = pg2[0], nxt.pg[1] = pg2[1];
     }
 }
 
@@ -501,7 +516,10 @@ __global__ __launch_bounds__(256) void kv_weights_rows_kernel(AttendArgs x) {
         pg[t] = uniform(j < len ? p.page_of(b, j) : -1);
         const int64_t vec = p.vec(max(pg[t], 0), hkv, j);
         Codes<DP> k;
-        k.load(p.kc + vec * (DP / 2), p.ks + vec * (DP / 32), g, r, pg[t] >= 0 && j + r < len);
+        if (p.pages)
+            k.load(p.kc + vec * (DP / 2), p.ks + vec * (DP / 32), g, r);
+        else
+            k.drop();
 #pragma unroll
         for (int s = 0; s < NS; ++s) kf[t][s] = fp4x8_to_bf16(k.w[s], e8m0_to_f32(k.e));
     }
