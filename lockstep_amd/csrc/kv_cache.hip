@@ -189,20 +189,25 @@ LSMX_DEV void scores(const Codes<DP> &k, const bf16x8 (&q)[RT][NT][DP / 32], f32
     }
 }
 
-// One workgroup: one sequence and key head, RT x 16 rows, a share of the keys;
+// One workgroup: one sequence and key head, RT x 16 of its rows, a share of the keys;
 // its 4 waves take tiles of 32 keys in turn and are joined at the end.  A wave
 // has the next tile's codes in flight while it works on one, and the page
 // numbers of the tile after that.
+//
+// Bound by the loads in flight, so that waves per SIMD count: 4 of them at 64 x
+// 8192 tokens of 8 key heads of 128 take 82 us = 5.2 TB/s (3: 91, 2: 101).
 template <typename TQ, int DP, int RT>
-__global__ __launch_bounds__(256) void kv_decode_kernel(AttendArgs x) {
+__global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(TQ, __bf16) ? 4 : 3) void kv_decode_kernel(AttendArgs x) {
     constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, NT = __is_same(TQ, __bf16) ? 1 : 2;
     __shared__ __attribute__((aligned(16))) uint8_t smem[4 * 32 * DP * 2];  // values of a wave's tile; then 16 x DP / 2 fp32 of a wave
     __shared__ float s_m[4][16], s_l[4][16];
     const AttnArgs &a = x.a;
     const Pool &p = x.p;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
-    const int bh = blockIdx.x / x.splits, sp = blockIdx.x - bh * x.splits, b = bh / a.kv_heads, hkv = bh - b * a.kv_heads;
-    const int rows = a.q_len * a.group;
+    const int rows = a.q_len * a.group, blocks = (rows + RT * 16 - 1) / (RT * 16);
+    // the blocks of rows of one share side by side: they read the same keys
+    const int rest = blockIdx.x / blocks, row0 = (blockIdx.x - rest * blocks) * RT * 16;
+    const int bh = rest / x.splits, sp = rest - bh * x.splits, b = bh / a.kv_heads, hkv = bh - b * a.kv_heads;
     const Tiles tiles(x, b);
     const int i0 = (int)((int64_t)tiles.n * sp / x.splits), i1 = (int)((int64_t)tiles.n * (sp + 1) / x.splits);
 
@@ -214,13 +219,12 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(AttendArgs x) {
         cur.load(p, hkv, g, r);
     }
     bf16x8 q[RT][NT][NS];
-    int pos[RT], low[RT];
+    int pos[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-        const int row = t * 16 + r;
+        const int row = row0 + t * 16 + r;
         load_rows<TQ, DP, NT>(a, b, hkv, row, g, row < rows, q[t]);
         pos[t] = row < rows ? div_by(row, a.by_group) + tiles.len - a.q_len : -1;
-        low[t] = window_low(pos[t], a.window);
     }
     f32x4 o[ND][RT];
     float m[RT], l[RT];
@@ -239,6 +243,10 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(AttendArgs x) {
         walk.find(i + 4 < i1 ? i + 4 : i, nxt);
         nxt.load(p, hkv, g, r);
         const int j0 = cur.j0;
+        // the lane's places in LDS, made anew each round: held over the loop they
+        // would take the registers of a wave
+        int lr = r;
+        asm volatile("" : "+v"(lr));
         // hidden keys: past a row's position, outside its window, or in no page
         const bool full = j0 + 31 <= pfirst && (cur.pg[0] | cur.pg[1]) >= 0 &&
                           (!a.window || j0 > tiles.len - 1 - a.window || j0 + 31 < a.sinks);
@@ -255,7 +263,7 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(AttendArgs x) {
             const float vsc = e8m0_to_f32(cur.v[t].e);
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
-                const int row = t * 16 + r, c = g * NS + s;
+                const int row = t * 16 + lr, c = g * NS + s;
                 *(bf16x8 *)(sv + row * DP + swz<NC>(row, c) * 8) = fp4x8_to_bf16(cur.v[t].w[s], vsc);
             }
         }
@@ -267,7 +275,7 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(AttendArgs x) {
                     const int j = j0 + t * 16 + g * 4 + e;
 #pragma unroll
                     for (int y = 0; y < RT; ++y) {
-                        const bool see = (cur.pg[t] >= 0) & sees(j, pos[y], low[y], a.sinks);
+                        const bool see = (cur.pg[t] >= 0) & sees(j, pos[y], window_low(pos[y], a.window), a.sinks);
                         st[t][y][e] = see ? st[t][y][e] : -INFINITY;
                     }
                 }
@@ -301,10 +309,10 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(AttendArgs x) {
         }
         // the wave's own LDS region: its writes above, its reads here, in order
         asm volatile("" ::: "memory");
-        const int row = g * 4 + (r >> 2);
+        const int row = g * 4 + (lr >> 2);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            const int c = d * 2 + ((r & 3) >> 1), e = (r & 1) * 4;
+            const int c = d * 2 + ((lr & 3) >> 1), e = (lr & 1) * 4;
             const bf16x8 vf = join<bf16x4, bf16x8>(read_tr<__bf16>(sv + row * DP + swz<NC>(row, c) * 8 + e),
                                                    read_tr<__bf16>(sv + (row + 16) * DP + swz<NC>(row + 16, c) * 8 + e));
 #pragma unroll
@@ -331,7 +339,7 @@ __global__ __launch_bounds__(256) void kv_decode_kernel(AttendArgs x) {
             for (int d = 0; d < ND / 2; ++d)
                 *(f32x4 *)(so + (wave * 16 + r) * HD + d * 16 + g * 4) = o[half * (ND / 2) + d][y];
             __syncthreads();
-            const int row = threadIdx.x >> 4, c = (threadIdx.x & 15) * (HD / 16), full = y * 16 + row;
+            const int row = threadIdx.x >> 4, c = (threadIdx.x & 15) * (HD / 16), full = row0 + y * 16 + row;
             float top = -INFINITY;
 #pragma unroll
             for (int w = 0; w < 4; ++w) top = fmaxf(top, s_m[w][row]);
@@ -682,13 +690,11 @@ __global__ __launch_bounds__(256) void kv_move_kernel(EvictArgs a) {
 template <typename TQ, int DP>
 hipError_t attend(const AttendArgs &x, hipStream_t s) {
     const int rows = x.a.q_len * x.a.group, bh = x.a.batch * x.a.kv_heads;
-    const dim3 grid((unsigned)x.splits * bh);
+    const unsigned grid = (unsigned)x.splits * bh;
     if (rows <= 16)
         kv_decode_kernel<TQ, DP, 1><<<grid, 256, 0, s>>>(x);
-    else if (rows <= 32)
-        kv_decode_kernel<TQ, DP, 2><<<grid, 256, 0, s>>>(x);
     else
-        kv_decode_kernel<TQ, DP, 4><<<grid, 256, 0, s>>>(x);
+        kv_decode_kernel<TQ, DP, 2><<<grid * ((rows + 31) / 32), 256, 0, s>>>(x);
     if (x.splits > 1) kv_join_kernel<TQ, DP><<<(unsigned)(rows * bh), 256, 0, s>>>(x);
     return hipGetLastError();
 }
