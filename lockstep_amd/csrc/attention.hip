@@ -65,10 +65,12 @@ struct DenseKV {
             dma_x4(ok ? (uint32_t)(j * (int)x_t + c * 8) * 2 : 0x80000000u, rs, lds + at * 16);
         }
     }
-    LSMX_DEV void fetch_k(int j0, T *to, int dim) { fetch(k, k_t, j0, to, dim); }
-    LSMX_DEV void fetch_v(int j0, T *to, int dim) { fetch(v, v_t, j0, to, dim); }
-    LSMX_DEV void land_k(T *, int *) { wait_dma(); }
-    LSMX_DEV void land_v(T *) { wait_dma(); }
+    LSMX_DEV void fetch(int j0, int, int, T *sk, T *sv, int *, int dim) {
+        fetch(k, k_t, j0, sk, dim);
+        fetch(v, v_t, j0, sv, dim);
+    }
+    LSMX_DEV void start(int j0, int, int, T *sk, T *sv, int *, int dim) { fetch(j0, 0, 0, sk, sv, nullptr, dim); }
+    LSMX_DEV void land() { wait_dma(); }
 };
 
 // Keys and values of a paged MXFP4 cache, expanded to bf16 on their way into
@@ -83,7 +85,7 @@ struct PagedKV {
     int b, h, k_len, row, part;
     uint32_t kr[NQ], vr[NQ];
     uint32_t ke, ve;
-    bool in;
+    int pg, pgn;  // page of the codes in registers, and of the next tile's
 
     LSMX_DEV static const AttnArgs &attn(const Args &a) { return a.a; }
     LSMX_DEV static bool find(const Args &x, int t, int size, Seq &s) {
@@ -101,9 +103,12 @@ struct PagedKV {
     LSMX_DEV void init(const Args &a, const Seq &s, int hkv) {
         p = &a.p, b = s.b, h = hkv, k_len = s.k_len, row = threadIdx.x >> 2, part = threadIdx.x & 3;
     }
-    // the thread's part of vector j: its codes, its block's scale; whether j is held
-    LSMX_DEV bool load(const uint8_t *codes, const uint8_t *scale, int j, uint32_t (&w)[NQ], uint32_t &e) {
-        const int pg = j < k_len ? p->page_of(b, j) : -1;
+    LSMX_DEV int page(int j0) const {
+        const int j = j0 + row;
+        return j0 >= 0 && j < k_len ? p->page_of(b, j) : -1;
+    }
+    // this thread's part of vector j
+    LSMX_DEV void codes(int j, const uint8_t *codes, const uint8_t *scale, uint32_t (&w)[NQ], uint32_t &e) {
 #pragma unroll
         for (int i = 0; i < NQ; ++i) w[i] = 0;
         e = 0;
@@ -116,20 +121,34 @@ struct PagedKV {
                 *(u32x2 *)w = *(const u32x2 *)c;
             e = scale[v * (DP / 32) + part * (DP / 32) / 4];
         }
-        return pg >= 0;
     }
     LSMX_DEV void store(T *to, const uint32_t (&w)[NQ], uint32_t e) {
         const float sc = e8m0_to_f32(e);
 #pragma unroll
         for (int i = 0; i < NQ; ++i) *(bf16x8 *)(to + row * DP + swz<NC>(row, part * NQ + i) * 8) = fp4x8_to_bf16(w[i], sc);
     }
-    LSMX_DEV void fetch_k(int j0, T *, int) { in = load(p->kc, p->ks, j0 + row, kr, ke); }
-    LSMX_DEV void fetch_v(int j0, T *, int) { load(p->vc, p->vs, j0 + row, vr, ve); }
-    LSMX_DEV void land_k(T *to, int *s_in) {
-        store(to, kr, ke);
-        if (part == 0) s_in[row] = in;
+    // The first tile j0 (next j1, then j2; -1: none) into LDS, the next one's
+    // codes on their way.
+    LSMX_DEV void start(int j0, int j1, int j2, T *sk, T *sv, int *s_in, int) {
+        pg = page(j0), pgn = page(j1);
+        load(j0);
+        fetch(j0, j1, j2, sk, sv, s_in, 0);
     }
-    LSMX_DEV void land_v(T *to) { store(to, vr, ve); }
+    LSMX_DEV void load(int j0) {
+        codes(j0 + row, p->kc, p->ks, kr, ke);
+        codes(j0 + row, p->vc, p->vs, vr, ve);
+    }
+    // Tile j0, whose codes are in registers, into LDS; those of j1 on their
+    // way, and the page of j2: each load has a round to land.
+    LSMX_DEV void fetch(int j0, int j1, int j2, T *sk, T *sv, int *s_in, int) {
+        store(sk, kr, ke);
+        store(sv, vr, ve);
+        if (part == 0) s_in[row] = pg >= 0;
+        pg = pgn;
+        load(j1);
+        pgn = page(j2);
+    }
+    LSMX_DEV void land() {}
 };
 
 // NW waves of RT x 16 rows.  TQ: type of q and o; T: type of the products'
@@ -184,12 +203,8 @@ __global__ __launch_bounds__(NW * 64, KV::kHoles ? (DP == 64 ? 2 : 1) : (DP == 6
 
     KV kv;
     kv.init(args, s, hkv);
-    if (t < t_hi) {
-        kv.fetch_k(t * kBN, sk[0], a.dim);
-        kv.fetch_v(t * kBN, sv[0], a.dim);
-        kv.land_k(sk[0], s_in[0]);
-        kv.land_v(sv[0]);
-    }
+    auto start_of = [&](int t) { return t < t_hi ? t * kBN : -1; };
+    if (t < t_hi) kv.start(t * kBN, start_of(tn), start_of(next(tn)), sk[0], sv[0], s_in[0], a.dim);
 
     // this lane's rows: wrow0 + r + 16 x
     int pos[RT], low[RT];
@@ -225,10 +240,12 @@ __global__ __launch_bounds__(NW * 64, KV::kHoles ? (DP == 64 ? 2 : 1) : (DP == 6
     const float lazy = kLazy / a.c;
 
     // scores of 32 keys from row j0 of a tile on
-    auto scores = [&](const T *ck, int j0, f32x4 (&z)[2][RT]) {
+    // (lr: r, opaque where the lane's places in LDS are made anew each time;
+    // held over the loop they would not fit the registers)
+    auto scores = [&](const T *ck, int j0, int lr, f32x4 (&z)[2][RT]) {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-            const int j = j0 + kt * 16 + r;
+            const int j = j0 + kt * 16 + lr;
 #pragma unroll
             for (int x = 0; x < RT; ++x) z[kt][x] = f32x4{0, 0, 0, 0};
 #pragma unroll
@@ -289,16 +306,18 @@ __global__ __launch_bounds__(NW * 64, KV::kHoles ? (DP == 64 ? 2 : 1) : (DP == 6
                 for (int d = 0; d < ND; ++d) o[d][x] *= alpha;
             }
         }
+        int lr = r;
+        asm volatile("" : "+v"(lr));
         X8 vf[ND];
-        const int j = jv + g * 4 + (r >> 2);
+        const int j = jv + g * 4 + (lr >> 2);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            const int c = d * 2 + ((r & 3) >> 1), e = (r & 1) * 4;
+            const int c = d * 2 + ((lr & 3) >> 1), e = (lr & 1) * 4;
             vf[d] = join<X4, X8>(read_tr<T>(cv + j * DP + swz<NC>(j, c) * 8 + e),
                                  read_tr<T>(cv + (j + 16) * DP + swz<NC>(j + 16, c) * 8 + e));
         }
         f32x4 zn[2][RT];
-        if constexpr (kMore) scores(ck, jk, zn);
+        if constexpr (kMore) scores(ck, jk, lr, zn);
         X8 pf[NT][RT];
 #pragma unroll
         for (int x = 0; x < RT; ++x) {
@@ -331,21 +350,20 @@ __global__ __launch_bounds__(NW * 64, KV::kHoles ? (DP == 64 ? 2 : 1) : (DP == 6
     wait_dma();
     __syncthreads();
     if (t < t_hi) {
-        scores(sk[0], 0, st);
+        scores(sk[0], 0, r, st);
         hide(t * kBN, s_in[0], st);
     }
     int n = 0;  // tile t is in buffer n
     while (t < t_hi) {
         const bool more = tn < t_hi;
         if (more) {
-            kv.fetch_k(tn * kBN, sk[n ^ 1], a.dim);
-            kv.fetch_v(tn * kBN, sv[n ^ 1], a.dim);
+            const int t2 = next(tn);
+            kv.fetch(tn * kBN, start_of(t2), start_of(next(t2)), sk[n ^ 1], sv[n ^ 1], s_in[n ^ 1], a.dim);
         }
         step(BoolC<true>{}, sk[n], 32, sv[n], 0);
         hide(t * kBN + 32, s_in[n] + (KV::kHoles ? 32 : 0), st);
         if (more) {
-            kv.land_k(sk[n ^ 1], s_in[n ^ 1]);
-            kv.land_v(sv[n ^ 1]);
+            kv.land();
             __syncthreads();
             step(BoolC<true>{}, sk[n ^ 1], 0, sv[n], 32);
             hide(tn * kBN, s_in[n ^ 1], st);
@@ -384,6 +402,9 @@ __global__ __launch_bounds__(NW * 64, KV::kHoles ? (DP == 64 ? 2 : 1) : (DP == 6
     }
 }
 
+#ifndef FEW
+#define FEW 512
+#endif
 // Row tiles over all sequences, and the grid of their items over 8 XCDs.
 void tiles_of(AttnArgs &a, int rows) {
     if (a.offsets)
@@ -396,17 +417,33 @@ void tiles_of(AttnArgs &a, int rows) {
 // Workgroups of 4 waves: two or three of them on a CU run out of step, and one's
 // products fall into another's exponentials.  (8 waves that share their tiles
 // were in step: 201 against 179 us at 2 x 4096 tokens, 32/8 heads of 128.)
-template <typename T, int DP, int RT>
+// 32 rows a wave, or 16 where 32 would leave CUs with less than two workgroups.
+bool few(const AttnArgs &a) {
+    const int64_t rows = (int64_t)(a.offsets ? a.tokens : a.q_len) * a.group * (a.offsets ? 1 : a.batch);
+    return rows * a.kv_heads < FEW * 128;
+}
+
+template <typename T, int DP>
 hipError_t fwd(AttnArgs a, hipStream_t s) {
-    tiles_of(a, 4 * RT * 16);
-    attn_fwd_kernel<T, T, DP, RT, 4, DenseKV<T, DP, 4>><<<(unsigned)a.per * 8, 256, 0, s>>>(a);
+    if (few(a)) {
+        tiles_of(a, 64);
+        attn_fwd_kernel<T, T, DP, 1, 4, DenseKV<T, DP, 4>><<<(unsigned)a.per * 8, 256, 0, s>>>(a);
+    } else {
+        tiles_of(a, 128);
+        attn_fwd_kernel<T, T, DP, 2, 4, DenseKV<T, DP, 4>><<<(unsigned)a.per * 8, 256, 0, s>>>(a);
+    }
     return hipGetLastError();
 }
 
 template <typename T, int DP>
 hipError_t chunk(AttendArgs x, hipStream_t s) {
-    tiles_of(x.a, 128);
-    attn_fwd_kernel<T, __bf16, DP, 2, 4, PagedKV<DP>><<<(unsigned)x.a.per * 8, 256, 0, s>>>(x);
+    if (few(x.a)) {
+        tiles_of(x.a, 64);
+        attn_fwd_kernel<T, __bf16, DP, 1, 4, PagedKV<DP>><<<(unsigned)x.a.per * 8, 256, 0, s>>>(x);
+    } else {
+        tiles_of(x.a, 128);
+        attn_fwd_kernel<T, __bf16, DP, 2, 4, PagedKV<DP>><<<(unsigned)x.a.per * 8, 256, 0, s>>>(x);
+    }
     return hipGetLastError();
 }
 
@@ -418,8 +455,8 @@ hipError_t launch_kv_chunk(const AttendArgs &x, int dtype, hipStream_t s) {
 }
 
 hipError_t launch_attn_fwd(const AttnArgs &a, int dtype, hipStream_t s) {
-    if (dtype == LSMX_BF16) return a.dim <= 64 ? fwd<__bf16, 64, 2>(a, s) : fwd<__bf16, 128, 2>(a, s);
-    return a.dim <= 64 ? fwd<_Float16, 64, 2>(a, s) : fwd<_Float16, 128, 2>(a, s);
+    if (dtype == LSMX_BF16) return a.dim <= 64 ? fwd<__bf16, 64>(a, s) : fwd<__bf16, 128>(a, s);
+    return a.dim <= 64 ? fwd<_Float16, 64>(a, s) : fwd<_Float16, 128>(a, s);
 }
 
 }  // namespace lsmx

@@ -535,39 +535,57 @@ __global__ __launch_bounds__(256) void kv_weights_rows_kernel(AttendArgs x) {
 #pragma unroll
     for (int t = 0; t < 4; ++t) sum[t] = f32x4{0, 0, 0, 0};
     const int row_hi = tok_hi * a.group;
+    // U tiles of rows at a time, the next U in flight: one tile's work is less
+    // than a load's latency
+    constexpr int U = 256 / DP;
     struct Row {
-        bf16x8 q[NT][NS];
+        typename Vec<TQ>::x8 q[NS];
         float lse;
         int pos;
     };
-    auto load = [&](int r0, Row &w) {
-        const int row = r0 + r;
-        const bool in = row < row_hi;
-        load_rows<TQ, DP, NT>(a, b, hkv, row, g, in, w.q);
-        const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
-        w.lse = a.lse[b * a.lse_b + h * a.lse_h + tok];
-        w.pos = in ? tok + first : -1;
-    };
-    Row cur, nxt;
-    int r0 = tok_lo * a.group + wave * 16;
-    if (r0 < row_hi) load(r0, cur);
-    for (; r0 < row_hi; r0 += 64) {
-        if (r0 + 64 < row_hi) load(r0 + 64, nxt);
-        const int low = window_low(cur.pos, a.window);
+    auto load = [&](int r0, Row (&w)[U]) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            f32x4 st{0, 0, 0, 0};
+        for (int u = 0; u < U; ++u) {
+            const int row = r0 + u * 64 + r;
+            const bool in = row < row_hi;
+            const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
+            const TQ *qp = (const TQ *)a.q + b * a.q_b + tok * a.q_t + h * a.q_h + g * (DP / 4);
+#pragma unroll
+            for (int s = 0; s < NS; ++s) w[u].q[s] = *(const typename Vec<TQ>::x8 *)(qp + s * 8);
+            w[u].lse = a.lse[b * a.lse_b + h * a.lse_h + tok];
+            w[u].pos = in ? tok + first : -1;
+        }
+    };
+    Row cur[U], nxt[U];
+    int r0 = tok_lo * a.group + wave * 16;
+    load(r0, cur);
+    for (; r0 < row_hi; r0 += 64 * U) {
+        load(r0 + 64 * U, nxt);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int low = window_low(cur[u].pos, a.window);
+            bf16x8 q[NT][NS];
 #pragma unroll
             for (int s = 0; s < NS; ++s)
+                if constexpr (NT == 1)
+                    q[0][s] = cur[u].q[s];
+                else
+                    split(cur[u].q[s], q[0][s], q[1][s]);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) st = mfma(kf[t][s], cur.q[n][s], st);
+            for (int t = 0; t < 4; ++t) {
+                f32x4 st{0, 0, 0, 0};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(st[e], a.c, -cur.lse));
-                sum[t][e] += sees(j0 + t * 16 + g * 4 + e, cur.pos, low, a.sinks) ? v : 0.f;
+                for (int s = 0; s < NS; ++s)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) st = mfma(kf[t][s], q[n][s], st);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(st[e], a.c, -cur[u].lse));
+                    sum[t][e] += sees(j0 + t * 16 + g * 4 + e, cur[u].pos, low, a.sinks) ? v : 0.f;
+                }
             }
+            cur[u] = nxt[u];
         }
-        cur = nxt;
     }
 #pragma unroll
     for (int t = 0; t < 4; ++t)
@@ -593,8 +611,10 @@ LSMX_DEV uint32_t rank_of(float w) {
 
 // One workgroup per sequence and key head: the rank of the last weight that
 // stays, by radix selection 8 bits at a time, then the kept positions in
-// ascending order.
+// ascending order.  PER: ranks a thread keeps in registers, which covers
+// 1024 PER positions; 0: they are read again in each round.
 constexpr int kSelect = 1024;
+template <int PER>
 __global__ __launch_bounds__(kSelect) void kv_select_kernel(EvictArgs a) {
     __shared__ int hist[256], s_scan[2][kSelect / 64], s_pick[2];
     const int bh = blockIdx.x, b = bh / a.p.kv_heads, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -607,83 +627,131 @@ __global__ __launch_bounds__(kSelect) void kv_select_kernel(EvictArgs a) {
     const bool all = n <= a.keep;
     int want = all ? 0 : a.keep - (n - (c1 - c0));  // of the candidates
     uint32_t prefix = 0;
+    float own[PER ? PER : 1];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) own[k] = k * kSelect + tid < n ? w[k * kSelect + tid] : 0.f;
+    // body(position, weight, whether it is one), by all threads alike
+    auto each = [&](auto body) {
+        if constexpr (PER > 0) {
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+                if (k * kSelect < n) body(k * kSelect + tid, own[k]);
+        } else {
+            for (int j = tid; j - tid < n; j += kSelect) body(j, j < n ? w[j] : 0.f);
+        }
+    };
     if (!all) {
         for (int shift = 24; shift >= 0; shift -= 8) {
             if (tid < 256) hist[tid] = 0;
             __syncthreads();
-            for (int j = c0 + tid; j < c1; j += kSelect) {
-                const uint32_t u = rank_of(w[j]);
-                if (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(u >> shift) & 255], 1);
-            }
+            each([&](int j, float x) {
+                const uint32_t u = rank_of(x);
+                if (j >= c0 && j < c1 && (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))))
+                    atomicAdd(&hist[(u >> shift) & 255], 1);
+            });
             __syncthreads();
-            if (tid == 0) {
-                int left = want, bin = 255;
-                while (bin > 0 && hist[bin] < left) left -= hist[bin--];
-                s_pick[0] = bin, s_pick[1] = left;
+            if (wave == 0) {
+                // the bin where the count from above reaches `want`: 4 bins a
+                // lane, the topmost in lane 0
+                int h[4], sum = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sum += h[k] = hist[255 - (lane * 4 + k)];
+                int above = sum;
+                for (int d = 1; d < 64; d <<= 1) {
+                    const int x = __shfl_up(above, d);
+                    if (lane >= d) above += x;
+                }
+                const uint64_t reach = __ballot(above >= want);
+                const int who = reach ? __ffsll((unsigned long long)reach) - 1 : 63;
+                if (lane == who) {
+                    int left = want - (above - sum), k = 0;
+                    while (k < 3 && h[k] < left) left -= h[k++];
+                    s_pick[0] = 255 - (lane * 4 + k), s_pick[1] = left;
+                }
             }
             __syncthreads();
             prefix |= (uint32_t)s_pick[0] << shift;
             want = s_pick[1];
-            __syncthreads();
         }
     }
     // prefix is the rank of the last that stays, `want` the number of its
     // equals that do (the first of them)
     int ties = 0, out = 0;
-    for (int j0 = 0; j0 < n; j0 += kSelect) {
-        const int j = j0 + tid;
-        const float x = j < n ? w[j] : 0.f;
+    each([&](int j, float x) {
         const uint32_t u = rank_of(x);
         const bool held = j < n && (all || j < c0 || j >= c1 || u > prefix);
         const bool tie = j < n && !all && j >= c0 && j < c1 && u == prefix;
-        const uint64_t bt = __ballot(tie);
+        const uint64_t below = (1ull << lane) - 1, bt = __ballot(tie);
         if (lane == 0) s_scan[0][wave] = __popcll(bt);
         __syncthreads();
-        int before = ties, all_ties = 0;
-        for (int i = 0; i < kSelect / 64; ++i) {
-            before += i < wave ? s_scan[0][i] : 0;
-            all_ties += s_scan[0][i];
-        }
-        before += __popcll(bt & ((1ull << lane) - 1));
-        const bool stay = held | (tie & (before < want));
+        // sums over the waves before, and over all
+        auto scan = [&](const int *v, int &before, int &total) {
+            const int x = lane < kSelect / 64 ? v[lane] : 0;
+            int y = lane < wave ? x : 0, z = x;
+#pragma unroll
+            for (int d = 1; d < kSelect / 64; d <<= 1) y += __shfl_xor(y, d), z += __shfl_xor(z, d);
+            before = lane_of(y, 0), total = lane_of(z, 0);
+        };
+        int before, total;
+        scan(s_scan[0], before, total);
+        const bool stay = held | (tie & (ties + before + __popcll(bt & below) < want));
+        ties += total;
         const uint64_t bs = __ballot(stay);
         if (lane == 0) s_scan[1][wave] = __popcll(bs);
         __syncthreads();
-        int at = out, all_out = 0;
-        for (int i = 0; i < kSelect / 64; ++i) {
-            at += i < wave ? s_scan[1][i] : 0;
-            all_out += s_scan[1][i];
-        }
-        at += __popcll(bs & ((1ull << lane) - 1));
+        scan(s_scan[1], before, total);
+        const int at = out + before + __popcll(bs & below);
         if (stay) index[at] = j, kept[at] = x;
-        ties += all_ties;
-        out += all_out;
-        __syncthreads();
-    }
+        out += total;
+    });
     for (int i = out + tid; i < a.keep; i += kSelect) index[i] = -1, kept[i] = 0.f;
 }
 
-// Moves the kept vectors to the new pages: 16 threads per token's key and
-// value vectors.
+// Moves the kept vectors to the new pages: 8 threads a token, 4 for its key's
+// codes and 4 for its value's; 4 tokens a thread, whose loads are in flight
+// together.
+template <int DP>
 __global__ __launch_bounds__(256) void kv_move_kernel(EvictArgs a) {
+    constexpr int NB = DP / 8, NW = NB / 4;  // bytes and words of codes of a thread
+    typedef uint32_t Words __attribute__((ext_vector_type(NW)));
     const Pool &p = a.p;
-    const int per = (a.keep + 15) / 16;
+    const int per = (a.keep + 127) / 128;
     const int bh = blockIdx.x / per, b = bh / p.kv_heads, h = bh - b * p.kv_heads;
-    const int to = (blockIdx.x - bh * per) * 16 + (threadIdx.x >> 4), c = threadIdx.x & 15;
-    if (to >= min(a.keep, a.out_max_pages << p.page_shift)) return;
-    const int from = a.index[(int64_t)bh * a.keep + to];
-    if (from < 0) return;
-    const int sp = p.page_of(b, from), dp = a.out_table[(int64_t)b * a.out_max_pages + (to >> p.page_shift)];
-    if (sp < 0 || (uint32_t)dp >= (uint32_t)p.pages) return;
-    const int64_t sv = p.vec(sp, h, from), dv = p.vec(dp, h, to);
-    const int words = p.dim / 8;  // of codes; scales: dim / 32 bytes
-    if (c < words) {
-        ((uint32_t *)p.kc)[dv * words + c] = ((const uint32_t *)p.kc)[sv * words + c];
-        ((uint32_t *)p.vc)[dv * words + c] = ((const uint32_t *)p.vc)[sv * words + c];
+    const int c = threadIdx.x & 3, is_v = (threadIdx.x >> 2) & 1, to0 = (blockIdx.x - bh * per) * 128 + (threadIdx.x >> 3);
+    uint8_t *codes = is_v ? p.vc : p.kc, *scale = is_v ? p.vs : p.ks;
+    int64_t src[4], dst[4];
+    Words w[4];
+    uint32_t e[4];
+    int from[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int to = to0 + i * 32;
+        from[i] = to < min(a.keep, a.out_max_pages << p.page_shift) ? a.index[(int64_t)bh * a.keep + to] : -1;
     }
-    if (c < p.dim / 32) {
-        p.ks[dv * (p.dim / 32) + c] = p.ks[sv * (p.dim / 32) + c];
-        p.vs[dv * (p.dim / 32) + c] = p.vs[sv * (p.dim / 32) + c];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int to = to0 + i * 32;
+        const int sp = from[i] >= 0 ? p.page_of(b, from[i]) : -1;
+        const int dp = from[i] >= 0 ? a.out_table[(int64_t)b * a.out_max_pages + (to >> p.page_shift)] : -1;
+        src[i] = sp >= 0 && (uint32_t)dp < (uint32_t)p.pages ? p.vec(sp, h, from[i]) : -1;
+        dst[i] = p.vec(max(dp, 0), h, to);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (src[i] < 0) continue;
+        w[i] = *(const Words *)(codes + src[i] * (DP / 2) + c * NB);
+        if (c == 0) e[i] = DP == 128 ? *(const uint32_t *)(scale + src[i] * 4) : *(const uint16_t *)(scale + src[i] * 2);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (src[i] < 0) continue;
+        *(Words *)(codes + dst[i] * (DP / 2) + c * NB) = w[i];
+        if (c == 0) {
+            if constexpr (DP == 128)
+                *(uint32_t *)(scale + dst[i] * 4) = e[i];
+            else
+                *(uint16_t *)(scale + dst[i] * 2) = (uint16_t)e[i];
+        }
     }
 }
 
@@ -750,9 +818,18 @@ hipError_t launch_kv_weights(const AttendArgs &x, int dtype, hipStream_t s) {
 }
 
 hipError_t launch_kv_evict(const EvictArgs &a, hipStream_t s) {
-    const int bh = a.batch * a.p.kv_heads;
-    kv_select_kernel<<<(unsigned)bh, kSelect, 0, s>>>(a);
-    kv_move_kernel<<<(unsigned)((a.keep + 15) / 16) * bh, 256, 0, s>>>(a);
+    const int bh = a.batch * a.p.kv_heads, cap = a.p.max_pages << a.p.page_shift;
+    if (cap <= 8 * kSelect)
+        kv_select_kernel<8><<<(unsigned)bh, kSelect, 0, s>>>(a);
+    else if (cap <= 32 * kSelect)
+        kv_select_kernel<32><<<(unsigned)bh, kSelect, 0, s>>>(a);
+    else
+        kv_select_kernel<0><<<(unsigned)bh, kSelect, 0, s>>>(a);
+    const unsigned grid = (unsigned)((a.keep + 127) / 128) * bh;
+    if (a.p.dim == 64)
+        kv_move_kernel<64><<<grid, 256, 0, s>>>(a);
+    else
+        kv_move_kernel<128><<<grid, 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
