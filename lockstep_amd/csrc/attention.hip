@@ -56,7 +56,7 @@ struct DenseKV {
     }
     LSMX_DEV void fetch(const T *x, int64_t x_t, int j0, T *to, int dim) {
         const v4i_rsrc rs = buf_rsrc(x + j0 * x_t, 0x7FFFFFFF);
-        const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+        const int wave = uniform((threadIdx.x >> 6) % NW), lane = threadIdx.x & 63;
         const uint32_t lds = lds_u32(to);
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
@@ -101,7 +101,7 @@ struct PagedKV {
         return true;
     }
     LSMX_DEV void init(const Args &a, const Seq &s, int hkv) {
-        p = &a.p, b = s.b, h = hkv, k_len = s.k_len, row = threadIdx.x >> 2, part = threadIdx.x & 3;
+        p = &a.p, b = s.b, h = hkv, k_len = s.k_len, row = (threadIdx.x & 255) >> 2, part = threadIdx.x & 3;
     }
     LSMX_DEV int page(int j0) const {
         const int j = j0 + row;
@@ -166,8 +166,8 @@ struct PagedKV {
 // a step is 32 keys).  2 x 4096 tokens, 32/8 heads of 128, window 1024: 184 us
 // = 656 TFLOP/s of the visible pairs; 16384 tokens of 8/1 heads of 64 through a
 // window of 4096: 227 us.
-template <typename TQ, typename T, int DP, int RT, int NW, typename KV>
-__global__ __launch_bounds__(NW * 64, KV::kHoles ? (DP == 64 ? 2 : 1) : (DP == 64 ? 3 : 2)) void attn_fwd_kernel(typename KV::Args args) {
+template <typename TQ, typename T, int DP, int RT, int NW, int KS, typename KV>
+__global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (DP == 64 ? 3 : 2)) void attn_fwd_kernel(typename KV::Args args) {
     constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, NT = __is_same(TQ, T) ? 1 : 2, BM = NW * RT * 16;
     // a row's maximum is followed only when it grows by a factor of 2^8: the
     // probabilities stay below 2^8 and O is rescaled a few times per row
@@ -176,8 +176,8 @@ __global__ __launch_bounds__(NW * 64, KV::kHoles ? (DP == 64 ? 2 : 1) : (DP == 6
     typedef typename Vec<T>::x4 X4;
     typedef typename Vec<TQ>::x8 Q8;
     typedef typename Vec<TQ>::x4 Q4;
-    __shared__ __attribute__((aligned(16))) T sk[2][kBN * DP], sv[2][kBN * DP];
-    __shared__ int s_in[2][KV::kHoles ? kBN : 1];
+    __shared__ __attribute__((aligned(16))) T s_kv[KS][2][2][kBN * DP];  // [group][keys, values][buffer]
+    __shared__ int s_held[KS][2][KV::kHoles ? kBN : 1];
 
     const AttnArgs &a = KV::attn(args);
     const int item = xcd_item(blockIdx.x, a.per);
@@ -186,7 +186,10 @@ __global__ __launch_bounds__(NW * 64, KV::kHoles ? (DP == 64 ? 2 : 1) : (DP == 6
     Seq s;
     if (!KV::find(args, item % a.tiles, BM, s)) return;
 
-    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
+    const int lane = threadIdx.x & 63, wave = uniform((threadIdx.x >> 6) % NW), g = lane >> 4, r = lane & 15;
+    const int group = KS == 1 ? 0 : uniform(threadIdx.x / (NW * 64));
+    T(&sk)[2][kBN * DP] = s_kv[group][0], (&sv)[2][kBN * DP] = s_kv[group][1];
+    auto &s_in = s_held[group];
     const int row0 = s.tile * BM, rows = s.q_len * a.group, wrow0 = row0 + wave * RT * 16;
 
     // the keys that some row of the tile sees: the sinks, then [lo, hi)
@@ -194,17 +197,20 @@ __global__ __launch_bounds__(NW * 64, KV::kHoles ? (DP == 64 ? 2 : 1) : (DP == 6
     const int pmax = div_by(min(row0 + BM, rows) - 1, a.by_group) + s.shift;
     const int hi = min(pmax + 1, s.k_len), lo = a.window ? max(0, pmin - a.window + 1) : 0;
     const int t_sink = (min(a.sinks, hi) + kBN - 1) / kBN, t_hi = hi > 0 ? (hi + kBN - 1) / kBN : 0;
-    const int t_lo = lo / kBN;
-    auto next = [&](int t) { return t + 1 < t_sink ? t + 1 : max(t + 1, t_lo); };
-    int t = t_sink > 0 ? 0 : t_lo, tn = next(t);
+    const int t_lo = max(lo / kBN, t_sink), nt = t_sink + max(0, t_hi - t_lo), rounds = (nt + KS - 1) / KS;
+    // first key of the group's tile of round k, -1 past the last
+    auto start_of = [&](int k) {
+        const int i = k * KS + group;
+        return i < nt ? (i < t_sink ? i : t_lo + i - t_sink) * kBN : -1;
+    };
     // and the positions of this wave's rows
     const int wmin = div_by(min(wrow0, rows - 1), a.by_group) + s.shift;
     const int wmax = div_by(min(wrow0 + RT * 16, rows) - 1, a.by_group) + s.shift;
 
     KV kv;
     kv.init(args, s, hkv);
-    auto start_of = [&](int t) { return t < t_hi ? t * kBN : -1; };
-    if (t < t_hi) kv.start(t * kBN, start_of(tn), start_of(next(tn)), sk[0], sv[0], s_in[0], a.dim);
+    int j0 = start_of(0);
+    if (j0 >= 0) kv.start(j0, start_of(1), start_of(2), sk[0], sv[0], s_in[0], a.dim);
 
     // this lane's rows: wrow0 + r + 16 x
     int pos[RT], low[RT];
@@ -307,7 +313,7 @@ __global__ __launch_bounds__(NW * 64, KV::kHoles ? (DP == 64 ? 2 : 1) : (DP == 6
             }
         }
         int lr = r;
-        asm volatile("" : "+v"(lr));
+        if constexpr (DP == 128 && !KV::kHoles) asm volatile("" : "+v"(lr));
         X8 vf[ND];
         const int j = jv + g * 4 + (lr >> 2);
 #pragma unroll
@@ -349,29 +355,56 @@ __global__ __launch_bounds__(NW * 64, KV::kHoles ? (DP == 64 ? 2 : 1) : (DP == 6
 
     wait_dma();
     __syncthreads();
-    if (t < t_hi) {
+    if (j0 >= 0) {
         scores(sk[0], 0, r, st);
-        hide(t * kBN, s_in[0], st);
+        hide(j0, s_in[0], st);
     }
-    int n = 0;  // tile t is in buffer n
-    while (t < t_hi) {
-        const bool more = tn < t_hi;
-        if (more) {
-            const int t2 = next(tn);
-            kv.fetch(tn * kBN, start_of(t2), start_of(next(t2)), sk[n ^ 1], sv[n ^ 1], s_in[n ^ 1], a.dim);
+    int n = 0;  // the round's tile is in buffer n
+    for (int k = 0; k < rounds; ++k) {
+        const int j1 = start_of(k + 1);
+        if (j1 >= 0) kv.fetch(j1, start_of(k + 2), start_of(k + 3), sk[n ^ 1], sv[n ^ 1], s_in[n ^ 1], a.dim);
+        if (j0 >= 0) {
+            step(BoolC<true>{}, sk[n], 32, sv[n], 0);
+            hide(j0 + 32, s_in[n] + (KV::kHoles ? 32 : 0), st);
         }
-        step(BoolC<true>{}, sk[n], 32, sv[n], 0);
-        hide(t * kBN + 32, s_in[n] + (KV::kHoles ? 32 : 0), st);
-        if (more) {
-            kv.land();
-            __syncthreads();
+        if (j1 >= 0) kv.land();
+        if (k + 1 < rounds) __syncthreads();
+        if (j1 >= 0) {
             step(BoolC<true>{}, sk[n ^ 1], 0, sv[n], 32);
-            hide(tn * kBN, s_in[n ^ 1], st);
-            __syncthreads();
-        } else {
+            hide(j1, s_in[n ^ 1], st);
+        } else if (j0 >= 0) {
             step(BoolC<false>{}, sk[0], 0, sv[n], 32);
         }
-        n ^= 1, t = tn, tn = next(tn);
+        if (k + 1 < rounds) __syncthreads();
+        n ^= 1, j0 = j1;
+    }
+
+    if constexpr (KS == 2) {
+        // the second group's sums through LDS to the first, which writes
+        static_assert(NW * 64 * RT * ND * 16 + NW * 64 * RT * 8 <= sizeof(s_kv), "");
+        float *x_o = (float *)&s_kv, *x_m = x_o + NW * 64 * RT * ND * 4;
+        const int me = wave * 64 + lane;
+        __syncthreads();
+        if (group == 1) {
+#pragma unroll
+            for (int x = 0; x < RT; ++x) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d) *(f32x4 *)(x_o + ((x * ND + d) * NW * 64 + me) * 4) = o[d][x];
+                x_m[(x * 2) * NW * 64 + me] = m[x], x_m[(x * 2 + 1) * NW * 64 + me] = l[x];
+            }
+        }
+        __syncthreads();
+        if (group == 1) return;
+#pragma unroll
+        for (int x = 0; x < RT; ++x) {
+            const float m2 = x_m[(x * 2) * NW * 64 + me], l2 = x_m[(x * 2 + 1) * NW * 64 + me], top = fmaxf(m[x], m2);
+            const float f1 = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[x] - top) * a.c);
+            const float f2 = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m2 - top) * a.c);
+            m[x] = top;
+            l[x] = l[x] * f1 + l2 * f2;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d][x] = o[d][x] * f1 + *(f32x4 *)(x_o + ((x * ND + d) * NW * 64 + me) * 4) * f2;
+        }
     }
 
 #pragma unroll
@@ -402,8 +435,9 @@ __global__ __launch_bounds__(NW * 64, KV::kHoles ? (DP == 64 ? 2 : 1) : (DP == 6
     }
 }
 
-#ifndef FEW
-#define FEW 512
+#ifndef F1
+#define F1 4096
+#define F2 2048
 #endif
 // Row tiles over all sequences, and the grid of their items over 8 XCDs.
 void tiles_of(AttnArgs &a, int rows) {
@@ -417,33 +451,39 @@ void tiles_of(AttnArgs &a, int rows) {
 // Workgroups of 4 waves: two or three of them on a CU run out of step, and one's
 // products fall into another's exponentials.  (8 waves that share their tiles
 // were in step: 201 against 179 us at 2 x 4096 tokens, 32/8 heads of 128.)
-// 32 rows a wave, or 16 where 32 would leave CUs with less than two workgroups.
-bool few(const AttnArgs &a) {
-    const int64_t rows = (int64_t)(a.offsets ? a.tokens : a.q_len) * a.group * (a.offsets ? 1 : a.batch);
-    return rows * a.kv_heads < FEW * 128;
+// Few rows leave SIMDs with less than two such waves: then 16 rows a wave, and
+// below that the keys in two halves, each with 4 waves of the workgroup.
+enum Form { kWide, kNarrow, kHalves };
+Form form_of(const AttnArgs &a) {
+    const int64_t waves = (int64_t)(a.offsets ? a.tokens : a.q_len) * a.group * (a.offsets ? 1 : a.batch) * a.kv_heads / 16;
+    return waves >= F1 ? kWide : waves >= F2 ? kNarrow : kHalves;
 }
 
 template <typename T, int DP>
 hipError_t fwd(AttnArgs a, hipStream_t s) {
-    if (few(a)) {
-        tiles_of(a, 64);
-        attn_fwd_kernel<T, T, DP, 1, 4, DenseKV<T, DP, 4>><<<(unsigned)a.per * 8, 256, 0, s>>>(a);
-    } else {
-        tiles_of(a, 128);
-        attn_fwd_kernel<T, T, DP, 2, 4, DenseKV<T, DP, 4>><<<(unsigned)a.per * 8, 256, 0, s>>>(a);
-    }
+    const Form f = form_of(a);
+    tiles_of(a, f == kWide ? 128 : 64);
+    const unsigned grid = (unsigned)a.per * 8;
+    if (f == kWide)
+        attn_fwd_kernel<T, T, DP, 2, 4, 1, DenseKV<T, DP, 4>><<<grid, 256, 0, s>>>(a);
+    else if (f == kNarrow)
+        attn_fwd_kernel<T, T, DP, 1, 4, 1, DenseKV<T, DP, 4>><<<grid, 256, 0, s>>>(a);
+    else
+        attn_fwd_kernel<T, T, DP, 1, 4, 2, DenseKV<T, DP, 4>><<<grid, 512, 0, s>>>(a);
     return hipGetLastError();
 }
 
 template <typename T, int DP>
 hipError_t chunk(AttendArgs x, hipStream_t s) {
-    if (few(x.a)) {
-        tiles_of(x.a, 64);
-        attn_fwd_kernel<T, __bf16, DP, 1, 4, PagedKV<DP>><<<(unsigned)x.a.per * 8, 256, 0, s>>>(x);
-    } else {
-        tiles_of(x.a, 128);
-        attn_fwd_kernel<T, __bf16, DP, 2, 4, PagedKV<DP>><<<(unsigned)x.a.per * 8, 256, 0, s>>>(x);
-    }
+    const Form f = form_of(x.a);
+    tiles_of(x.a, f == kWide ? 128 : 64);
+    const unsigned grid = (unsigned)x.a.per * 8;
+    if (f == kWide)
+        attn_fwd_kernel<T, __bf16, DP, 2, 4, 1, PagedKV<DP>><<<grid, 256, 0, s>>>(x);
+    else if (f == kNarrow)
+        attn_fwd_kernel<T, __bf16, DP, 1, 4, 1, PagedKV<DP>><<<grid, 256, 0, s>>>(x);
+    else
+        attn_fwd_kernel<T, __bf16, DP, 1, 4, 2, PagedKV<DP>><<<grid, 512, 0, s>>>(x);
     return hipGetLastError();
 }
 

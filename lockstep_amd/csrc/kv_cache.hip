@@ -501,9 +501,9 @@ __global__ __launch_bounds__(256) void kv_weights_kernel(AttendArgs x) {
 // Many rows: a workgroup owns 64 keys, whose operands stay in registers, and
 // its waves take tiles of 16 rows in turn; their sums are joined in LDS.
 template <typename TQ, int DP>
-__global__ __launch_bounds__(256) void kv_weights_rows_kernel(AttendArgs x) {
+__global__ __launch_bounds__(512) void kv_weights_rows_kernel(AttendArgs x) {
     constexpr int NS = DP / 32, NT = __is_same(TQ, __bf16) ? 1 : 2;
-    __shared__ __attribute__((aligned(16))) float s_sum[4][64];
+    __shared__ __attribute__((aligned(16))) float s_sum[8][64];
     const AttnArgs &a = x.a;
     const Pool &p = x.p;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
@@ -532,8 +532,13 @@ __global__ __launch_bounds__(256) void kv_weights_rows_kernel(AttendArgs x) {
         for (int s = 0; s < NS; ++s) kf[t][s] = fp4x8_to_bf16(k.w[s], e8m0_to_f32(k.e));
     }
     f32x4 sum[4];
+    uint32_t span[4][4];  // position p sees key j when 0 <= p - j <= span
 #pragma unroll
-    for (int t = 0; t < 4; ++t) sum[t] = f32x4{0, 0, 0, 0};
+    for (int t = 0; t < 4; ++t) {
+        sum[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) span[t][e] = a.window && j0 + t * 16 + g * 4 + e >= a.sinks ? a.window - 1 : 0x7FFFFFFF;
+    }
     const int row_hi = tok_hi * a.group;
     // U tiles of rows at a time, the next U in flight: one tile's work is less
     // than a load's latency
@@ -546,7 +551,7 @@ __global__ __launch_bounds__(256) void kv_weights_rows_kernel(AttendArgs x) {
     auto load = [&](int r0, Row (&w)[U]) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int row = r0 + u * 64 + r;
+            const int row = r0 + u * 128 + r;
             const bool in = row < row_hi;
             const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
             const TQ *qp = (const TQ *)a.q + b * a.q_b + tok * a.q_t + h * a.q_h + g * (DP / 4);
@@ -559,11 +564,10 @@ __global__ __launch_bounds__(256) void kv_weights_rows_kernel(AttendArgs x) {
     Row cur[U], nxt[U];
     int r0 = tok_lo * a.group + wave * 16;
     load(r0, cur);
-    for (; r0 < row_hi; r0 += 64 * U) {
-        load(r0 + 64 * U, nxt);
+    for (; r0 < row_hi; r0 += 128 * U) {
+        load(r0 + 128 * U, nxt);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int low = window_low(cur[u].pos, a.window);
             bf16x8 q[NT][NS];
 #pragma unroll
             for (int s = 0; s < NS; ++s)
@@ -581,7 +585,7 @@ __global__ __launch_bounds__(256) void kv_weights_rows_kernel(AttendArgs x) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(st[e], a.c, -cur[u].lse));
-                    sum[t][e] += sees(j0 + t * 16 + g * 4 + e, cur[u].pos, low, a.sinks) ? v : 0.f;
+                    sum[t][e] += (uint32_t)(cur[u].pos - (j0 + t * 16 + g * 4 + e)) <= span[t][e] ? v : 0.f;
                 }
             }
             cur[u] = nxt[u];
@@ -596,8 +600,12 @@ __global__ __launch_bounds__(256) void kv_weights_rows_kernel(AttendArgs x) {
         }
     __syncthreads();
     const int at = j0 + threadIdx.x;
-    if (threadIdx.x < 64 && at < len)
-        x.weights[(int64_t)bh * x.w_len + at] += s_sum[0][threadIdx.x] + s_sum[1][threadIdx.x] + s_sum[2][threadIdx.x] + s_sum[3][threadIdx.x];
+    if (threadIdx.x < 64 && at < len) {
+        float all = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) all += s_sum[i][threadIdx.x];
+        x.weights[(int64_t)bh * x.w_len + at] += all;
+    }
 }
 
 // ------------------------------------------------------------------ eviction
@@ -778,7 +786,7 @@ hipError_t weights(AttendArgs x, hipStream_t s) {
     else if (rows <= kDecodeRows)
         kv_weights_kernel<TQ, DP, 4><<<grid, 256, 0, s>>>(x);
     else
-        kv_weights_rows_kernel<TQ, DP><<<(unsigned)(((x.p.max_pages << x.p.page_shift) + 63) / 64) * bh, 256, 0, s>>>(x);
+        kv_weights_rows_kernel<TQ, DP><<<(unsigned)(((x.p.max_pages << x.p.page_shift) + 63) / 64) * bh, 512, 0, s>>>(x);
     return hipGetLastError();
 }
 
