@@ -120,6 +120,8 @@ def sink_window_attention(q, k, v, *, window=None, sinks=0, scale=None, offsets=
     for the matrix products.  Deterministic.  With return_lse also the natural
     log of each row's softmax sum, fp32 [B, H, Tq] or [H, N] (-inf for a row
     that sees nothing; not differentiable)."""
+    if not return_lse and (r := C.fast.attention(q, k, v, offsets, window, sinks, scale)) is not None:
+        return r
     if torch.is_autocast_enabled("cuda"):
         dt = torch.get_autocast_dtype("cuda")
         q, k, v = q.to(dt), k.to(dt), v.to(dt)

@@ -19,9 +19,14 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <ATen/autocast_mode.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <cmath>
 
 #include "../../include/lsmx.h"
 
@@ -441,6 +446,297 @@ PyObject *gemm_fp8(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// -------------------------------------------------------------- attention
+// What the attention kernels read in place: unit stride along the last axis, 16-byte
+// aligned vectors, tokens and the heads of a group within 32-bit offsets.
+bool in_reach(const Tensor &t, int64_t group) {
+    const int64_t d = t.dim();
+    if (t.numel() == 0 || t.stride(d - 1) != 1 || !al(t, 16)) return false;
+    for (int64_t i = 0; i < d - 1; ++i)
+        if (t.size(i) > 1 && t.stride(i) % 8) return false;
+    return (t.size(d - 3) <= 1 || t.stride(d - 3) < (1 << 22)) && (t.size(d - 2) <= 1 || t.stride(d - 2) * group < (1 << 29));
+}
+void strides_of(const Tensor &t, int64_t *s) {
+    const int64_t d = t.dim();
+    for (int i = 0; i < 3; ++i) {
+        const int64_t k = d - 4 + i;
+        s[i] = k >= 0 && t.size(k) > 1 ? t.stride(k) : 0;
+    }
+}
+bool bf16_or_f16(const Tensor &t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
+// an int >= lo, or None as 0
+bool int_arg(PyObject *o, int64_t lo, bool none, int64_t &v) {
+    if (none && o == Py_None) {
+        v = 0;
+        return true;
+    }
+    if (!PyLong_CheckExact(o)) return false;
+    int over = 0;
+    v = PyLong_AsLongLongAndOverflow(o, &over);
+    return !over && v >= lo;
+}
+// scale, or None as 1 / sqrt(D); positive and finite
+bool scale_arg(PyObject *o, int64_t D, double &v) {
+    if (o == Py_None)
+        v = 1.0 / std::sqrt((double)D);
+    else if (PyFloat_CheckExact(o))
+        v = PyFloat_AS_DOUBLE(o);
+    else
+        return false;
+    return v > 0.0 && v <= 3.0e38;
+}
+bool int32_on(const Tensor *t, const Tensor &like, int64_t dims) {
+    return t && t->scalar_type() == at::kInt && t->dim() == dims && t->is_contiguous() && t->device() == like.device();
+}
+
+struct Failed {
+    int rc;
+};
+
+lsmx_attention attention_args(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &o, const Tensor &rest,
+                              const Tensor &lse, const Tensor &offsets, int64_t window, int64_t sinks, double scale) {
+    lsmx_attention a{};
+    a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr(), a.o = o.data_ptr();
+    a.o_rest = rest.defined() ? rest.data_ptr() : nullptr;
+    a.lse = lse.data_ptr<float>();
+    a.dtype = dtype_of(q.scalar_type());
+    const int64_t d = q.dim();
+    a.batch = offsets.defined() ? offsets.numel() - 1 : q.size(0);
+    a.q_len = q.size(d - 3), a.k_len = k.size(d - 3), a.heads = q.size(d - 2), a.kv_heads = k.size(d - 2);
+    a.head_dim = q.size(d - 1);
+    strides_of(q, a.q_stride), strides_of(k, a.k_stride), strides_of(v, a.v_stride), strides_of(o, a.o_stride);
+    a.offsets = offsets.defined() ? offsets.data_ptr<int32_t>() : nullptr;
+    a.window = window, a.sinks = sinks, a.scale = (float)scale;
+    return a;
+}
+
+struct Forward {
+    Tensor o, rest, lse;
+};
+Forward attention_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &offsets, int64_t window,
+                          int64_t sinks, double scale, bool grad) {
+    Forward f;
+    const int64_t d = q.dim();
+    f.o = make(q.sizes(), q.scalar_type(), q);
+    if (grad) f.rest = make(q.sizes(), q.scalar_type(), q);
+    f.lse = d == 4 ? make({q.size(0), q.size(2), q.size(1)}, at::kFloat, q) : make({q.size(1), q.size(0)}, at::kFloat, q);
+    const lsmx_attention a = attention_args(q, k, v, f.o, f.rest, f.lse, offsets, window, sinks, scale);
+    if (const int rc = lsmx_attention_fwd(&a, stream_of(q))) throw Failed{rc};
+    return f;
+}
+
+// The same node as attention._SinkWindowAttention, in native code.
+struct Attention : torch::autograd::Function<Attention> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v,
+                          const std::optional<Tensor> &offsets, int64_t window, int64_t sinks, double scale) {
+        const Tensor off = offsets ? *offsets : Tensor();
+        const Forward f = attention_forward(q, k, v, off, window, sinks, scale, true);
+        ctx->save_for_backward({q, k, v, f.o, f.rest, f.lse, off});
+        ctx->saved_data["window"] = window;
+        ctx->saved_data["sinks"] = sinks;
+        ctx->saved_data["scale"] = scale;
+        return f.o;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        const auto s = ctx->get_saved_variables();
+        const Tensor &q = s[0], &k = s[1], &v = s[2];
+        std::vector<Tensor> d(3);
+        {
+            at::AutoGradMode off(false);
+            Tensor d_o = grads[0].defined() ? grads[0].to(q.scalar_type()) : at::zeros_like(q);
+            const int64_t group = q.size(-2) / k.size(-2);
+            if (!in_reach(d_o, group)) {
+                d_o = d_o.contiguous();
+                if (!al(d_o, 16)) d_o = d_o.clone();
+            }
+            for (int i = 0; i < 3; ++i) d[i] = make(s[i].sizes(), q.scalar_type(), q);
+            const lsmx_attention a = attention_args(q, k, v, s[3], s[4], s[5], s[6], ctx->saved_data["window"].toInt(),
+                                                    ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble());
+            const int64_t n = lsmx_attention_workspace(&a);
+            const Tensor ws = make({n}, at::kByte, q);
+            int64_t st[3];
+            strides_of(d_o, st);
+            TORCH_CHECK(lsmx_attention_bwd(&a, d_o.data_ptr(), st, d[0].data_ptr(), d[1].data_ptr(), d[2].data_ptr(),
+                                           ws.data_ptr(), n, stream_of(q)) == LSMX_OK,
+                        lsmx_last_error());
+        }
+        if (at::GradMode::is_enabled()) {  // create_graph: the gradients have none
+            auto err = std::make_shared<torch::autograd::DelayedError>(
+                "trying to differentiate twice a function that was marked with @once_differentiable", 3);
+            torch::autograd::variable_list in;
+            for (auto &t : d) in.push_back(t.detach().set_requires_grad(true));
+            d = (*err)(std::move(in));
+        }
+        return {d[0], d[1], d[2], Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// attention(q, k, v, offsets, window, sinks, scale) -> o
+PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    NONE_IF(n != 7);
+    const Tensor *q = plain(a[0]), *k = plain(a[1]), *v = plain(a[2]), *off = a[3] == Py_None ? nullptr : plain(a[3]);
+    NONE_IF(!q || !k || !v || (a[3] != Py_None && !off) || at::autocast::is_autocast_enabled(at::kCUDA));
+    const int64_t d = off ? 3 : 4;
+    NONE_IF(q->dim() != d || k->dim() != d || !k->sizes().equals(v->sizes()) || !bf16_or_f16(*q) ||
+            k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type() || k->device() != q->device() ||
+            v->device() != q->device() || (off && !int32_on(off, *q, 1)));
+    const int64_t H = q->size(d - 2), Hkv = k->size(d - 2), D = q->size(d - 1);
+    NONE_IF(q->numel() == 0 || k->numel() == 0 || k->size(0) != q->size(0) || k->size(d - 1) != D || H % Hkv || D % 8 ||
+            D > 128 || (off && off->numel() < 1) || !in_reach(*q, H / Hkv) || !in_reach(*k, 1) || !in_reach(*v, 1));
+    int64_t window, sinks;
+    double scale;
+    NONE_IF(!int_arg(a[4], 1, true, window) || !int_arg(a[5], 0, false, sinks) || !scale_arg(a[6], D, scale));
+    const Tensor none, &offsets = off ? *off : none;
+    const bool grad = at::GradMode::is_enabled() && (q->requires_grad() || k->requires_grad() || v->requires_grad());
+    Tensor o;
+    int rc = LSMX_OK;
+    {
+        NoGil released;
+        try {
+            o = grad ? Attention::apply(*q, *k, *v, off ? std::optional<Tensor>(*off) : std::nullopt, window, sinks, scale)
+                     : attention_forward(*q, *k, *v, offsets, window, sinks, scale, false).o;
+        } catch (const Failed &f) {
+            rc = f.rc;
+        }
+    }
+    if (rc != LSMX_OK) {
+        Py_XDECREF(PyObject_CallFunction(g_error, "i", rc));
+        return nullptr;
+    }
+    return THPVariable_Wrap(o);
+    END_HANDLE_TH_ERRORS
+}
+
+// -------------------------------------------------------------- cache
+// The cache of kv_cache._cache, or false for any form that it would refuse.
+bool cache_of(PyObject *pages, PyObject *table, PyObject *lengths, lsmx_kv_cache &c, const Tensor *&like) {
+    if (!PyTuple_Check(pages) || PyTuple_GET_SIZE(pages) != 4) return false;
+    const Tensor *p[4], *t = plain(table), *l = plain(lengths);
+    for (int i = 0; i < 4; ++i)
+        if (!(p[i] = plain(PyTuple_GET_ITEM(pages, i))) || p[i]->scalar_type() != at::kByte || p[i]->dim() != 4 ||
+            !p[i]->is_contiguous() || p[i]->numel() == 0)
+            return false;
+    const int64_t n = p[0]->size(0), h = p[0]->size(1), page = p[0]->size(2), D = 2 * p[0]->size(3);
+    const int64_t want[4] = {n, h, page, D / 32};
+    if ((D != 64 && D != 128) || page < 16 || page > 1024 || (page & (page - 1)) || !p[2]->sizes().equals(p[0]->sizes()) ||
+        !p[1]->sizes().equals(want) || !p[3]->sizes().equals(want))
+        return false;
+    like = p[0];
+    for (int i = 0; i < 4; ++i)
+        if (p[i]->device() != like->device() || !al(*p[i], 16)) return false;
+    if (!int32_on(t, *like, 2) || !int32_on(l, *like, 1) || l->size(0) != t->size(0) || t->numel() == 0) return false;
+    c = lsmx_kv_cache{p[0]->data_ptr<uint8_t>(), p[1]->data_ptr<uint8_t>(), p[2]->data_ptr<uint8_t>(), p[3]->data_ptr<uint8_t>(),
+                      n, page, h, D, t->data_ptr<int32_t>(), l->data_ptr<int32_t>(), t->size(0), t->size(1)};
+    return true;
+}
+// weights as kv_cache._check_weights wants them
+bool weights_ok(const Tensor *w, const lsmx_kv_cache &c, const Tensor &like) {
+    return w && w->scalar_type() == at::kFloat && w->is_contiguous() && w->dim() == 3 && w->size(0) == c.batch &&
+           w->size(1) == c.kv_heads && w->size(2) >= c.max_pages * c.page && w->device() == like.device();
+}
+
+// kv_append(pages, k, v, table, lengths, offsets, values) -> (k, v), or True
+PyObject *kv_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    NONE_IF(n != 7);
+    lsmx_kv_cache c;
+    const Tensor *like, *k = plain(a[1]), *v = plain(a[2]), *off = a[5] == Py_None ? nullptr : plain(a[5]);
+    NONE_IF(!k || !v || (a[5] != Py_None && !off) || !cache_of(a[0], a[3], a[4], c, like));
+    const int64_t d = off ? 3 : 4;
+    NONE_IF(k->dim() != d || !k->sizes().equals(v->sizes()) || !bf16_or_f16(*k) || v->scalar_type() != k->scalar_type() ||
+            k->device() != like->device() || v->device() != like->device() || k->size(d - 2) != c.kv_heads ||
+            k->size(d - 1) != c.head_dim || (off ? !int32_on(off, *like, 1) || off->size(0) != c.batch + 1 : k->size(0) != c.batch) ||
+            k->numel() == 0);
+    int64_t st[2][2];
+    const Tensor *kv[2] = {k, v};
+    for (int i = 0; i < 2; ++i) {
+        const Tensor &t = *kv[i];
+        NONE_IF(t.stride(d - 1) != 1 || !al(t, 16) || (t.size(d - 2) > 1 && t.stride(d - 2) % 8) ||
+                (t.size(d - 3) > 1 && t.stride(d - 3) % 8));
+        st[i][0] = t.size(d - 3) > 1 ? t.stride(d - 3) : d == 4 ? t.stride(0) : 0;
+        st[i][1] = t.size(d - 2) > 1 ? t.stride(d - 2) : 0;
+        // the sequences of a dense call one after another
+        NONE_IF(d == 4 && t.size(0) > 1 && (st[i][0] % 8 || t.stride(0) != st[i][0] * t.size(1)));
+    }
+    const bool values = a[6] == Py_True;
+    const int64_t tokens = off ? k->size(0) : k->size(0) * k->size(1);
+    Tensor ko, vo;
+    if (values) ko = make(k->sizes(), at::kBFloat16, *k), vo = make(k->sizes(), at::kBFloat16, *k);
+    void *s = stream_of(*k);
+    if (!launch([&] {
+            return lsmx_kv_append(&c, k->data_ptr(), st[0], v->data_ptr(), st[1], dtype_of(k->scalar_type()), tokens,
+                                  off ? 0 : k->size(1), off ? off->data_ptr<int32_t>() : nullptr,
+                                  values ? ko.data_ptr() : nullptr, values ? vo.data_ptr() : nullptr, s);
+        }))
+        return nullptr;
+    if (values) return wrap2(ko, vo);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// kv_attend(q, pages, table, lengths, window, sinks, scale, weights) -> o
+PyObject *kv_attend(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    NONE_IF(n != 8);
+    lsmx_kv_cache c;
+    const Tensor *like, *q = plain(a[0]), *w = a[7] == Py_None ? nullptr : plain(a[7]);
+    NONE_IF(!q || (a[7] != Py_None && !w) || !cache_of(a[1], a[2], a[3], c, like));
+    NONE_IF(q->dim() != 4 || !bf16_or_f16(*q) || q->device() != like->device() || q->numel() == 0 || q->size(0) != c.batch ||
+            q->size(3) != c.head_dim || q->size(2) % c.kv_heads || (w && !weights_ok(w, c, *like)) || q->stride(3) != 1 || !al(*q, 16));
+    for (int i = 0; i < 3; ++i) NONE_IF(q->size(i) > 1 && q->stride(i) % 8);
+    int64_t window, sinks, st[3];
+    double scale;
+    NONE_IF(!int_arg(a[4], 1, true, window) || !int_arg(a[5], 0, false, sinks) || !scale_arg(a[6], c.head_dim, scale));
+    strides_of(*q, st);
+    const Tensor o = make(q->sizes(), q->scalar_type(), *q);
+    const int64_t T = q->size(1), H = q->size(2), nws = lsmx_kv_attend_workspace(&c, T, H, window, sinks, w != nullptr);
+    PyObject *keep = nullptr;
+    if (nws) {
+        PyObject *dev = PyObject_GetAttrString(a[0], "device");
+        if (!dev) return nullptr;
+        keep = PyObject_CallFunction(g_workspace, "OL", dev, (long long)nws);
+        Py_DECREF(dev);
+        if (!keep) return nullptr;
+    }
+    void *ws = keep ? THPVariable_Unpack(keep).data_ptr() : nullptr, *s = stream_of(*q);
+    const bool ok = launch([&] {
+        return lsmx_kv_attend(&c, q->data_ptr(), st, dtype_of(q->scalar_type()), T, H, window, sinks, (float)scale,
+                              o.data_ptr(), w ? w->data_ptr<float>() : nullptr, w ? w->size(2) : 0, ws, nws, s);
+    });
+    Py_XDECREF(keep);
+    return ok ? THPVariable_Wrap(o) : nullptr;
+    END_HANDLE_TH_ERRORS
+}
+
+// kv_evict(pages, table, lengths, weights, keep, out_table, sinks, recent) -> (index, weights, lengths)
+PyObject *kv_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    NONE_IF(n != 8);
+    lsmx_kv_cache c;
+    const Tensor *like, *w = plain(a[3]), *out = plain(a[5]);
+    int64_t keep, sinks, recent;
+    NONE_IF(!w || !out || !cache_of(a[0], a[1], a[2], c, like) || !weights_ok(w, c, *like) || !int32_on(out, *like, 2) ||
+            !int_arg(a[4], 1, false, keep) || !int_arg(a[6], 0, false, sinks) || !int_arg(a[7], 0, false, recent));
+    const int64_t cap = c.max_pages * c.page, most = keep < cap ? keep : cap;
+    NONE_IF(keep >= (1 << 30) || sinks > keep || recent > keep - sinks || out->size(0) != c.batch || out->size(1) * c.page < most);
+    const Tensor index = make({c.batch, c.kv_heads, keep}, at::kInt, *like), kept = make({c.batch, c.kv_heads, keep}, at::kFloat, *like);
+    const Tensor len = make({c.batch}, at::kInt, *like);
+    void *s = stream_of(*like);
+    if (!launch([&] {
+            return lsmx_kv_evict(&c, w->data_ptr<float>(), w->size(2), keep, sinks, recent, out->data_ptr<int32_t>(),
+                                 out->size(1), index.data_ptr<int32_t>(), kept.data_ptr<float>(), len.data_ptr<int32_t>(), s);
+        }))
+        return nullptr;
+    PyObject *t = PyTuple_New(3);
+    if (!t) return nullptr;
+    PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(index));
+    PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(kept));
+    PyTuple_SET_ITEM(t, 2, THPVariable_Wrap(len));
+    return t;
+    END_HANDLE_TH_ERRORS
+}
+
 // init(check, workspace, next_epoch): the _capi functions the calls above use
 PyObject *init(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (n != 3) {
@@ -458,7 +754,8 @@ PyObject *init(PyObject *, PyObject *const *a, Py_ssize_t n) {
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(init),   FAST(quantize_pack), FAST(quantize_pack2), FAST(quantize), FAST(quantize_2d), FAST(pack),
-                         FAST(gemm_packed), FAST(linear), FAST(weight), FAST(gemm_fp8), {nullptr, nullptr, 0, nullptr}};
+                         FAST(gemm_packed), FAST(linear), FAST(weight), FAST(gemm_fp8),
+                         FAST(attention), FAST(kv_append), FAST(kv_attend), FAST(kv_evict), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -84,6 +84,8 @@ def append(pages, k, v, table, lengths, *, offsets=None, values=False):
     Positions below 0 (padding in front) or past the table are not written.
     The bytes are those of fp4.quantize_pack_mxfp4 on each head's vector.
     With values=True returns (k, v) as now held: bf16, exact."""
+    if (r := C.fast.kv_append(pages, k, v, table, lengths, offsets, values)) is not None:
+        return r if values else None
     c = _cache(pages, table, lengths)
     if k.dtype not in (torch.bfloat16, torch.float16) or v.dtype != k.dtype:
         raise TypeError(f"k and v must share bfloat16 or float16, got {k.dtype}, {v.dtype}")
@@ -127,6 +129,8 @@ def attend(q, pages, table, lengths, *, window=None, sinks=0, scale=None, weight
     weights (fp32 [B, Hkv, >= max_pages * page], contiguous): the softmax
     weight of every key, summed over the T tokens and the heads that share its
     head, is added in place.  Deterministic."""
+    if (r := C.fast.kv_attend(q, pages, table, lengths, window, sinks, scale, weights)) is not None:
+        return r
     c = _cache(pages, table, lengths)
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"q must be bfloat16 or float16, got {q.dtype}")
@@ -173,6 +177,8 @@ def evict(pages, table, lengths, weights, keep, out_table, *, sinks=0, recent=0)
     Returns (index int32 [B, Hkv, keep]: the positions they had, -1 past the
     last; weights fp32 [B, Hkv, keep]: theirs, 0 past the last; lengths int32
     [B]).  Afterwards positions, windows and sinks count the kept tokens."""
+    if (r := C.fast.kv_evict(pages, table, lengths, weights, keep, out_table, sinks, recent)) is not None:
+        return r
     c = _cache(pages, table, lengths)
     C.require_device(weights, out_table)
     _check_weights(weights, c)
