@@ -26,7 +26,6 @@ namespace {
 constexpr int kBM = 128;  // dQ: rows of a workgroup
 constexpr int kBN = 64;   // dQ: keys of a tile
 constexpr int kKM = 128;  // dK, dV: keys of a workgroup
-constexpr int kKN = 64;   // dK, dV: rows of a tile
 constexpr int kFar = 128; // far rows: rows of a tile
 
 // fp16 holds 2^-24 to 65504, and gradients are often small: P enters its
@@ -162,10 +161,13 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
         const T *ck = sk[n], *cv = sv[n];
         auto half = [&](auto all, int u) {
             const int ju = j0 + u * 32;
+            // places in LDS made anew each time: held, they would not fit
+            int lr = r;
+            if constexpr (DP == 128 && Range<T>::on) asm volatile("" : "+v"(lr));
             f32x4 st[2][2], dp[2][2];  // [16 keys][16 rows]
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
-                const int j = u * 32 + w * 16 + r;
+                const int j = u * 32 + w * 16 + lr;
                 st[w][0] = st[w][1] = dp[w][0] = dp[w][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int x = 0; x < NS; ++x) {
@@ -210,19 +212,27 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
                     }
                 }
             }
-            X8 df[2];
+            // bf16: one rounding of dS, as large as that of dQ itself.  fp16: two
+            // terms, for a type that is chosen for its digits
+            X8 df[2], dl[2];
 #pragma unroll
             for (int y = 0; y < 2; ++y)
 #pragma unroll
                 for (int w = 0; w < 2; ++w)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        df[y][w * 4 + i] = (T)(Range<T>::on ? st[w][y][i] * mul[y] : st[w][y][i]);
+                    for (int i = 0; i < 4; ++i) {
+                        const float ds = Range<T>::on ? st[w][y][i] * mul[y] : st[w][y][i];
+                        df[y][w * 4 + i] = (T)ds;
+                        if constexpr (Range<T>::on) dl[y][w * 4 + i] = (T)(ds - (float)df[y][w * 4 + i]);
+                    }
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
-                const X8 kf = columns<T, DP>(ck, u * 32, d, g, r);
-                dq[d][0] = mfma(kf, df[0], dq[d][0]);
-                dq[d][1] = mfma(kf, df[1], dq[d][1]);
+                const X8 kf = columns<T, DP>(ck, u * 32, d, g, lr);
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    dq[d][y] = mfma(kf, df[y], dq[d][y]);
+                    if constexpr (Range<T>::on) dq[d][y] = mfma(kf, dl[y], dq[d][y]);
+                }
             }
         };
 #pragma unroll
@@ -288,12 +298,14 @@ struct Rows {
     }
 };
 
-// 32 rows from row j0 of an LDS tile on against NK x 16 keys in registers.
-template <typename T, int DP, int NK>
+// 32 rows from row j0 of an LDS tile on against NK x 16 keys, whose K is in
+// registers, and V too or (VL) in LDS.
+template <typename T, int DP, int NK, bool VL>
 struct KeySums {
     static constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16;
     typedef typename Vec<T>::x8 X8;
-    X8 kf[NK][NS], vf[NK][NS];
+    X8 kf[NK][NS], vf[VL ? 1 : NK][NS];
+    const T *sv;  // VL: the first key's row of V
     f32x4 dk[ND][NK], dv[ND][NK];
     float mul[NK], limit[NK];
     // position p sees key y of the lane when 0 <= p - key <= span
@@ -318,20 +330,32 @@ struct KeySums {
 #pragma unroll
         for (int y = 0; y < NK; ++y) top[y] = 0.f;
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            const int j = j0 + w * 16 + r;
+        for (int w = 0; w < 2; ++w)
 #pragma unroll
             for (int y = 0; y < NK; ++y) pr[w][y] = ds[w][y] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int x = 0; x < NS; ++x) {
+        for (int x = 0; x < NS; ++x) {
+            X8 v[NK];
+#pragma unroll
+            for (int y = 0; y < NK; ++y)
+                if constexpr (VL)
+                    v[y] = *(const X8 *)(sv + (y * 16 + r) * DP + swz<NC>(y * 16 + r, x * 4 + g) * 8);
+                else
+                    v[y] = vf[y][x];
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const int j = j0 + w * 16 + r;
                 const X8 qf = *(const X8 *)(sq + j * DP + swz<NC>(j, x * 4 + g) * 8);
                 const X8 of = *(const X8 *)(so + j * DP + swz<NC>(j, x * 4 + g) * 8);
 #pragma unroll
                 for (int y = 0; y < NK; ++y) {
                     pr[w][y] = mfma(qf, kf[y][x], pr[w][y]);
-                    ds[w][y] = mfma(of, vf[y][x], ds[w][y]);
+                    ds[w][y] = mfma(of, v[y], ds[w][y]);
                 }
             }
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
             const f32x4 lse = *(const f32x4 *)(s_lse + j0 + w * 16 + g * 4);
             const f32x4 delta = *(const f32x4 *)(s_delta + j0 + w * 16 + g * 4);
             const i32x4 pos = *(const i32x4 *)(s_pos + j0 + w * 16 + g * 4);
@@ -424,7 +448,7 @@ __global__ __launch_bounds__(256) void attn_far_kernel(AttnArgs a) {
     const int row_lo = max(s.tile * a.chunk, first * a.group), row_hi = min((s.tile + 1) * a.chunk, rows);
     if (row_lo >= row_hi) return;
 
-    KeySums<T, DP, 1> sums;
+    KeySums<T, DP, 1, false> sums;
     sums.init(a, key);
     const T *kp = (const T *)a.k + s.b * a.k_b + (s.k0 + key) * a.k_t + hkv * a.k_h;
     const T *vp = (const T *)a.v + s.b * a.v_b + (s.k0 + key) * a.v_t + hkv * a.v_h;
@@ -465,14 +489,17 @@ __global__ __launch_bounds__(256) void attn_far_kernel(AttnArgs a) {
     }
 }
 
-// 320 registers at head 128: one wave per SIMD (held to 256, the spills took
-// 1350 us against 484 at 2 x 4096 tokens, 32/8 heads, window 1024).
+// Head 128: two waves per SIMD only with V in LDS, tiles of 32 rows and the LDS
+// places made anew each time (245 registers; with V in registers 320, one wave
+// per SIMD: 484 us at 2 x 4096 tokens, 32/8 heads, window 1024).
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attn_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
     constexpr int NS = DP / 32, ND = DP / 16;
+    constexpr bool VL = DP == 128;          // V in LDS
+    constexpr int kKN = VL ? 32 : 64;       // rows of a tile
     typedef typename Vec<T>::x8 X8;
     typedef typename Vec<T>::x4 X4;
-    __shared__ __attribute__((aligned(16))) T sq[2][kKN * DP], so[2][kKN * DP];
+    __shared__ __attribute__((aligned(16))) T sq[2][kKN * DP], so[2][kKN * DP], s_v[VL ? kKM * DP : 8];
     __shared__ __attribute__((aligned(16))) float s_lse[2][kKN], s_delta[2][kKN];
     __shared__ __attribute__((aligned(16))) int s_pos[2][kKN];
 
@@ -496,9 +523,17 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attn_dkv_kernel(AttnArg
         if (threadIdx.x < kKN) in.stats(row_lo + threadIdx.x, s_lse[0][threadIdx.x], s_delta[0][threadIdx.x], s_pos[0][threadIdx.x]);
     }
 
-    KeySums<T, DP, 2> sums;
+    KeySums<T, DP, 2, VL> sums;
     sums.init(a, key0 + wave * 32 + r);
     const int(&key)[2] = sums.key;
+    if constexpr (VL) {
+        const T *vp = (const T *)a.v + s.b * a.v_b + (s.k0 + key0) * a.v_t + hkv * a.v_h;
+        const int left = keys - key0, dim = a.dim, v_t = (int)a.v_t;
+        fetch_rows<T, DP>(buf_rsrc(vp, 0x7FFFFFFF), s_v, kKM, [=](int j, int c) {
+            return j < left && c * 8 < dim ? (uint32_t)(j * v_t + c * 8) * 2 : kZeros;
+        });
+        sums.sv = s_v + wave * 32 * DP;
+    }
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
         const T *kp = (const T *)a.k + s.b * a.k_b + (s.k0 + key[y]) * a.k_t + hkv * a.k_h;
@@ -508,7 +543,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attn_dkv_kernel(AttnArg
             const int c = x * 4 + g;
             const bool ok = key[y] < keys && c * 8 < a.dim;
             sums.kf[y][x] = ok ? *(const X8 *)(kp + c * 8) : X8{};
-            sums.vf[y][x] = ok ? *(const X8 *)(vp + c * 8) : X8{};
+            if constexpr (!VL) sums.vf[y][x] = ok ? *(const X8 *)(vp + c * 8) : X8{};
         }
     }
     const int wkey0 = key0 + wave * 32, wkey1 = wkey0 + 31;
@@ -528,7 +563,11 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attn_dkv_kernel(AttnArg
         const bool none = wkey0 > pmax || wkey0 > key1 || (a.window && wkey1 <= pmin - a.window && wkey0 >= a.sinks);
         if (!none) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) sums.add(sq[n], so[n], s_lse[n], s_delta[n], s_pos[n], u * 32, a.c, g, r);
+            for (int u = 0; u < kKN / 32; ++u) {
+                int lr = r;
+                if constexpr (VL) asm volatile("" : "+v"(lr));
+                sums.add(sq[n], so[n], s_lse[n], s_delta[n], s_pos[n], u * 32, a.c, g, lr);
+            }
         }
         wait_dma();
         if (more && threadIdx.x < kKN) s_lse[n ^ 1][threadIdx.x] = lse, s_delta[n ^ 1][threadIdx.x] = delta, s_pos[n ^ 1][threadIdx.x] = pos;
