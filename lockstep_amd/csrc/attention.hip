@@ -73,14 +73,13 @@ struct DenseKV {
     LSMX_DEV void land() { wait_dma(); }
 };
 
-// Keys and values of a paged MXFP4 cache, expanded to bf16 on their way into
-// LDS (exact).  Four of the 256 threads take a key's vector, and a value's.
-template <int DP>
+// Keys and values of a paged MXFP4 cache, expanded to the rows' type on their way into
+// LDS.  Four of the 256 threads take a key's vector, and a value's.
+template <typename T, int DP>
 struct PagedKV {
     static constexpr int NC = DP / 8, NQ = DP / 32;  // words of codes of a thread
     static constexpr bool kHoles = true;
     typedef AttendArgs Args;
-    typedef __bf16 T;
     const Pool *p;
     int b, h, k_len, row, part;
     uint32_t kr[NQ], vr[NQ];
@@ -123,9 +122,10 @@ struct PagedKV {
         }
     }
     LSMX_DEV void store(T *to, const uint32_t (&w)[NQ], uint32_t e) {
-        const float sc = e8m0_to_f32(e);
+        const float sc = block_scale<T>(e);
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) *(bf16x8 *)(to + row * DP + swz<NC>(row, part * NQ + i) * 8) = fp4x8_to_bf16(w[i], sc);
+        for (int i = 0; i < NQ; ++i)
+            *(typename Vec<T>::x8 *)(to + row * DP + swz<NC>(row, part * NQ + i) * 8) = fp4x8<T>(w[i], sc);
     }
     // The first tile j0 (next j1, then j2; -1: none) into LDS, the next one's
     // codes on their way.
@@ -151,9 +151,7 @@ struct PagedKV {
     LSMX_DEV void land() {}
 };
 
-// NW waves of RT x 16 rows.  TQ: type of q and o; T: type of the products'
-// operands.  fp16 rows against a cache (whose values need bf16's exponents)
-// enter as two bf16 terms, and so do their probabilities.
+// KS groups (each with its share of the keys) of NW waves of RT x 16 rows.
 //
 // The loop is pipelined over two key tiles: the scores of the next tile are
 // products that do not wait for anything, and stand between the exponentials
@@ -166,16 +164,14 @@ struct PagedKV {
 // a step is 32 keys).  2 x 4096 tokens, 32/8 heads of 128, window 1024: 184 us
 // = 656 TFLOP/s of the visible pairs; 16384 tokens of 8/1 heads of 64 through a
 // window of 4096: 227 us.
-template <typename TQ, typename T, int DP, int RT, int NW, int KS, typename KV>
+template <typename T, int DP, int RT, int NW, int KS, typename KV>
 __global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (DP == 64 ? 3 : 2)) void attn_fwd_kernel(typename KV::Args args) {
-    constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, NT = __is_same(TQ, T) ? 1 : 2, BM = NW * RT * 16;
+    constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, BM = NW * RT * 16;
     // a row's maximum is followed only when it grows by a factor of 2^8: the
     // probabilities stay below 2^8 and O is rescaled a few times per row
     constexpr float kLazy = 8.f;
     typedef typename Vec<T>::x8 X8;
     typedef typename Vec<T>::x4 X4;
-    typedef typename Vec<TQ>::x8 Q8;
-    typedef typename Vec<TQ>::x4 Q4;
     __shared__ __attribute__((aligned(16))) T s_kv[KS][2][2][kBN * DP];  // [group][keys, values][buffer]
     __shared__ int s_held[KS][2][KV::kHoles ? kBN : 1];
 
@@ -214,7 +210,7 @@ __global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (D
 
     // this lane's rows: wrow0 + r + 16 x
     int pos[RT], low[RT];
-    X8 qf[NT][RT][NS];
+    X8 qf[RT][NS];
 #pragma unroll
     for (int x = 0; x < RT; ++x) {
         const int row = wrow0 + r + 16 * x;
@@ -222,15 +218,11 @@ __global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (D
         const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
         pos[x] = in ? tok + s.shift : -1;
         low[x] = window_low(pos[x], a.window);
-        const TQ *qp = (const TQ *)a.q + s.b * a.q_b + (s.q0 + tok) * a.q_t + h * a.q_h;
+        const T *qp = (const T *)a.q + s.b * a.q_b + (s.q0 + tok) * a.q_t + h * a.q_h;
 #pragma unroll
         for (int st = 0; st < NS; ++st) {
             const int c = st * 4 + g;
-            const Q8 w = in && c * 8 < a.dim ? *(const Q8 *)(qp + c * 8) : Q8{};
-            if constexpr (NT == 1)
-                qf[0][x][st] = w;
-            else
-                split(w, qf[0][x][st], qf[1][x][st]);
+            qf[x][st] = in && c * 8 < a.dim ? *(const X8 *)(qp + c * 8) : X8{};
         }
     }
 
@@ -258,9 +250,7 @@ __global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (D
             for (int y = 0; y < NS; ++y) {
                 const X8 kf = *(const X8 *)(ck + j * DP + swz<NC>(j, y * 4 + g) * 8);
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int x = 0; x < RT; ++x) z[kt][x] = mfma(kf, qf[n][x][y], z[kt][x]);
+                for (int x = 0; x < RT; ++x) z[kt][x] = mfma(kf, qf[x][y], z[kt][x]);
             }
         }
     };
@@ -324,7 +314,7 @@ __global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (D
         }
         f32x4 zn[2][RT];
         if constexpr (kMore) scores(ck, jk, lr, zn);
-        X8 pf[NT][RT];
+        X8 pf[RT];
 #pragma unroll
         for (int x = 0; x < RT; ++x) {
 #pragma unroll
@@ -335,16 +325,13 @@ __global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (D
                     l[x] += p;
                     // the probabilities are the product's operand in the
                     // inputs' type; their sum is of the unrounded ones
-                    pf[0][x][kt * 4 + i] = (T)p;
-                    if constexpr (NT == 2) pf[1][x][kt * 4 + i] = (T)(p - (float)pf[0][x][kt * 4 + i]);
+                    pf[x][kt * 4 + i] = (T)p;
                 }
         }
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int x = 0; x < RT; ++x) o[d][x] = mfma(vf[d], pf[n][x], o[d][x]);
+            for (int x = 0; x < RT; ++x) o[d][x] = mfma(vf[d], pf[x], o[d][x]);
         if constexpr (kMore) {
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
@@ -417,16 +404,16 @@ __global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (D
         const int64_t o_at = s.b * a.o_b + (s.q0 + tok) * a.o_t + h * a.o_h;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            Q4 w, rest;
+            X4 w, rest;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float f = o[d][x][i] * inv;
-                w[i] = (TQ)f;
-                rest[i] = (TQ)(f - (float)w[i]);
+                w[i] = (T)f;
+                rest[i] = (T)(f - (float)w[i]);
             }
             if (d * 16 + g * 4 < a.dim) {
-                *(Q4 *)((TQ *)a.o + o_at + d * 16 + g * 4) = w;
-                if (a.o_lo) *(Q4 *)((TQ *)a.o_lo + o_at + d * 16 + g * 4) = rest;
+                *(X4 *)((T *)a.o + o_at + d * 16 + g * 4) = w;
+                if (a.o_lo) *(X4 *)((T *)a.o_lo + o_at + d * 16 + g * 4) = rest;
             }
         }
         if (a.lse && g == 0)
@@ -465,11 +452,11 @@ hipError_t fwd(AttnArgs a, hipStream_t s) {
     tiles_of(a, f == kWide ? 128 : 64);
     const unsigned grid = (unsigned)a.per * 8;
     if (f == kWide)
-        attn_fwd_kernel<T, T, DP, 2, 4, 1, DenseKV<T, DP, 4>><<<grid, 256, 0, s>>>(a);
+        attn_fwd_kernel<T, DP, 2, 4, 1, DenseKV<T, DP, 4>><<<grid, 256, 0, s>>>(a);
     else if (f == kNarrow)
-        attn_fwd_kernel<T, T, DP, 1, 4, 1, DenseKV<T, DP, 4>><<<grid, 256, 0, s>>>(a);
+        attn_fwd_kernel<T, DP, 1, 4, 1, DenseKV<T, DP, 4>><<<grid, 256, 0, s>>>(a);
     else
-        attn_fwd_kernel<T, T, DP, 1, 4, 2, DenseKV<T, DP, 4>><<<grid, 512, 0, s>>>(a);
+        attn_fwd_kernel<T, DP, 1, 4, 2, DenseKV<T, DP, 4>><<<grid, 512, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -479,11 +466,11 @@ hipError_t chunk(AttendArgs x, hipStream_t s) {
     tiles_of(x.a, f == kWide ? 128 : 64);
     const unsigned grid = (unsigned)x.a.per * 8;
     if (f == kWide)
-        attn_fwd_kernel<T, __bf16, DP, 2, 4, 1, PagedKV<DP>><<<grid, 256, 0, s>>>(x);
+        attn_fwd_kernel<T, DP, 2, 4, 1, PagedKV<T, DP>><<<grid, 256, 0, s>>>(x);
     else if (f == kNarrow)
-        attn_fwd_kernel<T, __bf16, DP, 1, 4, 1, PagedKV<DP>><<<grid, 256, 0, s>>>(x);
+        attn_fwd_kernel<T, DP, 1, 4, 1, PagedKV<T, DP>><<<grid, 256, 0, s>>>(x);
     else
-        attn_fwd_kernel<T, __bf16, DP, 1, 4, 2, PagedKV<DP>><<<grid, 512, 0, s>>>(x);
+        attn_fwd_kernel<T, DP, 1, 4, 2, PagedKV<T, DP>><<<grid, 512, 0, s>>>(x);
     return hipGetLastError();
 }
 

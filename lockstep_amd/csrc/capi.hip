@@ -901,7 +901,7 @@ static int64_t kv_span(const lsmx_kv_cache *c, int64_t q_len, int64_t window, in
 // where weights are asked for.
 struct KvPlan {
     int splits;
-    int64_t part, part_m, lse, bytes;
+    int64_t part_m, lse, bytes;
 };
 static KvPlan kv_plan(const lsmx_kv_cache *c, int64_t q_len, int64_t heads, int64_t window, int64_t sinks, bool weights) {
     KvPlan p{};

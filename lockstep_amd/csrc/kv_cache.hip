@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, int per_wg
         }
         if (a.k_out) {
             __bf16 *out = (__bf16 *)(is_v ? a.v_out : a.k_out) + ((int64_t)(t0 + i) * p.kv_heads + h) * p.dim + c * 8;
-            *(bf16x8 *)out = fp4x8_to_bf16(codes, e8m0_to_f32(e8));
+            *(bf16x8 *)out = fp4x8<__bf16>(codes, e8m0_to_f32(e8));
         }
     }
 }
@@ -157,35 +157,27 @@ struct Walk {
 
 // Rows of one (sequence, key head): row -> token and head, q fragments whose
 // contraction runs over quarter g of the vector in lane group g.
-template <typename TQ, int DP, int NT>
-LSMX_DEV void load_rows(const AttnArgs &a, int b, int hkv, int row, int g, bool in, bf16x8 (&q)[NT][DP / 32]) {
-    typedef typename Vec<TQ>::x8 Q8;
+template <typename T, int DP>
+LSMX_DEV void load_rows(const AttnArgs &a, int b, int hkv, int row, int g, bool in, typename Vec<T>::x8 (&q)[DP / 32]) {
+    typedef typename Vec<T>::x8 X8;
     const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
-    const TQ *qp = (const TQ *)a.q + b * a.q_b + tok * a.q_t + h * a.q_h + g * (DP / 4);
+    const T *qp = (const T *)a.q + b * a.q_b + tok * a.q_t + h * a.q_h + g * (DP / 4);
 #pragma unroll
-    for (int x = 0; x < DP / 32; ++x) {
-        const Q8 w = in ? *(const Q8 *)(qp + x * 8) : Q8{};
-        if constexpr (NT == 1)
-            q[0][x] = w;
-        else
-            split(w, q[0][x], q[1][x]);
-    }
+    for (int x = 0; x < DP / 32; ++x) q[x] = in ? *(const X8 *)(qp + x * 8) : X8{};
 }
 
 // The scores of 16 keys, lane 16g + r holding keys 4g..4g+3 of row r; the
 // lane's part of each vector is contracted as it lies in memory.
-template <int DP, int RT, int NT>
-LSMX_DEV void scores(const Codes<DP> &k, const bf16x8 (&q)[RT][NT][DP / 32], f32x4 (&st)[RT]) {
-    const float sc = e8m0_to_f32(k.e);
+template <typename T, int DP, int RT>
+LSMX_DEV void scores(const Codes<DP> &k, const typename Vec<T>::x8 (&q)[RT][DP / 32], f32x4 (&st)[RT]) {
+    const float sc = block_scale<T>(k.e);
 #pragma unroll
     for (int y = 0; y < RT; ++y) st[y] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int s = 0; s < DP / 32; ++s) {
-        const bf16x8 kf = fp4x8_to_bf16(k.w[s], sc);
+        const typename Vec<T>::x8 kf = fp4x8<T>(k.w[s], sc);
 #pragma unroll
-        for (int y = 0; y < RT; ++y)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) st[y] = mfma(kf, q[y][n][s], st[y]);
+        for (int y = 0; y < RT; ++y) st[y] = mfma(kf, q[y][s], st[y]);
     }
 }
 
@@ -196,9 +188,11 @@ LSMX_DEV void scores(const Codes<DP> &k, const bf16x8 (&q)[RT][NT][DP / 32], f32
 //
 // Bound by the loads in flight, so that waves per SIMD count: 4 of them at 64 x
 // 8192 tokens of 8 key heads of 128 take 82 us = 5.2 TB/s (3: 91, 2: 101).
-template <typename TQ, int DP, int RT>
-__global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(TQ, __bf16) ? 4 : 3) void kv_decode_kernel(AttendArgs x) {
-    constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, NT = __is_same(TQ, __bf16) ? 1 : 2;
+template <typename T, int DP, int RT>
+__global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(T, __bf16) ? 4 : 3) void kv_decode_kernel(AttendArgs x) {
+    constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16;
+    typedef typename Vec<T>::x8 X8;
+    typedef typename Vec<T>::x4 X4;
     __shared__ __attribute__((aligned(16))) uint8_t smem[4 * 32 * DP * 2];  // values of a wave's tile; then 16 x DP / 2 fp32 of a wave
     __shared__ float s_m[4][16], s_l[4][16];
     const AttnArgs &a = x.a;
@@ -218,12 +212,12 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(TQ, __bf16)
         walk.find(i, cur);
         cur.load(p, hkv, g, r);
     }
-    bf16x8 q[RT][NT][NS];
+    X8 q[RT][NS];
     int pos[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const int row = row0 + t * 16 + r;
-        load_rows<TQ, DP, NT>(a, b, hkv, row, g, row < rows, q[t]);
+        load_rows<T, DP>(a, b, hkv, row, g, row < rows, q[t]);
         pos[t] = row < rows ? div_by(row, a.by_group) + tiles.len - a.q_len : -1;
     }
     f32x4 o[ND][RT];
@@ -234,7 +228,7 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(TQ, __bf16)
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d][t] = f32x4{0, 0, 0, 0};
     }
-    __bf16 *sv = (__bf16 *)smem + wave * 32 * DP;
+    T *sv = (T *)smem + wave * 32 * DP;
     const int pfirst = tiles.len - a.q_len;
 
     for (; i < i1; i += 4) {
@@ -259,12 +253,12 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(TQ, __bf16)
         f32x4 st[2][RT];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            scores<DP, RT, NT>(cur.k[t], q, st[t]);
-            const float vsc = e8m0_to_f32(cur.v[t].e);
+            scores<T, DP, RT>(cur.k[t], q, st[t]);
+            const float vsc = block_scale<T>(cur.v[t].e);
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 const int row = t * 16 + lr, c = g * NS + s;
-                *(bf16x8 *)(sv + row * DP + swz<NC>(row, c) * 8) = fp4x8_to_bf16(cur.v[t].w[s], vsc);
+                *(X8 *)(sv + row * DP + swz<NC>(row, c) * 8) = fp4x8<T>(cur.v[t].w[s], vsc);
             }
         }
         if (!full) {
@@ -280,7 +274,7 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(TQ, __bf16)
                     }
                 }
         }
-        bf16x8 pf[RT][NT];
+        X8 pf[RT];
 #pragma unroll
         for (int y = 0; y < RT; ++y) {
             float mx = st[0][y][0];
@@ -303,8 +297,7 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(TQ, __bf16)
                 for (int e = 0; e < 4; ++e) {
                     const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][y][e], a.c, -mc));
                     l[y] += w;
-                    pf[y][0][t * 4 + e] = (__bf16)w;
-                    if constexpr (NT == 2) pf[y][1][t * 4 + e] = (__bf16)(w - (float)pf[y][0][t * 4 + e]);
+                    pf[y][t * 4 + e] = (T)w;
                 }
         }
         // the wave's own LDS region: its writes above, its reads here, in order
@@ -313,12 +306,10 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(TQ, __bf16)
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             const int c = d * 2 + ((lr & 3) >> 1), e = (lr & 1) * 4;
-            const bf16x8 vf = join<bf16x4, bf16x8>(read_tr<__bf16>(sv + row * DP + swz<NC>(row, c) * 8 + e),
-                                                   read_tr<__bf16>(sv + (row + 16) * DP + swz<NC>(row + 16, c) * 8 + e));
+            const X8 vf = join<X4, X8>(read_tr<T>(sv + row * DP + swz<NC>(row, c) * 8 + e),
+                                                   read_tr<T>(sv + (row + 16) * DP + swz<NC>(row + 16, c) * 8 + e));
 #pragma unroll
-            for (int y = 0; y < RT; ++y)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) o[d][y] = mfma(vf, pf[y][n], o[d][y]);
+            for (int y = 0; y < RT; ++y) o[d][y] = mfma(vf, pf[y], o[d][y]);
         }
         asm volatile("" ::: "memory");
         cur = nxt;
@@ -362,10 +353,10 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(TQ, __bf16)
                     if (half == 0 && (threadIdx.x & 15) == 0) x.part_m[at * 2] = top, x.part_m[at * 2 + 1] = tot;
                 } else {
                     const int tok = div_by(full, a.by_group), h = hkv * a.group + full - tok * a.group;
-                    TQ *op = (TQ *)a.o + b * a.o_b + tok * a.o_t + h * a.o_h + half * HD + c;
+                    T *op = (T *)a.o + b * a.o_b + tok * a.o_t + h * a.o_h + half * HD + c;
                     const float inv = tot > 0.f || tot != tot ? 1.f / tot : 0.f;
 #pragma unroll
-                    for (int e = 0; e < HD / 16; ++e) op[e] = (TQ)(acc[e] * inv);
+                    for (int e = 0; e < HD / 16; ++e) op[e] = (T)(acc[e] * inv);
                     if (a.lse && half == 0 && (threadIdx.x & 15) == 0)
                         a.lse[b * a.lse_b + h * a.lse_h + tok] = tot > 0.f ? mc + __log2f(tot) : tot != tot ? tot : -INFINITY;
                 }
@@ -375,7 +366,7 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(TQ, __bf16)
 }
 
 // Joins the shares of one row: 16 threads over the vector, 16 over the shares.
-template <typename TQ, int DP>
+template <typename T, int DP>
 __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs x) {
     constexpr int NE = DP / 16;
     __shared__ float s_top[4], s_tot[16], s_acc[16][DP + 4];
@@ -417,16 +408,17 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs x) {
     for (int i = 0; i < 16; ++i) sum += s_acc[i][threadIdx.x], tot += s_tot[i];
     const int tok = div_by(row, a.by_group), h = hkv * a.group + row - tok * a.group;
     const float inv = tot > 0.f || tot != tot ? 1.f / tot : 0.f;
-    ((TQ *)a.o)[b * a.o_b + tok * a.o_t + h * a.o_h + threadIdx.x] = (TQ)(sum * inv);
+    ((T *)a.o)[b * a.o_b + tok * a.o_t + h * a.o_h + threadIdx.x] = (T)(sum * inv);
     if (a.lse && threadIdx.x == 0)
         a.lse[b * a.lse_b + h * a.lse_h + tok] = tot > 0.f ? mc + __log2f(tot) : tot != tot ? tot : -INFINITY;
 }
 
 // ------------------------------------------------------------------ weights
 // weights[b, h, j] += sum over the rows of exp(s_ij - lse_i), the scores
-// recomputed from the keys' codes: 68 bytes a key at head 128, where scores
-// kept by the first pass would be 8 bytes a key and row.  Each sum has one owner and
-// one order.
+// recomputed from the keys' codes.  Each sum has one owner and one order.
+// (Scores kept by the first pass are fewer bytes for up to 8 rows at head 128,
+// but their short runs made that pass 118 us from 80 at 64 x 8192 tokens of 8
+// key heads and 4 rows, and adding them took 42, where this takes 60.)
 //
 // Few rows: their q stays in registers, and the waves run over the keys as in
 // kv_decode_kernel.
@@ -437,9 +429,10 @@ LSMX_DEV float sum_16(float x) {  // over the 16 lanes of a row of lanes
     x += u2f(__builtin_amdgcn_update_dpp(0, f2u(x), 0x140, 0xF, 0xF, true));  // row_mirror
     return x;
 }
-template <typename TQ, int DP, int RT>
+template <typename T, int DP, int RT>
 __global__ __launch_bounds__(256) void kv_weights_kernel(AttendArgs x) {
-    constexpr int NS = DP / 32, NT = __is_same(TQ, __bf16) ? 1 : 2;
+    constexpr int NS = DP / 32;
+    typedef typename Vec<T>::x8 X8;
     const AttnArgs &a = x.a;
     const Pool &p = x.p;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
@@ -453,14 +446,14 @@ __global__ __launch_bounds__(256) void kv_weights_kernel(AttendArgs x) {
     Walk walk(p, tiles, b, i, i1);
     walk.find(i, cur);
     cur.load(p, hkv, g, r);
-    bf16x8 q[RT][NT][NS];
+    X8 q[RT][NS];
     int pos[RT], low[RT];
     float lse[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const int row = t * 16 + r;
         const bool in = row < rows;
-        load_rows<TQ, DP, NT>(a, b, hkv, row, g, in, q[t]);
+        load_rows<T, DP>(a, b, hkv, row, g, in, q[t]);
         const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
         pos[t] = in ? tok + tiles.len - a.q_len : -1;
         low[t] = window_low(pos[t], a.window);
@@ -481,7 +474,7 @@ __global__ __launch_bounds__(256) void kv_weights_kernel(AttendArgs x) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x4 st[RT], sum{0, 0, 0, 0};
-            scores<DP, RT, NT>(cur.k[t], q, st);
+            scores<T, DP, RT>(cur.k[t], q, st);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
 #pragma unroll
@@ -500,10 +493,11 @@ __global__ __launch_bounds__(256) void kv_weights_kernel(AttendArgs x) {
 
 // Many rows: a workgroup owns 64 keys, whose operands stay in registers, and
 // its waves take tiles of 16 rows in turn; their sums are joined in LDS.
-template <typename TQ, int DP>
+template <typename T, int DP>
 __global__ __launch_bounds__(512) void kv_weights_rows_kernel(AttendArgs x) {
-    constexpr int NS = DP / 32, NT = __is_same(TQ, __bf16) ? 1 : 2;
+    constexpr int NS = DP / 32;
     __shared__ __attribute__((aligned(16))) float s_sum[8][64];
+    typedef typename Vec<T>::x8 X8;
     const AttnArgs &a = x.a;
     const Pool &p = x.p;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
@@ -516,7 +510,7 @@ __global__ __launch_bounds__(512) void kv_weights_rows_kernel(AttendArgs x) {
     int tok_hi = a.q_len;
     if (a.window && j0 >= a.sinks) tok_hi = min(tok_hi, min(j0 + 63, len - 1) + a.window - first);
     if (tok_lo >= tok_hi) return;
-    bf16x8 kf[4][NS];
+    X8 kf[4][NS];
     int pg[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -529,7 +523,7 @@ __global__ __launch_bounds__(512) void kv_weights_rows_kernel(AttendArgs x) {
         else
             k.drop();
 #pragma unroll
-        for (int s = 0; s < NS; ++s) kf[t][s] = fp4x8_to_bf16(k.w[s], e8m0_to_f32(k.e));
+        for (int s = 0; s < NS; ++s) kf[t][s] = fp4x8<T>(k.w[s], block_scale<T>(k.e));
     }
     f32x4 sum[4];
     uint32_t span[4][4];  // position p sees key j when 0 <= p - j <= span
@@ -544,7 +538,7 @@ __global__ __launch_bounds__(512) void kv_weights_rows_kernel(AttendArgs x) {
     // than a load's latency
     constexpr int U = 256 / DP;
     struct Row {
-        typename Vec<TQ>::x8 q[NS];
+        X8 q[NS];
         float lse;
         int pos;
     };
@@ -554,9 +548,9 @@ __global__ __launch_bounds__(512) void kv_weights_rows_kernel(AttendArgs x) {
             const int row = r0 + u * 128 + r;
             const bool in = row < row_hi;
             const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
-            const TQ *qp = (const TQ *)a.q + b * a.q_b + tok * a.q_t + h * a.q_h + g * (DP / 4);
+            const T *qp = (const T *)a.q + b * a.q_b + tok * a.q_t + h * a.q_h + g * (DP / 4);
 #pragma unroll
-            for (int s = 0; s < NS; ++s) w[u].q[s] = *(const typename Vec<TQ>::x8 *)(qp + s * 8);
+            for (int s = 0; s < NS; ++s) w[u].q[s] = *(const X8 *)(qp + s * 8);
             w[u].lse = a.lse[b * a.lse_b + h * a.lse_h + tok];
             w[u].pos = in ? tok + first : -1;
         }
@@ -568,20 +562,11 @@ __global__ __launch_bounds__(512) void kv_weights_rows_kernel(AttendArgs x) {
         load(r0 + 128 * U, nxt);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            bf16x8 q[NT][NS];
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-                if constexpr (NT == 1)
-                    q[0][s] = cur[u].q[s];
-                else
-                    split(cur[u].q[s], q[0][s], q[1][s]);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 f32x4 st{0, 0, 0, 0};
 #pragma unroll
-                for (int s = 0; s < NS; ++s)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) st = mfma(kf[t][s], q[n][s], st);
+                for (int s = 0; s < NS; ++s) st = mfma(kf[t][s], cur[u].q[s], st);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(st[e], a.c, -cur[u].lse));
@@ -684,34 +669,95 @@ __global__ __launch_bounds__(kSelect) void kv_select_kernel(EvictArgs a) {
     }
     // prefix is the rank of the last that stays, `want` the number of its
     // equals that do (the first of them)
-    int ties = 0, out = 0;
-    each([&](int j, float x) {
-        const uint32_t u = rank_of(x);
-        const bool held = j < n && (all || j < c0 || j >= c1 || u > prefix);
-        const bool tie = j < n && !all && j >= c0 && j < c1 && u == prefix;
-        const uint64_t below = (1ull << lane) - 1, bt = __ballot(tie);
-        if (lane == 0) s_scan[0][wave] = __popcll(bt);
-        __syncthreads();
-        // sums over the waves before, and over all
-        auto scan = [&](const int *v, int &before, int &total) {
-            const int x = lane < kSelect / 64 ? v[lane] : 0;
-            int y = lane < wave ? x : 0, z = x;
+    const uint64_t below = (1ull << lane) - 1;
+    auto held = [&](int j, uint32_t u) { return j < n && (all || j < c0 || j >= c1 || u > prefix); };
+    auto tie = [&](int j, uint32_t u) { return j < n && !all && j >= c0 && j < c1 && u == prefix; };
+    int out = 0;
+    if constexpr (PER > 0) {
+        // counts of all (round, wave) pairs at once: their sums before each pair
+        constexpr int NP = PER * (kSelect / 64), E = NP / 64;
+        __shared__ int s_pair[NP + 1];
+        auto scan = [&] {
+            __syncthreads();
+            if (wave == 0) {
+                int v[E], sum = 0;
 #pragma unroll
-            for (int d = 1; d < kSelect / 64; d <<= 1) y += __shfl_xor(y, d), z += __shfl_xor(z, d);
-            before = lane_of(y, 0), total = lane_of(z, 0);
+                for (int e = 0; e < E; ++e) sum += v[e] = s_pair[lane * E + e];
+                int upto = sum;
+                for (int d = 1; d < 64; d <<= 1) {
+                    const int x = __shfl_up(upto, d);
+                    if (lane >= d) upto += x;
+                }
+                int at = upto - sum;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    s_pair[lane * E + e] = at;
+                    at += v[e];
+                }
+                if (lane == 63) s_pair[NP] = at;
+            }
+            __syncthreads();
         };
-        int before, total;
-        scan(s_scan[0], before, total);
-        const bool stay = held | (tie & (ties + before + __popcll(bt & below) < want));
-        ties += total;
-        const uint64_t bs = __ballot(stay);
-        if (lane == 0) s_scan[1][wave] = __popcll(bs);
+        uint32_t stay = 0;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const uint64_t m = __ballot(tie(k * kSelect + tid, rank_of(own[k])));
+            if (lane == 0) s_pair[k * (kSelect / 64) + wave] = __popcll(m);
+        }
+        scan();
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int j = k * kSelect + tid;
+            const uint32_t u = rank_of(own[k]);
+            const bool t = tie(j, u);
+            const uint64_t m = __ballot(t);
+            const bool in = held(j, u) | (t & (s_pair[k * (kSelect / 64) + wave] + __popcll(m & below) < want));
+            stay |= (uint32_t)in << k;
+        }
         __syncthreads();
-        scan(s_scan[1], before, total);
-        const int at = out + before + __popcll(bs & below);
-        if (stay) index[at] = j, kept[at] = x;
-        out += total;
-    });
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const uint64_t m = __ballot((stay >> k) & 1);
+            if (lane == 0) s_pair[k * (kSelect / 64) + wave] = __popcll(m);
+        }
+        scan();
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const bool in = (stay >> k) & 1;
+            const uint64_t m = __ballot(in);
+            const int at = s_pair[k * (kSelect / 64) + wave] + __popcll(m & below);
+            if (in) index[at] = k * kSelect + tid, kept[at] = own[k];
+        }
+        out = s_pair[NP];
+    } else {
+        int ties = 0;
+        each([&](int j, float x) {
+            const uint32_t u = rank_of(x);
+            const bool t = tie(j, u);
+            const uint64_t bt = __ballot(t);
+            if (lane == 0) s_scan[0][wave] = __popcll(bt);
+            __syncthreads();
+            // sums over the waves before, and over all
+            auto scan = [&](const int *v, int &before, int &total) {
+                const int x = lane < kSelect / 64 ? v[lane] : 0;
+                int y = lane < wave ? x : 0, z = x;
+#pragma unroll
+                for (int d = 1; d < kSelect / 64; d <<= 1) y += __shfl_xor(y, d), z += __shfl_xor(z, d);
+                before = lane_of(y, 0), total = lane_of(z, 0);
+            };
+            int before, total;
+            scan(s_scan[0], before, total);
+            const bool in = held(j, u) | (t & (ties + before + __popcll(bt & below) < want));
+            ties += total;
+            const uint64_t bs = __ballot(in);
+            if (lane == 0) s_scan[1][wave] = __popcll(bs);
+            __syncthreads();
+            scan(s_scan[1], before, total);
+            const int at = out + before + __popcll(bs & below);
+            if (in) index[at] = j, kept[at] = x;
+            out += total;
+        });
+    }
     for (int i = out + tid; i < a.keep; i += kSelect) index[i] = -1, kept[i] = 0.f;
 }
 
@@ -763,30 +809,30 @@ __global__ __launch_bounds__(256) void kv_move_kernel(EvictArgs a) {
     }
 }
 
-template <typename TQ, int DP>
+template <typename T, int DP>
 hipError_t attend(const AttendArgs &x, hipStream_t s) {
     const int rows = x.a.q_len * x.a.group, bh = x.a.batch * x.a.kv_heads;
     const unsigned grid = (unsigned)x.splits * bh;
     if (rows <= 16)
-        kv_decode_kernel<TQ, DP, 1><<<grid, 256, 0, s>>>(x);
+        kv_decode_kernel<T, DP, 1><<<grid, 256, 0, s>>>(x);
     else
-        kv_decode_kernel<TQ, DP, 2><<<grid * ((rows + 31) / 32), 256, 0, s>>>(x);
-    if (x.splits > 1) kv_join_kernel<TQ, DP><<<(unsigned)(rows * bh), 256, 0, s>>>(x);
+        kv_decode_kernel<T, DP, 2><<<grid * ((rows + 31) / 32), 256, 0, s>>>(x);
+    if (x.splits > 1) kv_join_kernel<T, DP><<<(unsigned)(rows * bh), 256, 0, s>>>(x);
     return hipGetLastError();
 }
 
-template <typename TQ, int DP>
+template <typename T, int DP>
 hipError_t weights(AttendArgs x, hipStream_t s) {
     const int rows = x.a.q_len * x.a.group, bh = x.a.batch * x.a.kv_heads;
     const dim3 grid((unsigned)x.splits * bh);
     if (rows <= 16)
-        kv_weights_kernel<TQ, DP, 1><<<grid, 256, 0, s>>>(x);
+        kv_weights_kernel<T, DP, 1><<<grid, 256, 0, s>>>(x);
     else if (rows <= 32)
-        kv_weights_kernel<TQ, DP, 2><<<grid, 256, 0, s>>>(x);
+        kv_weights_kernel<T, DP, 2><<<grid, 256, 0, s>>>(x);
     else if (rows <= kDecodeRows)
-        kv_weights_kernel<TQ, DP, 4><<<grid, 256, 0, s>>>(x);
+        kv_weights_kernel<T, DP, 4><<<grid, 256, 0, s>>>(x);
     else
-        kv_weights_rows_kernel<TQ, DP><<<(unsigned)(((x.p.max_pages << x.p.page_shift) + 63) / 64) * bh, 512, 0, s>>>(x);
+        kv_weights_rows_kernel<T, DP><<<(unsigned)(((x.p.max_pages << x.p.page_shift) + 63) / 64) * bh, 512, 0, s>>>(x);
     return hipGetLastError();
 }
 
@@ -827,7 +873,9 @@ hipError_t launch_kv_weights(const AttendArgs &x, int dtype, hipStream_t s) {
 
 hipError_t launch_kv_evict(const EvictArgs &a, hipStream_t s) {
     const int bh = a.batch * a.p.kv_heads, cap = a.p.max_pages << a.p.page_shift;
-    if (cap <= 8 * kSelect)
+    if (cap <= 4 * kSelect)
+        kv_select_kernel<4><<<(unsigned)bh, kSelect, 0, s>>>(a);
+    else if (cap <= 8 * kSelect)
         kv_select_kernel<8><<<(unsigned)bh, kSelect, 0, s>>>(a);
     else if (cap <= 32 * kSelect)
         kv_select_kernel<32><<<(unsigned)bh, kSelect, 0, s>>>(a);

@@ -13,6 +13,7 @@ namespace lsmx {
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -239,24 +240,29 @@ struct EvictArgs {
     float *new_weights;
 };
 
-// The 8 elements of four bytes of codes, times 2^e of their block.
-LSMX_DEV bf16x8 fp4x8_to_bf16(uint32_t w, float sc) {
+// The 8 elements of four bytes of codes, times 2^e of their block (e: its E8M0
+// byte).  Exact in bf16; in fp16 (the operands of fp16 rows) too for values that
+// fp16 holds.  Blocks above it are clipped to its range, so that no
+// infinity meets a probability of 0, and below it the elements round to its
+// smallest ones.
+template <typename T>
+LSMX_DEV float block_scale(uint32_t e) {
+    if constexpr (__is_same(T, _Float16)) e = e == 255u ? e : min(e, 127u + 13u);
+    return e8m0_to_f32(e);
+}
+LSMX_DEV bf16x8 fp4x8_to(uint32_t w, float sc, bf16x8) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1);
     const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3);
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-
-// An fp16 vector as the sum of two bf16 ones, exact: 8 + 3 significant bits,
-// and bf16's exponents cover fp16's subnormals.
-LSMX_DEV void split(f16x8 x, bf16x8 &hi, bf16x8 &lo) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float f = (float)x[i];
-        hi[i] = (__bf16)f;
-        // an infinity or NaN stays in the first term alone
-        const float d = f - (float)hi[i];
-        lo[i] = (__bf16)(d == d ? d : 0.f);
-    }
+LSMX_DEV f16x8 fp4x8_to(uint32_t w, float sc, f16x8) {
+    const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 1);
+    const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 3);
+    return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+template <typename T>
+LSMX_DEV typename Vec<T>::x8 fp4x8(uint32_t w, float sc) {
+    return fp4x8_to(w, sc, typename Vec<T>::x8{});
 }
 
 // Rows (tokens x heads of a key head) up to which the keys of a sequence are
