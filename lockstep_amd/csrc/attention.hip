@@ -162,8 +162,9 @@ struct PagedKV {
 // cycles at head 128, 66% at 64, with the matrix unit at 34% and 32%), so that
 // waves per SIMD count: 2 at head 128, 3 at 64 (registers allow it only while
 // a step is 32 keys).  2 x 4096 tokens, 32/8 heads of 128, window 1024: 184 us
-// = 656 TFLOP/s of the visible pairs; 16384 tokens of 8/1 heads of 64 through a
-// window of 4096: 227 us.
+// = 656 TFLOP/s of the visible pairs (205 with the remainders of o stored for
+// the backward); 16384 tokens of 8/1 heads of 64 through a window of 4096:
+// 250 us = 483 TFLOP/s.
 template <typename T, int DP, int RT, int NW, int KS, typename KV>
 __global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (DP == 64 ? 3 : 2)) void attn_fwd_kernel(typename KV::Args args) {
     constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, BM = NW * RT * 16;
@@ -422,10 +423,6 @@ __global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (D
     }
 }
 
-#ifndef F1
-#define F1 4096
-#define F2 2048
-#endif
 // Row tiles over all sequences, and the grid of their items over 8 XCDs.
 void tiles_of(AttnArgs &a, int rows) {
     if (a.offsets)
@@ -438,12 +435,24 @@ void tiles_of(AttnArgs &a, int rows) {
 // Workgroups of 4 waves: two or three of them on a CU run out of step, and one's
 // products fall into another's exponentials.  (8 waves that share their tiles
 // were in step: 201 against 179 us at 2 x 4096 tokens, 32/8 heads of 128.)
-// Few rows leave SIMDs with less than two such waves: then 16 rows a wave, and
-// below that the keys in two halves, each with 4 waves of the workgroup.
+//
+// A wave of 32 rows (kWide) reads half as much of LDS per product as one of 16
+// (kNarrow), and is the faster when the rows give every SIMD as many as it
+// holds: 2 at head 128, 3 at 64.  With fewer rows twice as many waves are, and
+// below 2048 waves of 16 (two to a SIMD) the keys in two halves, each with 4
+// waves of the workgroup.  T tokens, causal, 32/8 heads, us:
+//             T    256    512   1024   1792   2560
+//   wide     64    9.7   14.9   25.1   39.8   54.4    128   13.3  20.9  36.6  58.7  80.9
+//   narrow         7.7   11.9   20.1   32.3   46.4           9.8  15.3  27.3  53.8  95.9
+//   halves         7.0    9.7   16.1   34.1   54.5           9.1  13.0  26.2  64.2 119.7
+// 16384 tokens of 8 heads of 64: wide 252, narrow 275.  Over the cache (4096
+// tokens, T newest, 32/8 heads of 64): halves 70, narrow 92, wide 111 at
+// T = 1024; 110, 105 and 109 at 1792.
 enum Form { kWide, kNarrow, kHalves };
+constexpr int kSimds = 1024;
 Form form_of(const AttnArgs &a) {
     const int64_t waves = (int64_t)(a.offsets ? a.tokens : a.q_len) * a.group * (a.offsets ? 1 : a.batch) * a.kv_heads / 16;
-    return waves >= F1 ? kWide : waves >= F2 ? kNarrow : kHalves;
+    return waves >= (a.dim <= 64 ? 6 : 4) * kSimds ? kWide : waves > 2 * kSimds ? kNarrow : kHalves;
 }
 
 template <typename T, int DP>
