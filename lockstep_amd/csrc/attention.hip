@@ -168,9 +168,9 @@ struct PagedKV {
 template <typename T, int DP, int RT, int NW, int KS, typename KV>
 __global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (DP == 64 ? 3 : 2)) void attn_fwd_kernel(typename KV::Args args) {
     constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, BM = NW * RT * 16;
-    // a row's maximum is followed only when it grows by a factor of 2^8: the
-    // probabilities stay below 2^8 and O is rescaled a few times per row
-    constexpr float kLazy = 8.f;
+    // a row's maximum is followed only when it grows by a factor of 2^8 (fp16:
+    // 2^4, below its range with the lift): O is rescaled a few times per row
+    constexpr float kLazy = kLift<T> > 0.f ? 4.f : 8.f;
     typedef typename Vec<T>::x8 X8;
     typedef typename Vec<T>::x4 X4;
     __shared__ __attribute__((aligned(16))) T s_kv[KS][2][2][kBN * DP];  // [group][keys, values][buffer]
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (D
                 const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[x] - top) * a.c);
                 m[x] = top;
                 limit[x] = top + lazy;
-                mc[x] = top == -INFINITY ? 0.f : top * a.c;
+                mc[x] = top == -INFINITY ? 0.f : top * a.c - kLift<T>;
                 l[x] *= alpha;
 #pragma unroll
                 for (int d = 0; d < ND; ++d) o[d][x] *= alpha;
@@ -419,7 +419,7 @@ __global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (D
         }
         if (a.lse && g == 0)
             a.lse[s.b * a.lse_b + h * a.lse_h + s.q0 + tok] =
-                sum > 0.f ? m[x] * a.c + __log2f(sum) : sum != sum ? sum : -INFINITY;
+                sum > 0.f ? m[x] * a.c - kLift<T> + __log2f(sum) : sum != sum ? sum : -INFINITY;
     }
 }
 

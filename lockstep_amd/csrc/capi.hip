@@ -850,7 +850,7 @@ static int kv_pool(const char *fn, const lsmx_kv_cache *c, lsmx::Pool *p) {
         return fail(LSMX_ERR_SHAPE, "%s: page=%lld must be a power of two, 16 to 1024", fn, (long long)c->page);
     if (c->head_dim != 64 && c->head_dim != 128)
         return fail(LSMX_ERR_SHAPE, "%s: head_dim=%lld must be 64 or 128", fn, (long long)c->head_dim);
-    if (c->pages >= lim || c->kv_heads >= lim || c->batch >= lim || c->max_pages * c->page >= lim ||
+    if (c->pages >= lim || c->kv_heads >= lim || c->batch >= lim || c->max_pages >= lim || c->max_pages * c->page >= lim ||
         c->batch * c->kv_heads >= lim)
         return fail(LSMX_ERR_SHAPE, "%s: too many pages, sequences or heads", fn);
     if (c->pages && (!c->k_codes || !c->k_scale || !c->v_codes || !c->v_scale))
@@ -874,7 +874,7 @@ int lsmx_kv_append(const lsmx_kv_cache *c, const void *k, const int64_t *k_strid
     if (int r = kv_pool(fn, c, &a.p)) return r;
     if (dtype != LSMX_BF16 && dtype != LSMX_F16) return fail(LSMX_ERR_DTYPE, "%s: dtype must be bf16 or fp16", fn);
     const int64_t lim = (int64_t)1 << 30;
-    if (tokens < 0 || tokens >= lim || per_seq < 0) return fail(LSMX_ERR_SHAPE, "%s: bad number of tokens", fn);
+    if (tokens < 0 || tokens >= lim || per_seq < 0 || per_seq >= lim) return fail(LSMX_ERR_SHAPE, "%s: bad number of tokens", fn);
     if (!offsets && tokens != per_seq * c->batch)
         return fail(LSMX_ERR_SHAPE, "%s: tokens=%lld is not per_seq=%lld for each of %lld sequences", fn,
                     (long long)tokens, (long long)per_seq, (long long)c->batch);
@@ -894,7 +894,7 @@ int lsmx_kv_append(const lsmx_kv_cache *c, const void *k, const int64_t *k_strid
 // What the keys of one call's rows span at most, whatever the lengths.
 static int64_t kv_span(const lsmx_kv_cache *c, int64_t q_len, int64_t window, int64_t sinks) {
     const int64_t cap = c->max_pages * c->page;
-    return window && window < cap && q_len + window + sinks < cap ? q_len + window + sinks : cap;
+    return window && window < cap && sinks < cap && q_len + window + sinks < cap ? q_len + window + sinks : cap;
 }
 
 // Splits, and the workspace: partial rows of the splits, then the rows' lse
@@ -924,8 +924,10 @@ static int kv_attend_check(const char *fn, const lsmx_kv_cache *c, int64_t q_len
         return fail(LSMX_ERR_SHAPE, "%s: heads=%lld must be a positive multiple of kv_heads=%lld", fn, (long long)heads,
                     (long long)c->kv_heads);
     if (window < 0 || sinks < 0) return fail(LSMX_ERR_ARG, "%s: negative window or sinks", fn);
-    const int64_t lim = (int64_t)1 << 30, rows = q_len * (heads / c->kv_heads), bh = c->batch * c->kv_heads;
-    if (q_len < 0 || q_len >= lim || heads >= lim || rows >= lim || (bh && (rows + 256) * bh >= lim) ||
+    const int64_t lim = (int64_t)1 << 30, bh = c->batch * c->kv_heads;
+    if (q_len < 0 || q_len >= lim || heads >= lim) return fail(LSMX_ERR_SHAPE, "%s: too many tokens or heads", fn);
+    const int64_t rows = q_len * (heads / c->kv_heads);
+    if (rows >= lim || (bh && (rows + 256) * bh >= lim) ||
         bh * (c->max_pages * c->page / 64 + 1) >= lim)
         return fail(LSMX_ERR_SHAPE, "%s: too many tokens, sequences or heads", fn);
     return LSMX_OK;
@@ -984,9 +986,9 @@ int lsmx_kv_evict(const lsmx_kv_cache *c, const float *weights, int64_t w_len, i
     lsmx::EvictArgs a{};
     if (int r = kv_pool(fn, c, &a.p)) return r;
     const int64_t lim = (int64_t)1 << 30;
-    if (keep < 1 || keep >= lim || sinks < 0 || recent < 0 || sinks + recent > keep)
+    if (keep < 1 || keep >= lim || sinks < 0 || recent < 0 || sinks > keep || recent > keep - sinks)
         return fail(LSMX_ERR_ARG, "%s: needs 1 <= keep and sinks + recent <= keep", fn);
-    if (out_max_pages < 0 || out_max_pages * c->page >= lim) return fail(LSMX_ERR_SHAPE, "%s: bad out_max_pages", fn);
+    if (out_max_pages < 0 || out_max_pages >= lim || out_max_pages * c->page >= lim) return fail(LSMX_ERR_SHAPE, "%s: bad out_max_pages", fn);
     const int64_t cap = c->max_pages * c->page, most = keep < cap ? keep : cap;
     if (out_max_pages * c->page < most)
         return fail(LSMX_ERR_SHAPE, "%s: out_table holds %lld tokens, %lld may stay", fn,

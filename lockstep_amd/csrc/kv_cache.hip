@@ -290,7 +290,7 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(T, __bf16) 
 #pragma unroll
                 for (int d = 0; d < ND; ++d) o[d][y] *= alpha;
             }
-            const float mc = m[y] == -INFINITY ? 0.f : m[y] * a.c;
+            const float mc = m[y] == -INFINITY ? 0.f : m[y] * a.c - kLift<T>;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(T, __bf16) 
 #pragma unroll
                     for (int e = 0; e < HD / 16; ++e) op[e] = (T)(acc[e] * inv);
                     if (a.lse && half == 0 && (threadIdx.x & 15) == 0)
-                        a.lse[b * a.lse_b + h * a.lse_h + tok] = tot > 0.f ? mc + __log2f(tot) : tot != tot ? tot : -INFINITY;
+                        a.lse[b * a.lse_b + h * a.lse_h + tok] = tot > 0.f ? mc - kLift<T> + __log2f(tot) : tot != tot ? tot : -INFINITY;
                 }
             }
         }
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs x) {
     const float inv = tot > 0.f || tot != tot ? 1.f / tot : 0.f;
     ((T *)a.o)[b * a.o_b + tok * a.o_t + h * a.o_h + threadIdx.x] = (T)(sum * inv);
     if (a.lse && threadIdx.x == 0)
-        a.lse[b * a.lse_b + h * a.lse_h + tok] = tot > 0.f ? mc + __log2f(tot) : tot != tot ? tot : -INFINITY;
+        a.lse[b * a.lse_b + h * a.lse_h + tok] = tot > 0.f ? mc - kLift<T> + __log2f(tot) : tot != tot ? tot : -INFINITY;
 }
 
 // ------------------------------------------------------------------ weights

@@ -240,6 +240,13 @@ struct EvictArgs {
     float *new_weights;
 };
 
+// Probabilities enter the product with the values relative to their row's
+// largest so far.  fp16 holds 2^-24 to 65504, so there they are lifted by
+// 2^kLift, with the sum of their row: one of 2^-25 still has all its bits, and what
+// a lost one leaves out is at most 2^-36 of the largest.  bf16 has fp32's range.
+template <typename T>
+constexpr float kLift = __is_same(T, _Float16) ? 11.f : 0.f;
+
 // The 8 elements of four bytes of codes, times 2^e of their block (e: its E8M0
 // byte).  Exact in bf16; in fp16 (the operands of fp16 rows) too for values that
 // fp16 holds.  Blocks above it are clipped to its range, so that no
