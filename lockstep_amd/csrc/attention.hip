@@ -40,6 +40,7 @@ struct DenseKV {
     static constexpr int NC = DP / 8, NU = kBN * NC / 64 / NW;  // loads of a wave, each of K and V
     static constexpr bool kHoles = false;
     typedef AttnArgs Args;
+    LSMX_DEV static int splits(const Args &) { return 1; }
     const T *k, *v;
     int64_t k_t, v_t;
     int k_len;
@@ -80,6 +81,7 @@ struct PagedKV {
     static constexpr int NC = DP / 8, NQ = DP / 32;  // words of codes of a thread
     static constexpr bool kHoles = true;
     typedef AttendArgs Args;
+    LSMX_DEV static int splits(const Args &a) { return a.splits; }
     const Pool *p;
     int b, h, k_len, row, part;
     uint32_t kr[NQ], vr[NQ];
@@ -166,7 +168,7 @@ struct PagedKV {
 // the backward); 16384 tokens of 8/1 heads of 64 through a window of 4096:
 // 250 us = 483 TFLOP/s.
 template <typename T, int DP, int RT, int NW, int KS, typename KV>
-__global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (DP == 64 ? 3 : 2)) void attn_fwd_kernel(typename KV::Args args) {
+__global__ __launch_bounds__(NW * KS * 64, DP == 64 && !KV::kHoles ? 3 : 2) void attn_fwd_kernel(typename KV::Args args) {
     constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, BM = NW * RT * 16;
     // a row's maximum is followed only when it grows by a factor of 2^8 (fp16:
     // 2^4, below its range with the lift): O is rescaled a few times per row
@@ -177,9 +179,10 @@ __global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (D
     __shared__ int s_held[KS][2][KV::kHoles ? kBN : 1];
 
     const AttnArgs &a = KV::attn(args);
-    const int item = xcd_item(blockIdx.x, a.per);
-    if (item >= a.tiles * a.kv_heads) return;
-    const int hkv = item / a.tiles;
+    // tiles of one share of the keys side by side
+    const int item = xcd_item(blockIdx.x, a.per), splits = KV::splits(args);
+    if (item >= a.tiles * a.kv_heads * splits) return;
+    const int rest = item / a.tiles, hkv = rest / splits, share = rest - hkv * splits;
     Seq s;
     if (!KV::find(args, item % a.tiles, BM, s)) return;
 
@@ -194,11 +197,13 @@ __global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (D
     const int pmax = div_by(min(row0 + BM, rows) - 1, a.by_group) + s.shift;
     const int hi = min(pmax + 1, s.k_len), lo = a.window ? max(0, pmin - a.window + 1) : 0;
     const int t_sink = (min(a.sinks, hi) + kBN - 1) / kBN, t_hi = hi > 0 ? (hi + kBN - 1) / kBN : 0;
-    const int t_lo = max(lo / kBN, t_sink), nt = t_sink + max(0, t_hi - t_lo), rounds = (nt + KS - 1) / KS;
+    const int t_lo = max(lo / kBN, t_sink), nt = t_sink + max(0, t_hi - t_lo);
+    const int first = (int)((int64_t)nt * share / splits), last = (int)((int64_t)nt * (share + 1) / splits);
+    const int rounds = (last - first + KS - 1) / KS;
     // first key of the group's tile of round k, -1 past the last
     auto start_of = [&](int k) {
-        const int i = k * KS + group;
-        return i < nt ? (i < t_sink ? i : t_lo + i - t_sink) * kBN : -1;
+        const int i = first + k * KS + group;
+        return i < last ? (i < t_sink ? i : t_lo + i - t_sink) * kBN : -1;
     };
     // and the positions of this wave's rows
     const int wmin = div_by(min(wrow0, rows - 1), a.by_group) + s.shift;
@@ -401,6 +406,15 @@ __global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (D
         const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
         const int row = wrow0 + r + 16 * x;
         if (row >= rows) continue;
+        if constexpr (KV::kHoles) {
+            if (splits > 1) {
+                const int64_t at = ((int64_t)(s.b * a.kv_heads + hkv) * splits + share) * rows + row;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) *(f32x4 *)(args.part + at * DP + d * 16 + g * 4) = o[d][x];
+                if (g == 0) args.part_m[at * 2] = m[x], args.part_m[at * 2 + 1] = sum;
+                continue;
+            }
+        }
         const int tok = div_by(row, a.by_group), h = hkv * a.group + row - tok * a.group;
         const int64_t o_at = s.b * a.o_b + (s.q0 + tok) * a.o_t + h * a.o_h;
 #pragma unroll
@@ -424,12 +438,12 @@ __global__ __launch_bounds__(NW * KS * 64, KV::kHoles ? (DP == 64 ? 2 : KS) : (D
 }
 
 // Row tiles over all sequences, and the grid of their items over 8 XCDs.
-void tiles_of(AttnArgs &a, int rows) {
+void tiles_of(AttnArgs &a, int rows, int splits = 1) {
     if (a.offsets)
         a.tiles = (int)(((int64_t)a.tokens * a.group + rows - 1) / rows) + a.batch + 2;
     else
         a.tiles = (int)(((int64_t)a.q_len * a.group + rows - 1) / rows) * a.batch;
-    a.per = (int)(((int64_t)a.tiles * a.kv_heads + 7) / 8);
+    a.per = (int)(((int64_t)a.tiles * a.kv_heads * splits + 7) / 8);
 }
 
 // Workgroups of 4 waves: two or three of them on a CU run out of step, and one's
@@ -445,9 +459,7 @@ void tiles_of(AttnArgs &a, int rows) {
 //   wide     64    9.7   14.9   25.1   39.8   54.4    128   13.3  20.9  36.6  58.7  80.9
 //   narrow         7.7   11.9   20.1   32.3   46.4           9.8  15.3  27.3  53.8  95.9
 //   halves         7.0    9.7   16.1   34.1   54.5           9.1  13.0  26.2  64.2 119.7
-// 16384 tokens of 8 heads of 64: wide 252, narrow 275.  Over the cache (4096
-// tokens, T newest, 32/8 heads of 64): halves 70, narrow 92, wide 111 at
-// T = 1024; 110, 105 and 109 at 1792.
+// 16384 tokens of 8 heads of 64: wide 252, narrow 275.
 enum Form { kWide, kNarrow, kHalves };
 constexpr int kSimds = 1024;
 Form form_of(const AttnArgs &a) {
@@ -469,17 +481,16 @@ hipError_t fwd(AttnArgs a, hipStream_t s) {
     return hipGetLastError();
 }
 
+// Over the cache: 16 rows a wave whatever their number (32, which expand the
+// codes half as often, hold one wave per SIMD at head 128 and two at 64: 2 x
+// 4096 newest tokens of 32/8 heads of 128 took 501 us against 428, 64: 211 both),
+// and the keys in shares where the rows are too few for the chip: 600 newest tokens of two
+// sequences, 16/4 heads of 64 in fp16, window 2048, in 3 shares 38 us and 6 to
+// join them, in two halves of a workgroup 49.
 template <typename T, int DP>
 hipError_t chunk(AttendArgs x, hipStream_t s) {
-    const Form f = form_of(x.a);
-    tiles_of(x.a, f == kWide ? 128 : 64);
-    const unsigned grid = (unsigned)x.a.per * 8;
-    if (f == kWide)
-        attn_fwd_kernel<T, DP, 2, 4, 1, PagedKV<T, DP>><<<grid, 256, 0, s>>>(x);
-    else if (f == kNarrow)
-        attn_fwd_kernel<T, DP, 1, 4, 1, PagedKV<T, DP>><<<grid, 256, 0, s>>>(x);
-    else
-        attn_fwd_kernel<T, DP, 1, 4, 2, PagedKV<T, DP>><<<grid, 512, 0, s>>>(x);
+    tiles_of(x.a, 64, x.splits);
+    attn_fwd_kernel<T, DP, 1, 4, 1, PagedKV<T, DP>><<<(unsigned)x.a.per * 8, 256, 0, s>>>(x);
     return hipGetLastError();
 }
 

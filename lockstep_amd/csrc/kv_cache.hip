@@ -365,6 +365,45 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(T, __bf16) 
     }
 }
 
+// Joins up to 16 shares of a row: 16 threads over the vector, 16 rows a
+// workgroup.  Bound by the shares' bytes: 19200 rows of 3 shares of 64, 5.6 us.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void kv_join_few_kernel(AttendArgs x) {
+    constexpr int NE = DP / 16;
+    const AttnArgs &a = x.a;
+    const int rows = a.q_len * a.group, c = (threadIdx.x & 15) * NE;
+    const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (i >= (int64_t)rows * a.batch * a.kv_heads) return;
+    const int bh = (int)(i / rows), row = (int)(i - (int64_t)bh * rows), b = bh / a.kv_heads, hkv = bh - b * a.kv_heads;
+    const int64_t at0 = (int64_t)bh * x.splits * rows + row;
+    float top = -INFINITY;
+    for (int s = 0; s < x.splits; ++s) top = fmaxf(top, x.part_m[(at0 + (int64_t)s * rows) * 2]);
+    const float mc = top == -INFINITY ? 0.f : top * a.c;
+    float tot = 0.f, acc[NE];
+#pragma unroll
+    for (int e = 0; e < NE; ++e) acc[e] = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < x.splits; ++s) {
+        const int64_t at = at0 + (int64_t)s * rows;
+        const float f = __builtin_amdgcn_exp2f(x.part_m[at * 2] * a.c - mc);
+        tot = __builtin_fmaf(x.part_m[at * 2 + 1], f, tot);
+#pragma unroll
+        for (int e = 0; e < NE; e += 4) {
+            const f32x4 w = *(const f32x4 *)(x.part + at * DP + c + e);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[e + k] = __builtin_fmaf(w[k], f, acc[e + k]);
+        }
+    }
+    const int tok = div_by(row, a.by_group), h = hkv * a.group + row - tok * a.group;
+    const float inv = tot > 0.f || tot != tot ? 1.f / tot : 0.f;
+    T *o = (T *)a.o + b * a.o_b + tok * a.o_t + h * a.o_h + c;
+#pragma unroll
+    for (int e = 0; e < NE; e += 4)
+        *(typename Vec<T>::x4 *)(o + e) = typename Vec<T>::x4{(T)(acc[e] * inv), (T)(acc[e + 1] * inv), (T)(acc[e + 2] * inv), (T)(acc[e + 3] * inv)};
+    if (a.lse && c == 0)
+        a.lse[b * a.lse_b + h * a.lse_h + tok] = tot > 0.f ? mc - kLift<T> + __log2f(tot) : tot != tot ? tot : -INFINITY;
+}
+
 // Joins the shares of one row: 16 threads over the vector, 16 over the shares.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs x) {
@@ -492,11 +531,16 @@ __global__ __launch_bounds__(256) void kv_weights_kernel(AttendArgs x) {
 }
 
 // Many rows: a workgroup owns 64 keys, whose operands stay in registers, and
-// its waves take tiles of 16 rows in turn; their sums are joined in LDS.
-template <typename T, int DP>
-__global__ __launch_bounds__(512) void kv_weights_rows_kernel(AttendArgs x) {
+// its waves take tiles of 16 rows in turn; their sums are joined in LDS.  Bound
+// by the loads of q in flight and, below some 500 workgroups, by their number:
+// 12 waves each then, else 4.  16/4 heads, T newest tokens of B sequences, us:
+//     head 64:  T = 600, B = 2, window 2048 (340 at work)  4 waves 35, 8: 34, 12: 31
+//               T = 600, B = 2 of 5000 (632)               4 waves 32, 8: 44, 12: 40
+//     head 128: T = 20, B = 8 of 4096 (2048)               4 waves 18, 8: 45, 12: 39
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void kv_weights_rows_kernel(AttendArgs x) {
     constexpr int NS = DP / 32;
-    __shared__ __attribute__((aligned(16))) float s_sum[8][64];
+    __shared__ __attribute__((aligned(16))) float s_sum[NW][64];
     typedef typename Vec<T>::x8 X8;
     const AttnArgs &a = x.a;
     const Pool &p = x.p;
@@ -536,7 +580,7 @@ __global__ __launch_bounds__(512) void kv_weights_rows_kernel(AttendArgs x) {
     const int row_hi = tok_hi * a.group;
     // U tiles of rows at a time, the next U in flight: one tile's work is less
     // than a load's latency
-    constexpr int U = 256 / DP;
+    constexpr int U = 128 / DP, kStep = NW * 16;
     struct Row {
         X8 q[NS];
         float lse;
@@ -545,7 +589,7 @@ __global__ __launch_bounds__(512) void kv_weights_rows_kernel(AttendArgs x) {
     auto load = [&](int r0, Row (&w)[U]) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int row = r0 + u * 128 + r;
+            const int row = r0 + u * kStep + r;
             const bool in = row < row_hi;
             const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
             const T *qp = (const T *)a.q + b * a.q_b + tok * a.q_t + h * a.q_h + g * (DP / 4);
@@ -558,21 +602,31 @@ __global__ __launch_bounds__(512) void kv_weights_rows_kernel(AttendArgs x) {
     Row cur[U], nxt[U];
     int r0 = tok_lo * a.group + wave * 16;
     load(r0, cur);
-    for (; r0 < row_hi; r0 += 128 * U) {
-        load(r0 + 128 * U, nxt);
+    for (; r0 < row_hi; r0 += kStep * U) {
+        load(r0 + kStep * U, nxt);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+            auto add = [&](auto all) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                f32x4 st{0, 0, 0, 0};
+                for (int t = 0; t < 4; ++t) {
+                    f32x4 st{0, 0, 0, 0};
 #pragma unroll
-                for (int s = 0; s < NS; ++s) st = mfma(kf[t][s], cur[u].q[s], st);
+                    for (int s = 0; s < NS; ++s) st = mfma(kf[t][s], cur[u].q[s], st);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(st[e], a.c, -cur[u].lse));
-                    sum[t][e] += (uint32_t)(cur[u].pos - (j0 + t * 16 + g * 4 + e)) <= span[t][e] ? v : 0.f;
+                    for (int e = 0; e < 4; ++e) {
+                        const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(st[e], a.c, -cur[u].lse));
+                        if constexpr (decltype(all)::value)
+                            sum[t][e] += v;
+                        else
+                            sum[t][e] += (uint32_t)(cur[u].pos - (j0 + t * 16 + g * 4 + e)) <= span[t][e] ? v : 0.f;
+                    }
                 }
-            }
+            };
+            // every row sees every key: most tiles
+            if (__all(cur[u].pos >= j0 + 63 && (!a.window || cur[u].pos < j0 + a.window || j0 + 63 < a.sinks)))
+                add(BoolC<true>{});
+            else
+                add(BoolC<false>{});
             cur[u] = nxt[u];
         }
     }
@@ -588,7 +642,7 @@ __global__ __launch_bounds__(512) void kv_weights_rows_kernel(AttendArgs x) {
     if (threadIdx.x < 64 && at < len) {
         float all = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) all += s_sum[i][threadIdx.x];
+        for (int i = 0; i < NW; ++i) all += s_sum[i][threadIdx.x];
         x.weights[(int64_t)bh * x.w_len + at] += all;
     }
 }
@@ -817,7 +871,16 @@ hipError_t attend(const AttendArgs &x, hipStream_t s) {
         kv_decode_kernel<T, DP, 1><<<grid, 256, 0, s>>>(x);
     else
         kv_decode_kernel<T, DP, 2><<<grid * ((rows + 31) / 32), 256, 0, s>>>(x);
-    if (x.splits > 1) kv_join_kernel<T, DP><<<(unsigned)(rows * bh), 256, 0, s>>>(x);
+    return hipGetLastError();
+}
+
+template <typename T, int DP>
+hipError_t join(const AttendArgs &x, hipStream_t s) {
+    const int64_t rows = (int64_t)x.a.q_len * x.a.group * x.a.batch * x.a.kv_heads;
+    if (x.splits > 16)
+        kv_join_kernel<T, DP><<<(unsigned)rows, 256, 0, s>>>(x);
+    else if (x.splits > 1)
+        kv_join_few_kernel<T, DP><<<(unsigned)((rows + 15) / 16), 256, 0, s>>>(x);
     return hipGetLastError();
 }
 
@@ -831,8 +894,14 @@ hipError_t weights(AttendArgs x, hipStream_t s) {
         kv_weights_kernel<T, DP, 2><<<grid, 256, 0, s>>>(x);
     else if (rows <= kDecodeRows)
         kv_weights_kernel<T, DP, 4><<<grid, 256, 0, s>>>(x);
-    else
-        kv_weights_rows_kernel<T, DP><<<(unsigned)(((x.p.max_pages << x.p.page_shift) + 63) / 64) * bh, 512, 0, s>>>(x);
+    else {
+        const int64_t cap = (int64_t)x.p.max_pages << x.p.page_shift, reach = (int64_t)x.a.q_len + x.a.window + x.a.sinks;
+        const unsigned tiles = (unsigned)((cap + 63) / 64) * bh;
+        if ((x.a.window && reach < cap ? reach : cap) / 64 * bh < 512)
+            kv_weights_rows_kernel<T, DP, 12><<<tiles, 768, 0, s>>>(x);
+        else
+            kv_weights_rows_kernel<T, DP, 4><<<tiles, 256, 0, s>>>(x);
+    }
     return hipGetLastError();
 }
 
@@ -850,20 +919,24 @@ hipError_t launch_kv_append(const AppendArgs &a, int dtype, hipStream_t s) {
 }
 
 // Shares of the keys: enough workgroups for 4 per CU, each of at least 256
-// keys (2 tiles per wave).
+// keys (2 tiles per wave).  A workgroup has all rows of a key head, or of many
+// rows 64; there the shares' sums are most of the bytes, and no more than 16 are
+// made (1.5 times as many workgroups: 37 + 7 us for 38 + 6, half: 43 + 5).
 int kv_attend_splits(int batch, int kv_heads, int rows, int64_t keys) {
-    if (rows > kDecodeRows) return 1;
-    const int64_t bh = (int64_t)batch * kv_heads;
-    const int64_t by_cu = (1024 + bh - 1) / bh, by_len = (keys + 255) / 256;
-    const int64_t n = by_cu < by_len ? by_cu : by_len;
-    return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
+    const int64_t bh = (int64_t)batch * kv_heads, items = rows > kDecodeRows ? bh * ((rows + 63) / 64) : bh;
+    const int64_t by_cu = rows > kDecodeRows ? (1024 + items / 2) / items : (1024 + items - 1) / items, by_len = (keys + 255) / 256;
+    const int64_t n = by_cu < by_len ? by_cu : by_len, most = rows > kDecodeRows ? 16 : 256;
+    return (int)(n < 1 ? 1 : n > most ? most : n);
 }
 
-
 hipError_t launch_kv_attend(const AttendArgs &x, int dtype, hipStream_t s) {
-    if (x.a.q_len * x.a.group > kDecodeRows) return launch_kv_chunk(x, dtype, s);
-    if (dtype == LSMX_BF16) return x.p.dim == 64 ? attend<__bf16, 64>(x, s) : attend<__bf16, 128>(x, s);
-    return x.p.dim == 64 ? attend<_Float16, 64>(x, s) : attend<_Float16, 128>(x, s);
+    const bool wide = x.p.dim == 128, bf16 = dtype == LSMX_BF16;
+    const hipError_t e = x.a.q_len * x.a.group > kDecodeRows ? launch_kv_chunk(x, dtype, s)
+                         : bf16                              ? (wide ? attend<__bf16, 128>(x, s) : attend<__bf16, 64>(x, s))
+                                : (wide ? attend<_Float16, 128>(x, s) : attend<_Float16, 64>(x, s));
+    if (e != hipSuccess) return e;
+    return bf16 ? (wide ? join<__bf16, 128>(x, s) : join<__bf16, 64>(x, s))
+                : (wide ? join<_Float16, 128>(x, s) : join<_Float16, 64>(x, s));
 }
 
 hipError_t launch_kv_weights(const AttendArgs &x, int dtype, hipStream_t s) {

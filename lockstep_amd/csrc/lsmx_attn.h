@@ -215,8 +215,8 @@ struct AttendArgs {
     Pool p;
     float *weights;       // [batch, kv_heads, w_len], or null
     int64_t w_len;
-    int splits;           // decode: workgroups per sequence and key head
-    float *part, *part_m; // decode: [batch kv_heads splits rows][DP] and [..][2]
+    int splits;           // shares of the keys, each with workgroups of its own
+    float *part, *part_m; // their sums: [batch kv_heads splits rows][DP] and [..][2]
 };
 
 struct AppendArgs {
