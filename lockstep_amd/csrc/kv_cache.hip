@@ -181,7 +181,7 @@ LSMX_DEV void scores(const Codes<DP> &k, const typename Vec<T>::x8 (&q)[RT][DP /
     }
 }
 
-// One workgroup: one sequence and key head, RT x 16 of its rows, a share of the keys;
+// One workgroup: one sequence and key head, its up to RT x 16 rows, a share of the keys;
 // its 4 waves take tiles of 32 keys in turn and are joined at the end.  A wave
 // has the next tile's codes in flight while it works on one, and the page
 // numbers of the tile after that.
@@ -198,10 +198,8 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(T, __bf16) 
     const AttnArgs &a = x.a;
     const Pool &p = x.p;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
-    const int rows = a.q_len * a.group, blocks = (rows + RT * 16 - 1) / (RT * 16);
-    // the blocks of rows of one share side by side: they read the same keys
-    const int rest = blockIdx.x / blocks, row0 = (blockIdx.x - rest * blocks) * RT * 16;
-    const int bh = rest / x.splits, sp = rest - bh * x.splits, b = bh / a.kv_heads, hkv = bh - b * a.kv_heads;
+    const int rows = a.q_len * a.group;
+    const int bh = blockIdx.x / x.splits, sp = blockIdx.x - bh * x.splits, b = bh / a.kv_heads, hkv = bh - b * a.kv_heads;
     const Tiles tiles(x, b);
     const int i0 = (int)((int64_t)tiles.n * sp / x.splits), i1 = (int)((int64_t)tiles.n * (sp + 1) / x.splits);
 
@@ -216,7 +214,7 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(T, __bf16) 
     int pos[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-        const int row = row0 + t * 16 + r;
+        const int row = t * 16 + r;
         load_rows<T, DP>(a, b, hkv, row, g, row < rows, q[t]);
         pos[t] = row < rows ? div_by(row, a.by_group) + tiles.len - a.q_len : -1;
     }
@@ -330,7 +328,7 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(T, __bf16) 
             for (int d = 0; d < ND / 2; ++d)
                 *(f32x4 *)(so + (wave * 16 + r) * HD + d * 16 + g * 4) = o[half * (ND / 2) + d][y];
             __syncthreads();
-            const int row = threadIdx.x >> 4, c = (threadIdx.x & 15) * (HD / 16), full = row0 + y * 16 + row;
+            const int row = threadIdx.x >> 4, c = (threadIdx.x & 15) * (HD / 16), full = y * 16 + row;
             float top = -INFINITY;
 #pragma unroll
             for (int w = 0; w < 4; ++w) top = fmaxf(top, s_m[w][row]);
@@ -459,8 +457,9 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs x) {
 // but their short runs made that pass 118 us from 80 at 64 x 8192 tokens of 8
 // key heads and 4 rows, and adding them took 42, where this takes 60.)
 //
-// Few rows: their q stays in registers, and the waves run over the keys as in
-// kv_decode_kernel.
+// Few rows: the q of RT x 16 stays in registers, and the waves run over the keys
+// as in kv_decode_kernel, once for each such block.  Bound by the codes' bytes:
+// 64 x 8192 tokens of 8 key heads of 128 and 4 rows each, 60 us = 5.3 TB/s.
 LSMX_DEV float sum_16(float x) {  // over the 16 lanes of a row of lanes
     x += u2f(__builtin_amdgcn_update_dpp(0, f2u(x), 0xB1, 0xF, 0xF, true));   // quad_perm 1,0,3,2
     x += u2f(__builtin_amdgcn_update_dpp(0, f2u(x), 0x4E, 0xF, 0xF, true));   // quad_perm 2,3,0,1
@@ -479,54 +478,56 @@ __global__ __launch_bounds__(256) void kv_weights_kernel(AttendArgs x) {
     const int rows = a.q_len * a.group;
     const Tiles tiles(x, b);
     const int i0 = (int)((int64_t)tiles.n * sp / x.splits), i1 = (int)((int64_t)tiles.n * (sp + 1) / x.splits);
-    Keys<DP, false> cur, nxt;
-    int i = i0 + wave;
-    if (i >= i1) return;
-    Walk walk(p, tiles, b, i, i1);
-    walk.find(i, cur);
-    cur.load(p, hkv, g, r);
-    X8 q[RT][NS];
-    int pos[RT], low[RT];
-    float lse[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int row = t * 16 + r;
-        const bool in = row < rows;
-        load_rows<T, DP>(a, b, hkv, row, g, in, q[t]);
-        const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
-        pos[t] = in ? tok + tiles.len - a.q_len : -1;
-        low[t] = window_low(pos[t], a.window);
-        lse[t] = a.lse[b * a.lse_b + h * a.lse_h + tok];
-    }
+    if (i0 + wave >= i1) return;
     float *w = x.weights + (int64_t)bh * x.w_len;
-    for (; i < i1; i += 4) {
-        const int j0 = cur.j0;
-        // lane r < 8 keeps the sums of key 16 (r / 4) + 4g + r % 4
-        const int mine = j0 + (r >> 2) * 16 + g * 4 + (r & 3);
-        const bool held = r < 8 && mine < tiles.len && (r < 4 ? cur.pg[0] : cur.pg[1]) >= 0;
-        float before = held ? w[mine] : 0.f;
-        // after the last tile this one again, from the cache: the loads of all
-        // rounds are alike, and the wait is for the round before
-        walk.find(i + 4 < i1 ? i + 4 : i, nxt);
-        nxt.load(p, hkv, g, r);
-        float own = 0.f;
+    for (int row0 = 0; row0 < rows; row0 += RT * 16) {
+        Keys<DP, false> cur, nxt;
+        int i = i0 + wave;
+        Walk walk(p, tiles, b, i, i1);
+        walk.find(i, cur);
+        cur.load(p, hkv, g, r);
+        X8 q[RT][NS];
+        int pos[RT], low[RT];
+        float lse[RT];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            f32x4 st[RT], sum{0, 0, 0, 0};
-            scores<T, DP, RT>(cur.k[t], q, st);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-#pragma unroll
-                for (int y = 0; y < RT; ++y) {
-                    const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(st[y][e], a.c, -lse[y]));
-                    sum[e] += sees(j0 + t * 16 + g * 4 + e, pos[y], low[y], a.sinks) ? v : 0.f;
-                }
-                const float all = sum_16(sum[e]);
-                own = r == t * 4 + e ? all : own;
-            }
+        for (int t = 0; t < RT; ++t) {
+            const int row = row0 + t * 16 + r;
+            const bool in = row < rows;
+            load_rows<T, DP>(a, b, hkv, row, g, in, q[t]);
+            const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
+            pos[t] = in ? tok + tiles.len - a.q_len : -1;
+            low[t] = window_low(pos[t], a.window);
+            lse[t] = a.lse[b * a.lse_b + h * a.lse_h + tok];
         }
-        if (held) w[mine] = before + own;
-        cur = nxt;
+        for (; i < i1; i += 4) {
+            const int j0 = cur.j0;
+            // lane r < 8 keeps the sums of key 16 (r / 4) + 4g + r % 4
+            const int mine = j0 + (r >> 2) * 16 + g * 4 + (r & 3);
+            const bool held = r < 8 && mine < tiles.len && (r < 4 ? cur.pg[0] : cur.pg[1]) >= 0;
+            float before = held ? w[mine] : 0.f;
+            // after the last tile this one again, from the cache: the loads of all
+            // rounds are alike, and the wait is for the round before
+            walk.find(i + 4 < i1 ? i + 4 : i, nxt);
+            nxt.load(p, hkv, g, r);
+            float own = 0.f;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                f32x4 st[RT], sum{0, 0, 0, 0};
+                scores<T, DP, RT>(cur.k[t], q, st);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                    for (int y = 0; y < RT; ++y) {
+                        const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(st[y][e], a.c, -lse[y]));
+                        sum[e] += sees(j0 + t * 16 + g * 4 + e, pos[y], low[y], a.sinks) ? v : 0.f;
+                    }
+                    const float all = sum_16(sum[e]);
+                    own = r == t * 4 + e ? all : own;
+                }
+            }
+            if (held) w[mine] = before + own;
+            cur = nxt;
+        }
     }
 }
 
@@ -870,7 +871,7 @@ hipError_t attend(const AttendArgs &x, hipStream_t s) {
     if (rows <= 16)
         kv_decode_kernel<T, DP, 1><<<grid, 256, 0, s>>>(x);
     else
-        kv_decode_kernel<T, DP, 2><<<grid * ((rows + 31) / 32), 256, 0, s>>>(x);
+        kv_decode_kernel<T, DP, 2><<<grid, 256, 0, s>>>(x);
     return hipGetLastError();
 }
 
@@ -887,20 +888,28 @@ hipError_t join(const AttendArgs &x, hipStream_t s) {
 template <typename T, int DP>
 hipError_t weights(AttendArgs x, hipStream_t s) {
     const int rows = x.a.q_len * x.a.group, bh = x.a.batch * x.a.kv_heads;
-    const dim3 grid((unsigned)x.splits * bh);
+    const int64_t cap = (int64_t)x.p.max_pages << x.p.page_shift, reach = (int64_t)x.a.q_len + x.a.window + x.a.sinks;
+    const int64_t keys = x.a.window && reach < cap ? reach : cap;
+    x.splits = kv_attend_splits(x.a.batch, x.a.kv_heads, 1, keys);
+    const unsigned grid = (unsigned)x.splits * bh;
+    // up to 64 rows are one pass over the codes; up to three passes are still
+    // faster than tiles of keys that each wait for the rows, where those would be
+    // many.  64 x 2048 tokens of 4 key heads of 128: 24, 44, 64, 83 us for 64, 128,
+    // 192, 256 rows, in tiles 60, 73, 83, 93; 8 x 4096 tokens: 10, 16, 24, 29 and 16, 20, 25,
+    // 28; one sequence (64 tiles a head): 128 rows 12 and 6.
+    const bool many = keys / 64 * bh >= 512;
     if (rows <= 16)
         kv_weights_kernel<T, DP, 1><<<grid, 256, 0, s>>>(x);
     else if (rows <= 32)
         kv_weights_kernel<T, DP, 2><<<grid, 256, 0, s>>>(x);
-    else if (rows <= kDecodeRows)
+    else if (rows <= (many ? 192 : 64))
         kv_weights_kernel<T, DP, 4><<<grid, 256, 0, s>>>(x);
     else {
-        const int64_t cap = (int64_t)x.p.max_pages << x.p.page_shift, reach = (int64_t)x.a.q_len + x.a.window + x.a.sinks;
         const unsigned tiles = (unsigned)((cap + 63) / 64) * bh;
-        if ((x.a.window && reach < cap ? reach : cap) / 64 * bh < 512)
-            kv_weights_rows_kernel<T, DP, 12><<<tiles, 768, 0, s>>>(x);
-        else
+        if (many)
             kv_weights_rows_kernel<T, DP, 4><<<tiles, 256, 0, s>>>(x);
+        else
+            kv_weights_rows_kernel<T, DP, 12><<<tiles, 768, 0, s>>>(x);
     }
     return hipGetLastError();
 }

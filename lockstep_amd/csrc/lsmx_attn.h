@@ -272,9 +272,11 @@ LSMX_DEV typename Vec<T>::x8 fp4x8(uint32_t w, float sc) {
     return fp4x8_to(w, sc, typename Vec<T>::x8{});
 }
 
-// Rows (tokens x heads of a key head) up to which the keys of a sequence are
-// split over workgroups; more rows run in tiles of 128.
-constexpr int kDecodeRows = 64;
+// Rows (tokens x heads of a key head) up to which each wave of the cache
+// attention has them all; more run in tiles of 64, 16 a wave.  With 64 rows: 27
+// us in tiles, 34 in blocks of 32 (8 x 4096 tokens of 4 key heads of 128), 20 and 17
+// for one such sequence; with 32 the tiles are mostly padding.
+constexpr int kDecodeRows = 32;
 // The number of the first tile (as find_tile counts them) of sequence s.
 LSMX_DEV int first_tile(const AttnArgs &a, const Seq &s, int size, int mult) {
     if (!a.offsets) return s.b * ((a.q_len * mult + size - 1) / size);

@@ -276,3 +276,28 @@ def test_layer_served(dev):
         layer.new_cache(1, 16, page_size=16).evict(4)
     with pytest.raises(RuntimeError, match="pack"):
         layer_of(dev).step(r(2, 1, 512), cache)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,T,D,window", [(2, 8, 64, None), (3, 12, 128, 300), (2, 17, 64, 500), (20, 30, 64, None),
+                                          (18, 45, 128, 900), (20, 52, 64, None), (18, 60, 128, None)])
+def test_cache_weights_of_some_rows(B, T, D, window, dt, dev):
+    """32 to 240 rows of a key head over few and many keys: each form of the
+    weights' pass, and the shares of attention's."""
+    from lockstep_amd import kv_cache as kc
+    H, Hkv, lens = 8, 2, [1000 - 7 * b for b in range(B)]
+    pages, table, lengths, (kv, vv), _ = filled(lens, Hkv, D, 64, dt, dev, seed=T)
+    q = inputs(B, T, 1, H, Hkv, D, dt, dev, seed=7)[0]
+    w0 = torch.rand((B, Hkv, table.shape[1] * 64), generator=torch.Generator(device=dev).manual_seed(1), device=dev)
+    w = w0.clone()
+    o = kc.attend(q, pages, table, lengths, window=window, sinks=3, weights=w)
+    for b in (0, B - 1):
+        ro, mag, rw, err = cache_formula(q[b], kv[b], vv[b], window, 3, 1.0 / math.sqrt(D))
+        bad = (o[b].double() - ro).abs() - 4 * U[dt] * mag - 1e-7
+        assert bad.max().item() <= 0, bad.max().item()
+        new = w0[b].double()
+        new[:, :lens[b]] += rw
+        tol = 2.0 ** -22 * new
+        tol[:, :lens[b]] += err
+        bad = (w[b].double() - new).abs() - tol
+        assert bad.max().item() <= 0, bad.max().item()
