@@ -77,6 +77,11 @@ LSMX_DEV typename Vec<T>::x8 columns(const T *t, int j0, int d, int g, int r) {
 }
 
 // ------------------------------------------------------------------ dQ, delta
+// Each workgroup owns 128 rows, a wave 32: q and dO in registers, the keys through
+// LDS as in the forward kernel.  delta comes first, from o and what o's rounding
+// left out.  Bound as attn_dkv_kernel is (vector unit 53%, matrix unit 35%, two
+// waves per SIMD): 2 x 4096 tokens, 32/8 heads of 128, window 1024: 265 us for
+// three products = 684 TFLOP/s of the visible pairs.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16;
@@ -402,6 +407,10 @@ struct KeySums {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) df[y][w * 4 + i] = (T)(ds[w][y][i] * mul[y]);
         }
+        // the wave that has its products ready goes first: its SIMD's other wave
+        // is then in its exponentials (417 -> 407 us; at the scores' products
+        // instead 452)
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             const X8 of = columns<T, DP>(so, j0, d, g, r), qf = columns<T, DP>(sq, j0, d, g, r);
@@ -411,6 +420,7 @@ struct KeySums {
                 dk[d][y] = mfma(qf, df[y], dk[d][y]);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
     }
     // the sums in their own units
     LSMX_DEV float k_unit(int y) const {
@@ -425,6 +435,9 @@ LSMX_DEV int far_token(const AttnArgs &a, const Seq &s, int j, int keys) {
     return min(j / kKM * kKM + kKM, keys) - 1 + a.window - s.shift;
 }
 
+// Bound by the loads of the chunks' rows, each used for 16 keys only: 25 us at 2 x
+// 4096 tokens, 32/8 heads of 128, window 1024, 4 sinks.
+//
 // Far rows: one chunk of rows, 16 sinks; the 4 waves take 32 rows each of a
 // tile of 128 and are joined in LDS.  part: [16 sinks][key head][chunk][dK, dV][16][DP].
 template <typename T, int DP>
@@ -489,9 +502,18 @@ __global__ __launch_bounds__(256) void attn_far_kernel(AttnArgs a) {
     }
 }
 
+// Each workgroup owns 128 keys, a wave 32 of them: K in registers, the sums of
+// dK and dV in 128 more, the rows through LDS.
+//
+// Bound by the two waves per SIMD that these registers leave: the vector unit is
+// busy 54% of the time, the matrix unit 33%, LDS 36%, and what one wave waits for
+// the other cannot always fill; 12% more is the sequence's end, whose keys fewer
+// rows see.  2 x 4096 tokens, 32/8 heads of 128, window 1024: 407 us for four
+// products = 593 TFLOP/s of the visible pairs.
+//
 // Head 128: two waves per SIMD only with V in LDS, tiles of 32 rows and the LDS
 // places made anew each time (245 registers; with V in registers 320, one wave
-// per SIMD: 484 us at 2 x 4096 tokens, 32/8 heads, window 1024).
+// per SIMD: 484 us).
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
     constexpr int NS = DP / 32, ND = DP / 16;

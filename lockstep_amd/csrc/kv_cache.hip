@@ -8,7 +8,10 @@ namespace {
 
 // ------------------------------------------------------------------ append
 // Four lanes quantize a 32-block (8 elements of 16 bits each); the rule and
-// the bytes are those of the quantizer (lsmx_q16.h).
+// the bytes are those of the quantizer (lsmx_q16.h).  A workgroup takes 512
+// blocks' parts of k and v, so that few new tokens still spread over the chip.
+// Bound by the bytes: 12000 tokens of 8 heads of 128, 25.5 us = 4.3 TB/s; 64 tokens,
+// a launch's own 4.6 us.
 constexpr int kAppendTokens = 64;  // most tokens of a workgroup
 
 template <typename T>
@@ -166,9 +169,10 @@ LSMX_DEV void load_rows(const AttnArgs &a, int b, int hkv, int row, int g, bool 
     for (int x = 0; x < DP / 32; ++x) q[x] = in ? *(const X8 *)(qp + x * 8) : X8{};
 }
 
-// The scores of 16 keys, lane 16g + r holding keys 4g..4g+3 of row r; the
-// lane's part of each vector is contracted as it lies in memory.
-template <typename T, int DP, int RT>
+// The scores of 16 keys, lane 16g + r holding keys 4g..4g+3 of row r (ROWS: rows
+// 4g..4g+3 of key r); the lane's part of each vector is contracted as it lies in
+// memory.
+template <typename T, int DP, int RT, bool ROWS = false>
 LSMX_DEV void scores(const Codes<DP> &k, const typename Vec<T>::x8 (&q)[RT][DP / 32], f32x4 (&st)[RT]) {
     const float sc = block_scale<T>(k.e);
 #pragma unroll
@@ -177,7 +181,7 @@ LSMX_DEV void scores(const Codes<DP> &k, const typename Vec<T>::x8 (&q)[RT][DP /
     for (int s = 0; s < DP / 32; ++s) {
         const typename Vec<T>::x8 kf = fp4x8<T>(k.w[s], sc);
 #pragma unroll
-        for (int y = 0; y < RT; ++y) st[y] = mfma(kf, q[y][s], st[y]);
+        for (int y = 0; y < RT; ++y) st[y] = ROWS ? mfma(q[y][s], kf, st[y]) : mfma(kf, q[y][s], st[y]);
     }
 }
 
@@ -402,7 +406,9 @@ __global__ __launch_bounds__(256) void kv_join_few_kernel(AttendArgs x) {
         a.lse[b * a.lse_b + h * a.lse_h + tok] = tot > 0.f ? mc - kLift<T> + __log2f(tot) : tot != tot ? tot : -INFINITY;
 }
 
-// Joins the shares of one row: 16 threads over the vector, 16 over the shares.
+// Joins the shares of one row: 16 threads over the vector, 16 over the shares;
+// for one long sequence, whose shares are many and rows few (32 rows of 128
+// shares of 128: 4.2 us, a launch and two dependent loads).
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs x) {
     constexpr int NE = DP / 16;
@@ -487,45 +493,56 @@ __global__ __launch_bounds__(256) void kv_weights_kernel(AttendArgs x) {
         walk.find(i, cur);
         cur.load(p, hkv, g, r);
         X8 q[RT][NS];
-        int pos[RT], low[RT];
-        float lse[RT];
+        int pos[RT][4];
+        float lse[RT][4];  // of rows 4g..4g+3; past the last: infinite, a weight of 0
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            const int row = row0 + t * 16 + r;
-            const bool in = row < rows;
-            load_rows<T, DP>(a, b, hkv, row, g, in, q[t]);
-            const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
-            pos[t] = in ? tok + tiles.len - a.q_len : -1;
-            low[t] = window_low(pos[t], a.window);
-            lse[t] = a.lse[b * a.lse_b + h * a.lse_h + tok];
+            load_rows<T, DP>(a, b, hkv, row0 + t * 16 + r, g, row0 + t * 16 + r < rows, q[t]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = row0 + t * 16 + g * 4 + e;
+                const bool in = row < rows;
+                const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
+                pos[t][e] = in ? tok + tiles.len - a.q_len : -1;
+                lse[t][e] = in ? a.lse[b * a.lse_b + h * a.lse_h + tok] : INFINITY;
+            }
         }
+        const int pfirst = div_by(row0, a.by_group) + tiles.len - a.q_len;
         for (; i < i1; i += 4) {
             const int j0 = cur.j0;
-            // lane r < 8 keeps the sums of key 16 (r / 4) + 4g + r % 4
-            const int mine = j0 + (r >> 2) * 16 + g * 4 + (r & 3);
-            const bool held = r < 8 && mine < tiles.len && (r < 4 ? cur.pg[0] : cur.pg[1]) >= 0;
+            // the first 32 lanes keep the sums of a key each
+            const int mine = j0 + (lane & 31);
+            const bool held = lane < 32 && mine < tiles.len && (g == 0 ? cur.pg[0] : cur.pg[1]) >= 0;
             float before = held ? w[mine] : 0.f;
             // after the last tile this one again, from the cache: the loads of all
             // rounds are alike, and the wait is for the round before
             walk.find(i + 4 < i1 ? i + 4 : i, nxt);
             nxt.load(p, hkv, g, r);
-            float own = 0.f;
+            const bool full = j0 + 31 <= pfirst && (!a.window || j0 > tiles.len - 1 - a.window || j0 + 31 < a.sinks);
+            float sum[2] = {0.f, 0.f};
+            auto add = [&](auto all) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                f32x4 st[RT], sum{0, 0, 0, 0};
-                scores<T, DP, RT>(cur.k[t], q, st);
+                for (int t = 0; t < 2; ++t) {
+                    f32x4 st[RT];  // rows 4g..4g+3 of key r
+                    scores<T, DP, RT, true>(cur.k[t], q, st);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                    for (int y = 0; y < RT; ++y)
 #pragma unroll
-                    for (int y = 0; y < RT; ++y) {
-                        const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(st[y][e], a.c, -lse[y]));
-                        sum[e] += sees(j0 + t * 16 + g * 4 + e, pos[y], low[y], a.sinks) ? v : 0.f;
-                    }
-                    const float all = sum_16(sum[e]);
-                    own = r == t * 4 + e ? all : own;
+                        for (int e = 0; e < 4; ++e) {
+                            const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(st[y][e], a.c, -lse[y][e]));
+                            if constexpr (decltype(all)::value)
+                                sum[t] += v;
+                            else
+                                sum[t] += sees(j0 + t * 16 + r, pos[y][e], window_low(pos[y][e], a.window), a.sinks) ? v : 0.f;
+                        }
                 }
-            }
-            if (held) w[mine] = before + own;
+            };
+            if (full)
+                add(BoolC<true>{});
+            else
+                add(BoolC<false>{});
+            const float s0 = sum_rows(sum[0]), s1 = sum_rows(sum[1]);
+            if (held) w[mine] = before + (g == 0 ? s0 : s1);
             cur = nxt;
         }
     }
@@ -659,7 +676,9 @@ LSMX_DEV uint32_t rank_of(float w) {
 
 // One workgroup per sequence and key head: the rank of the last weight that
 // stays, by radix selection 8 bits at a time, then the kept positions in
-// ascending order.  PER: ranks a thread keeps in registers, which covers
+// ascending order.  Bound by the four rounds' own latency (histogram in LDS, a
+// search of its bins): 256 x 8192 weights 16 us, 8 x 1500 10 us.
+// PER: ranks a thread keeps in registers, which covers
 // 1024 PER positions; 0: they are read again in each round.
 constexpr int kSelect = 1024;
 template <int PER>
@@ -818,7 +837,8 @@ __global__ __launch_bounds__(kSelect) void kv_select_kernel(EvictArgs a) {
 
 // Moves the kept vectors to the new pages: 8 threads a token, 4 for its key's
 // codes and 4 for its value's; 4 tokens a thread, whose loads are in flight
-// together.
+// together.  Bound by the bytes, read in runs of single tokens: 32 x 8 heads of
+// 4096 tokens of 128, 67 us = 4.3 TB/s.
 template <int DP>
 __global__ __launch_bounds__(256) void kv_move_kernel(EvictArgs a) {
     constexpr int NB = DP / 8, NW = NB / 4;  // bytes and words of codes of a thread
