@@ -461,11 +461,12 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs x) {
 // recomputed from the keys' codes.  Each sum has one owner and one order.
 // (Scores kept by the first pass are fewer bytes for up to 8 rows at head 128,
 // but their short runs made that pass 118 us from 80 at 64 x 8192 tokens of 8
-// key heads and 4 rows, and adding them took 42, where this takes 60.)
+// key heads and 4 rows, and adding them took 42, where this takes 47.)
 //
 // Few rows: the q of RT x 16 stays in registers, and the waves run over the keys
 // as in kv_decode_kernel, once for each such block.  Bound by the codes' bytes:
-// 64 x 8192 tokens of 8 key heads of 128 and 4 rows each, 60 us = 5.3 TB/s.
+// 64 sequences of up to 8192 tokens of 8 key heads of 128, 4 rows each, 47 us =
+// 5.0 TB/s.
 LSMX_DEV float sum_16(float x) {  // over the 16 lanes of a row of lanes
     x += u2f(__builtin_amdgcn_update_dpp(0, f2u(x), 0xB1, 0xF, 0xF, true));   // quad_perm 1,0,3,2
     x += u2f(__builtin_amdgcn_update_dpp(0, f2u(x), 0x4E, 0xF, 0xF, true));   // quad_perm 2,3,0,1
@@ -910,7 +911,11 @@ hipError_t weights(AttendArgs x, hipStream_t s) {
     const int rows = x.a.q_len * x.a.group, bh = x.a.batch * x.a.kv_heads;
     const int64_t cap = (int64_t)x.p.max_pages << x.p.page_shift, reach = (int64_t)x.a.q_len + x.a.window + x.a.sinks;
     const int64_t keys = x.a.window && reach < cap ? reach : cap;
-    x.splits = kv_attend_splits(x.a.batch, x.a.kv_heads, 1, keys);
+    // nothing is joined here: three times the shares of attention, for six waves per
+    // SIMD, while each has 1024 keys (64 x 8192 tokens of 8 key heads of 128: 47 us
+    // from 54; below, a share's start costs more: 64 x 2048 of 4 heads 12 from 10)
+    const int least = kv_attend_splits(x.a.batch, x.a.kv_heads, 1, keys);
+    x.splits = max(least, (int)min((int64_t)3 * least, keys / 1024));
     const unsigned grid = (unsigned)x.splits * bh;
     // up to 64 rows are one pass over the codes; up to three passes are still
     // faster than tiles of keys that each wait for the rows, where those would be
