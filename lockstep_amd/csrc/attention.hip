@@ -437,13 +437,13 @@ __global__ __launch_bounds__(NW * KS * 64, DP == 64 && !KV::kHoles ? 3 : 2) void
     }
 }
 
-// Row tiles over all sequences, and the grid of their items over 8 XCDs.
-void tiles_of(AttnArgs &a, int rows, int splits = 1) {
+// Row tiles over all sequences; the grid of their items.
+unsigned tiles_of(AttnArgs &a, int rows, int splits = 1) {
     if (a.offsets)
         a.tiles = (int)(((int64_t)a.tokens * a.group + rows - 1) / rows) + a.batch + 2;
     else
         a.tiles = (int)(((int64_t)a.q_len * a.group + rows - 1) / rows) * a.batch;
-    a.per = (int)(((int64_t)a.tiles * a.kv_heads * splits + 7) / 8);
+    return order_items(a, (int64_t)a.tiles * a.kv_heads * splits);
 }
 
 // Workgroups of 4 waves: two or three of them on a CU run out of step, and one's
@@ -470,8 +470,7 @@ Form form_of(const AttnArgs &a) {
 template <typename T, int DP>
 hipError_t fwd(AttnArgs a, hipStream_t s) {
     const Form f = form_of(a);
-    tiles_of(a, f == kWide ? 128 : 64);
-    const unsigned grid = (unsigned)a.per * 8;
+    const unsigned grid = tiles_of(a, f == kWide ? 128 : 64);
     if (f == kWide)
         attn_fwd_kernel<T, DP, 2, 4, 1, DenseKV<T, DP, 4>><<<grid, 256, 0, s>>>(a);
     else if (f == kNarrow)
@@ -489,8 +488,8 @@ hipError_t fwd(AttnArgs a, hipStream_t s) {
 // join them, in two halves of a workgroup 49.
 template <typename T, int DP>
 hipError_t chunk(AttendArgs x, hipStream_t s) {
-    tiles_of(x.a, 64, x.splits);
-    attn_fwd_kernel<T, DP, 1, 4, 1, PagedKV<T, DP>><<<(unsigned)x.a.per * 8, 256, 0, s>>>(x);
+    const unsigned grid = tiles_of(x.a, 64, x.splits);
+    attn_fwd_kernel<T, DP, 1, 4, 1, PagedKV<T, DP>><<<grid, 256, 0, s>>>(x);
     return hipGetLastError();
 }
 

@@ -430,6 +430,11 @@ struct KeySums {
     LSMX_DEV static float v_unit() { return Range<T>::on ? 1.f / 1024.f : 1.f; }
 };
 
+// Elements of one share's dK (or dV).
+LSMX_DEV int64_t share_size(const AttnArgs &a) {
+    return (a.offsets ? (int64_t)a.tokens : (int64_t)a.batch * a.k_len) * a.kv_heads * a.dim;
+}
+
 // The first token past the window of the key tile that holds key j.
 LSMX_DEV int far_token(const AttnArgs &a, const Seq &s, int j, int keys) {
     return min(j / kKM * kKM + kKM, keys) - 1 + a.window - s.shift;
@@ -502,8 +507,21 @@ __global__ __launch_bounds__(256) void attn_far_kernel(AttnArgs a) {
     }
 }
 
+// Rows (token, head) that see some key of tile `tile`, but for the far rows of
+// sinks: [first, second).
+struct RowSpan {
+    int lo, hi;
+};
+LSMX_DEV RowSpan rows_of_keys(const AttnArgs &a, const Seq &s, int keys) {
+    const int key0 = s.tile * kKM, key1 = min(key0 + kKM, keys) - 1;
+    int hi = s.q_len;
+    if (a.window && (a.chunk || key0 >= a.sinks)) hi = min(hi, key1 + a.window - s.shift);
+    return RowSpan{max(0, key0 - s.shift) * a.group, max(hi, 0) * a.group};
+}
+
 // Each workgroup owns 128 keys, a wave 32 of them: K in registers, the sums of
-// dK and dV in 128 more, the rows through LDS.
+// dK and dV in 128 more, the rows through LDS.  Few key tiles take their rows in
+// shares, whose sums go to memory in fp32 and are joined by a kernel of its own.
 //
 // Bound by the two waves per SIMD that these registers leave: the vector unit is
 // busy 54% of the time, the matrix unit 33%, LDS 36%, and what one wave waits for
@@ -526,19 +544,21 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) int s_pos[2][kKN];
 
     const int item = xcd_item(blockIdx.x, a.per);
-    if (item >= a.tiles * a.kv_heads) return;
-    const int hkv = item / a.tiles;
+    if (item >= a.tiles * a.kv_heads * a.shares) return;
+    const int rest = item / a.tiles, hkv = rest / a.shares, share = rest - hkv * a.shares;
     Seq s;
-    if (!find_tile(a, item % a.tiles, kKM, 1, a.k_len, s)) return;
+    if (!find_tile(a, item - rest * a.tiles, kKM, 1, a.k_len, s)) return;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
     const int keys = a.offsets ? s.q_len : s.k_len;  // of a dead sequence too
     const int key0 = s.tile * kKM, key1 = min(key0 + kKM, keys) - 1;
 
-    // the rows that see some key of the tile, but for the far rows of sinks
-    const int tok_lo = max(0, key0 - s.shift);
-    int tok_hi = s.q_len;
-    if (a.window && (a.chunk || key0 >= a.sinks)) tok_hi = min(tok_hi, key1 + a.window - s.shift);
-    const int row_lo = tok_lo * a.group, row_hi = max(tok_hi, 0) * a.group;
+    const RowSpan all = rows_of_keys(a, s, keys);
+    int row_lo = all.lo, row_hi = all.hi;
+    if (a.shares > 1) {
+        if (share && (int64_t)share * a.share_rows >= row_hi - row_lo) return;
+        row_lo += share * a.share_rows;
+        row_hi = min(row_hi, row_lo + a.share_rows);
+    }
     Rows<T, DP> in{a, s, hkv, row_hi};
     if (row_lo < row_hi) {
         in.fetch(row_lo, sq[0], so[0], kKN);
@@ -602,7 +622,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
 #pragma unroll
         for (int d = 0; d < ND; ++d) sums.dk[d][y] *= fk, sums.dv[d][y] *= fv;
         const int group = (wkey0 + y * 16) / 16;
-        if (a.chunk && wkey0 + y * 16 < min(a.sinks, keys)) {
+        if (a.chunk && share == 0 && wkey0 + y * 16 < min(a.sinks, keys)) {
             const int first = max(far_token(a, s, wkey0, keys), 0) * a.group, rows = s.q_len * a.group;
             const int slot0 = first_tile(a, s, a.chunk, a.group);
             for (int c = first / a.chunk; c * a.chunk < rows && first < rows; ++c) {
@@ -616,6 +636,17 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
         }
         if (key[y] >= keys) continue;
         const int64_t at = (((a.offsets ? s.k0 : (int64_t)s.b * a.k_len) + key[y]) * a.kv_heads + hkv) * a.dim;
+        if (a.shares > 1) {
+            const int64_t one = share_size(a);
+            float *to = a.share_part + 2 * share * one + at;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+                if (d * 16 + g * 4 < a.dim) {
+                    *(f32x4 *)(to + d * 16 + g * 4) = sums.dk[d][y];
+                    *(f32x4 *)(to + one + d * 16 + g * 4) = sums.dv[d][y];
+                }
+            continue;
+        }
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             X4 wk, wv;
@@ -629,6 +660,36 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
                 *(X4 *)((T *)a.dv + at + d * 16 + g * 4) = wv;
             }
         }
+    }
+}
+
+// Joins the shares of 16 keys, in their order.  Bound by the shares' bytes.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+    typedef typename Vec<T>::x4 X4;
+    const int item = blockIdx.x / 8, hkv = item / a.tiles;
+    Seq s;
+    if (!find_tile(a, item - hkv * a.tiles, kKM, 1, a.k_len, s)) return;
+    const int keys = a.offsets ? s.q_len : s.k_len, key0 = s.tile * kKM + (blockIdx.x & 7) * 16;
+    const RowSpan all = rows_of_keys(a, s, keys);
+    const int n = max(1, (all.hi - all.lo + a.share_rows - 1) / a.share_rows), quads = a.dim / 4;
+    const int64_t one = share_size(a);
+    for (int i = threadIdx.x; i < 16 * quads; i += 256) {
+        const int j = i / quads, key = key0 + j;
+        if (key >= keys) return;
+        const int64_t at = (((a.offsets ? s.k0 : (int64_t)s.b * a.k_len) + key) * a.kv_heads + hkv) * a.dim + (i - j * quads) * 4;
+        f32x4 dk{0, 0, 0, 0}, dv{0, 0, 0, 0};
+#pragma unroll 4
+        for (int c = 0; c < n; ++c) {
+            const float *p = a.share_part + 2 * c * one + at;
+            dk += *(const f32x4 *)p;
+            dv += *(const f32x4 *)(p + one);
+        }
+        X4 wk, wv;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) wk[e] = (T)(dk[e] * a.scale), wv[e] = (T)dv[e];
+        *(X4 *)((T *)a.dk + at) = wk;
+        *(X4 *)((T *)a.dv + at) = wv;
     }
 }
 
@@ -652,6 +713,38 @@ Far far_plan(const AttnArgs &a) {
     f.bytes = (int64_t)f.groups * a.kv_heads * f.slots * 2 * 16 * (a.dim <= 64 ? 64 : 128) * 4;
     return f;
 }
+// Shares of the rows of key tiles: where the longest tile would take over half as
+// long again as the chip for all, about 1024 workgroups in equal parts, none
+// below 512 rows, and the sums of no more than 512 MiB.
+struct Shares {
+    int n, rows;
+    int64_t bytes;
+};
+Shares share_plan(const AttnArgs &a, const Far &far) {
+    Shares p{1, 0, 0};
+    const int64_t keys = a.offsets ? a.tokens : (int64_t)a.batch * a.k_len, seqs = a.batch > 0 ? a.batch : 1;
+    const int64_t own = a.offsets ? a.tokens / seqs : a.q_len, most = a.offsets ? a.tokens : a.q_len;
+    const bool windowed = a.window && (far.chunk || !a.sinks);
+    // rows of the longest tile, and of all: a tile's reach, or half the sequence
+    const int64_t reach = (int64_t)a.window + kKM, longest = (windowed && reach < most ? reach : most) * a.group;
+    const int64_t mean = (windowed && reach < own / 2 ? reach : (own + 1) / 2) * a.group;
+    const int64_t total = (keys + kKM - 1) / kKM * a.kv_heads * mean;
+    if (!keys || !total || longest <= 512 || longest * 512 < total + total / 2) return p;
+    const int64_t one = keys * a.kv_heads * a.dim * 8, room = (int64_t)512 << 20;
+    int64_t rows = (total / 1024 + 127) / 128 * 128;
+    if (rows < 512) rows = 512;
+    if ((longest + rows - 1) / rows * one > room) {
+        const int64_t n = room / one;
+        if (n < 2) return p;
+        rows = ((longest + n - 1) / n + 127) / 128 * 128;
+    }
+    const int64_t n = (longest + rows - 1) / rows;
+    if ((keys / kKM + a.batch + 2) * a.kv_heads * n >= (int64_t)1 << 27) return p;
+    p.n = (int)n;
+    p.rows = (int)rows;
+    p.bytes = p.n > 1 ? p.n * one : 0;
+    return p;
+}
 int64_t delta_bytes(const AttnArgs &a) {
     const int64_t rows = (a.offsets ? (int64_t)a.tokens : (int64_t)a.batch * a.q_len) * a.heads;
     return (4 * rows + 255) / 256 * 256;
@@ -666,22 +759,28 @@ hipError_t bwd(const AttnArgs &in, hipStream_t s) {
     const int tokens = a.offsets ? a.tokens : a.q_len;
     if (tokens) {
         a.tiles = (int)(((int64_t)tokens * a.group + kBM - 1) / kBM) * many + pad;
-        a.per = (int)(((int64_t)a.tiles * a.kv_heads + 7) / 8);
-        attn_dq_kernel<T, DP><<<(unsigned)a.per * 8, 256, 0, s>>>(a);
+        attn_dq_kernel<T, DP><<<order_items(a, (int64_t)a.tiles * a.kv_heads), 256, 0, s>>>(a);
         if (far.chunk) {
             a.chunk = far.chunk, a.tiles = a.far_slots = far.slots;
             attn_far_kernel<T, DP><<<(unsigned)far.slots * a.kv_heads * far.groups, 256, 0, s>>>(a);
         }
     }
     a.tiles = ((a.offsets ? a.tokens : a.k_len) + kKM - 1) / kKM * many + pad;
-    a.per = (int)(((int64_t)a.tiles * a.kv_heads + 7) / 8);
-    if (a.tiles) attn_dkv_kernel<T, DP><<<(unsigned)a.per * 8, 256, 0, s>>>(a);
+    if (!a.tiles) return hipGetLastError();
+    const Shares shares = share_plan(a, far);
+    a.shares = shares.n, a.share_rows = shares.rows;
+    a.share_part = (float *)((uint8_t *)a.part + far.bytes);
+    attn_dkv_kernel<T, DP><<<order_items(a, (int64_t)a.tiles * a.kv_heads * a.shares), 256, 0, s>>>(a);
+    if (a.shares > 1) attn_join_kernel<T><<<(unsigned)(a.tiles * a.kv_heads * 8), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t attn_bwd_workspace(const AttnArgs &a) { return delta_bytes(a) + far_plan(a).bytes + 256; }
+int64_t attn_bwd_workspace(const AttnArgs &a) {
+    const Far far = far_plan(a);
+    return delta_bytes(a) + far.bytes + share_plan(a, far).bytes + 256;
+}
 
 hipError_t launch_attn_bwd(const AttnArgs &a, int dtype, hipStream_t s) {
     if (dtype == LSMX_BF16) return a.dim <= 64 ? bwd<__bf16, 64>(a, s) : bwd<__bf16, 128>(a, s);

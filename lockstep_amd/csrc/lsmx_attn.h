@@ -101,7 +101,7 @@ LSMX_DEV int div_by(int n, FastDiv f) { return f.d == 1 ? n : (int)(__umulhi((ui
 // Workgroup id -> work item so that consecutive items stay on one of the 8
 // XCDs (ids go to them in turn) and share its L2.  The grid is padded to a
 // multiple of 8; items past `total` are dropped by the caller.
-LSMX_DEV int xcd_item(int id, int per) { return (id & 7) * per + (id >> 3); }
+LSMX_DEV int xcd_item(int id, int per) { return per ? (id & 7) * per + (id >> 3) : id; }
 
 struct AttnArgs {
     const void *q, *k, *v;
@@ -126,7 +126,19 @@ struct AttnArgs {
     void *o_lo;          // o as computed less o as rounded, laid out as o (forward: null to leave out)
     float *part;         // far rows' partial gradients of the sinks
     int chunk, far_slots;  // rows of a chunk (0: no far rows apart), chunks of all sequences
+    float *share_part;     // dK and dV of each share of a key tile's rows: [share][dK, dV][key][kv head][dim]
+    int shares, share_rows;  // shares > 1: most of a tile, rows of one
 };
+
+// The order of a launch's items (tiles of one key head after the other): in
+// eighths over the XCDs, whose L2 then holds few heads' keys, where each takes
+// the same number of heads; else one after the other round the XCDs, so that the
+// long rows' tiles and the short rows' fall on all of them (5506 tokens of 5/1
+// heads of 64, causal: FIGURE).  Returns the grid.
+inline unsigned order_items(AttnArgs &a, int64_t items) {
+    a.per = a.kv_heads % 8 ? 0 : (int)((items + 7) / 8);
+    return (unsigned)((items + 7) / 8 * 8);
+}
 
 // One sequence of a packed or dense batch.
 struct Seq {
