@@ -166,7 +166,7 @@ struct PagedKV {
 // a step is 32 keys).  2 x 4096 tokens, 32/8 heads of 128, window 1024: 184 us
 // = 656 TFLOP/s of the visible pairs (205 with the remainders of o stored for
 // the backward); 16384 tokens of 8/1 heads of 64 through a window of 4096:
-// 250 us = 483 TFLOP/s.
+// 214 us = 562 TFLOP/s.
 template <typename T, int DP, int RT, int NW, int KS, typename KV>
 __global__ __launch_bounds__(NW * KS * 64, DP == 64 && !KV::kHoles ? 3 : 2) void attn_fwd_kernel(typename KV::Args args) {
     constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, BM = NW * RT * 16;
@@ -179,12 +179,12 @@ __global__ __launch_bounds__(NW * KS * 64, DP == 64 && !KV::kHoles ? 3 : 2) void
     __shared__ int s_held[KS][2][KV::kHoles ? kBN : 1];
 
     const AttnArgs &a = KV::attn(args);
-    // tiles of one share of the keys side by side
-    const int item = xcd_item(blockIdx.x, a.per), splits = KV::splits(args);
-    if (item >= a.tiles * a.kv_heads * splits) return;
-    const int rest = item / a.tiles, hkv = rest / splits, share = rest - hkv * splits;
+    const int splits = KV::splits(args);
+    const Item item = item_of(a, splits);
+    const int hkv = item.head, share = item.share;
+    if (hkv >= a.kv_heads) return;
     Seq s;
-    if (!KV::find(args, item % a.tiles, BM, s)) return;
+    if (!KV::find(args, item.tile, BM, s)) return;
 
     const int lane = threadIdx.x & 63, wave = uniform((threadIdx.x >> 6) % NW), g = lane >> 4, r = lane & 15;
     const int group = KS == 1 ? 0 : uniform(threadIdx.x / (NW * 64));
@@ -459,7 +459,7 @@ unsigned tiles_of(AttnArgs &a, int rows, int splits = 1) {
 //   wide     64    9.7   14.9   25.1   39.8   54.4    128   13.3  20.9  36.6  58.7  80.9
 //   narrow         7.7   11.9   20.1   32.3   46.4           9.8  15.3  27.3  53.8  95.9
 //   halves         7.0    9.7   16.1   34.1   54.5           9.1  13.0  26.2  64.2 119.7
-// 16384 tokens of 8 heads of 64: wide 252, narrow 275.
+// 16384 tokens of 8/1 heads of 64 through a window of 4096: wide 252, narrow 275.
 enum Form { kWide, kNarrow, kHalves };
 constexpr int kSimds = 1024;
 Form form_of(const AttnArgs &a) {

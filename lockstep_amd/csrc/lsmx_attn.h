@@ -98,11 +98,6 @@ inline FastDiv fast_div(uint32_t d) {
 }
 LSMX_DEV int div_by(int n, FastDiv f) { return f.d == 1 ? n : (int)(__umulhi((uint32_t)n, f.m) >> f.sh); }
 
-// Workgroup id -> work item so that consecutive items stay on one of the 8
-// XCDs (ids go to them in turn) and share its L2.  The grid is padded to a
-// multiple of 8; items past `total` are dropped by the caller.
-LSMX_DEV int xcd_item(int id, int per) { return per ? (id & 7) * per + (id >> 3) : id; }
-
 struct AttnArgs {
     const void *q, *k, *v;
     void *o;
@@ -116,7 +111,7 @@ struct AttnArgs {
     int window, sinks;       // window 0: none (then sinks is 0)
     float c;                 // scale * log2(e)
     FastDiv by_group;
-    int tiles, per;  // tiles per kv head over all sequences (dense: of one sequence times batch); items per XCD
+    int tiles, run;  // tiles per kv head over all sequences (dense: of one sequence times batch); items per XCD, or 0: see item_of
     // backward
     const void *d_o;
     int64_t do_b, do_t, do_h;
@@ -130,14 +125,29 @@ struct AttnArgs {
     int shares, share_rows;  // shares > 1: most of a tile, rows of one
 };
 
-// The order of a launch's items (tiles of one key head after the other): in
-// eighths over the XCDs, whose L2 then holds few heads' keys, where each takes
-// the same number of heads; else one after the other round the XCDs, so that the
-// long rows' tiles and the short rows' fall on all of them (5506 tokens of 5/1
-// heads of 64, causal: FIGURE).  Returns the grid.
+// The item of a workgroup: a tile of one key head, and one of `shares` shares.
+// Ids go to the 8 XCDs in turn.  A multiple of 8 key heads: `run` items in order on
+// each, so that its L2 holds one head's keys after the other.  Else the heads are
+// the ids' fastest part: an XCD still has one or few of them (4: one), all
+// XCDs long tiles and short ones, and the short come last (in runs an XCD had
+// the half of a head with the long rows: 5086 tokens of 32/4 heads of 128, causal,
+// 419 us against 303; 5506 of 5/1 heads of 64, 82 against 64).  The grid
+// is padded; items past the last are dropped by the caller.
+struct Item {
+    int tile, head, share;
+};
+LSMX_DEV Item item_of(const AttnArgs &a, int shares) {
+    const int id = blockIdx.x;
+    if (a.run) {
+        const int item = (id & 7) * a.run + (id >> 3), rest = item / a.tiles, head = rest / shares;
+        return Item{item - rest * a.tiles, head, rest - head * shares};
+    }
+    const int rest = id / a.kv_heads, share = rest / a.tiles;
+    return Item{rest - share * a.tiles, share < shares ? id - rest * a.kv_heads : a.kv_heads, share};
+}
 inline unsigned order_items(AttnArgs &a, int64_t items) {
-    a.per = a.kv_heads % 8 ? 0 : (int)((items + 7) / 8);
-    return (unsigned)((items + 7) / 8 * 8);
+    a.run = a.kv_heads % 8 ? 0 : (int)((items + 7) / 8);
+    return (unsigned)(a.run ? a.run * 8 : items);
 }
 
 // One sequence of a packed or dense batch.

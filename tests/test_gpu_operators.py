@@ -301,3 +301,43 @@ def test_cache_weights_of_some_rows(B, T, D, window, dt, dev):
         tol[:, :lens[b]] += err
         bad = (w[b].double() - new).abs() - tol
         assert bad.max().item() <= 0, bad.max().item()
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,Tq,Tk,H,Hkv,D,window,sinks", [
+    (1, 1500, 1500, 5, 1, 64, None, 0),      # few key tiles, long and short
+    (1, 700, 1300, 6, 2, 128, None, 0),      # keys before the queries
+    (1, 1300, 700, 4, 1, 80, None, 3),       # rows that see nothing
+    (2, 1100, 1100, 12, 3, 80, 200, 20),     # with the sinks' far rows apart
+    (1, 1100, 1100, 4, 1, 128, 300, 300),    # sinks past those
+])
+def test_gradients_in_shares(B, Tq, Tk, H, Hkv, D, window, sinks, dt, dev):
+    from lockstep_amd.attention import sink_window_attention
+    q, k, v, do = inputs(B, Tq, Tk, H, Hkv, D, dt, dev, seed=Tq)
+    x = [t.requires_grad_(True) for t in (q, k, v)]
+    o = sink_window_attention(*x, window=window, sinks=sinks)
+    grads = torch.autograd.grad(o, x, do, retain_graph=True)
+    for b in range(B):
+        ref = formula(*(t[b].detach() for t in x), window, sinks, 1.0 / math.sqrt(D), do[b])
+        close("o", o[b].detach(), ref["o"], ref["o_mag"], U[dt], 1)
+        for n, g in zip(("dq", "dk", "dv"), grads):
+            close(n, g[b], ref[n], ref[n + "_mag"], U[dt], 1)
+    assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(o, x, do)))
+
+
+@pytest.mark.parametrize("lens", [[1400], [3, 900, 0, 500], [200] * 9])
+def test_packed_gradients_in_shares(lens, dev):
+    from lockstep_amd.attention import sink_window_attention
+    N, H, Hkv, D = sum(lens) + 5, 8, 1, 128
+    q, k, v, do = (t[0] for t in inputs(1, N, N, H, Hkv, D, torch.bfloat16, dev, seed=len(lens)))
+    off = [sum(lens[:b]) for b in range(len(lens) + 1)]
+    x = [t.requires_grad_(True) for t in (q, k, v)]
+    o = sink_window_attention(*x, offsets=torch.tensor(off, dtype=torch.int32, device=dev))
+    grads = torch.autograd.grad(o, x, do)
+    for lo, hi in zip(off, off[1:]):
+        if hi > lo:
+            ref = formula(*(t[lo:hi].detach() for t in x), None, 0, 1.0 / math.sqrt(D), do[lo:hi])
+            close("o", o[lo:hi].detach(), ref["o"], ref["o_mag"], U[torch.bfloat16], 1)
+            for n, g in zip(("dq", "dk", "dv"), grads):
+                close(n, g[lo:hi], ref[n], ref[n + "_mag"], U[torch.bfloat16], 1)
+    assert all((g[off[-1]:] == 0).all() for g in grads)
