@@ -678,7 +678,7 @@ LSMX_DEV uint32_t rank_of(float w) {
 // One workgroup per sequence and key head: the rank of the last weight that
 // stays, by radix selection 8 bits at a time, then the kept positions in
 // ascending order.  Bound by the four rounds' own latency (histogram in LDS, a
-// search of its bins): 256 x 8192 weights 16 us, 8 x 1500 10 us.
+// search of its bins): 256 x 8192 weights 16 us, 8 x 1500 8 us.
 // PER: ranks a thread keeps in registers, which covers
 // 1024 PER positions; 0: they are read again in each round.
 constexpr int kSelect = 1024;
