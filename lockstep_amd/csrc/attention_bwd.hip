@@ -23,7 +23,6 @@
 namespace lsmx {
 namespace {
 
-constexpr int kBM = 128;  // dQ: rows of a workgroup
 constexpr int kBN = 64;   // dQ: keys of a tile
 constexpr int kKM = 128;  // dK, dV: keys of a workgroup
 constexpr int kFar = 128; // far rows: rows of a tile
@@ -77,14 +76,14 @@ LSMX_DEV typename Vec<T>::x8 columns(const T *t, int j0, int d, int g, int r) {
 }
 
 // ------------------------------------------------------------------ dQ, delta
-// Each workgroup owns 128 rows, a wave 32: q and dO in registers, the keys through
+// Each workgroup owns 64 RT rows, a wave 16 RT: q and dO in registers, the keys through
 // LDS as in the forward kernel.  delta comes first, from o and what o's rounding
 // left out.  Bound as attn_dkv_kernel is (vector unit 53%, matrix unit 35%, two
 // waves per SIMD): 2 x 4096 tokens, 32/8 heads of 128, window 1024: 265 us for
 // three products = 684 TFLOP/s of the visible pairs.
-template <typename T, int DP>
+template <typename T, int DP, int RT>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
-    constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16;
+    constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, kBM = 64 * RT;
     typedef typename Vec<T>::x8 X8;
     typedef typename Vec<T>::x4 X4;
     __shared__ __attribute__((aligned(16))) T sk[2][kBN * DP], sv[2][kBN * DP];
@@ -95,7 +94,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     Seq s;
     if (!find_tile(a, a.tiles - 1 - item.tile, kBM, a.group, a.q_len, s)) return;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
-    const int row0 = s.tile * kBM, rows = s.q_len * a.group, wrow0 = row0 + wave * 32;
+    const int row0 = s.tile * kBM, rows = s.q_len * a.group, wrow0 = row0 + wave * 16 * RT;
 
     const int pmin = div_by(row0, a.by_group) + s.shift;
     const int pmax = div_by(min(row0 + kBM, rows) - 1, a.by_group) + s.shift;
@@ -105,7 +104,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     auto next = [&](int t) { return t + 1 < t_sink ? t + 1 : max(t + 1, t_lo); };
     int t = t_sink > 0 ? 0 : t_lo, n = 0;
     const int wmin = div_by(min(wrow0, rows - 1), a.by_group) + s.shift;
-    const int wmax = wrow0 < rows ? div_by(min(wrow0 + 32, rows) - 1, a.by_group) + s.shift : -1;
+    const int wmax = wrow0 < rows ? div_by(min(wrow0 + 16 * RT, rows) - 1, a.by_group) + s.shift : -1;
 
     const T *kp = (const T *)a.k + s.b * a.k_b + s.k0 * a.k_t + hkv * a.k_h;
     const T *vp = (const T *)a.v + s.b * a.v_b + s.k0 * a.v_t + hkv * a.v_h;
@@ -120,12 +119,12 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     };
     if (t < t_hi) fetch(t * kBN, 0);
 
-    int pos[2], low[2];
-    int64_t q_at[2];
-    float lse[2], delta[2], mul[2] = {0.f, 0.f}, limit[2] = {0.f, 0.f};
-    X8 qf[2][NS], of[2][NS];
+    int pos[RT], low[RT];
+    int64_t q_at[RT];
+    float lse[RT], delta[RT], mul[RT] = {}, limit[RT] = {};
+    X8 qf[RT][NS], of[RT][NS];
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
+    for (int y = 0; y < RT; ++y) {
         const int row = wrow0 + r + 16 * y;
         const bool in = row < rows;
         const int tok = div_by(in ? row : 0, a.by_group), h = hkv * a.group + (in ? row : 0) - tok * a.group;
@@ -154,9 +153,11 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
         delta[y] = sum_rows(sum);
         if (in && g == 0) a.delta[l_at] = delta[y];
     }
-    f32x4 dq[ND][2];
+    f32x4 dq[ND][RT];
 #pragma unroll
-    for (int d = 0; d < ND; ++d) dq[d][0] = dq[d][1] = f32x4{0, 0, 0, 0};
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int y = 0; y < RT; ++y) dq[d][y] = f32x4{0, 0, 0, 0};
 
     wait_dma();
     __syncthreads();
@@ -169,30 +170,31 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
             // places in LDS made anew each time: held, they would not fit
             int lr = r;
             if constexpr (DP == 128 && Range<T>::on) asm volatile("" : "+v"(lr));
-            f32x4 st[2][2], dp[2][2];  // [16 keys][16 rows]
+            f32x4 st[2][RT], dp[2][RT];  // [16 keys][16 rows]
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 const int j = u * 32 + w * 16 + lr;
-                st[w][0] = st[w][1] = dp[w][0] = dp[w][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int y = 0; y < RT; ++y) st[w][y] = dp[w][y] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int x = 0; x < NS; ++x) {
                     const X8 kf = *(const X8 *)(ck + j * DP + swz<NC>(j, x * 4 + g) * 8);
                     const X8 vf = *(const X8 *)(cv + j * DP + swz<NC>(j, x * 4 + g) * 8);
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) {
+                    for (int y = 0; y < RT; ++y) {
                         st[w][y] = mfma(kf, qf[y][x], st[w][y]);
                         dp[w][y] = mfma(vf, of[y][x], dp[w][y]);
                     }
                 }
             }
             bool grow = false;
-            float top[2] = {0.f, 0.f};
+            float top[RT] = {};
 #pragma unroll
             for (int w = 0; w < 2; ++w)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) {
+                    for (int y = 0; y < RT; ++y) {
                         float ds = __builtin_amdgcn_exp2f(__builtin_fmaf(st[w][y][i], a.c, -lse[y])) *
                                    (dp[w][y][i] - delta[y]);
                         if constexpr (!decltype(all)::value) {
@@ -203,10 +205,11 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
                         if constexpr (Range<T>::on) top[y] = fmaxf(top[y], __builtin_fabsf(ds));
                     }
             if constexpr (Range<T>::on) {
-                grow = (top[0] > limit[0]) | (top[1] > limit[1]);
+                #pragma unroll
+                for (int y = 0; y < RT; ++y) grow = grow | (top[y] > limit[y]);
                 if (__any(grow)) {
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) {
+                    for (int y = 0; y < RT; ++y) {
                         const float most = max_rows(top[y]);
                         if (most > limit[y]) {
                             const float m = Range<T>::scale_for(most), f = mul[y] == 0.f ? 0.f : m / mul[y];
@@ -219,9 +222,9 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
             }
             // bf16: one rounding of dS, as large as that of dQ itself.  fp16: two
             // terms, for a type that is chosen for its digits
-            X8 df[2], dl[2];
+            X8 df[RT], dl[RT];
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
+            for (int y = 0; y < RT; ++y)
 #pragma unroll
                 for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -234,7 +237,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
             for (int d = 0; d < ND; ++d) {
                 const X8 kf = columns<T, DP>(ck, u * 32, d, g, lr);
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
+                for (int y = 0; y < RT; ++y) {
                     dq[d][y] = mfma(kf, df[y], dq[d][y]);
                     if constexpr (Range<T>::on) dq[d][y] = mfma(kf, dl[y], dq[d][y]);
                 }
@@ -255,7 +258,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
         __syncthreads();
     }
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
+    for (int y = 0; y < RT; ++y) {
         if (q_at[y] < 0) continue;
         T *p = (T *)a.dq + q_at[y];
         const float f = !Range<T>::on ? a.scale : mul[y] == 0.f ? 0.f : a.scale / mul[y];
@@ -762,8 +765,17 @@ hipError_t bwd(const AttnArgs &in, hipStream_t s) {
     const int pad = a.offsets ? a.batch + 2 : 0, many = a.offsets ? 1 : a.batch;
     const int tokens = a.offsets ? a.tokens : a.q_len;
     if (tokens) {
-        a.tiles = (int)(((int64_t)tokens * a.group + kBM - 1) / kBM) * many + pad;
-        attn_dq_kernel<T, DP><<<order_items(a, (int64_t)a.tiles * a.kv_heads), 256, 0, s>>>(a);
+        const int64_t rows = (int64_t)tokens * a.group;
+        // 32 rows a wave where that gives each CU a workgroup, else 16, which read
+        // twice as much of LDS per product: 216 and 252 workgroups of 128 rows (5506
+        // tokens of 5/1 heads of 64; 3 x 777 of 12, window 256, fp16) take 138 and 26
+        // us, 111 and 21 as twice as many of 64; 264 take 82 both, 536 take 39, 41
+        const bool wide = (rows + 127) / 128 * many * a.kv_heads >= 256;
+        a.tiles = (int)(wide ? (rows + 127) / 128 : (rows + 63) / 64) * many + pad;
+        if (wide)
+            attn_dq_kernel<T, DP, 2><<<order_items(a, (int64_t)a.tiles * a.kv_heads), 256, 0, s>>>(a);
+        else
+            attn_dq_kernel<T, DP, 1><<<order_items(a, (int64_t)a.tiles * a.kv_heads), 256, 0, s>>>(a);
         if (far.chunk) {
             a.chunk = far.chunk, a.tiles = a.far_slots = far.slots;
             attn_far_kernel<T, DP><<<(unsigned)far.slots * a.kv_heads * far.groups, 256, 0, s>>>(a);
