@@ -78,9 +78,9 @@ LSMX_DEV typename Vec<T>::x8 columns(const T *t, int j0, int d, int g, int r) {
 // ------------------------------------------------------------------ dQ, delta
 // Each workgroup owns 64 RT rows, a wave 16 RT: q and dO in registers, the keys through
 // LDS as in the forward kernel.  delta comes first, from o and what o's rounding
-// left out.  Bound as attn_dkv_kernel is (vector unit 53%, matrix unit 35%, two
-// waves per SIMD): 2 x 4096 tokens, 32/8 heads of 128, window 1024: 265 us for
-// three products = 684 TFLOP/s of the visible pairs.
+// left out.  Bound as attn_dkv_kernel is (before the second term vector unit 53%, matrix unit 35%; two
+// waves per SIMD): 2 x 4096 tokens, 32/8 heads of 128, window 1024: 330 us for
+// four products (dS in two terms) = 731 TFLOP/s of the visible pairs.
 template <typename T, int DP, int RT>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, kBM = 64 * RT;
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
             const int ju = j0 + u * 32;
             // places in LDS made anew each time: held, they would not fit
             int lr = r;
-            if constexpr (DP == 128 && Range<T>::on) asm volatile("" : "+v"(lr));
+            if constexpr (DP == 128) asm volatile("" : "+v"(lr));
             f32x4 st[2][RT], dp[2][RT];  // [16 keys][16 rows]
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
@@ -220,8 +220,10 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
                     }
                 }
             }
-            // bf16: one rounding of dS, as large as that of dQ itself.  fp16: two
-            // terms, for a type that is chosen for its digits
+            // two terms: the dS of a row cancel, so that one rounding of each is as
+            // much as 1.15 times that of dQ itself where the keys have a common part
+            // (both together 1.52 times the latter; with two terms 1.04).  330 us for
+            // 270.
             X8 df[RT], dl[RT];
 #pragma unroll
             for (int y = 0; y < RT; ++y)
@@ -231,7 +233,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
                     for (int i = 0; i < 4; ++i) {
                         const float ds = Range<T>::on ? st[w][y][i] * mul[y] : st[w][y][i];
                         df[y][w * 4 + i] = (T)ds;
-                        if constexpr (Range<T>::on) dl[y][w * 4 + i] = (T)(ds - (float)df[y][w * 4 + i]);
+                        dl[y][w * 4 + i] = (T)(ds - (float)df[y][w * 4 + i]);
                     }
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
@@ -239,7 +241,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
 #pragma unroll
                 for (int y = 0; y < RT; ++y) {
                     dq[d][y] = mfma(kf, df[y], dq[d][y]);
-                    if constexpr (Range<T>::on) dq[d][y] = mfma(kf, dl[y], dq[d][y]);
+                    dq[d][y] = mfma(kf, dl[y], dq[d][y]);
                 }
             }
         };
@@ -768,8 +770,8 @@ hipError_t bwd(const AttnArgs &in, hipStream_t s) {
         const int64_t rows = (int64_t)tokens * a.group;
         // 32 rows a wave where that gives each CU a workgroup, else 16, which read
         // twice as much of LDS per product: 216 and 252 workgroups of 128 rows (5506
-        // tokens of 5/1 heads of 64; 3 x 777 of 12, window 256, fp16) take 138 and 26
-        // us, 111 and 21 as twice as many of 64; 264 take 82 both, 536 take 39, 41
+        // tokens of 5/1 heads of 64; 3 x 777 of 12, window 256, fp16) took 138 and 26
+        // us, 111 and 21 as twice as many of 64; 264 took 82 both, 536 took 39, 41
         const bool wide = (rows + 127) / 128 * many * a.kv_heads >= 256;
         a.tiles = (int)(wide ? (rows + 127) / 128 : (rows + 63) / 64) * many + pad;
         if (wide)
