@@ -116,8 +116,10 @@ def sink_window_attention(q, k, v, *, window=None, sinks=0, scale=None, offsets=
     sinks: first tokens that stay visible past the window; scale: 1/sqrt(D).
 
     Differentiable in q, k and v.  Scores, softmax and every sum are held in
-    fp32; probabilities (and, backward, dS) are rounded to the inputs' type
-    for the matrix products.  Deterministic.  With return_lse also the natural
+    fp32; probabilities (and, backward, dS; for dq in two terms) are rounded to
+    the inputs' type for the matrix products.  A NaN or infinity in a key that
+    a row does not see does not reach the row's result; one in a value may, as
+    in a product with weights of 0.  Deterministic.  With return_lse also the natural
     log of each row's softmax sum, fp32 [B, H, Tq] or [H, N] (-inf for a row
     that sees nothing; not differentiable)."""
     if not return_lse and (r := C.fast.attention(q, k, v, offsets, window, sinks, scale)) is not None:

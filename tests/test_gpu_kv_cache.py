@@ -2,7 +2,7 @@
 
 Tolerances.  The values held are exact (E2M1 times a power of two), so the
 formula in 64 bits starts from them.  o: each probability is rounded once to
-bf16 (2^-9 of it; to 2^-17 for fp16 rows) and the result once to its type, so
+the rows' type and the result once, so
 |err| <= 4 u sum_j p_j |v_j| with u = 2^-8 (bf16) or 2^-11 (fp16) has room
 for the fp32 sums.  weights stay in fp32: a score's error is at most
 2^-20 (1 + scale sum |q_d k_d|) with room (chains of at most 128 terms in
