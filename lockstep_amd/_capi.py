@@ -212,12 +212,13 @@ _captured: list = []
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    """A device workspace of at least nbytes for the K slices of a GEMM.
+    """A device workspace of at least nbytes for the K slices of a GEMM, or the
+    key shares of an attention over a cache.
 
     Eager calls share one per (device, stream): calls on one stream are
     ordered, those of several host threads included (the library enqueues the
-    two launches of a sliced call with no other call's between them), so they
-    may share it.  It is kept for later calls and grown by
+    launches of a call that uses it with no other such call's between them, of
+    either operator), so they may share it.  It is kept for later calls and grown by
     replacing it with a larger one (the old one returns to torch's caching
     allocator, stream-ordered).
 

@@ -10,6 +10,10 @@
 #include "lsmx_attn.h"
 #include "lsmx_internal.h"
 
+namespace lsmx {
+std::mutex g_workspace_mu;
+}
+
 namespace {
 
 thread_local char g_err[512] = "";
@@ -971,10 +975,7 @@ int lsmx_kv_attend(const lsmx_kv_cache *c, const void *q, const int64_t *q_strid
     a.scale = scale, a.c = scale * 1.4426950408889634f, a.by_group = lsmx::fast_div((uint32_t)a.group);
     x.weights = weights, x.w_len = w_len, x.splits = plan.splits;
     x.part = (float *)ws, x.part_m = (float *)((uint8_t *)ws + plan.part_m);
-    // calls of several host threads on one stream may share a workspace: the
-    // launches of one stay together
-    static std::mutex mu;
-    std::lock_guard<std::mutex> lk(mu);
+    std::lock_guard<std::mutex> lk(lsmx::g_workspace_mu);
     if (int r = launched(lsmx::launch_kv_attend(x, dtype, (hipStream_t)stream), fn)) return r;
     return weights ? launched(lsmx::launch_kv_weights(x, dtype, (hipStream_t)stream), fn) : LSMX_OK;
 }

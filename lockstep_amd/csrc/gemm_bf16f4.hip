@@ -25,7 +25,6 @@
 // kernel and gemm_bf16f4_kernel half of a tile's A rows are rows of A0 and half
 // the same rows of A1: one weight tile in LDS feeds both batches and is read
 // from memory once per stage.
-#include <mutex>
 
 #include "lsmx_dma.h"
 #include "lsmx_store.h"
@@ -2005,11 +2004,6 @@ __global__ __launch_bounds__(256) void splitk_reduce_kernel(const float *__restr
     }
 }
 
-// The two launches of a sliced call, and no other thread's between them: all
-// host threads on a stream share its workspace, and a call's partials must
-// still be there when its reduction runs.
-static std::mutex g_slices_mu;
-
 // LA: 64 x 128 tiles have 128 registers per lane (two workgroups per CU), which
 // LA = 4 overruns by two
 template <int WM, int WN, int TM, int TN, int S, int LA>
@@ -2025,7 +2019,7 @@ static hipError_t launch_tile(GemmArgs g, int splits, hipStream_t s) {
 #define LSMX_T(CT)                                                                                                 \
     do {                                                                                                           \
         if (splits > 1) {                                                                                          \
-            std::lock_guard<std::mutex> lk(g_slices_mu);                                                           \
+            std::lock_guard<std::mutex> lk(g_workspace_mu);                                                        \
             hipLaunchKernelGGL((gemm_bf16f4_tile_kernel<LSMX_F32, true, WM, WN, TM, TN, S, LA, true>), grid, blk, 0, s, g); \
             hipLaunchKernelGGL((splitk_reduce_kernel<CT>), rgrid, rblk, 0, s, g.ws, splits, nb, Mp, Np, g.c, g.c1, \
                                g.ldc, g.M, g.N);                                                                   \

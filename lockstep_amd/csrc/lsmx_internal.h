@@ -1,9 +1,17 @@
 // Internal launcher interface between the C ABI (capi.hip) and the kernels.
 #pragma once
 
+#include <mutex>
+
 #include "lsmx_common.h"
 
 namespace lsmx {
+
+// Held by every call that passes partial results from one launch to the next
+// through its caller's workspace, over all of its launches (capi.hip): all host
+// threads on a stream may share one workspace, and a call's partials must still
+// be there when its join runs.
+extern std::mutex g_workspace_mu;
 
 // Compile-time arguments passed to the generic lambdas of the pipelined
 // kernels: a ring or register slot, a loader wave or not.

@@ -11,6 +11,8 @@
 //   dense M N K dtype mode nc            lsmx_gemm_dense_nb or lsmx_gemm_dense
 //   threads M N K n calls                n threads x calls of lsmx_gemm_bf16f4_ws on one stream;
 //                                        "split": launches of a call that another thread's interrupted
+//   mixed M N K n calls                  the same with every other call an lsmx_kv_attend of 8 long
+//                                        caches with weights, whose workspace is the same buffer
 //   kernels                              the names of all kernels in the library
 // A leading dimension of 0 stands for the dense one.
 #include <cxxabi.h>
@@ -118,6 +120,13 @@ int w4(int64_t M, int64_t N, int64_t K, int dual, int64_t need, int fmt, int64_t
     return L(lsmx_gemm_bf16f4_ws)(P(), dual ? P() : nullptr, lda, P<uint8_t>(), ldw, P(), lds, fmt, P(),
                                   dual ? P() : nullptr, LSMX_F32, N, M, N, K, need ? P() : nullptr, need, nullptr);
 }
+// 8 sequences of up to 8192 tokens, 2 key heads of 128: keys in shares, a join, the weights' pass
+int attend() {
+    const lsmx_kv_cache c{P<uint8_t>(), P<uint8_t>(), P<uint8_t>(), P<uint8_t>(), 1024, 64, 2, 128,
+                          P<int32_t>(), P<int32_t>(), 8, 128};
+    const int64_t st[3] = {1024, 1024, 128}, need = L(lsmx_kv_attend_workspace)(&c, 1, 8, 0, 0, 1);
+    return L(lsmx_kv_attend)(&c, P(), st, LSMX_BF16, 1, 8, 0, 0, 0.125f, P(), P<float>(), 8192, P(), need, nullptr);
+}
 }  // namespace
 
 int main(int argc, char **argv) {
@@ -165,7 +174,7 @@ int main(int argc, char **argv) {
                                  : L(lsmx_gemm_dense)(P(), P(), K, P(), P(), K, dt, mode, P<float>(), P<float>(), N, M, N,
                                                       K, 1, nullptr);
             std::cout << answer(rc) << std::endl;
-        } else if (op == "threads") {
+        } else if (op == "threads" || op == "mixed") {
             const int n = (int)arg(), calls = (int)arg();
             const int64_t need = L(lsmx_gemm_bf16f4_workspace)(M, N, K, 0);
             std::atomic<int> rc{0};
@@ -175,7 +184,11 @@ int main(int argc, char **argv) {
                 ts.emplace_back([&, i] {
                     for (int c = 0; c < calls; ++c) {
                         t_call = 1 + i * calls + c;
-                        if (w4(M, N, K, 0, need, LSMX_SCALE_E8M0, K, K / 2, K / 32) != 0) rc = 1;
+                        if (op == "mixed" && t_call % 2) {
+                            if (attend() != 0) rc = 1;
+                        } else if (w4(M, N, K, 0, need, LSMX_SCALE_E8M0, K, K / 2, K / 32) != 0) {
+                            rc = 1;
+                        }
                     }
                 });
             for (auto &t : ts) t.join();

@@ -41,6 +41,15 @@ def test_calls_of_several_threads_on_one_stream_keep_their_launches_together(tra
     assert r["split"] == 0
 
 
+def test_calls_that_share_a_workspace_keep_their_launches_together(trace):
+    """Sliced products and cache attention use one buffer per stream: the
+    partials of one must not be overwritten before its join has run."""
+    r, = trace(["mixed 20 4096 14336 4 20"])
+    # a product: slices and reduction; attention: shares, join and weights
+    assert r["rc"] == 0 and r["calls"] == 80 and r["launches"] == 40 * 2 + 40 * 3
+    assert r["split"] == 0
+
+
 @pytest.mark.parametrize("lda,ldb", [(1 << 19, 0), (0, 1 << 19), ((1 << 24) - 16, (1 << 24) - 16)])
 def test_quantizing_gemm_takes_long_rows_on_its_long_row_form(trace, lda, ldb):
     """32 rows of 2^19 bytes do not fit the plain form's 24-bit load offsets."""
