@@ -87,6 +87,7 @@ struct PagedKV {
     uint32_t kr[NQ], vr[NQ];
     uint32_t ke, ve;
     int pg, pgn;  // page of the codes in registers, and of the next tile's
+    bool bad;     // there were blocks that T does not hold
 
     LSMX_DEV static const AttnArgs &attn(const Args &a) { return a.a; }
     LSMX_DEV static bool find(const Args &x, int t, int size, Seq &s) {
@@ -102,7 +103,7 @@ struct PagedKV {
         return true;
     }
     LSMX_DEV void init(const Args &a, const Seq &s, int hkv) {
-        p = &a.p, b = s.b, h = hkv, k_len = s.k_len, row = (threadIdx.x & 255) >> 2, part = threadIdx.x & 3;
+        p = &a.p, b = s.b, h = hkv, k_len = s.k_len, row = (threadIdx.x & 255) >> 2, part = threadIdx.x & 3, bad = false;
     }
     LSMX_DEV int page(int j0) const {
         const int j = j0 + row;
@@ -112,7 +113,7 @@ struct PagedKV {
     LSMX_DEV void codes(int j, const uint8_t *codes, const uint8_t *scale, uint32_t (&w)[NQ], uint32_t &e) {
 #pragma unroll
         for (int i = 0; i < NQ; ++i) w[i] = 0;
-        e = 0;
+        e = 127;
         if (pg >= 0) {
             const int64_t v = p->vec(pg, h, j);
             const uint8_t *c = codes + v * (DP / 2) + part * (DP / 8);
@@ -125,6 +126,7 @@ struct PagedKV {
     }
     LSMX_DEV void store(T *to, const uint32_t (&w)[NQ], uint32_t e) {
         const float sc = block_scale<T>(e);
+        bad = bad | !holds<T>(e);
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
             *(typename Vec<T>::x8 *)(to + row * DP + swz<NC>(row, part * NQ + i) * 8) = fp4x8<T>(w[i], sc);
@@ -168,7 +170,7 @@ struct PagedKV {
 // the backward); 16384 tokens of 8/1 heads of 64 through a window of 4096:
 // 214 us = 562 TFLOP/s.
 template <typename T, int DP, int RT, int NW, int KS, typename KV>
-__global__ __launch_bounds__(NW * KS * 64, DP == 64 && !KV::kHoles ? 3 : 2) void attn_fwd_kernel(typename KV::Args args) {
+__global__ __launch_bounds__(NW * KS * 64, DP == 128 ? 2 : KV::kHoles ? 4 : 3) void attn_fwd_kernel(typename KV::Args args) {
     constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, BM = NW * RT * 16;
     // a row's maximum is followed only when it grows by a factor of 2^8 (fp16:
     // 2^4, below its range with the lift): O is rescaled a few times per row
@@ -372,6 +374,13 @@ __global__ __launch_bounds__(NW * KS * 64, DP == 64 && !KV::kHoles ? 3 : 2) void
         n ^= 1, j0 = j1;
     }
 
+    if constexpr (KV::kHoles && __is_same(T, _Float16)) {
+        if (uniform(__syncthreads_or(kv.bad))) {
+            attend_exact<T, DP, kBN>(args, s.b, hkv, share, row0, min(row0 + BM, rows), last - first,
+                                     [=](int i) { return (first + i < t_sink ? first + i : t_lo + first + i - t_sink) * kBN; });
+            return;
+        }
+    }
     if constexpr (KS == 2) {
         // the second group's sums through LDS to the first, which writes
         static_assert(NW * 64 * RT * ND * 16 + NW * 64 * RT * 8 <= sizeof(s_kv), "");

@@ -113,7 +113,7 @@ struct Codes {
     LSMX_DEV void drop() {
 #pragma unroll
         for (int i = 0; i < NW; ++i) w[i] = 0;
-        e = 0;
+        e = 127;
     }
 };
 
@@ -174,7 +174,9 @@ LSMX_DEV void load_rows(const AttnArgs &a, int b, int hkv, int row, int g, bool 
 // memory.
 template <typename T, int DP, int RT, bool ROWS = false>
 LSMX_DEV void scores(const Codes<DP> &k, const typename Vec<T>::x8 (&q)[RT][DP / 32], f32x4 (&st)[RT]) {
-    const float sc = block_scale<T>(k.e);
+    // (the branches of the general form keep the operands of two groups of keys from
+    // being made at once, which costs a wave per SIMD where registers are few)
+    const float sc = ROWS || RT > 1 ? e8m0_to_f32(k.e) : block_scale<T>(k.e);
 #pragma unroll
     for (int y = 0; y < RT; ++y) st[y] = f32x4{0, 0, 0, 0};
 #pragma unroll
@@ -193,7 +195,7 @@ LSMX_DEV void scores(const Codes<DP> &k, const typename Vec<T>::x8 (&q)[RT][DP /
 // Bound by the loads in flight, so that waves per SIMD count: 4 of them at 64 x
 // 8192 tokens of 8 key heads of 128 take 82 us = 5.2 TB/s (3: 91, 2: 101).
 template <typename T, int DP, int RT>
-__global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(T, __bf16) ? 4 : 3) void kv_decode_kernel(AttendArgs x) {
+__global__ __launch_bounds__(256, RT > 1 && DP == 128 ? 2 : 4) void kv_decode_kernel(AttendArgs x) {
     constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16;
     typedef typename Vec<T>::x8 X8;
     typedef typename Vec<T>::x4 X4;
@@ -232,6 +234,7 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(T, __bf16) 
     }
     T *sv = (T *)smem + wave * 32 * DP;
     const int pfirst = tiles.len - a.q_len;
+    uint64_t bad = 0;  // lanes with a block that T does not hold
 
     for (; i < i1; i += 4) {
         // after the last tile this one again, from the cache: the loads of all
@@ -250,13 +253,17 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(T, __bf16) 
             // what is in no row's sight must not reach a product as a NaN
 #pragma unroll
             for (int t = 0; t < 2; ++t)
-                if (cur.pg[t] < 0 || j0 + t * 16 + r >= tiles.len) cur.v[t].drop();
+                if (cur.pg[t] < 0 || j0 + t * 16 + r >= tiles.len) {
+                    cur.v[t].drop();
+                    if constexpr (__is_same(T, _Float16)) cur.k[t].e = 127;
+                }
         }
         f32x4 st[2][RT];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+            bad |= __ballot(!(holds<T>(cur.k[t].e) & holds<T>(cur.v[t].e)));
             scores<T, DP, RT>(cur.k[t], q, st[t]);
-            const float vsc = block_scale<T>(cur.v[t].e);
+            const float vsc = RT > 1 ? e8m0_to_f32(cur.v[t].e) : block_scale<T>(cur.v[t].e);
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 const int row = t * 16 + lr, c = g * NS + s;
@@ -315,6 +322,12 @@ __global__ __launch_bounds__(256, RT > 1 ? 2 : DP == 64 || __is_same(T, __bf16) 
         }
         asm volatile("" ::: "memory");
         cur = nxt;
+    }
+    if constexpr (__is_same(T, _Float16)) {
+        if (uniform(__syncthreads_or(bad != 0))) {
+            attend_exact<T, DP, 32>(x, b, hkv, sp, 0, rows, i1 - i0, [=](int k) { return tiles[i0 + k] * 32; });
+            return;
+        }
     }
 
     // join the waves, 16 rows at a time
@@ -474,6 +487,49 @@ LSMX_DEV float sum_16(float x) {  // over the 16 lanes of a row of lanes
     x += u2f(__builtin_amdgcn_update_dpp(0, f2u(x), 0x140, 0xF, 0xF, true));  // row_mirror
     return x;
 }
+// The weight of key j, vector vec, over every step-th row of [row0, row1), in fp32
+// (holds).
+template <typename T, int DP>
+LSMX_DEV float weight_exact(const AttendArgs &x, int b, int hkv, int j, int64_t vec, int row0, int row1, int step) {
+    const AttnArgs &a = x.a;
+    const int shift = x.p.length(b) - a.q_len;
+    float sum = 0.f;
+#pragma unroll 1
+    for (int row = row0; row < row1; row += step) {
+        const int tok = div_by(row, a.by_group), h = hkv * a.group + row - tok * a.group;
+        const T *q = (const T *)a.q + b * a.q_b + tok * a.q_t + h * a.q_h;
+        const float s = dot_exact(q, x.p.kc + vec * (DP / 2), x.p.ks + vec * (DP / 32), DP);
+        const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(s, a.c, -a.lse[b * a.lse_b + h * a.lse_h + tok]));
+        sum += sees(j, tok + shift, window_low(tok + shift, a.window), a.sinks) ? v : 0.f;
+    }
+    return sum;
+}
+// Whether T holds the blocks of a tile's keys before position len.
+template <typename T, int DP>
+LSMX_DEV bool all_held(const Keys<DP, false> &k, int len) {
+    if constexpr (!__is_same(T, _Float16)) return true;
+    const int r = threadIdx.x & 15;
+    return __all((holds<T>(k.k[0].e) | (k.j0 + r >= len)) & (holds<T>(k.k[1].e) | (k.j0 + 16 + r >= len)));
+}
+// The weights over the tiles i, i + 4, .. that it does not hold.
+template <typename T, int DP>
+LSMX_DEV void weights_exact(const AttendArgs &x, int b, int hkv, int i, int i1) {
+    int thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));  // as in attend_exact
+    const Pool &p = x.p;
+    const int lane = thread & 63, g = lane >> 4, r = lane & 15;
+    const Tiles tiles(x, b);
+    Walk walk(p, tiles, b, i, i1);
+    Keys<DP, false> cur;
+    for (; i < i1; i += 4) {
+        walk.find(i, cur);
+        cur.load(p, hkv, g, r);
+        const int j = cur.j0 + (lane & 31), pg = g == 0 ? cur.pg[0] : cur.pg[1];
+        if (!all_held<T, DP>(cur, tiles.len) && lane < 32 && j < tiles.len && pg >= 0)
+            x.weights[(int64_t)(b * x.a.kv_heads + hkv) * x.w_len + j] +=
+                weight_exact<T, DP>(x, b, hkv, j, p.vec(pg, hkv, j), 0, x.a.q_len * x.a.group, 1);
+    }
+}
 template <typename T, int DP, int RT>
 __global__ __launch_bounds__(256) void kv_weights_kernel(AttendArgs x) {
     constexpr int NS = DP / 32;
@@ -487,6 +543,7 @@ __global__ __launch_bounds__(256) void kv_weights_kernel(AttendArgs x) {
     const int i0 = (int)((int64_t)tiles.n * sp / x.splits), i1 = (int)((int64_t)tiles.n * (sp + 1) / x.splits);
     if (i0 + wave >= i1) return;
     float *w = x.weights + (int64_t)bh * x.w_len;
+    bool left = false;
     for (int row0 = 0; row0 < rows; row0 += RT * 16) {
         Keys<DP, false> cur, nxt;
         int i = i0 + wave;
@@ -520,6 +577,8 @@ __global__ __launch_bounds__(256) void kv_weights_kernel(AttendArgs x) {
             walk.find(i + 4 < i1 ? i + 4 : i, nxt);
             nxt.load(p, hkv, g, r);
             const bool full = j0 + 31 <= pfirst && (!a.window || j0 > tiles.len - 1 - a.window || j0 + 31 < a.sinks);
+            const bool ok = all_held<T, DP>(cur, full ? 0x7FFFFFFF : tiles.len);
+            left = left | !ok;
             float sum[2] = {0.f, 0.f};
             auto add = [&](auto all) {
 #pragma unroll
@@ -543,10 +602,11 @@ __global__ __launch_bounds__(256) void kv_weights_kernel(AttendArgs x) {
             else
                 add(BoolC<false>{});
             const float s0 = sum_rows(sum[0]), s1 = sum_rows(sum[1]);
-            if (held) w[mine] = before + (g == 0 ? s0 : s1);
+            if (held & ok) w[mine] = before + (g == 0 ? s0 : s1);
             cur = nxt;
         }
     }
+    if (left) weights_exact<T, DP>(x, b, hkv, i0 + wave, i1);
 }
 
 // Many rows: a workgroup owns 64 keys, whose operands stay in registers, and
@@ -575,6 +635,7 @@ __global__ __launch_bounds__(NW * 64) void kv_weights_rows_kernel(AttendArgs x) 
     if (tok_lo >= tok_hi) return;
     X8 kf[4][NS];
     int pg[4];
+    bool ok = true;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         const int j = j0 + t * 16;
@@ -587,6 +648,25 @@ __global__ __launch_bounds__(NW * 64) void kv_weights_rows_kernel(AttendArgs x) 
             k.drop();
 #pragma unroll
         for (int s = 0; s < NS; ++s) kf[t][s] = fp4x8<T>(k.w[s], block_scale<T>(k.e));
+        ok = ok && (holds<T>(k.e) || pg[t] < 0 || j + r >= len);
+    }
+    auto put = [&] {  // the waves' sums of the 64 keys
+        __syncthreads();
+        const int at = j0 + threadIdx.x;
+        if (threadIdx.x < 64 && at < len) {
+            float all = 0.f;
+#pragma unroll
+            for (int i = 0; i < NW; ++i) all += s_sum[i][threadIdx.x];
+            x.weights[(int64_t)bh * x.w_len + at] += all;
+        }
+    };
+    if constexpr (__is_same(T, _Float16)) {
+        if (!__all(ok)) {  // in every wave alike
+            const int j = j0 + lane, own = j < len ? p.page_of(b, j) : -1;
+            s_sum[wave][lane] = own < 0 ? 0.f : weight_exact<T, DP>(x, b, hkv, j, p.vec(own, hkv, j), tok_lo * a.group + wave, tok_hi * a.group, NW);
+            put();
+            return;
+        }
     }
     f32x4 sum[4];
     uint32_t span[4][4];  // position p sees key j when 0 <= p - j <= span
@@ -656,14 +736,7 @@ __global__ __launch_bounds__(NW * 64) void kv_weights_rows_kernel(AttendArgs x) 
             const float all = sum_16(sum[t][e]);
             if (r == 0) s_sum[wave][t * 16 + g * 4 + e] = pg[t] >= 0 ? all : 0.f;
         }
-    __syncthreads();
-    const int at = j0 + threadIdx.x;
-    if (threadIdx.x < 64 && at < len) {
-        float all = 0.f;
-#pragma unroll
-        for (int i = 0; i < NW; ++i) all += s_sum[i][threadIdx.x];
-        x.weights[(int64_t)bh * x.w_len + at] += all;
-    }
+    put();
 }
 
 // ------------------------------------------------------------------ eviction

@@ -269,16 +269,8 @@ struct EvictArgs {
 template <typename T>
 constexpr float kLift = __is_same(T, _Float16) ? 11.f : 0.f;
 
-// The 8 elements of four bytes of codes, times 2^e of their block (e: its E8M0
-// byte).  Exact in bf16; in fp16 (the operands of fp16 rows) too for values that
-// fp16 holds.  Blocks above it are clipped to its range, so that no
-// infinity meets a probability of 0, and below it the elements round to its
-// smallest ones.
-template <typename T>
-LSMX_DEV float block_scale(uint32_t e) {
-    if constexpr (__is_same(T, _Float16)) e = e == 255u ? e : min(e, 127u + 13u);
-    return e8m0_to_f32(e);
-}
+// The 8 elements of four bytes of codes, times their block's scale.  Exact in bf16,
+// which has E8M0's range; in fp16 where it holds them (holds).
 LSMX_DEV bf16x8 fp4x8_to(uint32_t w, float sc, bf16x8) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1);
     const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3);
@@ -292,6 +284,105 @@ LSMX_DEV f16x8 fp4x8_to(uint32_t w, float sc, f16x8) {
 template <typename T>
 LSMX_DEV typename Vec<T>::x8 fp4x8(uint32_t w, float sc) {
     return fp4x8_to(w, sc, typename Vec<T>::x8{});
+}
+
+// Rows in fp16 take the cached values in fp16 too (as bf16 operands they would need
+// two terms of everything, and 1.5 times as long), where it has all elements of a
+// block: 6 times 2^13 is the largest it holds, half of 2^-23 the smallest.  A cache
+// written from fp16 has no other blocks but those whose largest value is below 2^-21; one
+// written from bf16 may have any.  A workgroup that meets one takes its rows in
+// fp32 without matrix instructions (attend_exact), 20 to 80 times as long: 64 x 8192
+// tokens of 8 key heads of 128, 4 rows, 2.3 ms for 90 us.  A second form of the
+// kernels' loops with bf16 operands would be faster there, and cost the others a wave
+// per SIMD.
+template <typename T>
+LSMX_DEV bool holds(uint32_t e8m0) {
+    return !__is_same(T, _Float16) || e8m0 - (127u - 23u) <= 36u;
+}
+
+// The scale of a block that T holds (of others anything: their products are not used).
+template <typename T>
+LSMX_DEV float block_scale(uint32_t e8m0) {
+    if constexpr (__is_same(T, _Float16)) return u2f(e8m0 << 23);
+    return e8m0_to_f32(e8m0);
+}
+
+// The product of a row with a cached vector, in fp32.
+template <typename T>
+LSMX_DEV float dot_exact(const T *q, const uint8_t *codes, const uint8_t *scale, int dim) {
+    float sum = 0.f;
+#pragma unroll 1
+    for (int d = 0; d < dim; d += 8) {
+        const typename Vec<T>::x8 x = *(const typename Vec<T>::x8 *)(q + d);
+        const bf16x8 k = fp4x8<__bf16>(*(const uint32_t *)(codes + d / 2), e8m0_to_f32(scale[d >> 5]));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf((float)x[i], (float)k[i], sum);
+    }
+    return sum;
+}
+
+// Attention of rows [row0, row1) of sequence b and key head hkv over the keys of
+// `tiles` tiles of TS keys, the i-th from key key_of(i) on; writes what the kernels
+// write of a share.  A wave takes a row: its lanes the keys for the scores, then the
+// head's elements for the values.
+template <typename T, int DP, int TS, typename F>
+LSMX_DEV void attend_exact(const AttendArgs &x, int b, int hkv, int share, int row0, int row1, int tiles, F key_of) {
+    constexpr int NE = DP / 64;
+    const AttnArgs &a = x.a;
+    const Pool &p = x.p;
+    int thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));  // nothing made from it is shared with the caller's loop, and held over that
+    const int lane = thread & 63, len = p.length(b), rows = a.q_len * a.group;
+#pragma unroll 1
+    for (int row = row0 + uniform(thread >> 6); row < row1; row += blockDim.x >> 6) {
+        const int tok = div_by(row, a.by_group), h = hkv * a.group + row - tok * a.group, pos = tok + len - a.q_len;
+        const int low = window_low(pos, a.window);
+        const T *q = (const T *)a.q + b * a.q_b + tok * a.q_t + h * a.q_h;
+        float m = -INFINITY, l = 0.f, acc[NE] = {};
+#pragma unroll 1
+        for (int i = 0; i < tiles; ++i) {
+            const int j = key_of(i) + lane;
+            int pg = -1;
+            if (lane < TS && j < len && sees(j, pos, low, a.sinks)) pg = p.page_of(b, j);
+            const int64_t vec = p.vec(max(pg, 0), hkv, max(j, 0));
+            const float s = pg >= 0 ? dot_exact(q, p.kc + vec * (DP / 2), p.ks + vec * (DP / 32), DP) : -INFINITY;
+            float top = s;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+            top = fmaxf(top, m);
+            const float alpha = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - top) * a.c);
+            const float w = pg < 0 ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(s, a.c, top == -INFINITY ? 0.f : kLift<T> - top * a.c));
+            m = top;
+            l = __builtin_fmaf(l, alpha, w);
+#pragma unroll
+            for (int e = 0; e < NE; ++e) acc[e] *= alpha;
+#pragma unroll 1
+            for (int t = 0; t < TS; ++t) {
+                const int pt = lane_of(pg, t);
+                if (pt < 0) continue;
+                const float wt = u2f(lane_of(f2u(w), t));
+                const int64_t v = p.vec(pt, hkv, lane_of(j, t));
+                const uint32_t code = p.vc[v * (DP / 2) + lane * NE / 2] >> (NE == 1 ? 4 * (lane & 1) : 0);
+                const bf16x8 f = fp4x8<__bf16>(code, e8m0_to_f32(p.vs[v * (DP / 32) + lane * NE / 32]));
+#pragma unroll
+                for (int e = 0; e < NE; ++e) acc[e] = __builtin_fmaf(wt, (float)f[e], acc[e]);
+            }
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
+        if (x.splits > 1) {
+            const int64_t at = ((int64_t)(b * a.kv_heads + hkv) * x.splits + share) * rows + row;
+#pragma unroll
+            for (int e = 0; e < NE; ++e) x.part[at * DP + lane * NE + e] = acc[e];
+            if (lane == 0) x.part_m[at * 2] = m, x.part_m[at * 2 + 1] = l;
+            continue;
+        }
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) ((T *)a.o)[b * a.o_b + tok * a.o_t + h * a.o_h + lane * NE + e] = (T)(acc[e] * inv);
+        if (a.lse && lane == 0)
+            a.lse[b * a.lse_b + h * a.lse_h + tok] = l > 0.f ? m * a.c - kLift<T> + __log2f(l) : l != l ? l : -INFINITY;
+    }
 }
 
 // Rows (tokens x heads of a key head) up to which each wave of the cache

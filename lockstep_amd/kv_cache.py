@@ -123,9 +123,9 @@ def attend(q, pages, table, lengths, *, window=None, sinks=0, scale=None, weight
     sequence b has position lengths[b] - T + i and sees key j when j <= its
     position and (window is None, or j > position - window, or j < sinks).
     A row that sees nothing gives 0.  Returns o [B, T, H, D] in q's type.
-    Scores, softmax and sums are fp32; cached values are exact in bf16, and in
-    fp16 within its range (below 2^-14 they lose bits, above 65504 they are
-    cut); probabilities are rounded to q's type for the product with them.
+    Scores, softmax and sums are fp32; cached values enter as they are held
+    (fp16 rows over blocks that fp16 does not hold take a slow path in fp32);
+    probabilities are rounded to q's type for the product with them.
 
     weights (fp32 [B, Hkv, >= max_pages * page], contiguous): the softmax
     weight of every key, summed over the T tokens and the heads that share its
