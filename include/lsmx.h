@@ -528,7 +528,8 @@ int lsmx_kv_attend(const lsmx_kv_cache *c, const void *q, const int64_t *q_strid
 /* Cuts every sequence and key head to at most `keep` tokens: the first
  * `sinks`, the last `recent`, and of the others those with the largest
  * weights [batch, kv_heads, w_len] (ties: the lower position; -0 equals 0; a
- * NaN is above all), in their order (sinks + recent <= keep).  They are
+ * NaN is above all), in their order (sinks + recent <= keep).  Tokens whose id
+ * lies outside the pool do not stay and are not counted.  What stays is
  * copied to positions 0, 1, .. of the pages out_table [batch, out_max_pages]
  * of the same pool, which must not be pages of `table`.  index
  * [batch, kv_heads, keep]: the positions they had, -1 past the last;

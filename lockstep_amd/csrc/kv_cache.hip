@@ -757,37 +757,69 @@ LSMX_DEV uint32_t rank_of(float w) {
 constexpr int kSelect = 1024;
 template <int PER>
 __global__ __launch_bounds__(kSelect) void kv_select_kernel(EvictArgs a) {
-    __shared__ int hist[256], s_scan[2][kSelect / 64], s_pick[2];
+    __shared__ int hist[256], s_scan[2][kSelect / 64], s_lost[kSelect / 64], s_pick[2];
     const int bh = blockIdx.x, b = bh / a.p.kv_heads, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int n = a.p.length(b);
     const float *w = a.weights + (int64_t)bh * a.w_len;
     int32_t *index = a.index + (int64_t)bh * a.keep;
     float *kept = a.new_weights + (int64_t)bh * a.keep;
-    if (bh % a.p.kv_heads == 0 && tid == 0) a.new_lengths[b] = min(n, a.keep);
     const int c0 = min(a.sinks, n), c1 = max(c0, n - a.recent);  // candidates
-    const bool all = n <= a.keep;
-    int want = all ? 0 : a.keep - (n - (c1 - c0));  // of the candidates
-    uint32_t prefix = 0;
+    uint32_t prefix = 0, there = ~0u;  // bit k: of round k
     float own[PER ? PER : 1];
 #pragma unroll
     for (int k = 0; k < PER; ++k) own[k] = k * kSelect + tid < n ? w[k * kSelect + tid] : 0.f;
-    // body(position, weight, whether it is one), by all threads alike
+    // positions in no page are not there
+    bool lost = false;
+    for (int g = tid; g << a.p.page_shift < n; g += kSelect) lost = lost | (a.p.page_of(b, g << a.p.page_shift) < 0);
+    const bool any = __any(lost);
+    if (lane == 0) s_lost[wave] = any;
+    __syncthreads();
+    const bool holes = __any(s_lost[lane % (kSelect / 64)]);
+    if (PER > 0 && holes) {
+        for (int k = 0; k < PER; ++k) {
+            const int j = k * kSelect + tid;
+            if (j < n && a.p.page_of(b, j) < 0) there &= ~(1u << k);
+        }
+    }
+    // body(position, weight, whether it is there), by all threads alike
     auto each = [&](auto body) {
         if constexpr (PER > 0) {
 #pragma unroll
             for (int k = 0; k < PER; ++k)
-                if (k * kSelect < n) body(k * kSelect + tid, own[k]);
+                if (k * kSelect < n) body(k * kSelect + tid, own[k], (there >> k) & 1);
         } else {
-            for (int j = tid; j - tid < n; j += kSelect) body(j, j < n ? w[j] : 0.f);
+            if (holes) {
+                for (int j = tid; j - tid < n; j += kSelect) body(j, j < n ? w[j] : 0.f, j < n && a.p.page_of(b, j) >= 0);
+            } else {
+                for (int j = tid; j - tid < n; j += kSelect) body(j, j < n ? w[j] : 0.f, true);
+            }
         }
     };
+    int total = n, free = c1 - c0;
+    if (holes) {
+        if (tid < 2) s_pick[tid] = 0;
+        __syncthreads();
+        int gone = 0, gone_free = 0;
+        each([&](int j, float, bool in) {
+            const bool no = j < n && !in;
+            gone += no, gone_free += no && j >= c0 && j < c1;
+        });
+        atomicAdd(&s_pick[0], gone);
+        atomicAdd(&s_pick[1], gone_free);
+        __syncthreads();
+        total -= s_pick[0], free -= s_pick[1];
+        __syncthreads();
+    }
+    const bool all = total <= a.keep;
+    int want = all ? 0 : a.keep - (total - free);  // of the candidates
+    if (bh % a.p.kv_heads == 0 && tid == 0) a.new_lengths[b] = min(total, a.keep);
     if (!all) {
         for (int shift = 24; shift >= 0; shift -= 8) {
             if (tid < 256) hist[tid] = 0;
             __syncthreads();
-            each([&](int j, float x) {
+            each([&](int j, float x, bool in) {
                 const uint32_t u = rank_of(x);
-                if (j >= c0 && j < c1 && (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))))
+                if (in && j >= c0 && j < c1 && (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))))
                     atomicAdd(&hist[(u >> shift) & 255], 1);
             });
             __syncthreads();
@@ -818,8 +850,8 @@ __global__ __launch_bounds__(kSelect) void kv_select_kernel(EvictArgs a) {
     // prefix is the rank of the last that stays, `want` the number of its
     // equals that do (the first of them)
     const uint64_t below = (1ull << lane) - 1;
-    auto held = [&](int j, uint32_t u) { return j < n && (all || j < c0 || j >= c1 || u > prefix); };
-    auto tie = [&](int j, uint32_t u) { return j < n && !all && j >= c0 && j < c1 && u == prefix; };
+    auto held = [&](int j, uint32_t u, bool in) { return in && j < n && (all || j < c0 || j >= c1 || u > prefix); };
+    auto tie = [&](int j, uint32_t u, bool in) { return in && j < n && !all && j >= c0 && j < c1 && u == prefix; };
     int out = 0;
     if constexpr (PER > 0) {
         // counts of all (round, wave) pairs at once: their sums before each pair
@@ -849,7 +881,7 @@ __global__ __launch_bounds__(kSelect) void kv_select_kernel(EvictArgs a) {
         uint32_t stay = 0;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-            const uint64_t m = __ballot(tie(k * kSelect + tid, rank_of(own[k])));
+            const uint64_t m = __ballot(tie(k * kSelect + tid, rank_of(own[k]), (there >> k) & 1));
             if (lane == 0) s_pair[k * (kSelect / 64) + wave] = __popcll(m);
         }
         scan();
@@ -857,9 +889,9 @@ __global__ __launch_bounds__(kSelect) void kv_select_kernel(EvictArgs a) {
         for (int k = 0; k < PER; ++k) {
             const int j = k * kSelect + tid;
             const uint32_t u = rank_of(own[k]);
-            const bool t = tie(j, u);
+            const bool t = tie(j, u, (there >> k) & 1);
             const uint64_t m = __ballot(t);
-            const bool in = held(j, u) | (t & (s_pair[k * (kSelect / 64) + wave] + __popcll(m & below) < want));
+            const bool in = held(j, u, (there >> k) & 1) | (t & (s_pair[k * (kSelect / 64) + wave] + __popcll(m & below) < want));
             stay |= (uint32_t)in << k;
         }
         __syncthreads();
@@ -879,9 +911,9 @@ __global__ __launch_bounds__(kSelect) void kv_select_kernel(EvictArgs a) {
         out = s_pair[NP];
     } else {
         int ties = 0;
-        each([&](int j, float x) {
+        each([&](int j, float x, bool is) {
             const uint32_t u = rank_of(x);
-            const bool t = tie(j, u);
+            const bool t = tie(j, u, is);
             const uint64_t bt = __ballot(t);
             if (lane == 0) s_scan[0][wave] = __popcll(bt);
             __syncthreads();
@@ -895,7 +927,7 @@ __global__ __launch_bounds__(kSelect) void kv_select_kernel(EvictArgs a) {
             };
             int before, total;
             scan(s_scan[0], before, total);
-            const bool in = held(j, u) | (t & (ties + before + __popcll(bt & below) < want));
+            const bool in = held(j, u, is) | (t & (ties + before + __popcll(bt & below) < want));
             ties += total;
             const uint64_t bs = __ballot(in);
             if (lane == 0) s_scan[1][wave] = __popcll(bs);

@@ -170,6 +170,7 @@ def evict(pages, table, lengths, weights, keep, out_table, *, sinks=0, recent=0)
     The first `sinks` and the last `recent` tokens stay; of the others those
     with the largest weights (fp32 [B, Hkv, >= max_pages * page], as attend
     accumulates them; ties: the earlier token; a NaN counts as the largest).
+    Tokens in no page (an id outside the pool) do not stay, nor count.
     What stays keeps its order and is copied to positions 0, 1, .. of the
     pages of out_table (int32 [B, pages for `keep` tokens], same pool, other
     pages than table's: the old ones are free afterwards, or still another
