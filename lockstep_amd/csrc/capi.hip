@@ -774,7 +774,7 @@ static int attn_args(const char *fn, const lsmx_attention *a, bool bwd, lsmx::At
     const bool nq = a->batch && a->q_len, nk = a->batch && a->k_len;
     if ((nq || a->offsets) && a->q_len && (!a->q || !a->o)) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
     if ((nk || a->offsets) && a->k_len && (!a->k || !a->v)) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
-    if (bwd && nq && (!a->lse || !a->o_rest)) return fail(LSMX_ERR_ARG, "%s: null lse or o_rest", fn);
+    if (bwd && (nq || a->offsets) && a->q_len && (!a->lse || !a->o_rest)) return fail(LSMX_ERR_ARG, "%s: null lse or o_rest", fn);
     if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->o, 16) || !aligned(a->o_rest, 16) ||
         !aligned(a->lse, 4) || !aligned(a->offsets, 4))
         return fail(LSMX_ERR_ALIGN, "%s: operands must be 16-byte aligned", fn);

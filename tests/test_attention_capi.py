@@ -69,6 +69,17 @@ def test_attention_backward_refusals():
     assert lib.lsmx_attention_fwd(None, None) == C.ERR_ARG
 
 
+def test_attention_backward_of_tokens_in_no_sequence():
+    """Packed without a sequence: the tokens' gradients are written (zeros), so lse
+    and o_rest are read and must be there."""
+    lib, st = C.load(), I3(0, 256, 64)
+    for bad in (dict(lse=None), dict(o_rest=None)):
+        a = attention(batch=0, offsets=FAKE, **bad)
+        n = lib.lsmx_attention_workspace(ctypes.byref(a))
+        assert lib.lsmx_attention_bwd(ctypes.byref(a), FAKE, ctypes.byref(st), FAKE, FAKE, FAKE, FAKE, n, None) == C.ERR_ARG
+        assert "o_rest" in C.last_error()
+
+
 def cache(**kw):
     c = C.KVCache(FAKE, FAKE, FAKE, FAKE, 8, 16, 2, 64, FAKE, FAKE, 2, 4)
     for k, v in kw.items():
