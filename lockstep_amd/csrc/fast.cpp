@@ -654,7 +654,7 @@ PyObject *kv_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const Tensor &t = *kv[i];
         NONE_IF(t.stride(d - 1) != 1 || !al(t, 16) || (t.size(d - 2) > 1 && t.stride(d - 2) % 8) ||
                 (t.size(d - 3) > 1 && t.stride(d - 3) % 8));
-        st[i][0] = t.size(d - 3) > 1 ? t.stride(d - 3) : d == 4 ? t.stride(0) : 0;
+        st[i][0] = t.size(d - 3) > 1 ? t.stride(d - 3) : d == 4 && t.size(0) > 1 ? t.stride(0) : 0;
         st[i][1] = t.size(d - 2) > 1 ? t.stride(d - 2) : 0;
         // the sequences of a dense call one after another
         NONE_IF(d == 4 && t.size(0) > 1 && (st[i][0] % 8 || t.stride(0) != st[i][0] * t.size(1)));

@@ -55,3 +55,18 @@ def test_evict_leaves_out_what_is_in_no_page(lens, page, keep, sinks, recent, go
                 assert torch.equal(s[at, h], d[:, h])
         if not there:
             assert (o[b] == 0).all()
+
+
+def test_append_of_one_token_with_an_odd_stride(dev):
+    """The stride of an axis of one element means nothing."""
+    from lockstep_amd import fp4
+    from lockstep_amd import kv_cache as kc
+    base = torch.randn((3, 513), device=dev).half()
+    x = base[:, :512].view(3, 1, 8, 64)[0:1]
+    assert x.stride(0) % 8 and x.data_ptr() % 16 == 0
+    pages = kc.new_pages(1, 8, 64, 16, device=dev)
+    table, lengths = torch.zeros((1, 1), dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    kc.append(pages, x, x, table, lengths)
+    codes, scale = fp4.quantize_pack_mxfp4(x[0, 0].contiguous())
+    for c, s in (pages[:2], pages[2:]):
+        assert torch.equal(c[0, :, 0], codes) and torch.equal(s[0, :, 0], scale)
