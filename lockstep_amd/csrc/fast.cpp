@@ -659,7 +659,8 @@ PyObject *kv_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
         // the sequences of a dense call one after another
         NONE_IF(d == 4 && t.size(0) > 1 && (st[i][0] % 8 || t.stride(0) != st[i][0] * t.size(1)));
     }
-    const bool values = a[6] == Py_True;
+    const int values = PyObject_IsTrue(a[6]);
+    if (values < 0) return nullptr;
     const int64_t tokens = off ? k->size(0) : k->size(0) * k->size(1);
     Tensor ko, vo;
     if (values) ko = make(k->sizes(), at::kBFloat16, *k), vo = make(k->sizes(), at::kBFloat16, *k);

@@ -70,3 +70,14 @@ def test_append_of_one_token_with_an_odd_stride(dev):
     codes, scale = fp4.quantize_pack_mxfp4(x[0, 0].contiguous())
     for c, s in (pages[:2], pages[2:]):
         assert torch.equal(c[0, :, 0], codes) and torch.equal(s[0, :, 0], scale)
+
+
+@pytest.mark.parametrize("values", [1, "yes", True])
+def test_append_returns_values_for_any_true_flag(values, dev):
+    from lockstep_amd import kv_cache as kc
+    pages = kc.new_pages(1, 2, 64, 16, device=dev)
+    table, lengths = torch.zeros((1, 1), dtype=torch.int32, device=dev), torch.full((1,), 3, dtype=torch.int32, device=dev)
+    x = torch.randn((1, 3, 2, 64), device=dev).bfloat16()
+    k, v = kc.append(pages, x, x, table, lengths, values=values)
+    assert torch.equal(k, v) and k.shape == x.shape
+    assert kc.append(pages, x, x, table, lengths, values=0) is None
