@@ -17,6 +17,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _capi as C
 
@@ -115,7 +116,7 @@ def sink_window_attention(q, k, v, *, window=None, sinks=0, scale=None, offsets=
     window: keys a query sees, its own the last of them (None: all);
     sinks: first tokens that stay visible past the window; scale: 1/sqrt(D).
 
-    Differentiable in q, k and v.  Scores, softmax and every sum are held in
+    Differentiable in q, k and v (once, in reverse mode).  Scores, softmax and every sum are held in
     fp32; probabilities (and, backward, dS; for dq in two terms) are rounded to
     the inputs' type for the matrix products.  A NaN or infinity in a key that
     a row does not see does not reach the row's result; one in a value may, as
@@ -145,7 +146,9 @@ def sink_window_attention(q, k, v, *, window=None, sinks=0, scale=None, offsets=
     assert len({t.device for t in (q, k, v, *(() if offsets is None else (offsets,)))}) == 1, \
         "all tensors must be on one device"
     window, sinks, scale = check_mask(window, sinks, scale, D)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    # a dual tensor too goes to the node, which refuses it
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or \
+            any(forward_ad.unpack_dual(t).tangent is not None for t in (q, k, v)):
         o, lse = _SinkWindowAttention.apply(q, k, v, offsets, window, sinks, scale)
     else:
         *_, o, _, lse = _forward(q, k, v, offsets, window, sinks, scale, False)

@@ -489,6 +489,9 @@ bool int32_on(const Tensor *t, const Tensor &like, int64_t dims) {
     return t && t->scalar_type() == at::kInt && t->dim() == dims && t->is_contiguous() && t->device() == like.device();
 }
 
+// Forward-mode derivatives are refused by the Python path's node.
+bool dual(const Tensor &t) { return t._fw_grad(0).defined(); }
+
 struct Failed {
     int rc;
 };
@@ -576,7 +579,8 @@ PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     NONE_IF(n != 7);
     const Tensor *q = plain(a[0]), *k = plain(a[1]), *v = plain(a[2]), *off = a[3] == Py_None ? nullptr : plain(a[3]);
-    NONE_IF(!q || !k || !v || (a[3] != Py_None && !off) || at::autocast::is_autocast_enabled(at::kCUDA));
+    NONE_IF(!q || !k || !v || (a[3] != Py_None && !off) || at::autocast::is_autocast_enabled(at::kCUDA) || dual(*q) || dual(*k) ||
+            || dual(*v));
     const int64_t d = off ? 3 : 4;
     NONE_IF(q->dim() != d || k->dim() != d || !k->sizes().equals(v->sizes()) || !bf16_or_f16(*q) ||
             k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type() || k->device() != q->device() ||

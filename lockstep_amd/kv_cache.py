@@ -13,7 +13,7 @@ a pool of pages that sequences own through a block table:
 
 table is int32 [B, max_pages] and lengths int32 [B], both on the device; token
 j of sequence b lies in page table[b, j // page], slot j % page.  Entries past
-a sequence's pages are never read.  No call synchronizes.  Kernels:
+a sequence's pages are never read.  No call synchronizes, or is differentiable.  Kernels:
 lockstep_amd/csrc/kv_cache.hip, and attention.hip for many rows.
 """
 
@@ -129,7 +129,7 @@ def attend(q, pages, table, lengths, *, window=None, sinks=0, scale=None, weight
 
     weights (fp32 [B, Hkv, >= max_pages * page], contiguous): the softmax
     weight of every key, summed over the T tokens and the heads that share its
-    head, is added in place.  Deterministic."""
+    head, is added in place.  Deterministic.  The result has no gradient."""
     if (r := C.fast.kv_attend(q, pages, table, lengths, window, sinks, scale, weights)) is not None:
         return r
     c = _cache(pages, table, lengths)
