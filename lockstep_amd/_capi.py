@@ -201,6 +201,13 @@ def require_device(*tensors: torch.Tensor) -> None:
                 f"{t.device} (there is no CPU fallback)")
 
 
+def not_traced(name: str) -> None:
+    """torch.jit.trace records torch's own calls only: of a kernel's call it would
+    keep the allocation of the output, whose contents then are anything."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{name} cannot be traced: torch.jit.trace does not see the kernels' work")
+
+
 def slice_bytes(M: int, N: int, K: int, dual: bool) -> int:
     """Workspace bytes of the weight-only GEMM: 0 where it runs whole K."""
     L = load()

@@ -125,6 +125,7 @@ def sink_window_attention(q, k, v, *, window=None, sinks=0, scale=None, offsets=
     that sees nothing; not differentiable)."""
     if not return_lse and (r := C.fast.attention(q, k, v, offsets, window, sinks, scale)) is not None:
         return r
+    C.not_traced("sink_window_attention")
     if torch.is_autocast_enabled("cuda"):
         dt = torch.get_autocast_dtype("cuda")
         q, k, v = q.to(dt), k.to(dt), v.to(dt)

@@ -16,6 +16,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -489,7 +490,9 @@ bool int32_on(const Tensor *t, const Tensor &like, int64_t dims) {
     return t && t->scalar_type() == at::kInt && t->dim() == dims && t->is_contiguous() && t->device() == like.device();
 }
 
-// Forward-mode derivatives are refused by the Python path's node.
+// Under torch.jit.trace the Python path refuses the call; forward-mode
+// derivatives are refused by its node.
+bool traced() { return at::tracer::impl::is_dispatch_enabled(); }
 bool dual(const Tensor &t) { return t._fw_grad(0).defined(); }
 
 struct Failed {
@@ -579,8 +582,8 @@ PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     NONE_IF(n != 7);
     const Tensor *q = plain(a[0]), *k = plain(a[1]), *v = plain(a[2]), *off = a[3] == Py_None ? nullptr : plain(a[3]);
-    NONE_IF(!q || !k || !v || (a[3] != Py_None && !off) || at::autocast::is_autocast_enabled(at::kCUDA) || dual(*q) || dual(*k) ||
-            || dual(*v));
+    NONE_IF(!q || !k || !v || (a[3] != Py_None && !off) || at::autocast::is_autocast_enabled(at::kCUDA) || traced() || dual(*q) ||
+            dual(*k) || dual(*v));
     const int64_t d = off ? 3 : 4;
     NONE_IF(q->dim() != d || k->dim() != d || !k->sizes().equals(v->sizes()) || !bf16_or_f16(*q) ||
             k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type() || k->device() != q->device() ||
@@ -646,7 +649,7 @@ PyObject *kv_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     NONE_IF(n != 7);
     lsmx_kv_cache c;
     const Tensor *like, *k = plain(a[1]), *v = plain(a[2]), *off = a[5] == Py_None ? nullptr : plain(a[5]);
-    NONE_IF(!k || !v || (a[5] != Py_None && !off) || !cache_of(a[0], a[3], a[4], c, like));
+    NONE_IF(!k || !v || traced() || (a[5] != Py_None && !off) || !cache_of(a[0], a[3], a[4], c, like));
     const int64_t d = off ? 3 : 4;
     NONE_IF(k->dim() != d || !k->sizes().equals(v->sizes()) || !bf16_or_f16(*k) || v->scalar_type() != k->scalar_type() ||
             k->device() != like->device() || v->device() != like->device() || k->size(d - 2) != c.kv_heads ||
@@ -686,7 +689,7 @@ PyObject *kv_attend(PyObject *, PyObject *const *a, Py_ssize_t n) {
     NONE_IF(n != 8);
     lsmx_kv_cache c;
     const Tensor *like, *q = plain(a[0]), *w = a[7] == Py_None ? nullptr : plain(a[7]);
-    NONE_IF(!q || (a[7] != Py_None && !w) || !cache_of(a[1], a[2], a[3], c, like));
+    NONE_IF(!q || traced() || (a[7] != Py_None && !w) || !cache_of(a[1], a[2], a[3], c, like));
     NONE_IF(q->dim() != 4 || !bf16_or_f16(*q) || q->device() != like->device() || q->numel() == 0 || q->size(0) != c.batch ||
             q->size(3) != c.head_dim || q->size(2) % c.kv_heads || (w && !weights_ok(w, c, *like)) || q->stride(3) != 1 || !al(*q, 16));
     for (int i = 0; i < 3; ++i) NONE_IF(q->size(i) > 1 && q->stride(i) % 8);
@@ -721,7 +724,7 @@ PyObject *kv_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
     lsmx_kv_cache c;
     const Tensor *like, *w = plain(a[3]), *out = plain(a[5]);
     int64_t keep, sinks, recent;
-    NONE_IF(!w || !out || !cache_of(a[0], a[1], a[2], c, like) || !weights_ok(w, c, *like) || !int32_on(out, *like, 2) ||
+    NONE_IF(!w || !out || traced() || !cache_of(a[0], a[1], a[2], c, like) || !weights_ok(w, c, *like) || !int32_on(out, *like, 2) ||
             !int_arg(a[4], 1, false, keep) || !int_arg(a[6], 0, false, sinks) || !int_arg(a[7], 0, false, recent));
     const int64_t cap = c.max_pages * c.page, most = keep < cap ? keep : cap;
     NONE_IF(keep >= (1 << 30) || sinks > keep || recent > keep - sinks || out->size(0) != c.batch || out->size(1) * c.page < most);

@@ -86,6 +86,7 @@ def append(pages, k, v, table, lengths, *, offsets=None, values=False):
     With values=True returns (k, v) as now held: bf16, exact."""
     if (r := C.fast.kv_append(pages, k, v, table, lengths, offsets, values)) is not None:
         return r if values else None
+    C.not_traced("append")
     c = _cache(pages, table, lengths)
     if k.dtype not in (torch.bfloat16, torch.float16) or v.dtype != k.dtype:
         raise TypeError(f"k and v must share bfloat16 or float16, got {k.dtype}, {v.dtype}")
@@ -132,6 +133,7 @@ def attend(q, pages, table, lengths, *, window=None, sinks=0, scale=None, weight
     head, is added in place.  Deterministic.  The result has no gradient."""
     if (r := C.fast.kv_attend(q, pages, table, lengths, window, sinks, scale, weights)) is not None:
         return r
+    C.not_traced("attend")
     c = _cache(pages, table, lengths)
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"q must be bfloat16 or float16, got {q.dtype}")
@@ -181,6 +183,7 @@ def evict(pages, table, lengths, weights, keep, out_table, *, sinks=0, recent=0)
     [B]).  Afterwards positions, windows and sinks count the kept tokens."""
     if (r := C.fast.kv_evict(pages, table, lengths, weights, keep, out_table, sinks, recent)) is not None:
         return r
+    C.not_traced("evict")
     c = _cache(pages, table, lengths)
     C.require_device(weights, out_table)
     _check_weights(weights, c)

@@ -1,5 +1,5 @@
-"""The attention and cache calls under forward-mode derivatives: nothing
-is dropped without an error.  On the CPU with the kernels stubbed, which
+"""The attention and cache calls under forward-mode derivatives and torch.jit.trace:
+nothing is dropped without an error.  On the CPU with the kernels stubbed, which
 is the Python path; on the GPU the native one."""
 
 import pytest
@@ -7,6 +7,7 @@ import torch
 import torch.autograd.forward_ad as fw
 
 from lockstep_amd import _capi as C
+from lockstep_amd import kv_cache as kc
 from lockstep_amd.attention import sink_window_attention
 
 
@@ -46,10 +47,35 @@ def _forward_mode(dev):
                 assert sink_window_attention(*_inputs(dev)).shape == (1, 9, 4, 64)
 
 
+def _trace(dev):
+    q, k, v = _inputs(dev)
+    pages = kc.new_pages(4, 2, 64, 16, device=dev)
+    table = torch.zeros((1, 1), dtype=torch.int32, device=dev)
+    out = torch.ones((1, 1), dtype=torch.int32, device=dev)
+    lengths = torch.full((1,), 9, dtype=torch.int32, device=dev)
+    w = torch.zeros((1, 2, 16), device=dev)
+    calls = [(lambda a: sink_window_attention(a, k, v), q), (lambda a: kc.attend(a, pages, table, lengths), q),
+             (lambda a: kc.append(pages, a, v, table, lengths, values=True), k),
+             (lambda a: kc.evict(pages, table, lengths, a, 8, out), w)]
+    for f, x in calls:
+        with pytest.raises(RuntimeError, match="trac"):
+            torch.jit.trace(f, (x,), check_trace=False)
+        f(x)
+
+
 def test_forward_mode_python(stubs):
     _forward_mode(torch.device("cpu"))
+
+
+def test_trace_python(stubs):
+    _trace(torch.device("cpu"))
 
 
 @pytest.mark.gpu
 def test_forward_mode_native(dev):
     _forward_mode(dev)
+
+
+@pytest.mark.gpu
+def test_trace_native(dev):
+    _trace(dev)
