@@ -26,11 +26,14 @@ from .fp4_linear import MXFP4Linear
 from .mxfp4_gemm import mxfp4_linear_w
 
 
+_WEIGHT_ROWS = 16384  # rows of a pass over a prompt's weights (prefill)
+
+
 class LayerCache:
     """One layer's MXFP4 cache: `batch` sequences of up to `tokens` tokens.
 
-    track=True accumulates the tokens' softmax weights, and holds a second set
-    of pages for evict to move to.  lengths counts on the device; `used` is the
+    track=True accumulates the tokens' softmax weights, of prompts and of steps,
+    and holds a second set of pages for evict to move to.  lengths counts on the device; `used` is the
     host's bound on the longest of them, so that no call synchronizes."""
 
     def __init__(self, batch, tokens, kv_heads, head_dim, *, page_size=64, sinks=0, track=False, device="cuda"):
@@ -113,7 +116,8 @@ class MXFP4SelfAttention(nn.Module):
     def prefill(self, x, cache, offsets, longest=None):
         """Prompts packed as [N, dim] into an empty cache; attention is over
         their keys and values before quantization.  longest: the host's bound
-        on their lengths (default N)."""
+        on their lengths (default N).  A cache with track=True takes a second
+        pass, over the keys as it holds them, for the prompts' weights."""
         (w, s), (wo, so) = self._served()
         if cache.used:
             raise ValueError("prefill needs an empty cache; step continues one")
@@ -121,7 +125,18 @@ class MXFP4SelfAttention(nn.Module):
         cache.grow(x.shape[0] if longest is None else longest, offsets.diff())
         kv_cache.append(cache.pages, k, v, cache.table, cache.lengths, offsets=offsets)
         o = sink_window_attention(q, k, v, window=self.window, sinks=self.sinks, offsets=offsets)
+        if cache.weights is not None and x.shape[0]:
+            self._prompt_weights(q, cache, offsets, x.shape[0] if longest is None else longest)
         return mxfp4_linear_w(o.flatten(-2), wo, so)
+
+    def _prompt_weights(self, q, cache, offsets, longest):
+        """Adds the weights of packed prompts that fill the cache, the last T tokens
+        of every prompt at a time.  Rows before a prompt's first token see nothing."""
+        T = min(longest, max(64, _WEIGHT_ROWS // cache.lengths.numel()))
+        last = offsets[1:, None] - T + torch.arange(T, device=q.device)   # token of each row
+        for past in range(0, longest, T):
+            kv_cache.attend(q[(last - past).clamp(min=0)], cache.pages, cache.table, (cache.lengths - past).clamp(min=0),
+                            window=self.window, sinks=self.sinks, weights=cache.weights)
 
     @torch.no_grad()
     def step(self, x, cache):

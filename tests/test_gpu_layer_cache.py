@@ -1,0 +1,57 @@
+"""MXFP4SelfAttention's cache: the prompt's weights, evictions, captured steps."""
+
+import pytest
+import torch
+
+from .test_gpu_kv_cache import formula, held, reference_evict
+from .test_gpu_operators import layer_of
+
+pytestmark = pytest.mark.gpu
+
+
+def prompt_weights(layer, x, lens, cache, page, dev):
+    """In 64 bits: the weight of each held key over its prompt's queries, and the
+    bound on its error."""
+    from lockstep_amd import fp4
+    from lockstep_amd.mxfp4_gemm import mxfp4_linear_w
+    q = layer._split(mxfp4_linear_w(x, *layer.packed[0]))[0]
+    at = 0
+    for b, n in enumerate(lens):
+        if n:
+            kc, ks, _, _ = held(cache.pages, cache.table, b, n, page, dev)
+            k = fp4.dequantize_packed(kc.contiguous().flatten(0, 1), ks.contiguous().flatten(0, 1)).view(n, *kc.shape[1:2], -1)
+            _, _, w, err = formula(q[at:at + n], k, k, layer.window, layer.sinks, layer.head_dim ** -0.5)
+            yield b, n, w, err
+        at += n
+
+
+@pytest.mark.parametrize("rows", [16384, 128])     # in one pass, in several
+@pytest.mark.parametrize("window,sinks,lens", [(None, 2, [70, 0, 30, 200]), (40, 3, [300, 129]), (None, 0, [1])])
+def test_prefill_accumulates_the_prompts_weights(window, sinks, lens, rows, dev, monkeypatch):
+    from lockstep_amd import fp4_attention
+    monkeypatch.setattr(fp4_attention, "_WEIGHT_ROWS", rows, raising=False)
+    layer = layer_of(dev, window=window, sinks=sinks).pack()
+    for longest in (max(lens), None):
+        cache = layer.new_cache(len(lens), 512, page_size=16, track=True)
+        x = torch.randn((sum(lens), 512), generator=torch.Generator(device=dev).manual_seed(3), device=dev).bfloat16()
+        offsets = torch.tensor([sum(lens[:b]) for b in range(len(lens) + 1)], dtype=torch.int32, device=dev)
+        layer.prefill(x, cache, offsets, longest=longest)
+        for b, n, w, err in prompt_weights(layer, x, lens, cache, 16, dev):
+            bad = (cache.weights[b, :, :n].double() - w).abs() - err - 2.0 ** -20 * w
+            assert bad.max().item() <= 0, (b, bad.max().item())
+        for b, n in enumerate(lens):
+            assert (cache.weights[b, :, n:] == 0).all()
+
+
+def test_eviction_straight_after_a_prompt(dev):
+    """What stays is what the prompt attended to, not the first tokens, as with weights of 0."""
+    layer = layer_of(dev, sinks=1).pack()
+    cache = layer.new_cache(2, 256, page_size=16, track=True)
+    x = torch.randn((300, 512), generator=torch.Generator(device=dev).manual_seed(5), device=dev).bfloat16()
+    layer.prefill(x, cache, torch.tensor([0, 200, 300], dtype=torch.int32, device=dev), longest=200)
+    w = cache.weights.cpu()
+    index = cache.evict(64, recent=8)
+    for b, n in enumerate((200, 100)):
+        for h in range(2):
+            assert index[b, h].tolist() == reference_evict(w[b, h].tolist(), n, 64, 1, 8)
+            assert index[b, h].tolist() != reference_evict([0.0] * n, n, 64, 1, 8)
