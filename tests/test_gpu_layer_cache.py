@@ -44,7 +44,7 @@ def test_prefill_accumulates_the_prompts_weights(window, sinks, lens, rows, dev,
 
 
 def test_eviction_straight_after_a_prompt(dev):
-    """What stays is what the prompt attended to, not the first tokens, as with weights of 0."""
+    """What stays is what the prompt attended to: every token has a weight, its own at least."""
     layer = layer_of(dev, sinks=1).pack()
     cache = layer.new_cache(2, 256, page_size=16, track=True)
     x = torch.randn((300, 512), generator=torch.Generator(device=dev).manual_seed(5), device=dev).bfloat16()
@@ -54,4 +54,4 @@ def test_eviction_straight_after_a_prompt(dev):
     for b, n in enumerate((200, 100)):
         for h in range(2):
             assert index[b, h].tolist() == reference_evict(w[b, h].tolist(), n, 64, 1, 8)
-            assert index[b, h].tolist() != reference_evict([0.0] * n, n, 64, 1, 8)
+            assert (w[b, h, :n] > 0).all()
