@@ -33,8 +33,14 @@ class LayerCache:
     """One layer's MXFP4 cache: `batch` sequences of up to `tokens` tokens.
 
     track=True accumulates the tokens' softmax weights, of prompts and of steps,
-    and holds a second set of pages for evict to move to.  lengths counts on the device; `used` is the
-    host's bound on the longest of them, so that no call synchronizes."""
+    and holds a second set of pages for evict to move to.  lengths counts on the
+    device; `used` is the host's bound on the longest of them, so that no call
+    synchronizes.
+
+    All tensors stay where they are, so that a step captured in a graph goes on
+    after evictions.  Its replays count on the device alone: reserve() their tokens,
+    or those past the table are dropped.  (The capture runs nothing, but is
+    counted in `used`.)"""
 
     def __init__(self, batch, tokens, kv_heads, head_dim, *, page_size=64, sinks=0, track=False, device="cuda"):
         n = -(-tokens // page_size)
@@ -45,11 +51,15 @@ class LayerCache:
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.weights = torch.zeros((batch, kv_heads, n * page_size), device=device) if track else None
 
-    def grow(self, most, by):
-        """Counts new tokens: `by` for each sequence, at most `most`."""
+    def reserve(self, most):
+        """Counts at most `most` new tokens of a sequence on the host."""
         if self.used + most > self.tokens:
             raise ValueError(f"the cache holds {self.tokens} tokens, {self.used} + {most} asked for")
         self.used += most
+
+    def grow(self, most, by):
+        """Counts new tokens: `by` for each sequence, at most `most`."""
+        self.reserve(most)
         self.lengths += by
 
     def evict(self, keep, *, recent=0):
@@ -58,9 +68,12 @@ class LayerCache:
         (int32 [batch, kv_heads, keep], -1 past the last)."""
         if self.weights is None:
             raise ValueError("evict needs a cache made with track=True")
-        index, kept, self.lengths = kv_cache.evict(self.pages, self.table, self.lengths, self.weights, keep, self.other,
-                                                   sinks=self.sinks, recent=recent)
-        self.table, self.other = self.other, self.table
+        index, kept, lengths = kv_cache.evict(self.pages, self.table, self.lengths, self.weights, keep, self.other,
+                                              sinks=self.sinks, recent=recent)
+        self.lengths.copy_(lengths)
+        old = self.table.clone()
+        self.table.copy_(self.other)
+        self.other.copy_(old)
         n = min(keep, self.weights.shape[2])
         self.weights[:, :, :n] = kept[:, :, :n]
         self.weights[:, :, n:] = 0

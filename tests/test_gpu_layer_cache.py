@@ -55,3 +55,39 @@ def test_eviction_straight_after_a_prompt(dev):
         for h in range(2):
             assert index[b, h].tolist() == reference_evict(w[b, h].tolist(), n, 64, 1, 8)
             assert (w[b, h, :n] > 0).all()
+
+
+def test_captured_steps_go_on_after_an_eviction(dev):
+    """A captured step replays on what eager calls, evictions and other replays left."""
+    layer = layer_of(dev, window=50, sinks=2).pack()
+    g = torch.Generator(device=dev).manual_seed(9)
+    prompts = torch.randn((100, 512), generator=g, device=dev).bfloat16()
+    offsets = torch.tensor([0, 60, 100], dtype=torch.int32, device=dev)
+    caches = [layer.new_cache(2, 128, page_size=16, track=True) for _ in range(2)]
+    x = torch.randn((2, 1, 512), generator=g, device=dev).bfloat16()
+    for c in caches:
+        layer.prefill(prompts, c, offsets, longest=60)
+        layer.step(x, c)
+    eager, captured = caches
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer.step(x, eager)
+    torch.cuda.current_stream().wait_stream(side)
+    layer.step(x, captured)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer.step(x, captured)      # recorded, not run: its token is counted by the host alone
+    captured.used -= 1
+    for i in range(40):
+        x.copy_(torch.randn((2, 1, 512), generator=g, device=dev))
+        want = layer.step(x, eager)
+        captured.reserve(1)
+        graph.replay()
+        if i % 3 == 0:
+            torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+        assert torch.equal(captured.lengths, eager.lengths) and captured.used == eager.used
+        assert torch.equal(captured.weights, eager.weights)
+        if i % 13 == 12:
+            assert torch.equal(captured.evict(40, recent=6), eager.evict(40, recent=6))
