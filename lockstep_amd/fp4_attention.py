@@ -60,7 +60,21 @@ class LayerCache:
     def grow(self, most, by):
         """Counts new tokens: `by` for each sequence, at most `most`."""
         self.reserve(most)
-        self.lengths += by
+        try:
+            self.lengths += by
+        except RuntimeError:
+            self.used -= most
+            raise
+
+    def append(self, k, v, most, by, offsets=None):
+        """Writes new tokens and counts them; where the write is refused, nothing
+        is counted."""
+        self.grow(most, by)
+        try:
+            kv_cache.append(self.pages, k, v, self.table, self.lengths, offsets=offsets)
+        except Exception:
+            self.grow(-most, -by)
+            raise
 
     def evict(self, keep, *, recent=0):
         """Cuts every sequence to its `keep` most attended tokens: the sinks and
@@ -135,8 +149,7 @@ class MXFP4SelfAttention(nn.Module):
         if cache.used:
             raise ValueError("prefill needs an empty cache; step continues one")
         q, k, v = self._split(mxfp4_linear_w(x, w, s))
-        cache.grow(x.shape[0] if longest is None else longest, offsets.diff())
-        kv_cache.append(cache.pages, k, v, cache.table, cache.lengths, offsets=offsets)
+        cache.append(k, v, x.shape[0] if longest is None else longest, offsets.diff(), offsets)
         o = sink_window_attention(q, k, v, window=self.window, sinks=self.sinks, offsets=offsets)
         if cache.weights is not None and x.shape[0]:
             self._prompt_weights(q, cache, offsets, x.shape[0] if longest is None else longest)
@@ -156,8 +169,7 @@ class MXFP4SelfAttention(nn.Module):
         """The next T tokens of every sequence, x [B, T, dim], over the cache."""
         (w, s), (wo, so) = self._served()
         q, k, v = self._split(mxfp4_linear_w(x, w, s))
-        cache.grow(x.shape[1], x.shape[1])
-        kv_cache.append(cache.pages, k, v, cache.table, cache.lengths)
+        cache.append(k, v, x.shape[1], x.shape[1])
         o = kv_cache.attend(q, cache.pages, cache.table, cache.lengths, window=self.window, sinks=self.sinks,
                             weights=cache.weights)
         return mxfp4_linear_w(o.flatten(-2), wo, so)

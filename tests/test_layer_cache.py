@@ -37,3 +37,27 @@ def test_reserve_counts_what_a_replay_adds():
     with pytest.raises(ValueError, match="holds 40"):
         c.reserve(1)
     assert c.used == 40
+
+
+@pytest.fixture
+def layer(monkeypatch):
+    """A layer whose linears give zeros and whose attention is not reached."""
+    l = A.MXFP4SelfAttention(256, 4, 2).to(torch.bfloat16)
+    l.packed = ((384, None), (256, None))
+    monkeypatch.setattr(A, "mxfp4_linear_w", lambda x, n, s: x.new_zeros((*x.shape[:-1], n)))
+    return l
+
+
+def test_refused_calls_leave_the_cache_as_it_was(layer):
+    """Wrong batches, offsets and types are errors; no token of theirs is counted."""
+    c = layer.new_cache(3, 40, page_size=16, track=True)
+    x, off = torch.zeros((7, 256)).bfloat16(), torch.tensor([0, 3, 5, 7], dtype=torch.int32)
+    calls = [lambda: layer.prefill(x, c, off[:3]),            # two prompts for three sequences
+             lambda: layer.prefill(x, c, off.cpu()),          # CPU tensors
+             lambda: layer.step(torch.zeros((2, 1, 256)).bfloat16(), c),
+             lambda: layer.step(torch.zeros((3, 1, 256)), c),
+             lambda: c.grow(1, torch.zeros(2, dtype=torch.int32))]
+    for call in calls:
+        with pytest.raises((ValueError, AssertionError, TypeError, RuntimeError)):
+            call()
+        assert c.used == 0 and c.lengths.tolist() == [0, 0, 0]
