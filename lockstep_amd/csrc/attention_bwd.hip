@@ -75,15 +75,38 @@ LSMX_DEV typename Vec<T>::x8 columns(const T *t, int j0, int d, int g, int r) {
                                                           read_tr<T>(t + (j + 16) * DP + swz<NC>(j + 16, c) * 8 + e));
 }
 
+// acc and the sum of x, two elements at a time.
+LSMX_DEV float sum_of(bf16x8 x, float acc) {
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 one{(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) acc = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{x[i], x[i + 1]}, one, acc, false);
+    return acc;
+}
+
 // ------------------------------------------------------------------ dQ, delta
+// The dS of a row add up to 0, so that dQ_i = scale sum_j dS_ij (k_j - c_i) for any c_i.
+// They do so up to what the forward's rounded probabilities left in o, hence in
+// delta; with c_i near the keys' mean, this residue r_i = sum_j dS_ij, kept in fp32, does
+// not meet a common part of the keys: dQ_i = scale (sum_j dS_ij k_j - r_i c_i).  c_i is the
+// mean, by the row's probabilities, of the keys that it sees in the last tile of its
+// wave (a row that sees none of them keeps its residue).  Keys with a common part of twice
+// their spread: dQ's error was 2.0 to 2.2 times that of rounding it, of four times 3.4;
+// now 1.04.
+//
 // Each workgroup owns 64 RT rows, a wave 16 RT: q and dO in registers, the keys through
 // LDS as in the forward kernel.  delta comes first, from o and what o's rounding
 // left out.  Bound as attn_dkv_kernel is (before the second term vector unit 53%, matrix unit 35%; two
 // waves per SIMD): 2 x 4096 tokens, 32/8 heads of 128, window 1024: 330 us for
 // four products (dS in two terms) = 731 TFLOP/s of the visible pairs.
 template <typename T, int DP, int RT>
-__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs a) {
     constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, kBM = 64 * RT;
+    // bf16 at head 128: dS is summed as it enters the products, two elements an
+    // instruction, beside them (18 us where single additions before them took 25); fp16,
+    // and head 64, the other way round (8 x 2048 tokens of 16/4 heads of 64, causal: 14 us of 650,
+    // and 25)
+    constexpr bool kSumLate = DP == 128 && !Range<T>::on;
     typedef typename Vec<T>::x8 X8;
     typedef typename Vec<T>::x4 X4;
     __shared__ __attribute__((aligned(16))) T sk[2][kBN * DP], sv[2][kBN * DP];
@@ -105,6 +128,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     int t = t_sink > 0 ? 0 : t_lo, n = 0;
     const int wmin = div_by(min(wrow0, rows - 1), a.by_group) + s.shift;
     const int wmax = wrow0 < rows ? div_by(min(wrow0 + 16 * RT, rows) - 1, a.by_group) + s.shift : -1;
+    const int t_own = wmax >= 0 ? wmax / kBN : -1;  // the last tile that some row of the wave sees
 
     const T *kp = (const T *)a.k + s.b * a.k_b + s.k0 * a.k_t + hkv * a.k_h;
     const T *vp = (const T *)a.v + s.b * a.v_b + s.k0 * a.v_t + hkv * a.v_h;
@@ -121,7 +145,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
 
     int pos[RT], low[RT];
     int64_t q_at[RT];
-    float lse[RT], delta[RT], mul[RT] = {}, limit[RT] = {};
+    float lse[RT], delta[RT], mul[RT] = {}, limit[RT] = {}, rest[RT] = {};  // rest: sum of dS over the lane's keys
     X8 qf[RT][NS], of[RT][NS];
 #pragma unroll
     for (int y = 0; y < RT; ++y) {
@@ -202,6 +226,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
                             ds = sees(j, pos[y], low[y], a.sinks) ? ds : 0.f;
                         }
                         st[w][y][i] = ds;
+                        if constexpr (!kSumLate) rest[y] += ds;
                         if constexpr (Range<T>::on) top[y] = fmaxf(top[y], __builtin_fabsf(ds));
                     }
             if constexpr (Range<T>::on) {
@@ -244,6 +269,10 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
                     dq[d][y] = mfma(kf, dl[y], dq[d][y]);
                 }
             }
+            if constexpr (kSumLate) {
+#pragma unroll
+                for (int y = 0; y < RT; ++y) rest[y] = sum_of(df[y], sum_of(dl[y], rest[y]));
+            }
         };
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -254,6 +283,42 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
                 half(BoolC<true>{}, u);
             else
                 half(BoolC<false>{}, u);
+        }
+        if (t == t_own) {  // the rows' dS are complete: less r c (16 rows at a time: 32 do not fit)
+#pragma unroll
+            for (int y = 0; y < RT; ++y) {
+                X8 pf[2];
+                float mass = 0.f;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        int lr = r;
+                        asm volatile("" : "+v"(lr));  // as above
+                        const int j = u * 32 + w * 16 + lr;
+                        f32x4 st{0, 0, 0, 0};
+#pragma unroll
+                        for (int x = 0; x < NS; ++x)
+                            st = mfma(*(const X8 *)(ck + j * DP + swz<NC>(j, x * 4 + g) * 8), qf[y][x], st);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i], a.c, -lse[y]));
+                            const float p = sees(j0 + u * 32 + w * 16 + g * 4 + i, pos[y], low[y], a.sinks) ? e : 0.f;
+                            mass += p;
+                            pf[u][w * 4 + i] = (T)p;
+                        }
+                    }
+                mass = sum_rows(mass);
+                const float sum = sum_rows(rest[y]) * (Range<T>::on ? mul[y] : 1.f), f = mass > 0.f ? -sum / mass : 0.f;
+                int lr = r;
+                asm volatile("" : "+v"(lr));
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const f32x4 c = mfma(columns<T, DP>(ck, 32, d, g, lr), pf[1], mfma(columns<T, DP>(ck, 0, d, g, lr), pf[0], f32x4{0, 0, 0, 0}));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) dq[d][y][i] = __builtin_fmaf(f, c[i], dq[d][y][i]);
+                }
+            }
         }
         n ^= 1, t = tn;
         wait_dma();
