@@ -4,8 +4,8 @@ What stands between the linears of a block is the reference's
 train.py:46-52 with its linears replaced (fp4_linear.py:48-58); here the whole
 layer runs on this package's kernels:
 
-    layer = MXFP4SelfAttention(1024, heads=16, kv_heads=4, window=1024, sinks=4).cuda()
-    layer(x).sum().backward()                      # MXFP4 linears, sink_window_attention
+    layer = MXFP4SelfAttention(1024, heads=16, kv_heads=4, window=1024, sinks=4).cuda().bfloat16()
+    layer(x).sum().backward()                      # x bf16; MXFP4 linears, sink_window_attention
 
     layer.pack()                                   # weights to MXFP4, once
     cache = layer.new_cache(batch=8, tokens=4096, track=True)
@@ -100,7 +100,8 @@ class MXFP4SelfAttention(nn.Module):
     optional window and sinks, key heads shared by groups of query heads.
 
     Both linears are MXFP4Linear (quantized_backward as there).  head_dim =
-    dim // heads; 64 or 128 to serve.  Positions are the caller's business."""
+    dim // heads; 64 or 128 to serve.  Inputs are bf16 or fp16.  q and k
+    are taken as they are projected: positions enter with x, or not at all."""
 
     def __init__(self, dim, heads, kv_heads=None, *, window=None, sinks=0, quantized_backward=False):
         super().__init__()
