@@ -22,15 +22,6 @@ namespace {
 
 constexpr int kBN = 64;  // keys of a tile
 
-// Waits for a wave's own direct-to-LDS loads, which are issued in inline
-// assembly and not counted by the compiler.  It sees this wait, so that it
-// puts no wait for the rows' loads into the loop, where that would be one for
-// the tile in flight.
-LSMX_DEV void wait_dma() {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-    asm volatile("" ::: "memory");
-}
-
 // Keys and values as they lie in memory, loaded straight into LDS: lane l of
 // a load fills 16-byte position l, so the swizzle is in the addresses.  The
 // descriptor starts at the tile's first key; keys past the sequence and

@@ -60,11 +60,6 @@ LSMX_DEV void fetch_rows(v4i_rsrc rs, T *to, int rows, F offset) {
 }
 constexpr uint32_t kZeros = 0x80000000u;
 
-LSMX_DEV void wait_dma() {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0), seen by the compiler
-    asm volatile("" ::: "memory");
-}
-
 // Operand of 8 contraction rows 4g.., 16 + 4g.. of a tile from row j0 on, at
 // columns 16 d + r.
 template <typename T, int DP>

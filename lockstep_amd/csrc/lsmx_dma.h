@@ -45,4 +45,13 @@ LSMX_DEV void dma_x1(uint32_t off, v4i_rsrc r, uint32_t m0) {
                  "s"(__builtin_amdgcn_readfirstlane(m0)) : "memory");
 }
 
+// Waits for a wave's own direct-to-LDS loads, which are issued in inline
+// assembly and not counted by the compiler.  It sees this wait, so that it
+// puts no wait for the rows' loads into the loop, where that would be one for
+// the tile in flight.
+LSMX_DEV void wait_dma() {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    asm volatile("" ::: "memory");
+}
+
 }  // namespace lsmx
