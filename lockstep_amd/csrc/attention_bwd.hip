@@ -85,9 +85,10 @@ LSMX_DEV float sum_of(bf16x8 x, float acc) {
 // delta; with c_i near the keys' mean, this residue r_i = sum_j dS_ij, kept in fp32, does
 // not meet a common part of the keys: dQ_i = scale (sum_j dS_ij k_j - r_i c_i).  c_i is the
 // mean, by the row's probabilities, of the keys that it sees in the last tile of its
-// wave (a row that sees none of them keeps its residue).  Keys with a common part of twice
+// wave, less where these have less than their share of its probability (they may then be
+// nothing like its other keys, and a row that sees none of them keeps its residue).  Keys with a common part of twice
 // their spread: dQ's error was 2.0 to 2.2 times that of rounding it, of four times 3.4;
-// now 1.04.
+// now 1.07 and 1.1 to 1.2, and 1.03 without a common part.
 //
 // Each workgroup owns 64 RT rows, a wave 16 RT: q and dO in registers, the keys through
 // LDS as in the forward kernel.  delta comes first, from o and what o's rounding
@@ -139,7 +140,6 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs
     if (t < t_hi) fetch(t * kBN, 0);
 
     int pos[RT], low[RT];
-    int64_t q_at[RT];
     float lse[RT], delta[RT], mul[RT] = {}, limit[RT] = {}, rest[RT] = {};  // rest: sum of dS over the lane's keys
     X8 qf[RT][NS], of[RT][NS];
 #pragma unroll
@@ -150,8 +150,6 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs
         pos[y] = in ? tok + s.shift : -1;
         low[y] = window_low(pos[y], a.window);
         const int64_t l_at = s.b * a.lse_b + h * a.lse_h + s.q0 + tok;
-        const int64_t token = (a.offsets ? s.q0 : (int64_t)s.b * a.q_len) + tok;
-        q_at[y] = in ? (token * a.heads + h) * a.dim : -1;
         const T *qp = (const T *)a.q + s.b * a.q_b + (s.q0 + tok) * a.q_t + h * a.q_h;
         const T *dp = (const T *)a.d_o + s.b * a.do_b + (s.q0 + tok) * a.do_t + h * a.do_h;
         const int64_t o_at = s.b * a.o_b + (s.q0 + tok) * a.o_t + h * a.o_h;
@@ -283,7 +281,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs
 #pragma unroll
             for (int y = 0; y < RT; ++y) {
                 X8 pf[2];
-                float mass = 0.f;
+                float mass = 0.f, seen = 0.f;
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -298,13 +296,17 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i], a.c, -lse[y]));
-                            const float p = sees(j0 + u * 32 + w * 16 + g * 4 + i, pos[y], low[y], a.sinks) ? e : 0.f;
+                            const bool in = sees(j0 + u * 32 + w * 16 + g * 4 + i, pos[y], low[y], a.sinks);
+                            const float p = in ? e : 0.f;
                             mass += p;
+                            seen += in ? 1.f : 0.f;
                             pf[u][w * 4 + i] = (T)p;
                         }
                     }
-                mass = sum_rows(mass);
-                const float sum = sum_rows(rest[y]) * (Range<T>::on ? mul[y] : 1.f), f = mass > 0.f ? -sum / mass : 0.f;
+                const int near = a.window ? min(pos[y] + 1, a.window) : pos[y] + 1;
+                const float keys = (float)(near + min(a.sinks, pos[y] + 1 - near));  // that the row sees
+                const float share = fmaxf(sum_rows(mass), sum_rows(seen) / keys);
+                const float sum = sum_rows(rest[y]) * (Range<T>::on ? mul[y] : 1.f), f = share > 0.f ? -sum / share : 0.f;
                 int lr = r;
                 asm volatile("" : "+v"(lr));
 #pragma unroll
@@ -321,8 +323,10 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs
     }
 #pragma unroll
     for (int y = 0; y < RT; ++y) {
-        if (q_at[y] < 0) continue;
-        T *p = (T *)a.dq + q_at[y];
+        const int row = wrow0 + r + 16 * y;
+        if (row >= rows) continue;
+        const int tok = div_by(row, a.by_group), h = hkv * a.group + row - tok * a.group;
+        T *p = (T *)a.dq + (((a.offsets ? s.q0 : (int64_t)s.b * a.q_len) + tok) * a.heads + h) * a.dim;
         const float f = !Range<T>::on ? a.scale : mul[y] == 0.f ? 0.f : a.scale / mul[y];
 #pragma unroll
         for (int d = 0; d < ND; ++d) {

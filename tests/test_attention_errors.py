@@ -76,3 +76,20 @@ def test_errors_of_the_kernels(case, dt, dev):
     print({n: round(m, 3) for n, m in got.items()}, flush=True)
     assert got["dq"] < LIMIT, got
     assert all(got[n] < 1.6 for n in ("o", "dk", "dv")), got
+
+
+@pytest.mark.gpu
+def test_rows_whose_weight_is_on_the_sinks(dev):
+    """A window of one key and four sinks: rows that look at a sink alone take nothing
+    from their own key, element by element."""
+    from lockstep_amd.attention import sink_window_attention
+
+    from .test_gpu_attention import U, close
+    from .test_gpu_attention import formula as bounds
+    g = torch.Generator(device=dev).manual_seed(814236)
+    x = [torch.randn((2, 560, h, 64), generator=g, device=dev).bfloat16().requires_grad_(True) for h in (9, 3, 3)]
+    do = torch.randn((2, 560, 9, 64), generator=g, device=dev).bfloat16()
+    dq, = torch.autograd.grad(sink_window_attention(*x, window=1, sinks=4), x[:1], do)
+    for b in range(2):
+        ref = bounds(*(t[b].detach() for t in x), 1, 4, 0.125, do[b])
+        close("dq", dq[b], ref["dq"], ref["dq_mag"], U[torch.bfloat16], 1)
