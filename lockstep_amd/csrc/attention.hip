@@ -153,13 +153,15 @@ struct PagedKV {
 // of this one, which are as much work for the vector unit as both products
 // are for the matrix unit.
 //
-// Bound by the vector unit (exponentials, sums and conversions: 52% of its
-// cycles at head 128, 66% at 64, with the matrix unit at 34% and 32%), so that
-// waves per SIMD count: 2 at head 128, 3 at 64 (registers allow it only while
-// a step is 32 keys).  2 x 4096 tokens, 32/8 heads of 128, window 1024: 184 us
-// = 656 TFLOP/s of the visible pairs (205 with the remainders of o stored for
-// the backward); 16384 tokens of 8/1 heads of 64 through a window of 4096:
-// 214 us = 562 TFLOP/s.
+// Bound by what a wave waits for and the few others cannot fill: the vector unit
+// (exponentials, sums and conversions) is busy 58% of the cycles at head 128, the
+// matrix unit 30%, neither ever full.  Waves per SIMD count: 2 at head 128, 3 at 64
+// (registers allow it only while a step is 32 keys).  2 x 4096 tokens, 32/8 heads of
+// 128, window 1024: 174 us a call = 694 TFLOP/s of the visible pairs (with the
+// remainders of o stored for the backward 216 to 228); 16384 tokens of 8/1 heads
+// of 64 through a window of 4096: 191 us = 631 TFLOP/s (1024 almost equal workgroups, of
+// which 768 run at a time).  Heads of 72 to 120 take all products of 128, their
+// chunks past the head are zeros: 4096 causal tokens of 32/8 heads of 80 171 us, 128 176.
 template <typename T, int DP, int RT, int NW, int KS, typename KV>
 __global__ __launch_bounds__(NW * KS * 64, DP == 128 ? 2 : KV::kHoles ? 4 : 3) void attn_fwd_kernel(typename KV::Args args) {
     constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, BM = NW * RT * 16;

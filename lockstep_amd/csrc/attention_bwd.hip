@@ -7,7 +7,8 @@
 // Two kernels, so that every sum has one order (no atomics): one owns rows and
 // runs over their keys (dQ), the other owns keys and runs over the rows of all
 // heads that share them (dK, dV).  Both recompute S and dP:
-// seven products where one kernel with shared accumulators would take five.
+// eight products (dQ has dS in two terms) where one kernel with shared accumulators would
+// take five, or six.
 //
 // The sinks are seen by every row: their keys would keep one workgroup busy
 // with the whole sequence while the others have a window of it.  So the rows
@@ -95,9 +96,9 @@ LSMX_DEV float sum_of(bf16x8 x, float acc) {
 //
 // Each workgroup owns 64 RT rows, a wave 16 RT: q and dO in registers, the keys through
 // LDS as in the forward kernel.  delta comes first, from o and what o's rounding
-// left out.  Bound as attn_dkv_kernel is (before the second term vector unit 53%, matrix unit 35%; two
-// waves per SIMD): 2 x 4096 tokens, 32/8 heads of 128, window 1024: 330 us for
-// four products (dS in two terms) = 731 TFLOP/s of the visible pairs.
+// left out.  Bound as attn_dkv_kernel is (vector unit 63%, matrix unit 37%; two
+// waves per SIMD): 2 x 4096 tokens, 32/8 heads of 128, window 1024: 354 us for
+// four products (dS in two terms) = 682 TFLOP/s of the visible pairs.
 template <typename T, int DP, int RT>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs a) {
     constexpr int NC = DP / 8, NS = DP / 32, ND = DP / 16, kBM = 64 * RT;
@@ -241,10 +242,9 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs
                     }
                 }
             }
-            // two terms: the dS of a row cancel, so that one rounding of each is as
-            // much as 1.15 times that of dQ itself where the keys have a common part
-            // (both together 1.52 times the latter; with two terms 1.04).  330 us for
-            // 270.
+            // two terms: the dS of a row cancel, so that with one rounding of each the
+            // error of dQ is 1.4 times that of rounding it, and 2.5 times with keys that have a
+            // common part of twice their spread; with two 1.01 and 1.05.  (60 us of 330.)
             X8 df[RT], dl[RT];
 #pragma unroll
             for (int y = 0; y < RT; ++y)
