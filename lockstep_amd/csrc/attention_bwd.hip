@@ -73,7 +73,6 @@ LSMX_DEV typename Vec<T>::x8 columns(const T *t, int j0, int d, int g, int r) {
 
 // acc and the sum of x, two elements at a time.
 LSMX_DEV float sum_of(bf16x8 x, float acc) {
-    typedef short s16x2 __attribute__((ext_vector_type(2)));
     const bf16x2 one{(__bf16)1.f, (__bf16)1.f};
 #pragma unroll
     for (int i = 0; i < 8; i += 2) acc = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{x[i], x[i + 1]}, one, acc, false);
@@ -85,8 +84,9 @@ LSMX_DEV float sum_of(bf16x8 x, float acc) {
 // They do so up to what the forward's rounded probabilities left in o, hence in
 // delta; with c_i near sum_j P_ij k_j, this residue r_i = sum_j dS_ij, kept in fp32, does
 // not meet a common part of the keys: dQ_i = scale (sum_j dS_ij k_j - r_i c_i).  c_i takes
-// the keys of the wave's last tile as they are, with their P, and for the row's others the
-// tile's mean, as far as the row looks at keys in general: by its weight on the tile's
+// the keys of the wave's last tile as they are (of its halves that some row sees: what is
+// hidden from all may hold anything), with their P, and for the row's others their
+// mean, as far as the row looks at keys in general: by its weight on the tile's
 // keys, none counted above four times its share, against their share.  (A row that
 // looks at one key takes nothing from others; one of few keys has most in the tile.)
 // Keys with a common part of twice their spread: the error of dQ was 2.0 to 2.2 times
@@ -186,6 +186,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs
         const int j0 = t * kBN, tn = next(t);
         if (tn < t_hi) fetch(tn * kBN, n ^ 1);
         const T *ck = sk[n], *cv = sv[n];
+        // hidden from every row of the wave
+        auto unseen = [&](int ju) { return ju > wmax || (a.window && ju + 31 <= wmin - a.window && ju >= a.sinks); };
         auto half = [&](auto all, int u) {
             const int ju = j0 + u * 32;
             // places in LDS made anew each time: held, they would not fit
@@ -273,8 +275,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int ju = j0 + u * 32;
-            // hidden from every row, or seen by each
-            if (ju > wmax || (a.window && ju + 31 <= wmin - a.window && ju >= a.sinks)) continue;
+            if (unseen(ju)) continue;
             if (ju + 31 <= wmin && (!a.window || ju > wmax - a.window || ju + 31 < a.sinks))
                 half(BoolC<true>{}, u);
             else
@@ -286,9 +287,13 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs
                 const int near = a.window ? min(pos[y] + 1, a.window) : pos[y] + 1;
                 const float keys = (float)(near + min(a.sinks, pos[y] + 1 - near));  // that the row sees
                 X8 pf[2];
-                float mass = 0.f, even = 0.f, seen = 0.f;
+                float mass = 0.f, even = 0.f, seen = 0.f, held = 0.f;
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < 2; ++u) {
+                    pf[u] = X8{};
+                    const int ju = j0 + u * 32;
+                    if (unseen(ju)) continue;
+                    held += (float)min(32, s.k_len - ju);
 #pragma unroll
                     for (int w = 0; w < 2; ++w) {
                         int lr = r;
@@ -301,7 +306,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i], a.c, -lse[y]));
-                            const bool in = sees(j0 + u * 32 + w * 16 + g * 4 + i, pos[y], low[y], a.sinks);
+                            const bool in = sees(ju + w * 16 + g * 4 + i, pos[y], low[y], a.sinks);
                             const float p = in ? e : 0.f;
                             mass += p;
                             even += fminf(p * keys, 4.f);
@@ -309,20 +314,23 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void attn_dq_kernel(AttnArgs
                             pf[u][w * 4 + i] = (T)p;
                         }
                     }
+                }
                 const float sum = sum_rows(rest[y]) * (Range<T>::on ? mul[y] : 1.f);
                 const float other = fmaxf(1.f - sum_rows(mass), 0.f) * fminf(1.f, 2.f * sum_rows(even) / (sum_rows(seen) + 8.f));
-                const float each = keys >= 32.f ? other / (float)min(kBN, s.k_len - j0) : 0.f;
+                const float each = keys >= 32.f ? other / held : 0.f;
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < 2; ++u) {
+                    if (unseen(j0 + u * 32)) continue;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) pf[u][i] = (T)((float)pf[u][i] + each);
-                int lr = r;
-                asm volatile("" : "+v"(lr));
+                    int lr = r;
+                    asm volatile("" : "+v"(lr));
 #pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    const f32x4 c = mfma(columns<T, DP>(ck, 32, d, g, lr), pf[1], mfma(columns<T, DP>(ck, 0, d, g, lr), pf[0], f32x4{0, 0, 0, 0}));
+                    for (int d = 0; d < ND; ++d) {
+                        const f32x4 c = mfma(columns<T, DP>(ck, u * 32, d, g, lr), pf[u], f32x4{0, 0, 0, 0});
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) dq[d][y][i] = __builtin_fmaf(-sum, c[i], dq[d][y][i]);
+                        for (int i = 0; i < 4; ++i) dq[d][y][i] = __builtin_fmaf(-sum, c[i], dq[d][y][i]);
+                    }
                 }
             }
         }

@@ -93,3 +93,20 @@ def test_rows_whose_weight_is_on_the_sinks(dev):
     for b in range(2):
         ref = bounds(*(t[b].detach() for t in x), 1, 4, 0.125, do[b])
         close("dq", dq[b], ref["dq"], ref["dq_mag"], U[torch.bfloat16], 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,heads", [(64, 1), (64, 48), (200, 2)])
+def test_a_nan_key_ahead_does_not_reach_the_rows_behind(T, heads, dev):
+    """Key 40 is NaN: the first 32 rows have the dQ that they have without it."""
+    from lockstep_amd.attention import sink_window_attention
+    for D in (64, 128):
+        g = torch.Generator(device=dev).manual_seed(T)
+        q, k, v, do = (torch.randn((8, T, heads, D), generator=g, device=dev).bfloat16() for _ in range(4))
+        bad = k.clone()
+        bad[:, 40] = math.nan
+        got = []
+        for keys in (k, bad):
+            x = [t.clone().requires_grad_(True) for t in (q, keys, v)]
+            got.append(torch.autograd.grad(sink_window_attention(*x), x[:1], do)[0])
+        assert torch.equal(got[0][:, :32], got[1][:, :32]) and torch.isnan(got[1][:, 40:]).all()
