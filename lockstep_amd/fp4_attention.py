@@ -159,8 +159,9 @@ class MXFP4SelfAttention(nn.Module):
     def _prompt_weights(self, q, cache, offsets, longest):
         """Adds the weights of packed prompts that fill the cache, the last T tokens
         of every prompt at a time.  Rows before a prompt's first token see nothing."""
-        T = min(longest, max(64, _WEIGHT_ROWS // cache.lengths.numel()))
-        last = offsets[1:, None] - T + torch.arange(T, device=q.device)   # token of each row
+        T = max(min(longest, max(64, _WEIGHT_ROWS // cache.lengths.numel())), 1)
+        ends = offsets[1:, None].clamp(0, q.shape[0])
+        last = ends - T + torch.arange(T, device=q.device)   # token of each row
         for past in range(0, longest, T):
             kv_cache.attend(q[(last - past).clamp(min=0)], cache.pages, cache.table, (cache.lengths - past).clamp(min=0),
                             window=self.window, sinks=self.sinks, weights=cache.weights)

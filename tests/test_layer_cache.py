@@ -61,3 +61,16 @@ def test_refused_calls_leave_the_cache_as_it_was(layer):
         with pytest.raises((ValueError, AssertionError, TypeError, RuntimeError)):
             call()
         assert c.used == 0 and c.lengths.tolist() == [0, 0, 0]
+
+
+def test_prompt_weights_stay_within_the_rows(layer, monkeypatch):
+    """Offsets past the rows, or before them, are cut to them, as the kernels cut them."""
+    seen = []
+
+    def attend(q, pages, table, lengths, **kw):
+        seen.append(q.shape)
+    monkeypatch.setattr(A.kv_cache, "attend", attend)
+    c = _cache()
+    for off, longest in (([0, 3, 5, 900], 7), ([0, 3, 2 ** 31 - 1, 7], 40), ([-5, -3, 5, 7], 7), ([0, 3, 5, 7], 0)):
+        layer._prompt_weights(torch.zeros((7, 4, 64)), c, torch.tensor(off, dtype=torch.int32), longest)
+    assert seen == [(3, 7, 4, 64), (3, 40, 4, 64), (3, 7, 4, 64)]
