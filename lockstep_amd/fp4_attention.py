@@ -46,7 +46,7 @@ class LayerCache:
         n = -(-tokens // page_size)
         self.tokens, self.sinks, self.used = tokens, sinks, 0
         self.pages = kv_cache.new_pages((1 + track) * batch * n, kv_heads, head_dim, page_size, device)
-        ids = torch.arange((1 + track) * batch * n, dtype=torch.int32, device=device).view(-1, batch, n)
+        ids = torch.arange((1 + track) * batch * n, dtype=torch.int32, device=device).view(1 + track, batch, n)
         self.table, self.other = ids[0], ids[-1]
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.weights = torch.zeros((batch, kv_heads, n * page_size), device=device) if track else None
@@ -159,7 +159,7 @@ class MXFP4SelfAttention(nn.Module):
     def _prompt_weights(self, q, cache, offsets, longest):
         """Adds the weights of packed prompts that fill the cache, the last T tokens
         of every prompt at a time.  Rows before a prompt's first token see nothing."""
-        T = max(min(longest, max(64, _WEIGHT_ROWS // cache.lengths.numel())), 1)
+        T = max(min(longest, max(64, _WEIGHT_ROWS // max(cache.lengths.numel(), 1))), 1)
         ends = offsets[1:, None].clamp(0, q.shape[0])
         last = ends - T + torch.arange(T, device=q.device)   # token of each row
         for past in range(0, longest, T):

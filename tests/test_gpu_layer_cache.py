@@ -91,3 +91,11 @@ def test_captured_steps_go_on_after_an_eviction(dev):
         assert torch.equal(captured.weights, eager.weights)
         if i % 13 == 12:
             assert torch.equal(captured.evict(40, recent=6), eager.evict(40, recent=6))
+
+
+def test_a_prompt_of_no_sequence(dev):
+    layer = layer_of(dev).pack()
+    x = torch.randn((7, 512), generator=torch.Generator(device=dev).manual_seed(2), device=dev).bfloat16()
+    cache = layer.new_cache(0, 40, page_size=16, track=True)
+    assert (layer.prefill(x, cache, torch.zeros(1, dtype=torch.int32, device=dev)) == 0).all()
+    assert cache.weights.shape == (0, 2, 48)

@@ -43,7 +43,7 @@ def test_reserve_counts_what_a_replay_adds():
 def layer(monkeypatch):
     """A layer whose linears give zeros and whose attention is not reached."""
     l = A.MXFP4SelfAttention(256, 4, 2).to(torch.bfloat16)
-    l.packed = ((384, None), (256, None))
+    l.packed = ((512, None), (256, None))
     monkeypatch.setattr(A, "mxfp4_linear_w", lambda x, n, s: x.new_zeros((*x.shape[:-1], n)))
     return l
 
@@ -74,3 +74,10 @@ def test_prompt_weights_stay_within_the_rows(layer, monkeypatch):
     for off, longest in (([0, 3, 5, 900], 7), ([0, 3, 2 ** 31 - 1, 7], 40), ([-5, -3, 5, 7], 7), ([0, 3, 5, 7], 0)):
         layer._prompt_weights(torch.zeros((7, 4, 64)), c, torch.tensor(off, dtype=torch.int32), longest)
     assert seen == [(3, 7, 4, 64), (3, 40, 4, 64), (3, 7, 4, 64)]
+
+
+@pytest.mark.parametrize("batch,tokens", [(0, 40), (2, 0)])
+def test_an_empty_cache(batch, tokens):
+    for track in (True, False):
+        c = A.LayerCache(batch, tokens, 2, 64, page_size=16, track=track, device="cpu")
+        assert c.table.shape == c.other.shape == (batch, -(-tokens // 16)) and c.lengths.shape == (batch,)
