@@ -538,6 +538,98 @@ int lsmx_kv_evict(const lsmx_kv_cache *c, const float *weights, int64_t w_len, i
                   int64_t recent, const int32_t *out_table, int64_t out_max_pages, int32_t *index,
                   float *new_weights, int32_t *new_lengths, void *stream);
 
+/* ------------------------------------------------------------------- norm
+ * Root-mean-square norm with the residual's addition (an extension: the
+ * reference's model has no norm before its linears).  LSMX_F32 | BF16 | F16:
+ *
+ *   h = round(x + r)  (r NULL: h = x and is not written)
+ *   y = h (mean(h^2) + eps)^-1/2 w
+ *
+ * x [rows, ldx], r [rows, ldr]; h and y [rows, dim]; w [dim] of x's type or
+ * LSMX_F32.  codes, scale (both or neither): y before rounding as MXFP8, E4M3
+ * bytes [rows, dim] and E8M0 [rows, dim / 32]: the scale of 32 elements is the
+ * least power of two (from 2^-127) that keeps them within 448, 1 for zeros,
+ * NaN (255) for a block with an infinity or a NaN.  They need dim % 32 == 0,
+ * 16-byte aligned operands and rows, and codes 8-byte aligned. */
+int lsmx_rms_norm(const void *x, int64_t ldx, const void *r, int64_t ldr, int dtype, const void *w, int w_dtype,
+                  int64_t rows, int64_t dim, float eps, void *h, void *y, uint8_t *codes, uint8_t *scale, void *stream);
+
+/* Gradients from h (x itself without a residual), dy and dh (NULL: none), rows
+ * of ldh, lddy, lddh elements: dx [rows, dim] (the residual's too) and dw [dim]
+ * of w's type (NULL: not wanted).  ws: lsmx_rms_norm_bwd_workspace bytes,
+ * 16-byte aligned, no initial contents. */
+int64_t lsmx_rms_norm_bwd_workspace(int64_t rows, int64_t dim, int dtype);
+int lsmx_rms_norm_bwd(const void *h, int64_t ldh, const void *dy, int64_t lddy, const void *dh, int64_t lddh, int dtype,
+                      const void *w, int w_dtype, int64_t rows, int64_t dim, float eps, void *dx, void *dw, void *ws,
+                      int64_t ws_bytes, void *stream);
+
+/* ------------------------------------------------------------------ router
+ * Each row's choice of k of `experts` experts (an extension):
+ *
+ *   s = softmax(logits) or, sigmoid != 0, 1 / (1 + exp(-logits));  c = s + bias
+ *   of `groups` equal runs of experts those with the largest sums of their two
+ *   largest c stay, top_groups of them;  ids: the k largest c of what stays, in
+ *   that order, ties (of groups too) to the lowest index, a NaN first
+ *   weights = scale s / (renorm ? sum of the k : 1), 0 where the k sum to 0
+ *
+ * c is compared in 64 bits.  logits [rows, ld], LSMX_F32 | BF16 | F16; bias fp32
+ * [experts] or NULL; mask [rows] bytes or NULL: a row with 0 gets ids -1 and
+ * weights 0.  A row of nothing but -inf scores 0 under softmax.  experts <=
+ * 1024, groups <= 64, k <= 64. */
+typedef struct {
+    const void *logits;
+    int dtype;
+    int64_t rows, ld, experts, k;
+    int sigmoid;
+    int64_t groups, top_groups;
+    int renorm;
+    float scale;
+    const float *bias;
+    const uint8_t *mask;
+    float *weights;    /* [rows, k] */
+    int32_t *ids;      /* [rows, k] */
+} lsmx_route;
+int lsmx_route_fwd(const lsmx_route *a, void *stream);
+
+/* dlogits [rows, experts] of the logits' type from dweights [rows, k] and the
+ * forward call's ids; the choice itself has no gradient, nor has bias. */
+int lsmx_route_bwd(const lsmx_route *a, const float *dweights, void *dlogits, void *stream);
+
+/* The pairs p = token * k + slot sorted by ids[p], stable: order [pairs], and
+ * offsets [experts + 1], expert e's being order[offsets[e]] .. order[offsets[e + 1] - 1].
+ * Pairs whose id is no expert come behind.  pairs <= 2^21, experts <= 1024.
+ * ws: lsmx_dispatch_workspace bytes, 4-byte aligned, no initial contents. */
+int64_t lsmx_dispatch_workspace(int64_t pairs, int64_t experts);
+int lsmx_dispatch(const int32_t *ids, int64_t pairs, int64_t experts, int32_t *order, int32_t *offsets, void *ws,
+                  int64_t ws_bytes, void *stream);
+
+/* -------------------------------------------------------- experts' products
+ * Rows in MXFP8 times the MXFP4 weights of the expert of each pair (an
+ * extension of the weight-only products, mxfp4_gemm.py's weights many times
+ * over).  ids [tokens, k], order and offsets as lsmx_dispatch makes them.
+ * x [.., K] E4M3 bytes, x_scale [.., K / 32] E8M0; w [experts, N, K / 2] packed
+ * MXFP4, w_scale [experts, N, K / 32] E8M0; all dense, x and w 16-byte aligned.
+ * K % 128 == 0, an expert's weights below 2^31 bytes. */
+typedef struct {
+    const uint8_t *x, *x_scale, *w, *w_scale;
+    const int32_t *ids, *order, *offsets;
+    int64_t tokens, k, experts, N, K;
+} lsmx_experts;
+
+/* x [tokens, K]; N = 2 F, rows 0 .. F-1 of an expert the gate's, F .. 2F-1
+ * up's, F % 32 == 0.  h [tokens, k, F] E4M3 and h_scale [tokens, k, F / 32]:
+ * silu(x Wg^T) * (x Wu^T) in MXFP8, as lsmx_rms_norm makes it; pairs of no
+ * expert get zeros of scale 1. */
+int lsmx_expert_gated(const lsmx_experts *a, uint8_t *h, uint8_t *h_scale, void *stream);
+
+/* x [tokens, k, K]; y [tokens, N] = sum over a token's slots of weights
+ * [tokens, k] times x W^T of the slot's expert, in LSMX_F32 | BF16 | F16; slots
+ * of no expert add nothing.  ws: lsmx_expert_combine_workspace bytes, 16-byte
+ * aligned, no initial contents. */
+int64_t lsmx_expert_combine_workspace(const lsmx_experts *a);
+int lsmx_expert_combine(const lsmx_experts *a, const float *weights, void *y, int y_dtype, void *ws, int64_t ws_bytes,
+                        void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -75,10 +75,22 @@ SIGNATURES = {
     "lsmx_kv_attend_workspace": [_vp, _i64, _i64, _i64, _i64, _int],
     "lsmx_kv_attend": [_vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, ctypes.c_float, _vp, _vp, _i64, _vp, _i64, _vp],
     "lsmx_kv_evict": [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp],
+    "lsmx_rms_norm": [_vp, _i64, _vp, _i64, _int, _vp, _int, _i64, _i64, ctypes.c_float, _vp, _vp, _vp, _vp, _vp],
+    "lsmx_rms_norm_bwd_workspace": [_i64, _i64, _int],
+    "lsmx_rms_norm_bwd": [_vp, _i64, _vp, _i64, _vp, _i64, _int, _vp, _int, _i64, _i64, ctypes.c_float, _vp, _vp, _vp, _i64,
+                          _vp],
+    "lsmx_route_fwd": [_vp, _vp],
+    "lsmx_route_bwd": [_vp, _vp, _vp, _vp],
+    "lsmx_dispatch_workspace": [_i64, _i64],
+    "lsmx_dispatch": [_vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp],
+    "lsmx_expert_gated": [_vp, _vp, _vp, _vp],
+    "lsmx_expert_combine_workspace": [_vp],
+    "lsmx_expert_combine": [_vp, _vp, _vp, _int, _vp, _i64, _vp],
 }
 
 RET_I64 = ("lsmx_gemm_bf16f4_workspace", "lsmx_attention_workspace",
-           "lsmx_kv_attend_workspace")
+           "lsmx_kv_attend_workspace", "lsmx_rms_norm_bwd_workspace", "lsmx_dispatch_workspace",
+           "lsmx_expert_combine_workspace")
 
 
 class QItem(ctypes.Structure):
@@ -114,6 +126,19 @@ class KVCache(ctypes.Structure):
     _fields_ = [("k_codes", _vp), ("k_scale", _vp), ("v_codes", _vp), ("v_scale", _vp), ("pages", _i64), ("page", _i64),
                 ("kv_heads", _i64), ("head_dim", _i64), ("table", _vp), ("lengths", _vp), ("batch", _i64),
                 ("max_pages", _i64)]
+
+
+class Route(ctypes.Structure):
+    """lsmx_route of include/lsmx.h."""
+    _fields_ = [("logits", _vp), ("dtype", _int), ("rows", _i64), ("ld", _i64), ("experts", _i64), ("k", _i64),
+                ("sigmoid", _int), ("groups", _i64), ("top_groups", _i64), ("renorm", _int), ("scale", ctypes.c_float),
+                ("bias", _vp), ("mask", _vp), ("weights", _vp), ("ids", _vp)]
+
+
+class Experts(ctypes.Structure):
+    """lsmx_experts of include/lsmx.h."""
+    _fields_ = [("x", _vp), ("x_scale", _vp), ("w", _vp), ("w_scale", _vp), ("ids", _vp), ("order", _vp),
+                ("offsets", _vp), ("tokens", _i64), ("k", _i64), ("experts", _i64), ("N", _i64), ("K", _i64)]
 
 
 # Epochs for lsmx_scale_to_e8m0_batch's flag: unique within the process and
@@ -199,6 +224,15 @@ def require_device(*tensors: torch.Tensor) -> None:
             raise RuntimeError(
                 "lockstep_amd runs its MXFP4 ops on a gfx950 GPU only; got a tensor on "
                 f"{t.device} (there is no CPU fallback)")
+
+
+def one_device(*tensors: torch.Tensor) -> None:
+    assert len({t.device for t in tensors}) == 1, "all tensors must be on one device"
+
+
+def on_device_of(t: torch.Tensor):
+    """Makes t's device the current one: a launch on one of its streams needs that."""
+    return torch.cuda.device(t.device)
 
 
 def not_traced(name: str) -> None:

@@ -21,7 +21,7 @@ CSRC = PKG / "csrc"
 LIB = PKG / "liblsmx.so"
 FAST_LIB = PKG / "_fast.so"
 SOURCES = ["capi.hip", "quantize.hip", "gemm_f4f4.hip", "gemm_bf16f4.hip", "gemm_dense.hip", "gemm_dense_ring.hip", "gemm_f8f8.hip", "gemm_promote.hip",
-           "attention.hip", "attention_bwd.hip", "kv_cache.hip"]
+           "attention.hip", "attention_bwd.hip", "kv_cache.hip", "norm.hip", "route.hip", "experts.hip"]
 ARCH = "gfx950"
 
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 anywhere in the device code.

@@ -8,6 +8,7 @@
 #include <mutex>
 
 #include "lsmx_attn.h"
+#include "lsmx_block.h"
 #include "lsmx_internal.h"
 
 namespace lsmx {
@@ -1008,6 +1009,192 @@ int lsmx_kv_evict(const lsmx_kv_cache *c, const float *weights, int64_t w_len, i
     a.batch = (int)c->batch, a.keep = (int)keep, a.sinks = (int)sinks, a.recent = (int)recent;
     a.index = index, a.new_lengths = new_lengths, a.new_weights = new_weights;
     return launched(lsmx::launch_kv_evict(a, (hipStream_t)stream), fn);
+}
+
+// -------------------------------------------------------------------- norm
+static bool float_type(int dt) { return dt == LSMX_F32 || dt == LSMX_BF16 || dt == LSMX_F16; }
+
+static int norm_check(const char *fn, int dtype, int w_dtype, int64_t rows, int64_t dim, float eps) {
+    if (!float_type(dtype)) return fail(LSMX_ERR_DTYPE, "%s: dtype %d unsupported", fn, dtype);
+    if (w_dtype != dtype && w_dtype != LSMX_F32) return fail(LSMX_ERR_DTYPE, "%s: w must have x's type or be fp32", fn);
+    if (rows < 0 || rows >= (int64_t)1 << 31 || dim < 0 || dim >= (int64_t)1 << 31) return fail(LSMX_ERR_SHAPE, "%s: bad size", fn);
+    if (!(eps >= 0.f) || !(eps <= 3.0e38f)) return fail(LSMX_ERR_ARG, "%s: eps must be finite and not negative", fn);
+    return LSMX_OK;
+}
+
+int lsmx_rms_norm(const void *x, int64_t ldx, const void *r, int64_t ldr, int dtype, const void *w, int w_dtype,
+                  int64_t rows, int64_t dim, float eps, void *h, void *y, uint8_t *codes, uint8_t *scale, void *stream) {
+    const char *fn = "lsmx_rms_norm";
+    if (int c = norm_check(fn, dtype, w_dtype, rows, dim, eps)) return c;
+    const int es = elem_size(dtype);
+    if (rows && dim && (!x || !w || !y || (r && !h))) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (!codes != !scale) return fail(LSMX_ERR_ARG, "%s: codes and scale go together", fn);
+    if (ldx < dim || (r && ldr < dim)) return fail(LSMX_ERR_SHAPE, "%s: rows of x or r overlap", fn);
+    if (!aligned(x, es) || !aligned(r, es) || !aligned(w, elem_size(w_dtype)) || !aligned(h, es) || !aligned(y, es))
+        return fail(LSMX_ERR_ALIGN, "%s: misaligned pointer", fn);
+    if (codes) {
+        if (dim % 32) return fail(LSMX_ERR_SHAPE, "%s: dim=%lld must be a multiple of 32 for MXFP8", fn, (long long)dim);
+        if (!aligned(x, 16) || !aligned(r, 16) || !aligned(w, 16) || !aligned(h, 16) || !aligned(y, 16) || !aligned(codes, 8) ||
+            (ldx * es) % 16 || (r && (ldr * es) % 16))
+            return fail(LSMX_ERR_ALIGN, "%s: MXFP8 needs 16-byte aligned rows", fn);
+    }
+    if (int c = device_guard()) return c;
+    if (!rows || !dim) return LSMX_OK;
+    const lsmx::NormArgs a{x, r, w, dtype, w_dtype, rows, dim, ldx, ldr, eps, r ? h : nullptr, y, codes, scale};
+    return launched(lsmx::launch_norm_fwd(a, (hipStream_t)stream), fn);
+}
+
+int64_t lsmx_rms_norm_bwd_workspace(int64_t rows, int64_t dim, int dtype) {
+    if (norm_check("lsmx_rms_norm_bwd_workspace", dtype, dtype, rows, dim, 0.f)) return 0;
+    return rows && dim ? (int64_t)lsmx::norm_bwd_groups(rows, dim, dtype) * dim * 4 : 0;
+}
+
+int lsmx_rms_norm_bwd(const void *h, int64_t ldh, const void *dy, int64_t lddy, const void *dh, int64_t lddh, int dtype,
+                      const void *w, int w_dtype, int64_t rows, int64_t dim, float eps, void *dx, void *dw, void *ws,
+                      int64_t ws_bytes, void *stream) {
+    const char *fn = "lsmx_rms_norm_bwd";
+    if (int c = norm_check(fn, dtype, w_dtype, rows, dim, eps)) return c;
+    const int es = elem_size(dtype);
+    if (!rows && dw && dim) return fail(LSMX_ERR_SHAPE, "%s: no rows (dw is not written)", fn);
+    if (rows && dim && (!h || !dy || !w || !dx || (dw && !ws))) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (ldh < dim || lddy < dim || (dh && lddh < dim)) return fail(LSMX_ERR_SHAPE, "%s: rows overlap", fn);
+    if (!aligned(h, es) || !aligned(dy, es) || !aligned(dh, es) || !aligned(w, elem_size(w_dtype)) || !aligned(dx, es) ||
+        !aligned(dw, elem_size(w_dtype)) || !aligned(ws, 16))
+        return fail(LSMX_ERR_ALIGN, "%s: misaligned pointer", fn);
+    if (dw && ws_bytes < lsmx_rms_norm_bwd_workspace(rows, dim, dtype)) return fail(LSMX_ERR_ARG, "%s: workspace too small", fn);
+    if (int c = device_guard()) return c;
+    if (!rows || !dim) return LSMX_OK;
+    const lsmx::NormBwdArgs a{h, w, dy, dh, dtype, w_dtype, rows, dim, ldh, lddy, lddh, eps, dx, dw, (float *)ws};
+    return launched(lsmx::launch_norm_bwd(a, (hipStream_t)stream), fn);
+}
+
+// ------------------------------------------------------------------ router
+static int route_args(const char *fn, const lsmx_route *a, lsmx::RouteArgs *out) {
+    if (!a) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (!float_type(a->dtype)) return fail(LSMX_ERR_DTYPE, "%s: dtype %d unsupported", fn, a->dtype);
+    if (a->experts < 1 || a->experts > 1024) return fail(LSMX_ERR_SHAPE, "%s: experts=%lld must be 1 to 1024", fn, (long long)a->experts);
+    if (a->groups < 1 || a->groups > 64 || a->experts % a->groups)
+        return fail(LSMX_ERR_SHAPE, "%s: groups=%lld must be 1 to 64 and divide experts=%lld", fn, (long long)a->groups,
+                    (long long)a->experts);
+    if (a->top_groups < 1 || a->top_groups > a->groups)
+        return fail(LSMX_ERR_SHAPE, "%s: top_groups=%lld must be 1 to groups=%lld", fn, (long long)a->top_groups, (long long)a->groups);
+    if (a->k < 1 || a->k > 64 || a->k > a->experts / a->groups * a->top_groups)
+        return fail(LSMX_ERR_SHAPE, "%s: k=%lld must be 1 to 64 and at most the %lld experts that stay", fn, (long long)a->k,
+                    (long long)(a->experts / a->groups * a->top_groups));
+    if (a->rows < 0 || a->rows >= (int64_t)1 << 31) return fail(LSMX_ERR_SHAPE, "%s: bad number of rows", fn);
+    if (a->ld < a->experts) return fail(LSMX_ERR_SHAPE, "%s: rows of logits overlap", fn);
+    if (!(a->scale > 0.f) || !(a->scale <= 3.0e38f)) return fail(LSMX_ERR_ARG, "%s: scale must be positive and finite", fn);
+    if (a->rows && (!a->logits || !a->ids)) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (!aligned(a->logits, elem_size(a->dtype)) || !aligned(a->bias, 4) || !aligned(a->weights, 4) || !aligned(a->ids, 4))
+        return fail(LSMX_ERR_ALIGN, "%s: misaligned pointer", fn);
+    *out = lsmx::RouteArgs{a->logits, a->dtype, a->rows, a->ld, (int)a->experts, (int)a->k, a->sigmoid != 0, (int)a->groups,
+                           (int)a->top_groups, a->renorm != 0, a->scale, a->bias, a->mask, a->weights, a->ids, nullptr, nullptr};
+    return LSMX_OK;
+}
+
+int lsmx_route_fwd(const lsmx_route *a, void *stream) {
+    const char *fn = "lsmx_route_fwd";
+    lsmx::RouteArgs g;
+    if (int r = route_args(fn, a, &g)) return r;
+    if (g.rows && !g.weights) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (int r = device_guard()) return r;
+    if (!g.rows) return LSMX_OK;
+    return launched(lsmx::launch_route_fwd(g, (hipStream_t)stream), fn);
+}
+
+int lsmx_route_bwd(const lsmx_route *a, const float *dweights, void *dlogits, void *stream) {
+    const char *fn = "lsmx_route_bwd";
+    lsmx::RouteArgs g;
+    if (int r = route_args(fn, a, &g)) return r;
+    if (g.rows && (!dweights || !dlogits)) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (!aligned(dweights, 4) || !aligned(dlogits, elem_size(a->dtype))) return fail(LSMX_ERR_ALIGN, "%s: misaligned pointer", fn);
+    if (int r = device_guard()) return r;
+    if (!g.rows) return LSMX_OK;
+    g.dw = dweights, g.dlogits = dlogits;
+    return launched(lsmx::launch_route_bwd(g, (hipStream_t)stream), fn);
+}
+
+static int pairs_check(const char *fn, int64_t pairs, int64_t experts) {
+    if (experts < 1 || experts > 1024) return fail(LSMX_ERR_SHAPE, "%s: experts=%lld must be 1 to 1024", fn, (long long)experts);
+    if (pairs < 0 || pairs > (int64_t)1 << 21) return fail(LSMX_ERR_SHAPE, "%s: %lld pairs, at most 2^21", fn, (long long)pairs);
+    return LSMX_OK;
+}
+
+int64_t lsmx_dispatch_workspace(int64_t pairs, int64_t experts) {
+    return pairs_check("lsmx_dispatch_workspace", pairs, experts) ? 0 : lsmx::dispatch_workspace(pairs, (int)experts);
+}
+
+int lsmx_dispatch(const int32_t *ids, int64_t pairs, int64_t experts, int32_t *order, int32_t *offsets, void *ws,
+                  int64_t ws_bytes, void *stream) {
+    const char *fn = "lsmx_dispatch";
+    if (int r = pairs_check(fn, pairs, experts)) return r;
+    const int64_t need = lsmx::dispatch_workspace(pairs, (int)experts);
+    if (!offsets || (pairs && (!ids || !order)) || (need && !ws)) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (!aligned(ids, 4) || !aligned(order, 4) || !aligned(offsets, 4) || !aligned(ws, 4))
+        return fail(LSMX_ERR_ALIGN, "%s: misaligned pointer", fn);
+    if (ws_bytes < need) return fail(LSMX_ERR_ARG, "%s: workspace too small", fn);
+    if (int r = device_guard()) return r;
+    std::lock_guard<std::mutex> lk(lsmx::g_workspace_mu);
+    return launched(lsmx::launch_dispatch(ids, (int)pairs, (int)experts, order, offsets, (int32_t *)ws, (hipStream_t)stream), fn);
+}
+
+// ------------------------------------------------------- experts' products
+static int expert_args(const char *fn, const lsmx_experts *a, bool gated, lsmx::ExpertArgs *out) {
+    if (!a) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (a->k < 1 || a->k > 1024 || a->tokens < 0 || a->tokens > (int64_t)1 << 21)
+        return fail(LSMX_ERR_SHAPE, "%s: bad number of tokens or slots", fn);
+    if (int r = pairs_check(fn, a->tokens * a->k, a->experts)) return r;
+    if (a->K < 128 || a->K % 128 || a->K >= (int64_t)1 << 24)
+        return fail(LSMX_ERR_SHAPE, "%s: K=%lld must be a multiple of 128", fn, (long long)a->K);
+    if (a->N < 1 || a->N >= (int64_t)1 << 24 || a->N * a->K / 2 >= (int64_t)1 << 31)
+        return fail(LSMX_ERR_SHAPE, "%s: N=%lld: an expert's weights must stay below 2^31 bytes", fn, (long long)a->N);
+    if (gated && a->N % 64) return fail(LSMX_ERR_SHAPE, "%s: N=%lld must be a multiple of 64 (F of 32)", fn, (long long)a->N);
+    if (a->tokens && (!a->x || !a->x_scale || !a->w || !a->w_scale || !a->ids || !a->order || !a->offsets))
+        return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (!aligned(a->x, 16) || !aligned(a->w, 16) || !aligned(a->x_scale, 4) || !aligned(a->w_scale, 4) || !aligned(a->ids, 4) ||
+        !aligned(a->order, 4) || !aligned(a->offsets, 4))
+        return fail(LSMX_ERR_ALIGN, "%s: x and w must be 16-byte aligned, their scales 4-byte", fn);
+    *out = lsmx::ExpertArgs{};
+    out->x = a->x, out->xs = a->x_scale, out->w = a->w, out->ws = a->w_scale;
+    out->ids = a->ids, out->order = a->order, out->offsets = a->offsets;
+    out->pairs = (int)(a->tokens * a->k), out->k = (int)a->k, out->experts = (int)a->experts;
+    out->N = (int)a->N, out->K = (int)a->K, out->tokens = a->tokens;
+    out->ldz = (a->N + 3) / 4 * 4;
+    return LSMX_OK;
+}
+
+int lsmx_expert_gated(const lsmx_experts *a, uint8_t *h, uint8_t *h_scale, void *stream) {
+    const char *fn = "lsmx_expert_gated";
+    lsmx::ExpertArgs g;
+    if (int r = expert_args(fn, a, true, &g)) return r;
+    if (g.tokens && (!h || !h_scale)) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (!aligned(h, 4)) return fail(LSMX_ERR_ALIGN, "%s: h must be 4-byte aligned", fn);
+    if (int r = device_guard()) return r;
+    if (!g.tokens) return LSMX_OK;
+    g.h = h, g.hs = h_scale;
+    return launched(lsmx::launch_expert_gated(g, (hipStream_t)stream), fn);
+}
+
+int64_t lsmx_expert_combine_workspace(const lsmx_experts *a) {
+    lsmx::ExpertArgs g;
+    if (expert_args("lsmx_expert_combine_workspace", a, false, &g)) return 0;
+    return (int64_t)g.pairs * g.ldz * 4;
+}
+
+int lsmx_expert_combine(const lsmx_experts *a, const float *weights, void *y, int y_dtype, void *ws, int64_t ws_bytes,
+                        void *stream) {
+    const char *fn = "lsmx_expert_combine";
+    lsmx::ExpertArgs g;
+    if (int r = expert_args(fn, a, false, &g)) return r;
+    if (!float_type(y_dtype)) return fail(LSMX_ERR_DTYPE, "%s: y_dtype %d unsupported", fn, y_dtype);
+    if (g.tokens && (!weights || !y || !ws)) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
+    if (!aligned(weights, 4) || !aligned(y, elem_size(y_dtype)) || !aligned(ws, 16)) return fail(LSMX_ERR_ALIGN, "%s: misaligned pointer", fn);
+    if (ws_bytes < (int64_t)g.pairs * g.ldz * 4) return fail(LSMX_ERR_ARG, "%s: workspace too small", fn);
+    if (int r = device_guard()) return r;
+    if (!g.tokens) return LSMX_OK;
+    g.z = (float *)ws, g.weights = weights, g.y = y, g.y_dtype = y_dtype;
+    std::lock_guard<std::mutex> lk(lsmx::g_workspace_mu);
+    return launched(lsmx::launch_expert_combine(g, (hipStream_t)stream), fn);
 }
 
 }  // extern "C"

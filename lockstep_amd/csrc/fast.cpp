@@ -745,6 +745,174 @@ PyObject *kv_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// --------------------------------------------- norm, router, experts' products
+// dense storage of a type on the current device, which launches need; gradients
+// and forward-mode derivatives go through the Python path's nodes
+bool dense(const Tensor *t, at::ScalarType s) { return t && t->scalar_type() == s && t->is_contiguous(); }
+bool here(const Tensor &t) { return t.device().index() == c10::hip::current_device(); }
+bool wants_grad(const Tensor *t) { return t && ((at::GradMode::is_enabled() && t->requires_grad()) || dual(*t)); }
+bool bool_arg(PyObject *o, bool &v) {
+    v = o == Py_True;
+    return PyBool_Check(o);
+}
+std::vector<int64_t> with_last(at::IntArrayRef shape, std::initializer_list<int64_t> last, int64_t drop) {
+    std::vector<int64_t> v(shape.begin(), shape.end() - drop);
+    v.insert(v.end(), last);
+    return v;
+}
+PyObject *wrap_all(std::initializer_list<const Tensor *> ts) {
+    Py_ssize_t n = 0, i = 0;
+    for (const Tensor *t : ts) n += t->defined();
+    PyObject *r = PyTuple_New(n);
+    if (!r) return nullptr;
+    for (const Tensor *t : ts)
+        if (t->defined()) PyTuple_SET_ITEM(r, i++, THPVariable_Wrap(*t));
+    return r;
+}
+
+// rms_norm(x, weight, residual, eps, mxfp8) -> y, or (y, h), with (codes, scale)
+PyObject *rms_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    NONE_IF(n != 5);
+    const Tensor *x = plain(a[0]), *w = plain(a[1]), *r = a[2] == Py_None ? nullptr : plain(a[2]);
+    bool mx;
+    NONE_IF(!x || !w || (a[2] != Py_None && !r) || !PyFloat_CheckExact(a[3]) || !bool_arg(a[4], mx) || traced());
+    const double eps = PyFloat_AS_DOUBLE(a[3]);
+    const at::ScalarType dt = x->scalar_type();
+    NONE_IF(dtype_of(dt) < 0 || x->dim() < 1 || x->numel() == 0 || !x->is_contiguous() || (r && (!dense(r, dt) || !r->sizes().equals(x->sizes()))) ||
+            (w->scalar_type() != dt && w->scalar_type() != at::kFloat) || w->dim() != 1 || !w->is_contiguous() ||
+            w->size(0) != x->size(-1) || w->device() != x->device() || (r && r->device() != x->device()) || !here(*x) ||
+            wants_grad(x) || wants_grad(w) || wants_grad(r) || !(eps >= 0.0 && eps <= 3.0e38));
+    const int64_t D = x->size(-1), rows = x->numel() / D;
+    NONE_IF(mx && (D % 32 || !al(*x, 16) || !al(*w, 16) || (r && !al(*r, 16))));
+    const Tensor y = make(x->sizes(), dt, *x), h = r ? make(x->sizes(), dt, *x) : Tensor();
+    Tensor codes, scale;
+    if (mx) {
+        codes = make(x->sizes(), at::kFloat8_e4m3fn, *x);
+        scale = make(with_last(x->sizes(), {D / 32}, 1), at::kByte, *x);
+    }
+    void *s = stream_of(*x);
+    if (!launch([&] {
+            return lsmx_rms_norm(x->data_ptr(), D, r ? r->data_ptr() : nullptr, r ? D : 0, dtype_of(dt), w->data_ptr(),
+                                 dtype_of(w->scalar_type()), rows, D, (float)eps, r ? h.data_ptr() : nullptr, y.data_ptr(),
+                                 mx ? (uint8_t *)codes.data_ptr() : nullptr, mx ? scale.data_ptr<uint8_t>() : nullptr, s);
+        }))
+        return nullptr;
+    return r || mx ? wrap_all({&y, &h, &codes, &scale}) : THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// route(logits, k, bias, scoring, groups, top_groups, renormalize, scale, mask) -> (weights, experts)
+PyObject *route(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    NONE_IF(n != 9);
+    const Tensor *l = plain(a[0]), *b = a[2] == Py_None ? nullptr : plain(a[2]), *m = a[8] == Py_None ? nullptr : plain(a[8]);
+    int64_t k, groups, top;
+    bool renorm;
+    NONE_IF(!l || (a[2] != Py_None && !b) || (a[8] != Py_None && !m) || traced() || !int_arg(a[1], 1, false, k) ||
+            !int_arg(a[4], 1, false, groups) || !int_arg(a[5], 1, false, top) || !bool_arg(a[6], renorm) ||
+            !PyFloat_CheckExact(a[7]) || !PyUnicode_CheckExact(a[3]));
+    const bool soft = PyUnicode_CompareWithASCIIString(a[3], "softmax") == 0;
+    NONE_IF(!soft && PyUnicode_CompareWithASCIIString(a[3], "sigmoid") != 0);
+    NONE_IF(dtype_of(l->scalar_type()) < 0 || l->dim() < 1 || l->numel() == 0 || !l->is_contiguous() || !here(*l) || wants_grad(l));
+    const int64_t E = l->size(-1), rows = l->numel() / E;
+    const at::IntArrayRef lead = l->sizes().slice(0, l->dim() - 1);
+    const double scale = PyFloat_AS_DOUBLE(a[7]);
+    NONE_IF(E > 1024 || groups > 64 || E % groups || top > groups || k > 64 || k > E / groups * top || !(scale > 0.0 && scale <= 3.0e38) ||
+            (b && (!dense(b, at::kFloat) || b->dim() != 1 || b->size(0) != E || b->device() != l->device() || dual(*b))) ||
+            (m && (!dense(m, at::kBool) || !m->sizes().equals(lead) || m->device() != l->device())));
+    const std::vector<int64_t> shape = with_last(lead, {k}, 0);
+    const Tensor w = make(shape, at::kFloat, *l), ids = make(shape, at::kInt, *l);
+    lsmx_route g{l->data_ptr(), dtype_of(l->scalar_type()), rows, E, E, k, !soft, groups, top, renorm, (float)scale,
+                 b ? b->data_ptr<float>() : nullptr, m ? (const uint8_t *)m->data_ptr() : nullptr, w.data_ptr<float>(), ids.data_ptr<int32_t>()};
+    void *s = stream_of(*l);
+    if (!launch([&] { return lsmx_route_fwd(&g, s); })) return nullptr;
+    return wrap2(w, ids);
+    END_HANDLE_TH_ERRORS
+}
+
+// dispatch(experts, num_experts) -> (order, offsets)
+PyObject *dispatch(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    NONE_IF(n != 2);
+    const Tensor *ids = plain(a[0]);
+    int64_t E;
+    NONE_IF(!dense(ids, at::kInt) || ids->dim() < 1 || traced() || !int_arg(a[1], 1, false, E) || E > 1024 || ids->numel() == 0 ||
+            ids->numel() > (1 << 21) || !here(*ids));
+    const int64_t pairs = ids->numel(), nws = lsmx_dispatch_workspace(pairs, E);
+    const Tensor order = make({pairs}, at::kInt, *ids), offsets = make({E + 1}, at::kInt, *ids);
+    const Tensor ws = nws ? make({nws}, at::kByte, *ids) : Tensor();
+    void *s = stream_of(*ids);
+    if (!launch([&] {
+            return lsmx_dispatch(ids->data_ptr<int32_t>(), pairs, E, order.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(),
+                                 nws ? ws.data_ptr() : nullptr, nws, s);
+        }))
+        return nullptr;
+    return wrap2(order, offsets);
+    END_HANDLE_TH_ERRORS
+}
+
+// The product of experts._check, or false for any form that it would convert or
+// refuse.  slots: rows are [.., k, K], else [.., K].
+bool experts_of(PyObject *const *a, bool slots, lsmx_experts &g, const Tensor *&x, const Tensor *&ids) {
+    if (!PyTuple_Check(a[4]) || PyTuple_GET_SIZE(a[4]) != 3 || traced()) return false;
+    const Tensor *xs = plain(a[1]), *w = plain(a[2]), *ws = plain(a[3]);
+    const Tensor *order = plain(PyTuple_GET_ITEM(a[4], 1)), *off = plain(PyTuple_GET_ITEM(a[4], 2));
+    x = plain(a[0]), ids = plain(PyTuple_GET_ITEM(a[4], 0));
+    if (!x || !(dense(x, at::kFloat8_e4m3fn) || dense(x, at::kByte)) || !dense(xs, at::kByte) || !dense(w, at::kByte) ||
+        !dense(ws, at::kByte) || !dense(ids, at::kInt) || !dense(order, at::kInt) || !dense(off, at::kInt))
+        return false;
+    for (const Tensor *t : {xs, w, ws, ids, order, off})
+        if (t->device() != x->device()) return false;
+    if (!here(*x) || w->dim() != 3 || w->numel() == 0 || ids->dim() < 1 || ids->numel() == 0 || !al(*x, 16) || !al(*w, 16) ||
+        !al(*xs, 4) || !al(*ws, 4))
+        return false;
+    const int64_t E = w->size(0), N = w->size(1), K = 2 * w->size(2), k = ids->size(-1);
+    const at::IntArrayRef lead = slots ? ids->sizes() : ids->sizes().slice(0, ids->dim() - 1);
+    if (K % 128 || E > 1024 || k > 1024 || ids->numel() > (1 << 21) || N * K / 2 >= ((int64_t)1 << 31) ||
+        !ws->sizes().equals({E, N, K / 32}) || !x->sizes().equals(with_last(lead, {K}, 0)) ||
+        !xs->sizes().equals(with_last(lead, {K / 32}, 0)) || order->dim() != 1 || order->numel() != ids->numel() ||
+        off->dim() != 1 || off->numel() != E + 1)
+        return false;
+    g = lsmx_experts{(const uint8_t *)x->data_ptr(), xs->data_ptr<uint8_t>(), w->data_ptr<uint8_t>(), ws->data_ptr<uint8_t>(),
+                     ids->data_ptr<int32_t>(), order->data_ptr<int32_t>(), off->data_ptr<int32_t>(), ids->numel() / k, k, E, N, K};
+    return true;
+}
+
+// expert_gated(x, x_scale, w, w_scale, d) -> (h, h_scale)
+PyObject *expert_gated(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    NONE_IF(n != 5);
+    lsmx_experts g;
+    const Tensor *x, *ids;
+    NONE_IF(!experts_of(a, false, g, x, ids) || g.N % 64);
+    const Tensor h = make(with_last(ids->sizes(), {g.N / 2}, 0), at::kFloat8_e4m3fn, *x);
+    const Tensor hs = make(with_last(ids->sizes(), {g.N / 64}, 0), at::kByte, *x);
+    void *s = stream_of(*x);
+    if (!launch([&] { return lsmx_expert_gated(&g, (uint8_t *)h.data_ptr(), hs.data_ptr<uint8_t>(), s); })) return nullptr;
+    return wrap2(h, hs);
+    END_HANDLE_TH_ERRORS
+}
+
+// expert_combine(h, h_scale, w, w_scale, d, weights, out_dtype) -> y
+PyObject *expert_combine(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    NONE_IF(n != 7);
+    lsmx_experts g;
+    const Tensor *x, *ids, *w = plain(a[5]);
+    const at::ScalarType ot = out_type(a[6]);
+    NONE_IF(ot == at::ScalarType::Undefined || !dense(w, at::kFloat) || !experts_of(a, true, g, x, ids) ||
+            !w->sizes().equals(ids->sizes()) || w->device() != x->device());
+    const Tensor y = make(with_last(ids->sizes(), {g.N}, 1), ot, *x);
+    const int64_t nws = lsmx_expert_combine_workspace(&g);
+    const Tensor ws = make({nws}, at::kByte, *x);
+    void *s = stream_of(*x);
+    if (!launch([&] { return lsmx_expert_combine(&g, w->data_ptr<float>(), y.data_ptr(), dtype_of(ot), ws.data_ptr(), nws, s); }))
+        return nullptr;
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
 // init(check, workspace, next_epoch): the _capi functions the calls above use
 PyObject *init(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (n != 3) {
@@ -763,7 +931,8 @@ PyObject *init(PyObject *, PyObject *const *a, Py_ssize_t n) {
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(init),   FAST(quantize_pack), FAST(quantize_pack2), FAST(quantize), FAST(quantize_2d), FAST(pack),
                          FAST(gemm_packed), FAST(linear), FAST(weight), FAST(gemm_fp8),
-                         FAST(attention), FAST(kv_append), FAST(kv_attend), FAST(kv_evict), {nullptr, nullptr, 0, nullptr}};
+                         FAST(attention), FAST(kv_append), FAST(kv_attend), FAST(kv_evict), FAST(rms_norm), FAST(route),
+                         FAST(dispatch), FAST(expert_gated), FAST(expert_combine), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
