@@ -746,11 +746,10 @@ PyObject *kv_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
 }
 
 // --------------------------------------------- norm, router, experts' products
-// dense storage of a type on the current device, which launches need; gradients
-// and forward-mode derivatives go through the Python path's nodes
+// dense storage of a type on the current device, which launches need;
+// forward-mode derivatives go to the Python path's nodes, which refuse them
 bool dense(const Tensor *t, at::ScalarType s) { return t && t->scalar_type() == s && t->is_contiguous(); }
 bool here(const Tensor &t) { return t.device().index() == c10::hip::current_device(); }
-bool wants_grad(const Tensor *t) { return t && ((at::GradMode::is_enabled() && t->requires_grad()) || dual(*t)); }
 bool bool_arg(PyObject *o, bool &v) {
     v = o == Py_True;
     return PyBool_Check(o);
@@ -760,15 +759,94 @@ std::vector<int64_t> with_last(at::IntArrayRef shape, std::initializer_list<int6
     v.insert(v.end(), last);
     return v;
 }
-PyObject *wrap_all(std::initializer_list<const Tensor *> ts) {
-    Py_ssize_t n = 0, i = 0;
-    for (const Tensor *t : ts) n += t->defined();
-    PyObject *r = PyTuple_New(n);
+PyObject *wrap_all(const std::vector<Tensor> &ts) {
+    PyObject *r = PyTuple_New((Py_ssize_t)ts.size());
     if (!r) return nullptr;
-    for (const Tensor *t : ts)
-        if (t->defined()) PyTuple_SET_ITEM(r, i++, THPVariable_Wrap(*t));
+    for (size_t i = 0; i < ts.size(); ++i) PyTuple_SET_ITEM(r, (Py_ssize_t)i, THPVariable_Wrap(ts[i]));
     return r;
 }
+
+// Raises for a failed call made inside a node, where the engine carries C++
+// exceptions.
+void must(int rc) { TORCH_CHECK(rc == LSMX_OK, lsmx_last_error()); }
+
+// Gradients that have none of their own (create_graph), as once_differentiable
+// gives them.
+torch::autograd::variable_list once(torch::autograd::variable_list d) {
+    if (!at::GradMode::is_enabled()) return d;
+    auto err = std::make_shared<torch::autograd::DelayedError>(
+        "trying to differentiate twice a function that was marked with @once_differentiable", (int)d.size());
+    torch::autograd::variable_list in;
+    for (auto &t : d) in.push_back(t.defined() ? t.detach().set_requires_grad(true) : t);
+    return (*err)(std::move(in));
+}
+
+struct NormOut {
+    Tensor y, h, codes, scale;
+};
+NormOut norm_forward(const Tensor &x, const Tensor &w, const Tensor &r, double eps, bool mx) {
+    const int64_t D = x.size(-1);
+    NormOut o;
+    o.y = make(x.sizes(), x.scalar_type(), x);
+    if (r.defined()) o.h = make(x.sizes(), x.scalar_type(), x);
+    if (mx) {
+        o.codes = make(x.sizes(), at::kFloat8_e4m3fn, x);
+        o.scale = make(with_last(x.sizes(), {D / 32}, 1), at::kByte, x);
+    }
+    if (const int rc = lsmx_rms_norm(x.data_ptr(), D, r.defined() ? r.data_ptr() : nullptr, r.defined() ? D : 0, dtype_of(x.scalar_type()),
+                                     w.data_ptr(), dtype_of(w.scalar_type()), x.numel() / D, D, (float)eps,
+                                     r.defined() ? o.h.data_ptr() : nullptr, o.y.data_ptr(), mx ? (uint8_t *)o.codes.data_ptr() : nullptr,
+                                     mx ? o.scale.data_ptr<uint8_t>() : nullptr, stream_of(x)))
+        throw Failed{rc};
+    return o;
+}
+
+// The same node as norm._AddRMSNorm, in native code.
+struct Norm : torch::autograd::Function<Norm> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &w,
+                                                  const std::optional<Tensor> &r, double eps, bool mx) {
+        NormOut o = norm_forward(x, w, r ? *r : Tensor(), eps, mx);
+        ctx->save_for_backward({r ? o.h : x, w});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["residual"] = r.has_value();
+        ctx->set_materialize_grads(false);
+        torch::autograd::variable_list out{o.y};
+        if (r) out.push_back(o.h);
+        if (mx) {
+            out.push_back(o.codes), out.push_back(o.scale);
+            ctx->mark_non_differentiable({o.codes, o.scale});
+        }
+        return out;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        const auto s = ctx->get_saved_variables();
+        const Tensor &h = s[0], &w = s[1];
+        const bool residual = ctx->saved_data["residual"].toBool();
+        Tensor dy = grads[0], dh = residual ? grads[1] : Tensor(), dx, dw;
+        if (!dy.defined()) {
+            dx = dh;
+        } else {
+            at::AutoGradMode off(false);
+            const int64_t D = h.size(-1), rows = h.numel() / D;
+            const int dt = dtype_of(h.scalar_type());
+            dy = dy.to(h.scalar_type()).contiguous();
+            if (dh.defined()) dh = dh.to(h.scalar_type()).contiguous();
+            dx = make(h.sizes(), h.scalar_type(), h);
+            Tensor ws;
+            int64_t n = 0;
+            if (ctx->needs_input_grad(1)) {
+                dw = make(w.sizes(), w.scalar_type(), w);
+                n = lsmx_rms_norm_bwd_workspace(rows, D, dt);
+                ws = make({n}, at::kByte, h);
+            }
+            must(lsmx_rms_norm_bwd(h.data_ptr(), D, dy.data_ptr(), D, dh.defined() ? dh.data_ptr() : nullptr, dh.defined() ? D : 0, dt,
+                                   w.data_ptr(), dtype_of(w.scalar_type()), rows, D, (float)ctx->saved_data["eps"].toDouble(),
+                                   dx.data_ptr(), dw.defined() ? dw.data_ptr() : nullptr, n ? ws.data_ptr() : nullptr, n, stream_of(h)));
+        }
+        auto d = once({dx, dw, residual ? dx : Tensor()});
+        return {d[0], d[1], d[2], Tensor(), Tensor()};
+    }
+};
 
 // rms_norm(x, weight, residual, eps, mxfp8) -> y, or (y, h), with (codes, scale)
 PyObject *rms_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
@@ -782,25 +860,82 @@ PyObject *rms_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
     NONE_IF(dtype_of(dt) < 0 || x->dim() < 1 || x->numel() == 0 || !x->is_contiguous() || (r && (!dense(r, dt) || !r->sizes().equals(x->sizes()))) ||
             (w->scalar_type() != dt && w->scalar_type() != at::kFloat) || w->dim() != 1 || !w->is_contiguous() ||
             w->size(0) != x->size(-1) || w->device() != x->device() || (r && r->device() != x->device()) || !here(*x) ||
-            wants_grad(x) || wants_grad(w) || wants_grad(r) || !(eps >= 0.0 && eps <= 3.0e38));
-    const int64_t D = x->size(-1), rows = x->numel() / D;
-    NONE_IF(mx && (D % 32 || !al(*x, 16) || !al(*w, 16) || (r && !al(*r, 16))));
-    const Tensor y = make(x->sizes(), dt, *x), h = r ? make(x->sizes(), dt, *x) : Tensor();
-    Tensor codes, scale;
-    if (mx) {
-        codes = make(x->sizes(), at::kFloat8_e4m3fn, *x);
-        scale = make(with_last(x->sizes(), {D / 32}, 1), at::kByte, *x);
+            dual(*x) || dual(*w) || (r && dual(*r)) || !(eps >= 0.0 && eps <= 3.0e38));
+    NONE_IF(mx && (x->size(-1) % 32 || !al(*x, 16) || !al(*w, 16) || (r && !al(*r, 16))));
+    const bool grad = at::GradMode::is_enabled() && (x->requires_grad() || w->requires_grad() || (r && r->requires_grad()));
+    torch::autograd::variable_list out;
+    int rc = LSMX_OK;
+    {
+        NoGil released;
+        try {
+            if (grad) {
+                out = Norm::apply(*x, *w, r ? std::optional<Tensor>(*r) : std::nullopt, eps, mx);
+            } else {
+                NormOut o = norm_forward(*x, *w, r ? *r : Tensor(), eps, mx);
+                for (const Tensor &t : {o.y, o.h, o.codes, o.scale})
+                    if (t.defined()) out.push_back(t);
+            }
+        } catch (const Failed &f) {
+            rc = f.rc;
+        }
     }
-    void *s = stream_of(*x);
-    if (!launch([&] {
-            return lsmx_rms_norm(x->data_ptr(), D, r ? r->data_ptr() : nullptr, r ? D : 0, dtype_of(dt), w->data_ptr(),
-                                 dtype_of(w->scalar_type()), rows, D, (float)eps, r ? h.data_ptr() : nullptr, y.data_ptr(),
-                                 mx ? (uint8_t *)codes.data_ptr() : nullptr, mx ? scale.data_ptr<uint8_t>() : nullptr, s);
-        }))
+    if (rc != LSMX_OK) {
+        Py_XDECREF(PyObject_CallFunction(g_error, "i", rc));
         return nullptr;
-    return r || mx ? wrap_all({&y, &h, &codes, &scale}) : THPVariable_Wrap(y);
+    }
+    return out.size() > 1 ? wrap_all(out) : THPVariable_Wrap(out[0]);
     END_HANDLE_TH_ERRORS
 }
+
+lsmx_route route_args(const Tensor &l, int64_t k, bool sigmoid, int64_t groups, int64_t top, bool renorm, double scale) {
+    lsmx_route g{};
+    const int64_t E = l.size(-1);
+    g.logits = l.data_ptr(), g.dtype = dtype_of(l.scalar_type()), g.rows = l.numel() / E, g.ld = E, g.experts = E, g.k = k;
+    g.sigmoid = sigmoid, g.groups = groups, g.top_groups = top, g.renorm = renorm, g.scale = (float)scale;
+    return g;
+}
+struct RouteOut {
+    Tensor weights, ids;
+};
+RouteOut route_forward(const Tensor &l, lsmx_route g) {
+    const std::vector<int64_t> shape = with_last(l.sizes(), {g.k}, 1);
+    RouteOut o{make(shape, at::kFloat, l), make(shape, at::kInt, l)};
+    g.weights = o.weights.data_ptr<float>(), g.ids = o.ids.data_ptr<int32_t>();
+    if (const int rc = lsmx_route_fwd(&g, stream_of(l))) throw Failed{rc};
+    return o;
+}
+
+// The same node as experts._Route, in native code.
+struct Route : torch::autograd::Function<Route> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const Tensor &l, const std::optional<Tensor> &bias,
+                                                  const std::optional<Tensor> &mask, int64_t k, bool sigmoid, int64_t groups, int64_t top,
+                                                  bool renorm, double scale) {
+        lsmx_route g = route_args(l, k, sigmoid, groups, top, renorm, scale);
+        g.bias = bias ? bias->data_ptr<float>() : nullptr;
+        g.mask = mask ? (const uint8_t *)mask->data_ptr() : nullptr;
+        const RouteOut o = route_forward(l, g);
+        ctx->save_for_backward({l, o.ids});
+        ctx->saved_data["k"] = k, ctx->saved_data["sigmoid"] = sigmoid, ctx->saved_data["renorm"] = renorm, ctx->saved_data["scale"] = scale;
+        ctx->mark_non_differentiable({o.ids});
+        return {o.weights, o.ids};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        const auto s = ctx->get_saved_variables();
+        const Tensor &l = s[0], &ids = s[1];
+        Tensor dl;
+        {
+            at::AutoGradMode off(false);
+            dl = make(l.sizes(), l.scalar_type(), l);
+            const Tensor dw = grads[0].defined() ? grads[0].to(at::kFloat).contiguous() : at::zeros_like(ids, at::kFloat);
+            // the groups only decide the choice
+            lsmx_route g = route_args(l, ctx->saved_data["k"].toInt(), ctx->saved_data["sigmoid"].toBool(), 1, 1,
+                                      ctx->saved_data["renorm"].toBool(), ctx->saved_data["scale"].toDouble());
+            g.ids = ids.data_ptr<int32_t>();
+            must(lsmx_route_bwd(&g, dw.data_ptr<float>(), dl.data_ptr(), stream_of(l)));
+        }
+        return {once({dl})[0], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
 
 // route(logits, k, bias, scoring, groups, top_groups, renormalize, scale, mask) -> (weights, experts)
 PyObject *route(PyObject *, PyObject *const *a, Py_ssize_t n) {
@@ -814,20 +949,37 @@ PyObject *route(PyObject *, PyObject *const *a, Py_ssize_t n) {
             !PyFloat_CheckExact(a[7]) || !PyUnicode_CheckExact(a[3]));
     const bool soft = PyUnicode_CompareWithASCIIString(a[3], "softmax") == 0;
     NONE_IF(!soft && PyUnicode_CompareWithASCIIString(a[3], "sigmoid") != 0);
-    NONE_IF(dtype_of(l->scalar_type()) < 0 || l->dim() < 1 || l->numel() == 0 || !l->is_contiguous() || !here(*l) || wants_grad(l));
-    const int64_t E = l->size(-1), rows = l->numel() / E;
+    NONE_IF(dtype_of(l->scalar_type()) < 0 || l->dim() < 1 || l->numel() == 0 || !l->is_contiguous() || !here(*l) || dual(*l));
+    const int64_t E = l->size(-1);
     const at::IntArrayRef lead = l->sizes().slice(0, l->dim() - 1);
     const double scale = PyFloat_AS_DOUBLE(a[7]);
     NONE_IF(E > 1024 || groups > 64 || E % groups || top > groups || k > 64 || k > E / groups * top || !(scale > 0.0 && scale <= 3.0e38) ||
             (b && (!dense(b, at::kFloat) || b->dim() != 1 || b->size(0) != E || b->device() != l->device() || dual(*b))) ||
             (m && (!dense(m, at::kBool) || !m->sizes().equals(lead) || m->device() != l->device())));
-    const std::vector<int64_t> shape = with_last(lead, {k}, 0);
-    const Tensor w = make(shape, at::kFloat, *l), ids = make(shape, at::kInt, *l);
-    lsmx_route g{l->data_ptr(), dtype_of(l->scalar_type()), rows, E, E, k, !soft, groups, top, renorm, (float)scale,
-                 b ? b->data_ptr<float>() : nullptr, m ? (const uint8_t *)m->data_ptr() : nullptr, w.data_ptr<float>(), ids.data_ptr<int32_t>()};
-    void *s = stream_of(*l);
-    if (!launch([&] { return lsmx_route_fwd(&g, s); })) return nullptr;
-    return wrap2(w, ids);
+    RouteOut o;
+    int rc = LSMX_OK;
+    {
+        NoGil released;
+        try {
+            if (at::GradMode::is_enabled() && l->requires_grad()) {
+                const auto v = Route::apply(*l, b ? std::optional<Tensor>(b->detach()) : std::nullopt, m ? std::optional<Tensor>(*m) : std::nullopt,
+                                            k, !soft, groups, top, renorm, scale);
+                o = {v[0], v[1]};
+            } else {
+                lsmx_route g = route_args(*l, k, !soft, groups, top, renorm, scale);
+                g.bias = b ? b->data_ptr<float>() : nullptr;
+                g.mask = m ? (const uint8_t *)m->data_ptr() : nullptr;
+                o = route_forward(*l, g);
+            }
+        } catch (const Failed &f) {
+            rc = f.rc;
+        }
+    }
+    if (rc != LSMX_OK) {
+        Py_XDECREF(PyObject_CallFunction(g_error, "i", rc));
+        return nullptr;
+    }
+    return wrap2(o.weights, o.ids);
     END_HANDLE_TH_ERRORS
 }
 

@@ -257,22 +257,25 @@ __global__ __launch_bounds__(TPR) void norm_bwd_kernel(NormBwdArgs a) {
     }
 }
 
-// dw: the shares of `groups` workgroups added up, 64 columns a workgroup, its
-// 16 waves every 16th share each.
+// dw: the shares of `groups` workgroups added up, 16 columns a workgroup, its 64
+// sets of 16 lanes every 64th share each.
 template <int DT>
 __global__ __launch_bounds__(1024) void norm_dw_kernel(const float *part, int groups, int64_t dim, void *dw) {
-    __shared__ float red[16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+    __shared__ float red[16][16];
+    const int c = threadIdx.x & 15, set = threadIdx.x >> 4;
+    const int64_t col = (int64_t)blockIdx.x * 16 + c;
     float s = 0.f;
     if (col < dim)
-        for (int g = wave; g < groups; g += 16) s += part[g * dim + col];
-    red[wave][lane] = s;
+#pragma unroll 4
+        for (int g = set; g < groups; g += 64) s += part[g * dim + col];
+    s += __shfl_xor(s, 16, 64);
+    s += __shfl_xor(s, 32, 64);
+    if ((threadIdx.x & 63) < 16) red[threadIdx.x >> 6][c] = s;
     __syncthreads();
-    if (wave == 0 && col < dim) {
+    if (threadIdx.x < 16 && col < dim) {
         s = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s += red[i][lane];
+        for (int i = 0; i < 16; ++i) s += red[i][c];
         ((typename Elem<DT>::S *)dw)[col] = Elem<DT>::store(s);
     }
 }
@@ -346,7 +349,7 @@ hipError_t launch_norm_bwd(const NormBwdArgs &a, hipStream_t s) {
     hipError_t e = a.dtype == LSMX_F32 ? bwd_of<LSMX_F32>(a, s) : a.dtype == LSMX_BF16 ? bwd_of<LSMX_BF16>(a, s) : bwd_of<LSMX_F16>(a, s);
     if (e != hipSuccess || !a.dw) return e;
     const int groups = norm_bwd_groups(a.rows, a.dim, a.dtype);
-    const unsigned grid = (unsigned)((a.dim + 63) / 64);
+    const unsigned grid = (unsigned)((a.dim + 15) / 16);
     if (a.w_dtype == LSMX_F32)
         norm_dw_kernel<LSMX_F32><<<grid, 1024, 0, s>>>(a.part, groups, a.dim, a.dw);
     else if (a.w_dtype == LSMX_BF16)

@@ -13,10 +13,58 @@ namespace lsmx {
 
 namespace {
 
-LSMX_DEV double shfl_d(double v, int m) {
+// A lane's value from N lanes on, around its 16.
+template <int N>
+LSMX_DEV uint32_t ror16(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + N, 0xF, 0xF, true);
+}
+template <int N>
+LSMX_DEV double ror16(double v) {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)u, m, 64), hi = (uint32_t)__shfl_xor((int)(uint32_t)(u >> 32), m, 64);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+    return __builtin_bit_cast(double, (uint64_t)ror16<N>((uint32_t)(u >> 32)) << 32 | ror16<N>((uint32_t)u));
+}
+// max over 16 lanes, in all of them
+LSMX_DEV uint32_t max16(uint32_t v) {
+    v = max(v, ror16<1>(v));
+    v = max(v, ror16<2>(v));
+    v = max(v, ror16<4>(v));
+    return max(v, ror16<8>(v));
+}
+LSMX_DEV float sum16(float v) {
+    v += u2f(ror16<1>(f2u(v)));
+    v += u2f(ror16<2>(f2u(v)));
+    v += u2f(ror16<4>(f2u(v)));
+    return v + u2f(ror16<8>(f2u(v)));
+}
+LSMX_DEV uint32_t lane_of(uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); }
+LSMX_DEV double lane_of(double v, int l) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)lane_of((uint32_t)(u >> 32), l) << 32 | lane_of((uint32_t)u, l));
+}
+LSMX_DEV uint32_t wave_max(uint32_t v) {
+    v = max16(v);
+    return max(max(lane_of(v, 0), lane_of(v, 16)), max(lane_of(v, 32), lane_of(v, 48)));
+}
+LSMX_DEV double wave_sum(double v) {
+    v += ror16<1>(v);
+    v += ror16<2>(v);
+    v += ror16<4>(v);
+    v += ror16<8>(v);
+    return lane_of(v, 0) + lane_of(v, 16) + (lane_of(v, 32) + lane_of(v, 48));
+}
+LSMX_DEV double wave_max(double v) {   // of numbers
+    auto up = [](double p, double q) { return q > p ? q : p; };
+    v = up(v, ror16<1>(v));
+    v = up(v, ror16<2>(v));
+    v = up(v, ror16<4>(v));
+    v = up(v, ror16<8>(v));
+    return up(up(lane_of(v, 0), lane_of(v, 16)), up(lane_of(v, 32), lane_of(v, 48)));
+}
+// order of the numbers as unsigned words: -0 is 0, a NaN above all; 0 is below all
+LSMX_DEV uint64_t ordered(double f) {
+    if (f != f) return ~0ull;
+    const uint64_t u = __builtin_bit_cast(uint64_t, f + 0.0);
+    return u ^ ((uint64_t)((int64_t)u >> 63) | 1ull << 63);
 }
 
 // The order in which values are chosen: a NaN before all, then the larger, of
@@ -33,11 +81,10 @@ LSMX_DEV double logit(const RouteArgs &a, int64_t row, int e) {
     return (double)Elem<DT>::load(((const typename Elem<DT>::S *)a.logits)[row * a.ld + e]);
 }
 
-// Scores of a row, NPL a lane (expert lane + 64 j); beyond the last: -inf in
-// `l` and 0 in `s`.  A row of nothing but -inf scores 0 throughout.
+// Logits l and scores s of a row, NPL a lane (expert lane + 64 j); beyond the
+// last: -inf and 0.  A row of nothing but -inf scores 0 throughout.
 template <int DT, int NPL>
-LSMX_DEV void scores(const RouteArgs &a, int64_t row, int lane, double (&s)[NPL]) {
-    double l[NPL];
+LSMX_DEV void scores(const RouteArgs &a, int64_t row, int lane, double (&l)[NPL], double (&s)[NPL]) {
 #pragma unroll
     for (int j = 0; j < NPL; ++j) l[j] = lane + 64 * j < a.experts ? logit<DT>(a, row, lane + 64 * j) : -__builtin_inf();
     if (a.sigmoid) {
@@ -45,58 +92,49 @@ LSMX_DEV void scores(const RouteArgs &a, int64_t row, int lane, double (&s)[NPL]
         for (int j = 0; j < NPL; ++j) s[j] = 1.0 / (1.0 + exp(-l[j]));
         return;
     }
-    double m = -__builtin_inf();
-    bool nan = false;
+    double m = -__builtin_inf(), t = 0.0;
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) m = l[j] > m ? l[j] : m, nan |= l[j] != l[j];
+    for (int j = 0; j < NPL; ++j) m = l[j] > m ? l[j] : m;
+    m = wave_max(m);
 #pragma unroll
-    for (int x = 1; x < 64; x *= 2) {
-        const double o = shfl_d(m, x);
-        m = o > m ? o : m;
-    }
-    double t = 0.0;
-#pragma unroll
-    for (int j = 0; j < NPL; ++j) s[j] = m == -__builtin_inf() && !nan ? 0.0 : exp(l[j] - m), t += s[j];
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) t += shfl_d(t, x);
+    for (int j = 0; j < NPL; ++j) s[j] = l[j] == -__builtin_inf() ? 0.0 : exp(l[j] - m), t += s[j];
+    t = wave_sum(t);
 #pragma unroll
     for (int j = 0; j < NPL; ++j) s[j] = t == 0.0 ? 0.0 : s[j] / t;
 }
 
+// The row by a whole wave, in 64 bits throughout; row_of_c: `experts` doubles of
+// LDS of its own, where there are groups.  Without a bias experts rank by
+// their logits, the order of the scores.
 template <int DT, int NPL>
-__global__ __launch_bounds__(256) void route_fwd_kernel(RouteArgs a) {
-    extern __shared__ double lds[];  // a wave's row of c, where there are groups
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row = (int64_t)blockIdx.x * 4 + wave;
-    if (row >= a.rows) return;  // no barrier below: a wave works alone
+LSMX_DEV void exact_row(const RouteArgs &a, int64_t row, int lane, double *row_of_c) {
     float *wo = a.weights + row * a.k;
     int32_t *io = a.ids + row * a.k;
     if (a.mask && !a.mask[row]) {
         if (lane < a.k) wo[lane] = 0.f, io[lane] = -1;
         return;
     }
-    double s[NPL], c[NPL];
-    bool live[NPL];
-    scores<DT, NPL>(a, row, lane, s);
+    double l[NPL], s[NPL];
+    uint64_t key[NPL];
+    scores<DT, NPL>(a, row, lane, l, s);
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
         const int e = lane + 64 * j;
-        live[j] = e < a.experts;
-        c[j] = a.bias && live[j] ? s[j] + (double)a.bias[e] : s[j];
+        if (a.bias && e < a.experts) l[j] = s[j] + (double)a.bias[e];
+        key[j] = e < a.experts ? ordered(l[j]) : 0;
     }
     if (a.top_groups < a.groups) {
-        double *mine = lds + wave * a.experts;
 #pragma unroll
         for (int j = 0; j < NPL; ++j)
-            if (live[j]) mine[lane + 64 * j] = c[j];
+            if (key[j]) row_of_c[lane + 64 * j] = a.bias ? l[j] : s[j];
         __builtin_amdgcn_wave_barrier();
         const int size = a.experts / a.groups;
         // lane g scores group g (groups <= 64)
         double score = 0.0;
         if (lane < a.groups) {
-            double u = mine[lane * size], v = -__builtin_inf();
+            double u = row_of_c[lane * size], v = -__builtin_inf();
             for (int i = 1; i < size; ++i) {
-                const double x = mine[lane * size + i];
+                const double x = row_of_c[lane * size + i];
                 if (before(x, 0, u, 1))
                     v = u, u = x;
                 else if (before(x, 0, v, 1))
@@ -106,42 +144,323 @@ __global__ __launch_bounds__(256) void route_fwd_kernel(RouteArgs a) {
         }
         // a group stays when fewer than top_groups are before it
         int ahead = 0;
-        for (int g = 0; g < a.groups; ++g) {
-            const uint64_t u = __builtin_bit_cast(uint64_t, score);
-            const double o = __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(u >> 32), g) << 32 |
-                                                            (uint32_t)__builtin_amdgcn_readlane((uint32_t)u, g));
-            ahead += g != lane && before(o, g, score, lane);
-        }
+        for (int g = 0; g < a.groups; ++g) ahead += g != lane && before(lane_of(score, g), g, score, lane);
         const uint64_t stay = __builtin_amdgcn_ballot_w64(lane < a.groups && ahead < a.top_groups);
 #pragma unroll
         for (int j = 0; j < NPL; ++j)
-            if (live[j]) live[j] = (stay >> ((lane + 64 * j) / size)) & 1;
+            if (!((stay >> (min(lane + 64 * j, a.experts - 1) / size)) & 1)) key[j] = 0;
+        __builtin_amdgcn_wave_barrier();
     }
     float w = 0.f, total = 0.f;
     for (int j = 0; j < a.k; ++j) {
         // the first of this lane's, then of all lanes'
-        double best = -__builtin_inf(), sc = 0.0;
-        int at = 0x7FFFFFFF;
+        uint64_t best = 0;
+        int at = 0;
 #pragma unroll
         for (int i = 0; i < NPL; ++i)
-            if (live[i] && (at == 0x7FFFFFFF || before(c[i], lane + 64 * i, best, at))) best = c[i], at = lane + 64 * i, sc = s[i];
-        int first = at;
-        double fb = best;
+            if (key[i] > best) best = key[i], at = lane + 64 * i;
+        const uint32_t hi = wave_max((uint32_t)(best >> 32)), lo = wave_max((uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
+        const bool mine = best == ((uint64_t)hi << 32 | lo);
+        const int first = 0xFFFF - (int)wave_max(mine ? 0xFFFFu - (uint32_t)at : 0u);
+        float f = 0.f;
 #pragma unroll
-        for (int x = 1; x < 64; x *= 2) {
-            const double ob = shfl_d(fb, x);
-            const int oa = __shfl_xor(first, x, 64);
-            if (oa != 0x7FFFFFFF && (first == 0x7FFFFFFF || before(ob, oa, fb, first))) fb = ob, first = oa;
+        for (int i = 0; i < NPL; ++i) {
+            if (i == first >> 6) f = (float)s[i];
+            if (lane + 64 * i == first) key[i] = 0;
         }
-        const int from = first & 63;
-        const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, (float)sc), __builtin_amdgcn_readfirstlane(from)));
+        f = u2f(lane_of(f2u(f), first & 63));
         if (lane == j) w = f, io[j] = first;
         total += f;
-#pragma unroll
-        for (int i = 0; i < NPL; ++i)
-            if (lane + 64 * i == first) live[i] = false;
     }
     if (lane < a.k) wo[lane] = a.renorm ? (total == 0.f ? 0.f : a.scale * (w / total)) : a.scale * w;
+}
+
+template <int DT, int NPL>
+__global__ __launch_bounds__(256) void route_fwd_kernel(RouteArgs a) {
+    extern __shared__ double lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+    if (row >= a.rows) return;  // no barrier below: a wave works alone
+    exact_row<DT, NPL>(a, row, lane, lds + wave * a.experts);
+}
+
+// ---------------------------------------------------------- 16 lanes a row
+// Up to 256 experts and 16 choices: four rows a wave, V experts a lane (expert
+// lane * v + j, v = ceil(experts / 16)).  Ranks are kept as words that order
+// like the numbers, the index within the lane in the low bits; each lane sorts
+// its own once, and a choice is then a maximum over 16 heads.
+//
+// Without a bias experts rank by their logits: 16-bit logits leave room for the
+// whole index, and words never tie.  Otherwise ranks are fp32 within 2^-20 of
+// the score's size (two roundings of exp, one of the sum and the quotient), 4
+// low bits lost: together within 4e-6 (1 + |c|).  Where two neighbours of the
+// choice, or two groups, are too near to be told apart, the wave takes that row
+// again in 64 bits.
+
+// order of the numbers as unsigned words; 0 is below all
+LSMX_DEV uint32_t ordered(float f) {
+    const uint32_t u = f2u(f + 0.f);   // -0 as 0
+    return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+}
+LSMX_DEV float unordered(uint32_t u) { return u2f(u & 0x80000000u ? u ^ 0x80000000u : ~u); }
+
+// descending, by merging (V a power of two)
+template <int V>
+LSMX_DEV void sort_down(uint32_t (&k)[V]) {
+#pragma unroll
+    for (int p = 1; p < V; p *= 2)
+#pragma unroll
+        for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+            for (int j = q % p; j + q < V; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; ++i)
+                    if (i + j + q < V && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+                        const uint32_t x = max(k[i + j], k[i + j + q]), y = min(k[i + j], k[i + j + q]);
+                        k[i + j] = x, k[i + j + q] = y;
+                    }
+}
+
+// a lane's logits: v of them from expert lane * v on, -inf past the last
+template <int DT, int V>
+LSMX_DEV void lane_logits(const RouteArgs &a, int64_t row, int l16, int v, bool vec, float (&l)[V]) {
+    typedef typename Elem<DT>::S S;
+    const S *p = (const S *)a.logits + row * a.ld + l16 * v;
+    constexpr int N = 16 / (int)sizeof(S) < V ? 16 / (int)sizeof(S) : V;
+    typedef S W __attribute__((ext_vector_type(N)));
+    if (vec) {
+#pragma unroll
+        for (int j = 0; j < V; j += N) {
+            const W w = *(const W *)(p + j);
+#pragma unroll
+            for (int i = 0; i < N; ++i) l[j + i] = Elem<DT>::load(w[i]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) l[j] = Elem<DT>::load(p[min(j, a.experts - 1 - l16 * v)]);   // every lane loads something
+#pragma unroll
+        for (int j = 0; j < V; ++j) l[j] = j < v && l16 * v + j < a.experts ? l[j] : -__builtin_inff();
+    }
+}
+// full vectors in every lane, aligned
+template <int DT, int V>
+LSMX_DEV bool whole_vectors(const RouteArgs &a, int v) {
+    constexpr int N = (16 / (int)sizeof(typename Elem<DT>::S) < V ? 16 : V * (int)sizeof(typename Elem<DT>::S));
+    return v == V && a.experts == 16 * V && (uintptr_t)a.logits % N == 0 && a.ld * (int)sizeof(typename Elem<DT>::S) % N == 0;
+}
+
+// within 2^-22 of 1
+LSMX_DEV float sigmoid(float l) { return __builtin_amdgcn_rcpf(1.f + __expf(-l)); }
+
+template <int DT, int V>
+__global__ __launch_bounds__(256) void route_fwd16_kernel(RouteArgs a) {
+    extern __shared__ double lds[];   // a row of c for each wave, where there are groups
+    __shared__ int chosen[16][16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, r = threadIdx.x >> 4;
+    const int64_t row0 = (int64_t)blockIdx.x * 16 + wave * 4, row = row0 + (lane >> 4);
+    if (row0 >= a.rows) return;   // no barrier below: a wave works alone
+    const bool live = row < a.rows;
+    const int64_t at = live ? row : a.rows - 1;
+    const int v = (a.experts + 15) / 16;
+    float l[V], c[V];
+    lane_logits<DT, V>(a, at, l16, v, whole_vectors<DT, V>(a, v), l);
+    const bool grouped = a.top_groups < a.groups, scored = a.bias != nullptr;
+    // the row's largest logit, and whether 64 bits have to look at it
+    uint32_t top = 0;
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < V; ++j) top = max(top, ordered(l[j])), odd |= !(l[j] < __builtin_inff());
+    top = max16(top);
+    const float m = unordered(top);
+    // the sum of a softmax, where something needs it
+    float inv = 1.f;
+    const bool summed = !a.sigmoid && (scored || grouped || !a.renorm);
+    if (summed) {
+        float t = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) t += m == -__builtin_inff() ? 0.f : __expf(l[j] - m);
+        t = sum16(t);
+        inv = t > 0.f ? 1.f / t : 0.f;
+    }
+    auto score = [&](float x) __attribute__((always_inline)) {
+        return a.sigmoid ? sigmoid(x) : x == -__builtin_inff() ? 0.f : __expf(x - m) * inv;
+    };
+    // ranks as words
+    const bool whole = DT != LSMX_F32 && !scored;   // with the whole index
+    const uint32_t low = whole ? (DT == LSMX_BF16 ? 0xFFFFu : 0x1FFFu) : 15u;
+    uint32_t k[V];
+    if (scored) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) c[j] = a.bias[min(l16 * v + j, a.experts - 1)];
+#pragma unroll
+        for (int j = 0; j < V; ++j) c[j] += score(l[j]), odd |= !(c[j] < __builtin_inff());
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) c[j] = l[j];
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int e = l16 * v + j;
+        const uint32_t in = j < v && e < a.experts ? ~0u : 0u;
+        k[j] = ((ordered(c[j]) & ~low) | (low - (whole ? e : j))) & in;
+    }
+    sort_down<V>(k);
+    bool near = false;
+    if (grouped) {
+        // 16 / groups lanes a group: its two largest from their lanes' two
+        uint32_t u = k[0], w = V > 1 ? k[1] : 0u;
+        const int per = 16 / a.groups, by = 31 - __builtin_clz(per);
+        auto merge = [&](uint32_t ou, uint32_t ow) __attribute__((always_inline)) {
+            w = max(min(u, ou), max(w, ow));
+            u = max(u, ou);
+        };
+        if (per > 1) merge(__shfl_xor((int)u, 1, 64), __shfl_xor((int)w, 1, 64));
+        if (per > 2) merge(__shfl_xor((int)u, 2, 64), __shfl_xor((int)w, 2, 64));
+        if (per > 4) merge(__shfl_xor((int)u, 4, 64), __shfl_xor((int)w, 4, 64));
+        const float fu = unordered(u & ~low), fw = unordered(w & ~low);
+        const bool two = a.experts > a.groups;   // else a group's one is its score
+        const float s = scored ? fu + (two ? fw : 0.f) : score(fu) + (two ? score(fw) : 0.f);
+        // groups surely and perhaps ahead of this lane's, each counted by its lanes
+        int ahead = 0, perhaps = 0;
+        const int mine = l16 >> by;
+        const float tol = 2e-5f * (1.f + __builtin_fabsf(s));
+        auto look = [&](int o16, float o) __attribute__((always_inline)) {
+            const bool other = (o16 & 15) >> by != mine;
+            ahead += other && o > s + tol;
+            perhaps += other && !(o < s - tol);
+        };
+#define LOOK(n) look(l16 - n, u2f(ror16<n>(f2u(s))))
+        LOOK(1), LOOK(2), LOOK(3), LOOK(4), LOOK(5), LOOK(6), LOOK(7), LOOK(8), LOOK(9), LOOK(10), LOOK(11), LOOK(12), LOOK(13),
+            LOOK(14), LOOK(15);
+#undef LOOK
+        const bool out = ahead >> by >= a.top_groups;
+        near = !out && perhaps >> by >= a.top_groups;
+        if (out) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) k[j] = 0;
+        }
+    }
+    uint32_t last = 0;
+    const int rounds = whole ? a.k : a.k + 1;   // one more to see whether the last choice is sure
+    for (int j = 0; j < rounds; ++j) {
+        const uint32_t best = max16(k[0]);
+        const bool win = k[0] == best;
+        if (win && j < a.k) chosen[r][j] = whole ? (int)(low - (best & low)) : l16 * v + (int)(low - (best & low));
+        if (!whole && best != 0) {
+            const uint32_t wins = (uint32_t)(__builtin_amdgcn_ballot_w64(win) >> (lane & 48)) & 0xFFFFu;
+            near |= (wins & (wins - 1)) != 0;
+            if (j > 0) {
+                const float p = unordered(last & ~low), q = unordered(best & ~low);
+                near |= scored ? !(p - q > 5e-6f * (1.f + __builtin_fabsf(p))) : (last & ~low) == (best & ~low);
+            }
+        }
+        last = best;
+        const uint32_t up = win ? ~0u : 0u;
+#pragma unroll
+        for (int i = 0; i + 1 < V; ++i) k[i] = (k[i + 1] & up) | (k[i] & ~up);
+        k[V - 1] &= ~up;
+    }
+    __builtin_amdgcn_wave_barrier();
+    const bool masked = live && a.mask && !a.mask[row];
+    const int id = l16 < a.k ? chosen[r][l16] : 0;
+    // the chosen's scores, with the whole precision of exp
+    auto exact = [&](float x) __attribute__((always_inline)) {
+        return a.sigmoid ? 1.f / (1.f + expf(-x)) : x == -__builtin_inff() ? 0.f : expf(x - m) * inv;
+    };
+    float f = 0.f;
+    if (l16 < a.k) f = exact(Elem<DT>::load(((const typename Elem<DT>::S *)a.logits)[at * a.ld + min((uint32_t)id, (uint32_t)(a.experts - 1))]));
+    const float total = sum16(f);
+    const float weight = a.renorm ? (total == 0.f ? 0.f : a.scale * (f / total)) : a.scale * f;
+    uint64_t again = __builtin_amdgcn_ballot_w64(live && !masked && (odd || near));
+    if (live && l16 < a.k && !(again >> (lane & 48) & 0xFFFF)) {
+        a.weights[row * a.k + l16] = masked ? 0.f : weight;
+        a.ids[row * a.k + l16] = masked ? -1 : id;
+    }
+    while (again) {   // a row at a time
+        const int which = __builtin_ctzll(again) >> 4;
+        exact_row<DT, (V + 3) / 4>(a, row0 + which, lane, lds + wave * a.experts);
+        again &= ~(0xFFFFull << (16 * which));
+    }
+}
+
+// The gradient with 16 lanes a row, in fp32.
+template <int DT, int V>
+__global__ __launch_bounds__(256) void route_bwd16_kernel(RouteArgs a) {
+    typedef typename Elem<DT>::S S;
+    __shared__ float g_of[16][16 * V];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, r = threadIdx.x >> 4;
+    const int64_t row0 = (int64_t)blockIdx.x * 16 + wave * 4, row = row0 + (lane >> 4);
+    if (row0 >= a.rows) return;   // no barrier below: a wave works alone
+    const bool live = row < a.rows;
+    const int64_t at = live ? row : a.rows - 1;
+    const int v = (a.experts + 15) / 16;
+    const bool vec = whole_vectors<DT, V>(a, v);
+    const int id = l16 < a.k ? a.ids[at * a.k + l16] : -1;
+    const float dw = l16 < a.k ? a.dw[at * a.k + l16] : 0.f;
+    const bool there = (uint32_t)id < (uint32_t)a.experts;
+    float l[V];
+    lane_logits<DT, V>(a, at, l16, v, vec, l);
+#pragma unroll
+    for (int j = 0; j < V; ++j) g_of[r][l16 * V + j] = 0.f;
+    float m = -__builtin_inff(), inv = 1.f;
+    if (!a.sigmoid) {
+        // a NaN stays one in the sum below
+#pragma unroll
+        for (int j = 0; j < V; ++j) m = fmaxf(m, l[j]);
+        m = fmaxf(m, u2f(ror16<1>(f2u(m))));
+        m = fmaxf(m, u2f(ror16<2>(f2u(m))));
+        m = fmaxf(m, u2f(ror16<4>(f2u(m))));
+        m = fmaxf(m, u2f(ror16<8>(f2u(m))));
+        float t = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) l[j] = l[j] == -__builtin_inff() ? 0.f : expf(l[j] - m), t += l[j];
+        t = sum16(t);
+        inv = t == 0.f ? 0.f : 1.f / t;
+    }
+    auto score = [&](float x) __attribute__((always_inline)) {
+        return a.sigmoid ? 1.f / (1.f + expf(-x)) : x == -__builtin_inff() ? 0.f : expf(x - m) * inv;
+    };
+    const float own = there ? score(Elem<DT>::load(((const S *)a.logits)[at * a.ld + id])) : 0.f;
+    float g = a.scale * dw;
+    if (a.renorm) {
+        const float total = sum16(own), da = sum16(dw * own);
+        g = total == 0.f ? 0.f : a.scale * (dw - da / total) / total;
+    }
+    if (!there) g = 0.f;
+    const float mean = sum16(g * own);
+    __builtin_amdgcn_wave_barrier();
+    if (there) g_of[r][id / v * V + id % v] = g;
+    __builtin_amdgcn_wave_barrier();
+    const bool any = (__builtin_amdgcn_ballot_w64(there) >> (lane & 48)) & 0xFFFF;   // a masked row has no gradient
+    float d[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float x = g_of[r][l16 * V + j];
+        if (a.sigmoid) {
+            const float s = score(l[j]);
+            d[j] = x == 0.f ? 0.f : x * s * (1.f - s);
+        } else {
+            d[j] = l[j] * inv * (x - mean);
+        }
+        if (!any) d[j] = 0.f;
+    }
+    if (!live) return;
+    S *out = (S *)a.dlogits + row * a.experts + l16 * v;
+    constexpr int N = 16 / (int)sizeof(S) < V ? 16 / (int)sizeof(S) : V;
+    typedef S W __attribute__((ext_vector_type(N)));
+    if (vec && (uintptr_t)a.dlogits % 16 == 0) {
+#pragma unroll
+        for (int j = 0; j < V; j += N) {
+            W w;
+#pragma unroll
+            for (int i = 0; i < N; ++i) w[i] = Elem<DT>::store(d[j + i]);
+            *(W *)(out + j) = w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j < v && l16 * v + j < a.experts) out[j] = Elem<DT>::store(d[j]);
+    }
 }
 
 template <int DT, int NPL>
@@ -151,8 +470,8 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(RouteArgs a) {
     const int64_t row = (int64_t)blockIdx.x * 4 + wave;
     if (row >= a.rows) return;
     S *out = (S *)a.dlogits + row * a.experts;
-    double s[NPL], d[NPL];
-    scores<DT, NPL>(a, row, lane, s);
+    double l[NPL], s[NPL], d[NPL];
+    scores<DT, NPL>(a, row, lane, l, s);
     const int id = lane < a.k ? a.ids[row * a.k + lane] : -1;
     const double dw = lane < a.k ? (double)a.dw[row * a.k + lane] : 0.0;
     // a lane's chosen score, then the sums over the chosen
@@ -164,27 +483,19 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(RouteArgs a) {
 #pragma unroll
         for (int i = 0; i < NPL; ++i)
             if (i == e / 64) v = s[i];
-        const uint64_t u = __builtin_bit_cast(uint64_t, v);
-        v = __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(u >> 32), e & 63) << 32 |
-                                           (uint32_t)__builtin_amdgcn_readlane((uint32_t)u, e & 63));
+        v = lane_of(v, e & 63);
         if (lane == j) own = v;
     }
-    double total = own, da = dw * own;
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) total += shfl_d(total, x), da += shfl_d(da, x);
+    const double total = wave_sum(own), da = wave_sum(dw * own);
     double g = a.scale * dw;   // gradient of a lane's chosen score
     if (a.renorm) g = total == 0.0 ? 0.0 : a.scale * (dw - da / total) / total;
     if (id < 0) g = 0.0;
-    double mean = g * own;
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) mean += shfl_d(mean, x);
+    const double mean = wave_sum(g * own);
 #pragma unroll
     for (int i = 0; i < NPL; ++i) d[i] = 0.0;
     for (int j = 0; j < a.k; ++j) {
         const int e = __builtin_amdgcn_readlane(id, j);
-        const uint64_t u = __builtin_bit_cast(uint64_t, g);
-        const double v = __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(u >> 32), j) << 32 |
-                                                        (uint32_t)__builtin_amdgcn_readlane((uint32_t)u, j));
+        const double v = lane_of(g, j);
 #pragma unroll
         for (int i = 0; i < NPL; ++i)
             if (e == lane + 64 * i) d[i] = v;
@@ -198,10 +509,30 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(RouteArgs a) {
         }
 }
 
+// What 16 lanes a row take: their experts in registers, the groups as whole
+// lanes.
+bool in16(const RouteArgs &a) {
+    return a.experts <= 256 && a.k <= 16 && (a.top_groups == a.groups || (a.experts % 16 == 0 && 16 % a.groups == 0));
+}
+
 template <int DT>
 hipError_t fwd_of(const RouteArgs &a, hipStream_t s) {
-    const unsigned grid = (unsigned)((a.rows + 3) / 4);
     const size_t lds = a.top_groups < a.groups ? (size_t)a.experts * 4 * sizeof(double) : 0;
+    if (in16(a)) {
+        const unsigned grid = (unsigned)((a.rows + 15) / 16);
+        if (a.experts <= 16)
+            route_fwd16_kernel<DT, 1><<<grid, 256, lds, s>>>(a);
+        else if (a.experts <= 32)
+            route_fwd16_kernel<DT, 2><<<grid, 256, lds, s>>>(a);
+        else if (a.experts <= 64)
+            route_fwd16_kernel<DT, 4><<<grid, 256, lds, s>>>(a);
+        else if (a.experts <= 128)
+            route_fwd16_kernel<DT, 8><<<grid, 256, lds, s>>>(a);
+        else
+            route_fwd16_kernel<DT, 16><<<grid, 256, lds, s>>>(a);
+        return hipGetLastError();
+    }
+    const unsigned grid = (unsigned)((a.rows + 3) / 4);
     if (a.experts <= 64)
         route_fwd_kernel<DT, 1><<<grid, 256, lds, s>>>(a);
     else if (a.experts <= 128)
@@ -216,6 +547,20 @@ hipError_t fwd_of(const RouteArgs &a, hipStream_t s) {
 }
 template <int DT>
 hipError_t bwd_of(const RouteArgs &a, hipStream_t s) {
+    if (a.experts <= 256 && a.k <= 16) {
+        const unsigned grid = (unsigned)((a.rows + 15) / 16);
+        if (a.experts <= 16)
+            route_bwd16_kernel<DT, 1><<<grid, 256, 0, s>>>(a);
+        else if (a.experts <= 32)
+            route_bwd16_kernel<DT, 2><<<grid, 256, 0, s>>>(a);
+        else if (a.experts <= 64)
+            route_bwd16_kernel<DT, 4><<<grid, 256, 0, s>>>(a);
+        else if (a.experts <= 128)
+            route_bwd16_kernel<DT, 8><<<grid, 256, 0, s>>>(a);
+        else
+            route_bwd16_kernel<DT, 16><<<grid, 256, 0, s>>>(a);
+        return hipGetLastError();
+    }
     const unsigned grid = (unsigned)((a.rows + 3) / 4);
     if (a.experts <= 64)
         route_bwd_kernel<DT, 1><<<grid, 256, 0, s>>>(a);

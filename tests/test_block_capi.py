@@ -171,10 +171,10 @@ def test_arguments_are_refused_on_the_gpu(dev):
             norm.add_rms_norm(**{"x": x, "weight": w, **bad})
     with pytest.raises(ValueError, match="eps"):
         norm.add_rms_norm(x, w, eps=-1)
-    with pytest.raises(RuntimeError, match="once_differentiable|twice|does not require grad"):
+    with pytest.raises(RuntimeError, match="twice|does not require grad"):
         a = x.clone().requires_grad_(True)
         g, = torch.autograd.grad(norm.add_rms_norm(a, w).sum(), a, create_graph=True)
-        torch.autograd.grad(g.sum(), a)
+        g.sum().backward()
     for bad in (dict(k=0), dict(k=65), dict(groups=3), dict(groups=4, top_groups=5), dict(k=17, groups=4), dict(scale=0), dict(scale=float("inf"))):
         with pytest.raises(ValueError):
             experts.route(x, **{"k": 2, **bad})
