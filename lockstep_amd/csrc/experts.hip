@@ -462,7 +462,6 @@ template <bool GATED>
 hipError_t products(const ExpertArgs &a, hipStream_t s) {
     if (a.K < 512) return stream<GATED, 1, 8>(a, s);
     const int64_t per = a.pairs / a.experts;
-    }
     return per <= 8 ? stream<GATED, 1, 8>(a, s) : per <= 32 ? stream<GATED, 4, 4>(a, s) : per <= 256 ? tiles<GATED, 128>(a, s) : tiles<GATED, 256>(a, s);
 }
 
