@@ -1149,6 +1149,9 @@ static int expert_args(const char *fn, const lsmx_experts *a, bool gated, lsmx::
     if (a->N < 1 || a->N >= (int64_t)1 << 24 || a->N * a->K / 2 >= (int64_t)1 << 31)
         return fail(LSMX_ERR_SHAPE, "%s: N=%lld: an expert's weights must stay below 2^31 bytes", fn, (long long)a->N);
     if (gated && a->N % 64) return fail(LSMX_ERR_SHAPE, "%s: N=%lld must be a multiple of 64 (F of 32)", fn, (long long)a->N);
+    // workgroups of the smallest tiles
+    if ((a->tokens * a->k / 16 + a->experts + 2) * (a->N / 64 + 1) >= (int64_t)1 << 31 || a->tokens * (a->N / 2048 + 1) >= (int64_t)1 << 31)
+        return fail(LSMX_ERR_SHAPE, "%s: too many pairs times rows", fn);
     if (a->tokens && (!a->x || !a->x_scale || !a->w || !a->w_scale || !a->ids || !a->order || !a->offsets))
         return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
     if (!aligned(a->x, 16) || !aligned(a->w, 16) || !aligned(a->x_scale, 4) || !aligned(a->w_scale, 4) || !aligned(a->ids, 4) ||
@@ -1159,7 +1162,7 @@ static int expert_args(const char *fn, const lsmx_experts *a, bool gated, lsmx::
     out->ids = a->ids, out->order = a->order, out->offsets = a->offsets;
     out->pairs = (int)(a->tokens * a->k), out->k = (int)a->k, out->experts = (int)a->experts;
     out->N = (int)a->N, out->K = (int)a->K, out->tokens = a->tokens;
-    out->ldz = (a->N + 3) / 4 * 4;
+    out->ldz = (a->N + 7) / 8 * 8;
     return LSMX_OK;
 }
 

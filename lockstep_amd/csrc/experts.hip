@@ -9,7 +9,14 @@
 // that a lane's four results are four rows of W for one pair.  Lane (i, g),
 // g = lane / 16, supplies A's K 32g .. 32g+31 of row i, B's K 16g .. 16g+15
 // and 64+16g .. of pair i, and block g's scales; its results are W's rows
-// 4g .. 4g+3 for pair i.
+// 4g .. 4g+3 for pair i (checked on the device against the products).
+//
+// The instruction adds eight products at a time, keeping 13 bits below the
+// largest exponent among them; beyond those eight its sums are fp32.  E4M3 spans
+// more than that: rows with both large and small codes lose 4e-6 of a result
+// (rms, normal values).  The forms that wait for memory take each row's codes of
+// 2 and more and those below in two instructions, which is exact; the form for
+// many rows, bound by the matrix cores, does not (twice its time).
 //
 // Pairs come sorted by expert (order, offsets); a workgroup finds the expert
 // and the pairs of its tile from the offsets.  Nothing in order or offsets is
@@ -23,18 +30,43 @@ namespace lsmx {
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 
 __device__ v4f mfma_f4f8(v4i a, v8i b, v4f c, int cbsz, int blgp, int opsel_a, int scale_a, int opsel_b, int scale_b)
     __asm("llvm.amdgcn.mfma.scale.f32.16x16x128.f8f6f4.v4i32.v8i32");
 
 namespace {
 
+// The codes of magnitude 2 and more (bit 6 of a byte), the others 0.
+LSMX_DEV v8i large_codes(v8i x) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t b = (uint32_t)x[i] & 0x40404040u;
+        x[i] &= (int)((b << 2) - (b >> 6));
+    }
+    return x;
+}
+
+// ---------------------------------------------------------------- the tiles
 // What a workgroup does: block `block` of W's rows for the pairs
 // order[start .. start + n), all of expert `expert`, or of no expert where that
 // is `experts`.  n = 0: nothing.
 struct Tile {
     int expert, start, n, block;
 };
+
+LSMX_DEV int lane_of(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+
+// Sums of a wave's lanes up to each.
+LSMX_DEV int scan64(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast 15, 31
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
 
 // Every expert's pairs in tiles of `height`, then those of the pairs of no
 // expert, each tile `blocks` times; an expert's tiles of one block are
@@ -44,52 +76,66 @@ struct Tile {
 LSMX_DEV Tile find_tile(const int32_t *offsets, int experts, int pairs, int height, int blocks) {
     const int lane = threadIdx.x & 63;
     const int per = (experts + 64) / 64;   // of experts + 1 entries
-    // lane's entries: first .. first + per - 1
-    const int first = lane * per;
-    auto at = [&](int e) __attribute__((always_inline)) { return e > experts ? pairs : min(max(offsets[e], 0), pairs); };
-    int mine = 0, lo = at(min(first, experts + 1));
+    const int first = lane * per;          // a lane's: first .. first + per - 1
+    auto at = [&](int e) __attribute__((always_inline)) {
+        const int v = offsets[min(e, experts)];
+        return e > experts ? pairs : min(max(v, 0), pairs);
+    };
+    const int begin = at(first);
+    int mine = 0, lo = begin, n0 = 0;
     for (int i = 0; i < per; ++i) {
-        const int hi = at(min(first + i + 1, experts + 1));
-        if (first + i <= experts) mine += (max(hi - lo, 0) + height - 1) / height;
+        const int hi = at(first + i + 1), n = first + i <= experts ? max(hi - lo, 0) : 0;
+        mine += (n + height - 1) / height;
+        n0 = n;
         lo = hi;
     }
-    int inc = mine;
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-        const int o = __shfl_up(inc, m, 64);
-        if (lane >= m) inc += o;
-    }
-    const int all = __builtin_amdgcn_readlane(inc, 63) * blocks, chunk = (all + 7) / 8;
+    const int inc = scan64(mine), all = lane_of(inc, 63) * blocks, chunk = (all + 7) / 8;
     const int unit = (int)(blockIdx.x & 7) * chunk + (int)(blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= chunk || unit >= all) return Tile{0, 0, 0, 0};
     const int owner = __builtin_ctzll(__builtin_amdgcn_ballot_w64(inc * blocks > unit));
-    int left = unit - (__builtin_amdgcn_readlane(inc, owner) - __builtin_amdgcn_readlane(mine, owner)) * blocks;
-    int e = owner * per;
-    for (int i = 0; i < per; ++i, ++e) {
-        const int lo2 = at(e), n = max(at(e + 1) - lo2, 0), tiles = (n + height - 1) / height;
-        if (left < tiles * blocks) {
-            const int m = left % tiles;
-            return Tile{e, lo2 + m * height, min(n - m * height, height), left / tiles};
+    int left = unit - (lane_of(inc, owner) - lane_of(mine, owner)) * blocks;
+    int e = owner * per, start = lane_of(begin, owner), n = lane_of(n0, owner);
+    if (per > 1) {
+        for (int i = 0; i < per; ++i, ++e) {
+            start = __builtin_amdgcn_readfirstlane(at(e));
+            n = max(__builtin_amdgcn_readfirstlane(at(e + 1)) - start, 0);
+            const int units = (n + height - 1) / height * blocks;
+            if (left < units) break;
+            left -= units;
         }
-        left -= tiles * blocks;
+        if (e >= owner * per + per) return Tile{0, 0, 0, 0};
     }
-    return Tile{0, 0, 0, 0};
+    const int tiles = (n + height - 1) / height;
+    if (tiles == 0) return Tile{0, 0, 0, 0};
+    const int block = left / tiles, m = left - block * tiles;
+    return Tile{e, start + m * height, min(n - m * height, height), block};
 }
 // Workgroups that hold every tile, whatever the offsets.
 int64_t tile_units(int64_t pairs, int64_t experts, int64_t height, int64_t blocks) {
     return ((pairs / height + (experts + 1 < pairs ? experts + 1 : pairs)) * blocks + 7) / 8 * 8;
 }
 
+// The pair of row r of a tile, -1 where there is none.
+LSMX_DEV int pair_at(const ExpertArgs &a, const Tile &tile, int r) {
+    const uint32_t p = (uint32_t)a.order[tile.start + min(r, tile.n - 1)];
+    return r < tile.n && p < (uint32_t)a.pairs ? (int)p : -1;
+}
+// The row of x of a tile's row r (of its last past the end).
+template <bool GATED>
+LSMX_DEV int64_t x_row(const ExpertArgs &a, const Tile &tile, int r) {
+    const uint32_t p = (uint32_t)a.order[tile.start + min(r, tile.n - 1)], q = p < (uint32_t)a.pairs ? p : 0u;
+    return GATED ? q / (uint32_t)a.k : q;
+}
+
 // g sigmoid(g) u.  exp(-g) past the type's range gives the sigmoid's 0 or 1; the
 // reciprocal is within 1 step of fp32.
 LSMX_DEV float silu_times(float g, float u) { return g * __builtin_amdgcn_rcpf(1.f + __expf(-g)) * u; }
 
-// Zeros of scale 1 in elements f0 .. f0 + nf - 1 of the rows of n pairs.
-template <int NT, typename P>
-LSMX_DEV void zero_rows(const ExpertArgs &a, const P &pair_of, int n, int f0, int nf) {
+// Zeros of scale 1 in elements f0 .. f0 + nf - 1 of a tile's rows.
+LSMX_DEV void zero_rows(const ExpertArgs &a, const Tile &tile, int threads, int f0, int nf) {
     const int F = a.N / 2, words = nf / 4, each = words + nf / 32;
-    for (int q = threadIdx.x; q < n * each; q += NT) {
-        const int p = pair_of(q / each), w = q % each;
+    for (int q = threadIdx.x; q < tile.n * each; q += threads) {
+        const int p = pair_at(a, tile, q / each), w = q % each;
         if (p < 0) continue;
         if (w < words)
             *(uint32_t *)(a.h + (int64_t)p * F + f0 + 4 * w) = 0;
@@ -98,30 +144,25 @@ LSMX_DEV void zero_rows(const ExpertArgs &a, const P &pair_of, int n, int f0, in
     }
 }
 
-// ------------------------------------------------------------ few rows
-// A workgroup of KW waves: 64 rows of W (gated: 32 of the gate, the same 32 of
-// up) for up to 16 NT pairs of one expert.  The waves split K, stream the
-// weights from memory into registers and add their sums up in LDS.
-template <bool GATED, int NT, int KW>
-__global__ __launch_bounds__(64 * KW) void expert_stream_kernel(ExpertArgs a) {
-    constexpr int C = 16 * NT;
-    __shared__ __attribute__((aligned(16))) float sum[KW][64][C];
-    __shared__ int pair_of[C];
+// ------------------------------------------------------------ few workgroups
+// 8 waves for 64 rows of W (gated: 32 of the gate, the same 32 of up) and up to
+// 16 pairs of one expert: the waves split K, take the weights from memory
+// straight into registers, two steps of 128 at a time, and add their sums up in
+// LDS.
+template <bool GATED>
+__global__ __launch_bounds__(512) void expert_stream_kernel(ExpertArgs a) {
+    constexpr int KW = 8;
+    __shared__ __attribute__((aligned(16))) float sum[KW][64][16];
+    __shared__ int pair_of[16];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), i16 = lane & 15, g = lane >> 4;
-    const Tile tile = find_tile(a.offsets, a.experts, a.pairs, C, (a.N + 63) / 64);
-    const int nb = tile.block;
+    const Tile tile = find_tile(a.offsets, a.experts, a.pairs, 16, (a.N + 63) / 64);
     if (tile.n == 0) return;
-    if (t < C) {
-        const uint32_t p = t < tile.n ? (uint32_t)a.order[tile.start + t] : 0xFFFFFFFFu;
-        pair_of[t] = p < (uint32_t)a.pairs ? (int)p : -1;
-    }
-    __syncthreads();
-    const int F = a.N / 2;
+    const int nb = tile.block, F = a.N / 2;
     if (tile.expert == a.experts) {   // pairs of no expert: rows of zeros
-        if constexpr (GATED) zero_rows<64 * KW>(a, [&](int r) { return pair_of[r]; }, tile.n, nb * 32, 32);
+        if constexpr (GATED) zero_rows(a, tile, 512, nb * 32, 32);
         return;
     }
-    const int kb = a.K / 32;
+    const int kb = a.K / 32, steps = a.K / 128, s0 = steps * wave / KW, s1 = steps * (wave + 1) / KW;
     // four tiles of 16 rows of W
     const uint8_t *wp[4], *sp[4];
 #pragma unroll
@@ -131,125 +172,106 @@ __global__ __launch_bounds__(64 * KW) void expert_stream_kernel(ExpertArgs a) {
         wp[r] = a.w + n * (a.K / 2) + 16 * g;
         sp[r] = a.ws + n * kb + g;
     }
-    const uint8_t *xp[NT], *xsp[NT];
+    const int64_t row = x_row<GATED>(a, tile, i16);
+    const uint8_t *xp = a.x + row * a.K + 16 * g, *xsp = a.xs + row * kb + g;
+    if (t < 16) pair_of[t] = pair_at(a, tile, t);
+    v4f acc[4];
 #pragma unroll
-    for (int c = 0; c < NT; ++c) {
-        const int p = max(pair_of[c * 16 + i16], 0);
-        const int64_t row = GATED ? p / a.k : p;
-        xp[c] = a.x + row * a.K + 16 * g;
-        xsp[c] = a.xs + row * kb + g;
-    }
-    v4f acc[4][NT];
+    for (int r = 0; r < 4; ++r) acc[r] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int s = s0; s < s1; s += 2) {
+        v4i w[2][4];
+        v8i x[2];
+        int ws[2][4], xs[2];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+        for (int u = 0; u < 2; ++u) {
+            const int64_t q = min(s + u, s1 - 1);
 #pragma unroll
-        for (int c = 0; c < NT; ++c) acc[r][c] = v4f{0.f, 0.f, 0.f, 0.f};
-    const int steps = a.K / 128, s1 = steps * (wave + 1) / KW;
-    for (int s = steps * wave / KW; s < s1; ++s) {
-        v4i w[4];
-        v8i x[NT];
-        int ws[4], xs[NT];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            w[r] = *(const v4i *)(wp[r] + (int64_t)s * 64);
-            ws[r] = sp[r][s * 4];
+            for (int r = 0; r < 4; ++r) {
+                w[u][r] = *(const v4i *)(wp[r] + q * 64);
+                ws[u][r] = sp[r][q * 4];
+            }
+            const v4i lo = *(const v4i *)(xp + q * 128), hi = *(const v4i *)(xp + q * 128 + 64);
+            x[u] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            xs[u] = xsp[q * 4];
         }
 #pragma unroll
-        for (int c = 0; c < NT; ++c) {
-            const v4i lo = *(const v4i *)(xp[c] + (int64_t)s * 128), hi = *(const v4i *)(xp[c] + (int64_t)s * 128 + 64);
-            x[c] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            xs[c] = xsp[c][s * 4];
+        for (int u = 0; u < 2; ++u) {
+            if (s + u >= s1) continue;
+            const v8i big = large_codes(x[u]), small = x[u] ^ big;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[r] = mfma_f4f8(w[u][r], big, acc[r], 4, 0, 0, ws[u][r], 0, xs[u]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[r] = mfma_f4f8(w[u][r], small, acc[r], 4, 0, 0, ws[u][r], 0, xs[u]);
         }
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int c = 0; c < NT; ++c) acc[r][c] = mfma_f4f8(w[r], x[c], acc[r][c], 4, 0, 0, ws[r], 0, xs[c]);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int c = 0; c < NT; ++c)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) sum[wave][r * 16 + 4 * g + q][c * 16 + i16] = acc[r][c][q];
+        for (int q = 0; q < 4; ++q) sum[wave][r * 16 + 4 * g + q][i16] = acc[r][q];
     __syncthreads();
-    auto total = [&](int row, int col) __attribute__((always_inline)) {
-        float v = sum[0][row][col];
+    auto total = [&](int r, int c) __attribute__((always_inline)) {
+        float v = sum[0][r][c];
 #pragma unroll
-        for (int w = 1; w < KW; ++w) v += sum[w][row][col];
+        for (int w = 1; w < KW; ++w) v += sum[w][r][c];
         return v;
     };
     if constexpr (GATED) {
-        // 8 threads a pair, 4 elements each
-        for (int q = t; q < C * 8; q += 64 * KW) {
-            const int c = q / 8, f = q % 8 * 4;
-            float v[4];
-            uint32_t am = 0;
+        // 32 threads a pair, one element each
+        const int c = t / 32, f = t % 32, p = pair_of[c];
+        const float v = silu_times(total(f, c), total(32 + f, c));
+        uint32_t am = f2u(v) & 0x7FFFFFFFu;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] = silu_times(total(f + j, c), total(32 + f + j, c));
-                am = max(am, f2u(v[j]) & 0x7FFFFFFFu);
-            }
-#pragma unroll
-            for (int m = 1; m < 8; m *= 2) am = max(am, (uint32_t)__shfl_xor((int)am, m, 64));
-            const uint32_t byte = mx8_byte(am);
-            const float m = mx8_inverse(byte);
-            const int p = pair_of[c];
-            if (p >= 0) {
-                *(uint32_t *)(a.h + (int64_t)p * F + nb * 32 + f) = e4m3_x4(v[0] * m, v[1] * m, v[2] * m, v[3] * m);
-                if (f == 0) a.hs[(int64_t)p * (F / 32) + nb] = (uint8_t)byte;
-            }
+        for (int m = 1; m < 32; m *= 2) am = max(am, (uint32_t)__shfl_xor((int)am, m, 64));
+        const uint32_t byte = mx8_byte(am);
+        if (p >= 0) {
+            a.h[(int64_t)p * F + nb * 32 + f] = (uint8_t)e4m3_x4(v * mx8_inverse(byte), 0.f, 0.f, 0.f);
+            if (f == 0) a.hs[(int64_t)p * (F / 32) + nb] = (uint8_t)byte;
         }
     } else {
-        for (int q = t; q < C * 64; q += 64 * KW) {
-            const int c = q / 64, n = nb * 64 + q % 64, p = pair_of[c];
-            if (p >= 0 && n < a.N) a.z[(int64_t)p * a.ldz + n] = total(q % 64, c);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int c = t / 64 + 8 * q, n = nb * 64 + t % 64, p = pair_of[c];
+            if (p >= 0 && n < a.N) a.z[(int64_t)p * a.ldz + n] = total(t % 64, c);
         }
     }
 }
 
-// ------------------------------------------------------------ many rows
-// A workgroup of 8 waves, WM along W and 8 / WM along the pairs: 256 rows of W
-// (gated: of 128 elements the gate's and up's, 256 / WM / 2 of each in a wave)
-// for up to BT pairs of one expert.  Stages of 128 K go straight from memory
-// into a ring of three LDS slots, two stages ahead of their use: pairs' rows
-// by the addresses of each lane's own row, so that nothing is gathered first.
-// One barrier a stage: after it the stage is there for every wave, and the slot
-// of the stage before is free.
-template <int BT>
+// ------------------------------------------------------------- LDS tiles
+// A workgroup of WM * WT waves, WM along W and WT along the pairs: 256 rows of W
+// (gated: of 128 elements the gate's and up's, 128 / WM of each in a wave) for
+// up to BT pairs of one expert.  Stages of 128 K go straight from memory into a
+// ring of three LDS slots, two stages ahead of their use: pairs' rows by the
+// addresses of each lane's own row, so that nothing is gathered first.  Scales
+// come four stages at a time: a load of 4 bytes a row would read as many cache
+// lines each stage as the codes do.  One barrier a stage.
+template <int BT, int NW>
 struct TileShape {
-    static constexpr int WM = BT == 256 ? 2 : 4, WT = 8 / WM;
+    static constexpr int WM = NW == 4 || BT < 256 ? 4 : 2, WT = NW / WM, NT = 64 * NW;
     static constexpr int A = 256 / WM / 16, B = BT / WT / 16;   // 16 x 16 tiles of a wave
     static constexpr int XB = BT * 128, WB = 256 * 64;          // bytes of a stage
-    static constexpr int SLOT = XB + WB, ROWS = BT + 256;
-    static constexpr int LDS = 3 * SLOT + 2 * ROWS * 16;        // and two groups of 4 stages' scales
-    static constexpr int XL = XB / 16 / 512;                    // 16-byte loads of a thread
+    static constexpr int SLOT = XB + WB, ROWS = 256 + (BT < 64 ? 64 : BT);
+    static constexpr int LDS = 3 * SLOT + 2 * ROWS * 16;        // and two groups of four stages' scales
+    static constexpr int XL = XB < NT * 16 ? 1 : XB / 16 / NT, WL = WB / 16 / NT, L = XL + WL;   // 16-byte loads of a thread
+    static constexpr int SETS = ROWS / 64, SL = (SETS + NW - 1) / NW;   // scales
 };
 
 LSMX_DEV void dma16(const uint8_t *p, uint32_t m0) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(__builtin_amdgcn_readfirstlane(m0)) : "memory");
 }
-LSMX_DEV void dma4(const uint8_t *p, uint32_t m0) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(__builtin_amdgcn_readfirstlane(m0)) : "memory");
-}
 
-template <bool GATED, int BT>
-__global__ __launch_bounds__(512, 2) void expert_tile_kernel(ExpertArgs a) {
-    typedef TileShape<BT> S;
-    constexpr int A = S::A, B = S::B;
+template <bool GATED, int BT, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void expert_tile_kernel(ExpertArgs a) {
+    typedef TileShape<BT, NW> S;
+    constexpr int A = S::A, B = S::B, L = S::L, G = 4;   // G: stages of a group of scales
+    constexpr bool EXACT = BT == 16;   // in time that its loads leave over (64 pairs: 55 us, exact 83)
     __shared__ __attribute__((aligned(16))) uint8_t lds[S::LDS];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), i16 = lane & 15, g = lane >> 4;
     const int wm = wave % S::WM, wt = wave / S::WM;
-    const int F = a.N / 2;
     const Tile tile = find_tile(a.offsets, a.experts, a.pairs, BT, (a.N + 255) / 256);
-    const int nb = tile.block;
     if (tile.n == 0) return;
-    // the pair of row r of the tile, -1 past the last
-    auto pair_of = [&](int r) __attribute__((always_inline)) {
-        const uint32_t p = r < tile.n ? (uint32_t)a.order[tile.start + r] : 0xFFFFFFFFu;
-        return p < (uint32_t)a.pairs ? (int)p : -1;
-    };
+    const int nb = tile.block, F = a.N / 2;
     if (tile.expert == a.experts) {
-        if constexpr (GATED) zero_rows<512>(a, pair_of, tile.n, nb * 128, min(128, F - nb * 128));
+        if constexpr (GATED) zero_rows(a, tile, S::NT, nb * 128, min(128, F - nb * 128));
         return;
     }
     const int kb = a.K / 32, nk = a.K / 128;
@@ -264,45 +286,47 @@ __global__ __launch_bounds__(512, 2) void expert_tile_kernel(ExpertArgs a) {
             return first + min(nb * 256 + r, a.N - 1);
         }
     };
-    auto x_row = [&](int r) __attribute__((always_inline)) {
-        const int p = max(pair_of(min(r, tile.n - 1)), 0);
-        return (int64_t)(GATED ? p / a.k : p);
-    };
     // a thread's shares of a stage.  16-byte chunk c of a pair's row lies at
     // c ^ (row & 7), of a weight's row at c ^ (row / 2 & 3): the rows that are
-    // read together then cover the banks.
-    const uint8_t *xp[S::XL], *wp[2], *sp;
+    // read together then cover the banks.  Where a stage's pairs are fewer than
+    // the threads, several waves load the same.
+    constexpr int XW = S::XB / 1024 < NW ? S::XB / 1024 : NW;
+    const uint8_t *xp[S::XL], *wp[S::WL], *sp[S::SL];
 #pragma unroll
-    for (int i = 0; i < S::XL; ++i) xp[i] = a.x + x_row(i * 64 + wave * 8 + lane / 8) * a.K + ((lane & 7) ^ (lane >> 3)) * 16;
+    for (int i = 0; i < S::XL; ++i)
+        xp[i] = a.x + x_row<GATED>(a, tile, i * 8 * NW + wave % XW * 8 + lane / 8) * a.K + ((lane & 7) ^ (lane >> 3)) * 16;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-        wp[i] = a.w + w_row(i * 128 + wave * 16 + lane / 4) * (a.K / 2) + ((lane & 3) ^ (lane >> 3 & 3)) * 16;
-    // scales, 16 bytes a row for four stages: waves 0 .. 3 the weights', the
-    // others the pairs'
-    if (wave < 4)
-        sp = a.ws + w_row(wave * 64 + lane) * kb;
-    else
-        sp = a.xs + x_row(min((wave - 4) * 64 + lane, BT - 1)) * kb;
+    for (int i = 0; i < S::WL; ++i)
+        wp[i] = a.w + w_row(i * 16 * NW + wave * 16 + lane / 4) * (a.K / 2) + ((lane & 3) ^ (lane >> 3 & 3)) * 16;
+    // scales in sets of 64 rows: four of the weights, then the pairs'
+    auto set_of = [&](int i) __attribute__((always_inline)) { return min(wave + i * NW, S::SETS - 1); };
+#pragma unroll
+    for (int i = 0; i < S::SL; ++i) {
+        const int u = set_of(i);
+        sp[i] = u < 4 ? a.ws + w_row(u * 64 + lane) * kb : a.xs + x_row<GATED>(a, tile, min((u - 4) * 64 + lane, BT - 1)) * kb;
+    }
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
-    constexpr int L = S::XL + 2;   // loads of a stage
     // load i of a stage, and the way to the next stage's: 1, or 0 past the last
     auto load = [&](int i, uint32_t slot, int step) __attribute__((always_inline)) {
         if (i < S::XL) {
-            dma16(xp[i], base + slot + (i * 8 + wave) * 1024);
+            dma16(xp[i], base + slot + (i * NW + wave % XW) * 1024);
             xp[i] += 128 * step;
         } else {
-            dma16(wp[i - S::XL], base + slot + S::XB + ((i - S::XL) * 8 + wave) * 1024);
+            dma16(wp[i - S::XL], base + slot + S::XB + ((i - S::XL) * NW + wave) * 1024);
             wp[i - S::XL] += 64 * step;
         }
     };
-    // the scales of stages 4 n .. 4 n + 3, the last group's moved back to where
+    // the scales of the G stages from G n on, the last group's moved back to where
     // it ends with the row (nk >= 4)
-    auto group = [&](int n) __attribute__((always_inline)) { return min(4 * n, nk - 4); };
     auto load_scales = [&](int n) __attribute__((always_inline)) {
-        if (wave < 4 + BT / 64) dma16(sp + group(n) * 4, base + 3 * S::SLOT + (n & 1) * S::ROWS * 16 + wave * 1024);
+        const uint32_t to = base + 3 * S::SLOT + (n & 1) * S::ROWS * 4 * G;
+        const int at = min(G * n, nk - G) * 4;
+#pragma unroll
+        for (int i = 0; i < S::SL; ++i) dma16(sp[i] + at, to + set_of(i) * 1024);
     };
-    auto scales_of = [&](int kt) __attribute__((always_inline)) {
-        return (uint32_t)(3 * S::SLOT + (kt >> 2 & 1) * S::ROWS * 16 + (kt - group(kt >> 2)) * 4);
+    // where stage kt's scales lie, kt = G n + i
+    auto scales_of = [&](int n, int i) __attribute__((always_inline)) {
+        return (uint32_t)(3 * S::SLOT + (n & 1) * S::ROWS * 4 * G + (i + max(G * n + G - nk, 0)) * 4);
     };
     v4f acc[A][B];
 #pragma unroll
@@ -310,7 +334,7 @@ __global__ __launch_bounds__(512, 2) void expert_tile_kernel(ExpertArgs a) {
 #pragma unroll
         for (int j = 0; j < B; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
     const int x0 = (wt * B * 16 + i16) * 128 + ((g ^ (lane & 7)) << 4), w0 = S::XB + (wm * A * 16 + i16) * 64 + ((g ^ (lane >> 1 & 3)) << 4);
-    const int ws0 = (wm * A * 16 + i16) * 16 + g, xs0 = (256 + wt * B * 16 + i16) * 16 + g;
+    const int ws0 = (wm * A * 16 + i16) * 4 * G + g, xs0 = (256 + wt * B * 16 + i16) * 4 * G + g;
     v8i x[B];
     v4i w[A];
     int xs[B], ws[A];
@@ -318,11 +342,22 @@ __global__ __launch_bounds__(512, 2) void expert_tile_kernel(ExpertArgs a) {
         const uint8_t *sl = lds + slot;
         const v4i lo = *(const v4i *)(sl + x0 + j * 2048), hi = *(const v4i *)(sl + (x0 ^ 64) + j * 2048);
         x[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        xs[j] = lds[sc + xs0 + j * 256];
+        xs[j] = lds[sc + xs0 + j * 64 * G];
     };
     auto read_w = [&](int i, uint32_t slot, uint32_t sc) __attribute__((always_inline)) {
         w[i] = *(const v4i *)(lds + slot + w0 + i * 1024);
-        ws[i] = lds[sc + ws0 + i * 256];
+        ws[i] = lds[sc + ws0 + i * 64 * G];
+    };
+    // products of W's tiles i0 .. i1 - 1 with pairs' tile j
+    auto multiply = [&](int i0, int i1, int j) __attribute__((always_inline)) {
+        const v8i big = EXACT ? large_codes(x[j]) : x[j];
+#pragma unroll
+        for (int i = i0; i < i1; ++i) acc[i][j] = mfma_f4f8(w[i], big, acc[i][j], 4, 0, 0, ws[i], 0, xs[j]);
+        if constexpr (EXACT) {
+            const v8i small = x[j] ^ big;
+#pragma unroll
+            for (int i = i0; i < i1; ++i) acc[i][j] = mfma_f4f8(w[i], small, acc[i][j], 4, 0, 0, ws[i], 0, xs[j]);
+        }
     };
     // waits for this wave's reads and for all but its last n loads, then for the
     // other waves
@@ -332,13 +367,14 @@ __global__ __launch_bounds__(512, 2) void expert_tile_kernel(ExpertArgs a) {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
+    static_assert(2 * L < 16, "the count of a wait");
     load_scales(0);
 #pragma unroll
     for (int k = 0; k < 3; ++k)
 #pragma unroll
         for (int i = 0; i < L; ++i) load(i, k * S::SLOT, k + 1 < nk);
     wait(SlotC<2 * L>{});
-    uint32_t sc = scales_of(0);
+    uint32_t sc = scales_of(0, 0);
 #pragma unroll
     for (int i = 0; i < A / 2; ++i) read_w(i, 0, sc);
 #pragma unroll
@@ -349,19 +385,18 @@ __global__ __launch_bounds__(512, 2) void expert_tile_kernel(ExpertArgs a) {
     // one between the products of the second half and of the next stage's first
     // (in one burst they keep the waves from issuing).  During the second half
     // the next stage is read, each pair's rows once their last product is issued.
-    // The loop has no branches: past the last stage it loads that again, and
-    // reads what it does not use.
+    // Past the last stage the loop loads that again, and reads what it does not
+    // use, without branches.
     uint32_t now = 0, before = 2 * S::SLOT;
     constexpr int L0 = L - L / 2;   // loads of the second half
-    int step = 0;
+    int step = 0, gn = 0, gi = 0;   // kt = G gn + gi
     for (int kt = 0; kt < nk; ++kt) {
         const uint32_t next = now == 2 * S::SLOT ? 0 : now + S::SLOT;
 #pragma unroll
         for (int j = 0; j < B; ++j) {
 #pragma unroll
             for (int i = A / 2 * j / B; i < A / 2 * (j + 1) / B; ++i) read_w(A / 2 + i, now, sc);
-#pragma unroll
-            for (int i = 0; i < A / 2; ++i) acc[i][j] = mfma_f4f8(w[i], x[j], acc[i][j], 4, 0, 0, ws[i], 0, xs[j]);
+            multiply(0, A / 2, j);
             if (kt > 0)
 #pragma unroll
                 for (int i = L0 + L / 2 * j / B; i < L0 + L / 2 * (j + 1) / B; ++i) load(i, before, step);
@@ -369,15 +404,15 @@ __global__ __launch_bounds__(512, 2) void expert_tile_kernel(ExpertArgs a) {
         }
         wait(SlotC<L>{});
         step = kt + 4 < nk;
-        sc = scales_of(min(kt + 1, nk - 1));
-        if ((kt & 3) == 0 && kt + 4 < nk) load_scales(kt / 4 + 1);
+        if (gi == 0 && G * (gn + 1) < nk) load_scales(gn + 1);
+        if (++gi == G) gi = 0, ++gn;
+        sc = kt + 1 < nk ? scales_of(gn, gi) : sc;
 #pragma unroll
         for (int i = 0; i < A / 2; ++i) read_w(i, next, sc);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < B; ++j) {
-#pragma unroll
-            for (int i = A / 2; i < A; ++i) acc[i][j] = mfma_f4f8(w[i], x[j], acc[i][j], 4, 0, 0, ws[i], 0, xs[j]);
+            multiply(A / 2, A, j);
             __builtin_amdgcn_sched_barrier(0);
             read_x(j, next, sc);
 #pragma unroll
@@ -389,7 +424,7 @@ __global__ __launch_bounds__(512, 2) void expert_tile_kernel(ExpertArgs a) {
     wait_dma();   // nothing may land in LDS after the workgroup
 #pragma unroll
     for (int j = 0; j < B; ++j) {
-        const int p = pair_of((wt * B + j) * 16 + i16);
+        const int p = pair_at(a, tile, (wt * B + j) * 16 + i16);
         if constexpr (GATED) {
             // a block of 32 elements of a pair: two tiles in four lanes
 #pragma unroll
@@ -413,6 +448,36 @@ __global__ __launch_bounds__(512, 2) void expert_tile_kernel(ExpertArgs a) {
                     if (g == 0) a.hs[(int64_t)p * (F / 32) + f / 32] = (uint8_t)byte;
                 }
             }
+        } else if (a.zs) {
+            // rows of z in 16 bits: fp16 over the largest power of two among 64
+            // elements, 2^-12 of each
+#pragma unroll
+            for (int b = 0; b < A / 4; ++b) {
+                uint32_t am = 0;
+#pragma unroll
+                for (int i = 4 * b; i < 4 * b + 4; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const uint32_t u = f2u(acc[i][j][q]) & 0x7FFFFFFFu;
+                        am = max(am, u < 0x7F800000u ? u : 0u);   // infinities and NaN stay what they are
+                    }
+                am = max(am, (uint32_t)__shfl_xor((int)am, 16, 64));
+                am = max(am, (uint32_t)__shfl_xor((int)am, 32, 64));
+                const uint32_t e = max(am >> 23, 16u) - 14u;   // the largest below 2^15
+                const float m = u2f((254u - e) << 23);
+                const int n = nb * 256 + (wm * A + 4 * b) * 16;
+                if (p >= 0 && n < a.N) {
+                    _Float16 *z = (_Float16 *)a.z + (int64_t)p * a.ldz + n + 4 * g;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        v4h o;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) o[q] = (_Float16)(acc[4 * b + i][j][q] * m);
+                        if (n + 16 * i + 4 * g < a.N) *(v4h *)(z + 16 * i) = o;
+                    }
+                    if (g == 0) a.zs[(int64_t)p * ((a.N + 63) / 64) + n / 64] = u2f(e << 23);
+                }
+            }
         } else if (p >= 0) {
 #pragma unroll
             for (int i = 0; i < A; ++i) {
@@ -424,63 +489,88 @@ __global__ __launch_bounds__(512, 2) void expert_tile_kernel(ExpertArgs a) {
 }
 
 // y_t = sum_j weight_tj z_tj over the pairs that have an expert, in the order of
-// their slots.
-template <int DT>
+// their slots; 8 elements a thread.
+template <int DT, bool HALF>
 __global__ __launch_bounds__(256) void expert_join_kernel(ExpertArgs a) {
     typedef typename Elem<DT>::S S;
-    const int64_t token = blockIdx.y + (int64_t)blockIdx.z * 65535;
-    if (token >= a.tokens) return;
-    const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
+    const int chunks = (a.N + 7) / 8, blocks = (chunks + 255) / 256;
+    const int64_t token = blockIdx.x / blocks;
+    const int n = ((blockIdx.x % blocks) * 256 + threadIdx.x) * 8;
     if (n >= a.N) return;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    float v[8] = {};
+#pragma unroll 4
     for (int j = 0; j < a.k; ++j) {
         const int64_t p = token * a.k + j;
         if ((uint32_t)a.ids[p] >= (uint32_t)a.experts) continue;
-        const float w = a.weights[p];
-        const v4f z = *(const v4f *)(a.z + p * a.ldz + n);
+        if constexpr (HALF) {
+            const float w = a.weights[p] * a.zs[p * ((a.N + 63) / 64) + n / 64];
+            typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+            const v8h z = *(const v8h *)((const _Float16 *)a.z + p * a.ldz + n);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += w * z[i];
+            for (int i = 0; i < 8; ++i) v[i] += w * (float)z[i];
+        } else {
+            const float w = a.weights[p];
+            const v4f z0 = *(const v4f *)(a.z + p * a.ldz + n), z1 = *(const v4f *)(a.z + p * a.ldz + n + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += w * z0[i], v[4 + i] += w * z1[i];
+        }
     }
+    S *y = (S *)a.y + token * a.N + n;
+    typedef S V __attribute__((ext_vector_type(8), aligned(16)));
+    if (a.N % 8 == 0 && (uintptr_t)a.y % 16 == 0) {
+        V o;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (n + i < a.N) ((S *)a.y)[token * a.N + n + i] = Elem<DT>::store(v[i]);
+        for (int i = 0; i < 8; ++i) o[i] = Elem<DT>::store(v[i]);
+        *(V *)y = o;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (n + i < a.N) y[i] = Elem<DT>::store(v[i]);
+    }
 }
 
-template <bool GATED, int NT, int KW>
+template <bool GATED>
 hipError_t stream(const ExpertArgs &a, hipStream_t s) {
-    const int64_t units = tile_units(a.pairs, a.experts, 16 * NT, (a.N + 63) / 64);
-    expert_stream_kernel<GATED, NT, KW><<<(unsigned)units, 64 * KW, 0, s>>>(a);
+    expert_stream_kernel<GATED><<<(unsigned)tile_units(a.pairs, a.experts, 16, (a.N + 63) / 64), 512, 0, s>>>(a);
     return hipGetLastError();
 }
-template <bool GATED, int BT>
+template <bool GATED, int BT, int NW>
 hipError_t tiles(const ExpertArgs &a, hipStream_t s) {
-    const int64_t units = tile_units(a.pairs, a.experts, BT, (a.N + 255) / 256);
-    expert_tile_kernel<GATED, BT><<<(unsigned)units, 512, 0, s>>>(a);
+    expert_tile_kernel<GATED, BT, NW><<<(unsigned)tile_units(a.pairs, a.experts, BT, (a.N + 255) / 256), 64 * NW, 0, s>>>(a);
     return hipGetLastError();
 }
 template <bool GATED>
 hipError_t products(const ExpertArgs &a, hipStream_t s) {
-    if (a.K < 512) return stream<GATED, 1, 8>(a, s);
+    if (a.K < 512) return stream<GATED>(a, s);
     const int64_t per = a.pairs / a.experts;
-    return per <= 8 ? stream<GATED, 1, 8>(a, s) : per <= 32 ? stream<GATED, 4, 4>(a, s) : per <= 256 ? tiles<GATED, 128>(a, s) : tiles<GATED, 256>(a, s);
+    if (a.pairs * ((a.N + 63) / 64) <= 384) return stream<GATED>(a, s);
+    if (per <= 4) return tiles<GATED, 16, 4>(a, s);
+    if (per <= 80) return tiles<GATED, 64, 8>(a, s);
+    return per <= 400 ? tiles<GATED, 128, 8>(a, s) : tiles<GATED, 256, 8>(a, s);
+}
+
+template <int DT>
+hipError_t join(const ExpertArgs &a, hipStream_t s) {
+    const int64_t chunks = (a.N + 7) / 8, grid = (chunks + 255) / 256 * a.tokens;
+    if (a.zs)
+        expert_join_kernel<DT, true><<<(unsigned)grid, 256, 0, s>>>(a);
+    else
+        expert_join_kernel<DT, false><<<(unsigned)grid, 256, 0, s>>>(a);
+    return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_expert_gated(const ExpertArgs &a, hipStream_t s) { return products<true>(a, s); }
 
-hipError_t launch_expert_combine(const ExpertArgs &a, hipStream_t s) {
-    hipError_t e = hipSuccess;
-    if (a.pairs) e = products<false>(a, s);
+hipError_t launch_expert_combine(const ExpertArgs &a0, hipStream_t s) {
+    ExpertArgs a = a0;
+    // bf16 sums of many rows take the pairs' rows in 16 bits, where writing and
+    // reading them costs more than the products
+    if (a.y_dtype == LSMX_BF16 && a.K >= 512 && a.pairs / a.experts > 80) a.zs = (float *)((uint8_t *)a.z + (int64_t)a.pairs * a.ldz * 2);
+    const hipError_t e = products<false>(a, s);
     if (e != hipSuccess) return e;
-    const dim3 grid((a.N + 1023) / 1024, (unsigned)(a.tokens < 65535 ? a.tokens : 65535), (unsigned)((a.tokens + 65534) / 65535));
-    if (a.y_dtype == LSMX_F32)
-        expert_join_kernel<LSMX_F32><<<grid, 256, 0, s>>>(a);
-    else if (a.y_dtype == LSMX_BF16)
-        expert_join_kernel<LSMX_BF16><<<grid, 256, 0, s>>>(a);
-    else
-        expert_join_kernel<LSMX_F16><<<grid, 256, 0, s>>>(a);
-    return hipGetLastError();
+    return a.y_dtype == LSMX_F32 ? join<LSMX_F32>(a, s) : a.y_dtype == LSMX_BF16 ? join<LSMX_BF16>(a, s) : join<LSMX_F16>(a, s);
 }
 
 }  // namespace lsmx

@@ -86,8 +86,9 @@ struct ExpertArgs {
     const int32_t *ids, *order, *offsets;
     int pairs, k, experts, N, K;
     uint8_t *h, *hs;         // gated: [pairs, N / 2], [pairs, N / 64]
-    float *z;                // combine: the pairs' rows, [pairs, ldz]
-    int64_t ldz;
+    float *z;                // combine: the pairs' rows, [pairs, ldz]; with zs in
+    int64_t ldz;             // fp16 over [pairs, ceil(N / 64)] powers of two
+    float *zs;
     const float *weights;
     void *y;
     int y_dtype;

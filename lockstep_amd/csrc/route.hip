@@ -582,6 +582,17 @@ hipError_t bwd_of(const RouteArgs &a, hipStream_t s) {
 // experts count as expert `experts`, behind the others.
 constexpr int kDispWaves = 16, kDispPairs = 4096;
 
+// Sums of a wave's lanes up to each.
+LSMX_DEV int scan64(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast 15, 31
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+
 // One round of a wave: each lane's rank among the wave's pairs of its expert so
 // far, the counts brought up to date.
 LSMX_DEV int round_rank(int e, int bits, uint16_t *hist, bool live) {
@@ -618,20 +629,22 @@ __global__ __launch_bounds__(1024) void dispatch_count_kernel(const int32_t *ids
 }
 
 // order and offsets.  counts null: one workgroup, which counts for itself.
+template <int ROUNDS>
 __global__ __launch_bounds__(1024) void dispatch_kernel(const int32_t *ids, int pairs, int experts, int bits,
                                                         const int32_t *counts, int32_t *order, int32_t *offsets) {
     extern __shared__ int lds_i[];   // bases [experts + 1], totals [experts + 1], counts [waves][experts + 1]
+    const int threads = blockDim.x, waves = threads / 64;
     const int n = experts + 1;
     int *base = lds_i, *scan = lds_i + n;
     uint16_t *hists = (uint16_t *)(lds_i + 2 * n);   // at most kDispPairs
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    for (int i = t; i < kDispWaves * n; i += 1024) hists[i] = 0;
+    for (int i = t; i < waves * n; i += threads) hists[i] = 0;
     __syncthreads();
     uint16_t *hist = hists + wave * n;
-    int e[kDispPairs / 1024], rank[kDispPairs / 1024];
+    int e[ROUNDS], rank[ROUNDS];
 #pragma unroll
-    for (int r = 0; r < kDispPairs / 1024; ++r) {
-        const int p = blockIdx.x * kDispPairs + wave * (kDispPairs / kDispWaves) + r * 64 + lane;
+    for (int r = 0; r < ROUNDS; ++r) {
+        const int p = blockIdx.x * kDispPairs + wave * (64 * ROUNDS) + r * 64 + lane;
         const bool live = p < pairs;
         e[r] = live ? expert_of(ids, p, experts) : 0;
         rank[r] = round_rank(e[r], bits, hist, live);
@@ -639,9 +652,9 @@ __global__ __launch_bounds__(1024) void dispatch_kernel(const int32_t *ids, int 
     __syncthreads();
     // expert x: pairs of earlier workgroups, of all, and the waves' counts turned
     // into where each begins
-    for (int x = t; x < n; x += 1024) {
+    for (int x = t; x < n; x += threads) {
         int run = 0;
-        for (int w = 0; w < kDispWaves; ++w) {
+        for (int w = 0; w < waves; ++w) {
             const int c = hists[w * n + x];
             hists[w * n + x] = (uint16_t)run;
             run += c;
@@ -665,22 +678,17 @@ __global__ __launch_bounds__(1024) void dispatch_kernel(const int32_t *ids, int 
         for (int x0 = 0; x0 < n; x0 += 64) {
             const int x = x0 + lane;
             const int v = x < n ? scan[x] : 0;
-            int inc = v;
-#pragma unroll
-            for (int m = 1; m < 64; m *= 2) {
-                const int o = __shfl_up(inc, m, 64);
-                if (lane >= m) inc += o;
-            }
+            const int inc = scan64(v);
             if (x < n) scan[x] = carry + inc - v;
-            carry += __shfl(inc, 63, 64);
+            carry += __builtin_amdgcn_readlane(inc, 63);
         }
     }
     __syncthreads();
     if (blockIdx.x == 0)
-        for (int x = t; x < n; x += 1024) offsets[x] = scan[x];
+        for (int x = t; x < n; x += threads) offsets[x] = scan[x];
 #pragma unroll
-    for (int r = 0; r < kDispPairs / 1024; ++r) {
-        const int p = blockIdx.x * kDispPairs + wave * (kDispPairs / kDispWaves) + r * 64 + lane;
+    for (int r = 0; r < ROUNDS; ++r) {
+        const int p = blockIdx.x * kDispPairs + wave * (64 * ROUNDS) + r * 64 + lane;
         if (p < pairs) order[scan[e[r]] + base[e[r]] + hist[e[r]] + rank[r]] = p;
     }
 }
@@ -708,8 +716,13 @@ hipError_t launch_dispatch(const int32_t *ids, int pairs, int experts, int32_t *
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    const size_t lds = (size_t)(experts + 1) * (8 + 2 * kDispWaves);
-    dispatch_kernel<<<blocks, 1024, lds, s>>>(ids, pairs, experts, bits, blocks > 1 ? ws : nullptr, order, offsets);
+    // up to 1024 pairs: a round for each wave, as many waves as it takes
+    const int waves = pairs <= 1024 ? (pairs + 63) / 64 + (pairs == 0) : kDispWaves;
+    const size_t lds = (size_t)(experts + 1) * (8 + 2 * waves);
+    if (pairs <= 1024)
+        dispatch_kernel<1><<<1, 64 * waves, lds, s>>>(ids, pairs, experts, bits, nullptr, order, offsets);
+    else
+        dispatch_kernel<kDispPairs / 1024><<<blocks, 1024, lds, s>>>(ids, pairs, experts, bits, blocks > 1 ? ws : nullptr, order, offsets);
     return hipGetLastError();
 }
 
