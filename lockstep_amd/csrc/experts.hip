@@ -251,7 +251,7 @@ struct TileShape {
     static constexpr int XB = BT * 128, WB = 256 * 64;          // bytes of a stage
     static constexpr int SLOT = XB + WB, ROWS = 256 + (BT < 64 ? 64 : BT);
     static constexpr int LDS = 3 * SLOT + 2 * ROWS * 16;        // and two groups of four stages' scales
-    static constexpr int XL = XB < NT * 16 ? 1 : XB / 16 / NT, WL = WB / 16 / NT, L = XL + WL;   // 16-byte loads of a thread
+    static constexpr int XL = (XB / 16 + NT - 1) / NT, WL = WB / 16 / NT, L = XL + WL;   // 16-byte loads of a thread
     static constexpr int SETS = ROWS / 64, SL = (SETS + NW - 1) / NW;   // scales
 };
 
@@ -263,7 +263,7 @@ template <bool GATED, int BT, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void expert_tile_kernel(ExpertArgs a) {
     typedef TileShape<BT, NW> S;
     constexpr int A = S::A, B = S::B, L = S::L, G = 4;   // G: stages of a group of scales
-    constexpr bool EXACT = BT == 16;   // in time that its loads leave over (64 pairs: 55 us, exact 83)
+    constexpr bool EXACT = BT == 16;   // in time that its loads leave over (64 pairs a tile: 55 us, exact 83)
     __shared__ __attribute__((aligned(16))) uint8_t lds[S::LDS];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), i16 = lane & 15, g = lane >> 4;
     const int wm = wave % S::WM, wt = wave / S::WM;
@@ -290,11 +290,11 @@ __global__ __launch_bounds__(64 * NW, 2) void expert_tile_kernel(ExpertArgs a) {
     // c ^ (row & 7), of a weight's row at c ^ (row / 2 & 3): the rows that are
     // read together then cover the banks.  Where a stage's pairs are fewer than
     // the threads, several waves load the same.
-    constexpr int XW = S::XB / 1024 < NW ? S::XB / 1024 : NW;
+    auto x_set = [&](int i) __attribute__((always_inline)) { return min(i * NW + wave, S::XB / 1024 - 1); };   // of 8 rows
     const uint8_t *xp[S::XL], *wp[S::WL], *sp[S::SL];
 #pragma unroll
     for (int i = 0; i < S::XL; ++i)
-        xp[i] = a.x + x_row<GATED>(a, tile, i * 8 * NW + wave % XW * 8 + lane / 8) * a.K + ((lane & 7) ^ (lane >> 3)) * 16;
+        xp[i] = a.x + x_row<GATED>(a, tile, x_set(i) * 8 + lane / 8) * a.K + ((lane & 7) ^ (lane >> 3)) * 16;
 #pragma unroll
     for (int i = 0; i < S::WL; ++i)
         wp[i] = a.w + w_row(i * 16 * NW + wave * 16 + lane / 4) * (a.K / 2) + ((lane & 3) ^ (lane >> 3 & 3)) * 16;
@@ -309,7 +309,7 @@ __global__ __launch_bounds__(64 * NW, 2) void expert_tile_kernel(ExpertArgs a) {
     // load i of a stage, and the way to the next stage's: 1, or 0 past the last
     auto load = [&](int i, uint32_t slot, int step) __attribute__((always_inline)) {
         if (i < S::XL) {
-            dma16(xp[i], base + slot + (i * NW + wave % XW) * 1024);
+            dma16(xp[i], base + slot + x_set(i) * 1024);
             xp[i] += 128 * step;
         } else {
             dma16(wp[i - S::XL], base + slot + S::XB + ((i - S::XL) * NW + wave) * 1024);
@@ -328,6 +328,9 @@ __global__ __launch_bounds__(64 * NW, 2) void expert_tile_kernel(ExpertArgs a) {
     auto scales_of = [&](int n, int i) __attribute__((always_inline)) {
         return (uint32_t)(3 * S::SLOT + (n & 1) * S::ROWS * 4 * G + (i + max(G * n + G - nk, 0)) * 4);
     };
+    int pair[B];   // of this lane's results
+#pragma unroll
+    for (int j = 0; j < B; ++j) pair[j] = pair_at(a, tile, (wt * B + j) * 16 + i16);
     v4f acc[A][B];
 #pragma unroll
     for (int i = 0; i < A; ++i)
@@ -374,6 +377,20 @@ __global__ __launch_bounds__(64 * NW, 2) void expert_tile_kernel(ExpertArgs a) {
 #pragma unroll
         for (int i = 0; i < L; ++i) load(i, k * S::SLOT, k + 1 < nk);
     wait(SlotC<2 * L>{});
+    if (S::WT > 1 && wt * B * 16 >= tile.n) {
+        // a wave without pairs only loads: the other one of its SIMD multiplies
+        uint32_t slot = 0;
+        for (int kt = 0; kt < nk; ++kt) {
+            wait(SlotC<L>{});
+            if (kt % G == 0 && kt + G < nk) load_scales(kt / G + 1);
+            const int step = kt + 4 < nk;
+#pragma unroll
+            for (int i = 0; i < L; ++i) load(i, slot, step);
+            slot = slot == 2 * S::SLOT ? 0 : slot + S::SLOT;
+        }
+        wait_dma();
+        return;
+    }
     uint32_t sc = scales_of(0, 0);
 #pragma unroll
     for (int i = 0; i < A / 2; ++i) read_w(i, 0, sc);
@@ -424,7 +441,7 @@ __global__ __launch_bounds__(64 * NW, 2) void expert_tile_kernel(ExpertArgs a) {
     wait_dma();   // nothing may land in LDS after the workgroup
 #pragma unroll
     for (int j = 0; j < B; ++j) {
-        const int p = pair_at(a, tile, (wt * B + j) * 16 + i16);
+        const int p = pair[j];
         if constexpr (GATED) {
             // a block of 32 elements of a pair: two tiles in four lanes
 #pragma unroll
@@ -545,8 +562,11 @@ hipError_t products(const ExpertArgs &a, hipStream_t s) {
     const int64_t per = a.pairs / a.experts;
     if (a.pairs * ((a.N + 63) / 64) <= 384) return stream<GATED>(a, s);
     if (per <= 4) return tiles<GATED, 16, 4>(a, s);
-    if (per <= 80) return tiles<GATED, 64, 8>(a, s);
-    return per <= 400 ? tiles<GATED, 128, 8>(a, s) : tiles<GATED, 256, 8>(a, s);
+    if (per <= 24) return tiles<GATED, 32, 4>(a, s);
+    if (per <= 96) return tiles<GATED, 48, 4>(a, s);
+    // 256 pairs where such tiles fill the CUs three times over, or are full
+    const int64_t units = (a.pairs / 256 + a.experts / 2) * ((a.N + 255) / 256);
+    return per > 400 || units >= 768 ? tiles<GATED, 256, 8>(a, s) : tiles<GATED, 128, 8>(a, s);
 }
 
 template <int DT>
@@ -567,7 +587,7 @@ hipError_t launch_expert_combine(const ExpertArgs &a0, hipStream_t s) {
     ExpertArgs a = a0;
     // bf16 sums of many rows take the pairs' rows in 16 bits, where writing and
     // reading them costs more than the products
-    if (a.y_dtype == LSMX_BF16 && a.K >= 512 && a.pairs / a.experts > 80) a.zs = (float *)((uint8_t *)a.z + (int64_t)a.pairs * a.ldz * 2);
+    if (a.y_dtype == LSMX_BF16 && a.K >= 512 && a.pairs / a.experts > 24) a.zs = (float *)((uint8_t *)a.z + (int64_t)a.pairs * a.ldz * 2);
     const hipError_t e = products<false>(a, s);
     if (e != hipSuccess) return e;
     return a.y_dtype == LSMX_F32 ? join<LSMX_F32>(a, s) : a.y_dtype == LSMX_BF16 ? join<LSMX_BF16>(a, s) : join<LSMX_F16>(a, s);
