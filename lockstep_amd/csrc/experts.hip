@@ -21,6 +21,7 @@
 // Pairs come sorted by expert (order, offsets); a workgroup finds the expert
 // and the pairs of its tile from the offsets.  Nothing in order or offsets is
 // trusted to be in range.
+#include <cstdlib>
 #include "lsmx_block.h"
 #include "lsmx_dma.h"
 #include "lsmx_internal.h"
@@ -560,6 +561,16 @@ template <bool GATED>
 hipError_t products(const ExpertArgs &a, hipStream_t s) {
     if (a.K < 512) return stream<GATED>(a, s);
     const int64_t per = a.pairs / a.experts;
+    if (const char *f = getenv("LSMX_EXP")) {
+        switch (atoi(f)) {
+            case 1: return stream<GATED>(a, s);
+            case 16: return tiles<GATED, 16, 4>(a, s);
+            case 32: return tiles<GATED, 32, 4>(a, s);
+            case 48: return tiles<GATED, 48, 4>(a, s);
+            case 128: return tiles<GATED, 128, 8>(a, s);
+            case 256: return tiles<GATED, 256, 8>(a, s);
+        }
+    }
     if (a.pairs * ((a.N + 63) / 64) <= 384) return stream<GATED>(a, s);
     if (per <= 4) return tiles<GATED, 16, 4>(a, s);
     if (per <= 24) return tiles<GATED, 32, 4>(a, s);

@@ -252,8 +252,9 @@ LSMX_DEV bool whole_vectors(const RouteArgs &a, int v) {
 // within 2^-22 of 1
 LSMX_DEV float sigmoid(float l) { return __builtin_amdgcn_rcpf(1.f + __expf(-l)); }
 
-template <int DT, int V>
+template <int DT, int V, int KM>   // k <= KM
 __global__ __launch_bounds__(256) void route_fwd16_kernel(RouteArgs a) {
+    constexpr int H = KM + 1 < V ? KM + 1 : V;   // of a lane's, those that can be chosen or be next
     extern __shared__ double lds[];   // a row of c for each wave, where there are groups
     __shared__ int chosen[16][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, r = threadIdx.x >> 4;
@@ -262,7 +263,7 @@ __global__ __launch_bounds__(256) void route_fwd16_kernel(RouteArgs a) {
     const bool live = row < a.rows;
     const int64_t at = live ? row : a.rows - 1;
     const int v = (a.experts + 15) / 16;
-    float l[V], c[V];
+    float l[V];
     lane_logits<DT, V>(a, at, l16, v, whole_vectors<DT, V>(a, v), l);
     const bool grouped = a.top_groups < a.groups, scored = a.bias != nullptr;
     // the row's largest logit, and whether 64 bits have to look at it
@@ -290,26 +291,31 @@ __global__ __launch_bounds__(256) void route_fwd16_kernel(RouteArgs a) {
     const uint32_t low = whole ? (DT == LSMX_BF16 ? 0xFFFFu : 0x1FFFu) : 15u;
     uint32_t k[V];
     if (scored) {
+        float c[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) c[j] = a.bias[min(l16 * v + j, a.experts - 1)];
 #pragma unroll
-        for (int j = 0; j < V; ++j) c[j] += score(l[j]), odd |= !(c[j] < __builtin_inff());
+        for (int j = 0; j < V; ++j) {
+            c[j] += score(l[j]);
+            odd |= !(c[j] < __builtin_inff());
+            k[j] = ordered(c[j]);
+        }
     } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) c[j] = l[j];
+        for (int j = 0; j < V; ++j) k[j] = ordered(l[j]);
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int e = l16 * v + j;
         const uint32_t in = j < v && e < a.experts ? ~0u : 0u;
-        k[j] = ((ordered(c[j]) & ~low) | (low - (whole ? e : j))) & in;
+        k[j] = ((k[j] & ~low) | (low - (whole ? e : j))) & in;
     }
     sort_down<V>(k);
     bool near = false;
     if (grouped) {
         // 16 / groups lanes a group: its two largest from their lanes' two
         uint32_t u = k[0], w = V > 1 ? k[1] : 0u;
-        const int per = 16 / a.groups, by = 31 - __builtin_clz(per);
+        const int per = 16 / a.groups;
         auto merge = [&](uint32_t ou, uint32_t ow) __attribute__((always_inline)) {
             w = max(min(u, ou), max(w, ow));
             u = max(u, ou);
@@ -320,21 +326,21 @@ __global__ __launch_bounds__(256) void route_fwd16_kernel(RouteArgs a) {
         const float fu = unordered(u & ~low), fw = unordered(w & ~low);
         const bool two = a.experts > a.groups;   // else a group's one is its score
         const float s = scored ? fu + (two ? fw : 0.f) : score(fu) + (two ? score(fw) : 0.f);
-        // groups surely and perhaps ahead of this lane's, each counted by its lanes
+        // groups surely and perhaps ahead of this lane's
         int ahead = 0, perhaps = 0;
-        const int mine = l16 >> by;
         const float tol = 2e-5f * (1.f + __builtin_fabsf(s));
-        auto look = [&](int o16, float o) __attribute__((always_inline)) {
-            const bool other = (o16 & 15) >> by != mine;
-            ahead += other && o > s + tol;
-            perhaps += other && !(o < s - tol);
+        auto look = [&](float o) __attribute__((always_inline)) {
+            ahead += o > s + tol;
+            perhaps += !(o < s - tol);
         };
-#define LOOK(n) look(l16 - n, u2f(ror16<n>(f2u(s))))
-        LOOK(1), LOOK(2), LOOK(3), LOOK(4), LOOK(5), LOOK(6), LOOK(7), LOOK(8), LOOK(9), LOOK(10), LOOK(11), LOOK(12), LOOK(13),
-            LOOK(14), LOOK(15);
+#define LOOK(n) look(u2f(ror16<n>(f2u(s))))
+        LOOK(8);
+        if (per <= 4) LOOK(4), LOOK(12);
+        if (per <= 2) LOOK(2), LOOK(6), LOOK(10), LOOK(14);
+        if (per <= 1) LOOK(1), LOOK(3), LOOK(5), LOOK(7), LOOK(9), LOOK(11), LOOK(13), LOOK(15);
 #undef LOOK
-        const bool out = ahead >> by >= a.top_groups;
-        near = !out && perhaps >> by >= a.top_groups;
+        const bool out = ahead >= a.top_groups;
+        near = !out && perhaps >= a.top_groups;
         if (out) {
 #pragma unroll
             for (int j = 0; j < V; ++j) k[j] = 0;
@@ -357,8 +363,8 @@ __global__ __launch_bounds__(256) void route_fwd16_kernel(RouteArgs a) {
         last = best;
         const uint32_t up = win ? ~0u : 0u;
 #pragma unroll
-        for (int i = 0; i + 1 < V; ++i) k[i] = (k[i + 1] & up) | (k[i] & ~up);
-        k[V - 1] &= ~up;
+        for (int i = 0; i + 1 < H; ++i) k[i] = (k[i + 1] & up) | (k[i] & ~up);
+        k[H - 1] &= ~up;
     }
     __builtin_amdgcn_wave_barrier();
     const bool masked = live && a.mask && !a.mask[row];
@@ -509,6 +515,14 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(RouteArgs a) {
         }
 }
 
+template <int DT, int V>
+void fwd16(const RouteArgs &a, unsigned grid, size_t lds, hipStream_t s) {
+    if (a.k <= 8)
+        route_fwd16_kernel<DT, V, 8><<<grid, 256, lds, s>>>(a);
+    else
+        route_fwd16_kernel<DT, V, 16><<<grid, 256, lds, s>>>(a);
+}
+
 // What 16 lanes a row take: their experts in registers, the groups as whole
 // lanes.
 bool in16(const RouteArgs &a) {
@@ -521,15 +535,15 @@ hipError_t fwd_of(const RouteArgs &a, hipStream_t s) {
     if (in16(a)) {
         const unsigned grid = (unsigned)((a.rows + 15) / 16);
         if (a.experts <= 16)
-            route_fwd16_kernel<DT, 1><<<grid, 256, lds, s>>>(a);
+            fwd16<DT, 1>(a, grid, lds, s);
         else if (a.experts <= 32)
-            route_fwd16_kernel<DT, 2><<<grid, 256, lds, s>>>(a);
+            fwd16<DT, 2>(a, grid, lds, s);
         else if (a.experts <= 64)
-            route_fwd16_kernel<DT, 4><<<grid, 256, lds, s>>>(a);
+            fwd16<DT, 4>(a, grid, lds, s);
         else if (a.experts <= 128)
-            route_fwd16_kernel<DT, 8><<<grid, 256, lds, s>>>(a);
+            fwd16<DT, 8>(a, grid, lds, s);
         else
-            route_fwd16_kernel<DT, 16><<<grid, 256, lds, s>>>(a);
+            fwd16<DT, 16>(a, grid, lds, s);
         return hipGetLastError();
     }
     const unsigned grid = (unsigned)((a.rows + 3) / 4);
