@@ -1046,7 +1046,7 @@ int lsmx_rms_norm(const void *x, int64_t ldx, const void *r, int64_t ldr, int dt
 
 int64_t lsmx_rms_norm_bwd_workspace(int64_t rows, int64_t dim, int dtype) {
     if (norm_check("lsmx_rms_norm_bwd_workspace", dtype, dtype, rows, dim, 0.f)) return 0;
-    return rows && dim ? (int64_t)lsmx::norm_bwd_groups(rows, dim, dtype) * dim * 4 : 0;
+    return rows && dim ? (int64_t)lsmx::norm_bwd_groups(rows) * dim * 4 : 0;
 }
 
 int lsmx_rms_norm_bwd(const void *h, int64_t ldh, const void *dy, int64_t lddy, const void *dh, int64_t lddh, int dtype,

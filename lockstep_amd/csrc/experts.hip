@@ -15,13 +15,21 @@
 // largest exponent among them; beyond those eight its sums are fp32.  E4M3 spans
 // more than that: rows with both large and small codes lose 4e-6 of a result
 // (rms, normal values).  The forms that wait for memory take each row's codes of
-// 2 and more and those below in two instructions, which is exact; the form for
-// many rows, bound by the matrix cores, does not (twice its time).
+// 2 and more and those below in two instructions, which is exact; the forms for
+// many rows, bound by the matrix cores, do not (twice the instructions).
+//
+// What bounds them.  Few rows: an expert's weights are read once, F N 17/32
+// bytes each, at the rate of a large copy (4.9 TB/s): 64 tokens that choose 8 of
+// 128 experts, K = 4096, F = 1024, read nearly all of 571 MB in 110 us.  Many
+// rows: the matrix cores, which alone, from registers, run these types at 3.6
+// PF/s; 8192 tokens of 4 of 32 experts, K = 4096, F = 2048 take 460 us gated
+// (2.4 PF/s; codes and weights through LDS keep them busy half of the time, the
+// gate and its rounding are a tenth of a tile), 362 us combined (K = 2048, N =
+// 4096; the products 250 us, a pair's rows written and read 110).
 //
 // Pairs come sorted by expert (order, offsets); a workgroup finds the expert
 // and the pairs of its tile from the offsets.  Nothing in order or offsets is
 // trusted to be in range.
-#include <cstdlib>
 #include "lsmx_block.h"
 #include "lsmx_dma.h"
 #include "lsmx_internal.h"
@@ -57,17 +65,6 @@ struct Tile {
 };
 
 LSMX_DEV int lane_of(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
-
-// Sums of a wave's lanes up to each.
-LSMX_DEV int scan64(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast 15, 31
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-    return v;
-}
 
 // Every expert's pairs in tiles of `height`, then those of the pairs of no
 // expert, each tile `blocks` times; an expert's tiles of one block are
@@ -109,6 +106,7 @@ LSMX_DEV Tile find_tile(const int32_t *offsets, int experts, int pairs, int heig
     const int tiles = (n + height - 1) / height;
     if (tiles == 0) return Tile{0, 0, 0, 0};
     const int block = left / tiles, m = left - block * tiles;
+    if (left < 0 || block >= blocks) return Tile{0, 0, 0, 0};   // sums that passed 31 bits: no dispatch's offsets
     return Tile{e, start + m * height, min(n - m * height, height), block};
 }
 // Workgroups that hold every tile, whatever the offsets.
@@ -149,7 +147,9 @@ LSMX_DEV void zero_rows(const ExpertArgs &a, const Tile &tile, int threads, int 
 // 8 waves for 64 rows of W (gated: 32 of the gate, the same 32 of up) and up to
 // 16 pairs of one expert: the waves split K, take the weights from memory
 // straight into registers, two steps of 128 at a time, and add their sums up in
-// LDS.
+// LDS.  With so few workgroups the time is one pass over K in latency: 8 waves
+// a workgroup shorten it, and a ring in LDS would only lengthen it (4 experts,
+// K = 2048, F = 1024: 8.3 us).
 template <bool GATED>
 __global__ __launch_bounds__(512) void expert_stream_kernel(ExpertArgs a) {
     constexpr int KW = 8;
@@ -245,6 +245,10 @@ __global__ __launch_bounds__(512) void expert_stream_kernel(ExpertArgs a) {
 // addresses of each lane's own row, so that nothing is gathered first.  Scales
 // come four stages at a time: a load of 4 bytes a row would read as many cache
 // lines each stage as the codes do.  One barrier a stage.
+//
+// Tiles of up to 48 pairs have four waves and half of the LDS, two workgroups a
+// CU: one's loads stand under the other's products.  128 and 256 pairs, where
+// an expert has them, read W less often.
 template <int BT, int NW>
 struct TileShape {
     static constexpr int WM = NW == 4 || BT < 256 ? 4 : 2, WT = NW / WM, NT = 64 * NW;
@@ -264,7 +268,7 @@ template <bool GATED, int BT, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void expert_tile_kernel(ExpertArgs a) {
     typedef TileShape<BT, NW> S;
     constexpr int A = S::A, B = S::B, L = S::L, G = 4;   // G: stages of a group of scales
-    constexpr bool EXACT = BT == 16;   // in time that its loads leave over (64 pairs a tile: 55 us, exact 83)
+    constexpr bool EXACT = BT == 16;   // in time that its loads leave over (at 64 pairs: 55 us, exact 83)
     __shared__ __attribute__((aligned(16))) uint8_t lds[S::LDS];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), i16 = lane & 15, g = lane >> 4;
     const int wm = wave % S::WM, wt = wave / S::WM;
@@ -467,8 +471,9 @@ __global__ __launch_bounds__(64 * NW, 2) void expert_tile_kernel(ExpertArgs a) {
                 }
             }
         } else if (a.zs) {
-            // rows of z in 16 bits: fp16 over the largest power of two among 64
-            // elements, 2^-12 of each
+            // rows of z in 16 bits: fp16 with a power of two for 64 elements that
+            // puts the largest at 2^14 to 2^15; within 2^-11 of each down to 2^-28
+            // of the largest, an eighth of bf16's own rounding
 #pragma unroll
             for (int b = 0; b < A / 4; ++b) {
                 uint32_t am = 0;
@@ -507,7 +512,8 @@ __global__ __launch_bounds__(64 * NW, 2) void expert_tile_kernel(ExpertArgs a) {
 }
 
 // y_t = sum_j weight_tj z_tj over the pairs that have an expert, in the order of
-// their slots; 8 elements a thread.
+// their slots, in fp32; 8 elements a thread.  Sums by atomics in the products'
+// epilogue would need no z, but their order, and the result, would change.
 template <int DT, bool HALF>
 __global__ __launch_bounds__(256) void expert_join_kernel(ExpertArgs a) {
     typedef typename Elem<DT>::S S;
@@ -521,11 +527,11 @@ __global__ __launch_bounds__(256) void expert_join_kernel(ExpertArgs a) {
         const int64_t p = token * a.k + j;
         if ((uint32_t)a.ids[p] >= (uint32_t)a.experts) continue;
         if constexpr (HALF) {
-            const float w = a.weights[p] * a.zs[p * ((a.N + 63) / 64) + n / 64];
+            const float w = a.weights[p], scale = a.zs[p * ((a.N + 63) / 64) + n / 64];
             typedef _Float16 v8h __attribute__((ext_vector_type(8)));
             const v8h z = *(const v8h *)((const _Float16 *)a.z + p * a.ldz + n);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += w * (float)z[i];
+            for (int i = 0; i < 8; ++i) v[i] += w * ((float)z[i] * scale);
         } else {
             const float w = a.weights[p];
             const v4f z0 = *(const v4f *)(a.z + p * a.ldz + n), z1 = *(const v4f *)(a.z + p * a.ldz + n + 4);
@@ -557,27 +563,42 @@ hipError_t tiles(const ExpertArgs &a, hipStream_t s) {
     expert_tile_kernel<GATED, BT, NW><<<(unsigned)tile_units(a.pairs, a.experts, BT, (a.N + 255) / 256), 64 * NW, 0, s>>>(a);
     return hipGetLastError();
 }
-template <bool GATED>
-hipError_t products(const ExpertArgs &a, hipStream_t s) {
-    if (a.K < 512) return stream<GATED>(a, s);
+// Pairs of a tile, or 0 for the stream kernel.  us at 32 experts, K = 2048,
+// F = 1024, by pairs an expert (gated; combine, its K = 1024, alike):
+//            1     4     8    24    48    96   128   256   512  1024
+//   stream  14.3  26.3  31.7
+//     16    12.7  15.3  20.0  29.6  33.1  53.3
+//     32    11.9  14.5  14.9  19.4  28.4  32.6  40.2
+//     48    12.9  15.2  15.5  21.5  21.9  30.0  39.1  55.1  107   226
+//    128    13.4  15.3  15.7  20.2  30.3  35.0  35.1  55.1   90.7 191
+//    256    18.3  19.8  19.9  21.7  28.8  46.5  45.4  58.0   88.2 153
+// and with 128 experts, where the weights do not stay in the caches:
+//     16    26.7  45.1  53.9  81.5 128
+//     32    26.4  44.9  47.2  61.5  85.3
+//     48    27.1  45.9  47.6  58.2  77.6 113.5 136   258   446   814
+//    128    31.9  54.6  56.8  64.3  82.1 110.1 132   206   362   671
+//    256    39.1  71.4  72.0  75.1  88.5 116.4 131   188   322   575
+// Pairs are not spread evenly; 16 where it costs little, for its exact products.
+int height_of(const ExpertArgs &a) {
+    // a tile needs two groups' worth of stages; up to 384 workgroups, more waves
+    // for each (4 pairs, K = 2048, F = 1024: 8.3 against 10.0 us)
+    if (a.K < 512 || (int64_t)a.pairs * ((a.N + 63) / 64) <= 384) return 0;
     const int64_t per = a.pairs / a.experts;
-    if (const char *f = getenv("LSMX_EXP")) {
-        switch (atoi(f)) {
-            case 1: return stream<GATED>(a, s);
-            case 16: return tiles<GATED, 16, 4>(a, s);
-            case 32: return tiles<GATED, 32, 4>(a, s);
-            case 48: return tiles<GATED, 48, 4>(a, s);
-            case 128: return tiles<GATED, 128, 8>(a, s);
-            case 256: return tiles<GATED, 256, 8>(a, s);
-        }
-    }
-    if (a.pairs * ((a.N + 63) / 64) <= 384) return stream<GATED>(a, s);
-    if (per <= 4) return tiles<GATED, 16, 4>(a, s);
-    if (per <= 24) return tiles<GATED, 32, 4>(a, s);
-    if (per <= 96) return tiles<GATED, 48, 4>(a, s);
-    // 256 pairs where such tiles fill the CUs three times over, or are full
+    if (per <= 96) return per <= 4 ? 16 : per <= 24 ? 32 : 48;
+    // full tiles, or as many as fill the 256 CUs three times
     const int64_t units = (a.pairs / 256 + a.experts / 2) * ((a.N + 255) / 256);
-    return per > 400 || units >= 768 ? tiles<GATED, 256, 8>(a, s) : tiles<GATED, 128, 8>(a, s);
+    return per > 400 || units >= 768 ? 256 : 128;
+}
+template <bool GATED>
+hipError_t products(const ExpertArgs &a, int height, hipStream_t s) {
+    switch (height) {
+        case 16: return tiles<GATED, 16, 4>(a, s);
+        case 32: return tiles<GATED, 32, 4>(a, s);
+        case 48: return tiles<GATED, 48, 4>(a, s);
+        case 128: return tiles<GATED, 128, 8>(a, s);
+        case 256: return tiles<GATED, 256, 8>(a, s);
+        default: return stream<GATED>(a, s);
+    }
 }
 
 template <int DT>
@@ -592,14 +613,16 @@ hipError_t join(const ExpertArgs &a, hipStream_t s) {
 
 }  // namespace
 
-hipError_t launch_expert_gated(const ExpertArgs &a, hipStream_t s) { return products<true>(a, s); }
+hipError_t launch_expert_gated(const ExpertArgs &a, hipStream_t s) { return products<true>(a, height_of(a), s); }
 
 hipError_t launch_expert_combine(const ExpertArgs &a0, hipStream_t s) {
     ExpertArgs a = a0;
-    // bf16 sums of many rows take the pairs' rows in 16 bits, where writing and
-    // reading them costs more than the products
-    if (a.y_dtype == LSMX_BF16 && a.K >= 512 && a.pairs / a.experts > 24) a.zs = (float *)((uint8_t *)a.z + (int64_t)a.pairs * a.ldz * 2);
-    const hipError_t e = products<false>(a, s);
+    const int height = height_of(a);
+    // bf16 sums of many rows take the pairs' rows in 16 bits.  us with them in 32
+    // and in 16, 128 experts, K = 1024, N = 2048, by pairs an expert:
+    //   32 45.7 43.9   48 53.7 51.8   96 97.3 76.8   192 164 145   512 409 318
+    if (a.y_dtype == LSMX_BF16 && height >= 48) a.zs = (float *)((uint8_t *)a.z + (int64_t)a.pairs * a.ldz * 2);
+    const hipError_t e = products<false>(a, height, s);
     if (e != hipSuccess) return e;
     return a.y_dtype == LSMX_F32 ? join<LSMX_F32>(a, s) : a.y_dtype == LSMX_BF16 ? join<LSMX_BF16>(a, s) : join<LSMX_F16>(a, s);
 }

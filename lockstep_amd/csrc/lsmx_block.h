@@ -51,6 +51,17 @@ LSMX_DEV uint32_t e4m3_x4(float a, float b, float c, float d) {
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
+// Sums of a wave's lanes up to each.
+LSMX_DEV int scan64(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast 15, 31
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+
 // --------------------------------------------------------------- arguments
 struct NormArgs {
     const void *x, *r, *w;   // r null: no residual
@@ -96,7 +107,7 @@ struct ExpertArgs {
 };
 
 hipError_t launch_norm_fwd(const NormArgs &a, hipStream_t s);
-int norm_bwd_groups(int64_t rows, int64_t dim, int dtype);
+int norm_bwd_groups(int64_t rows);
 hipError_t launch_norm_bwd(const NormBwdArgs &a, hipStream_t s);
 hipError_t launch_route_fwd(const RouteArgs &a, hipStream_t s);
 hipError_t launch_route_bwd(const RouteArgs &a, hipStream_t s);

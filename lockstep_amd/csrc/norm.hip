@@ -6,7 +6,9 @@
 // Forward and backward read each operand once: a row stays in the registers
 // of the threads that hold it (fp32) between the sum of squares and the
 // output.  Sums are fp32; they have one order, so results do not depend on
-// the run.  Memory bound.
+// the run.  Memory bound: 8192 rows of 8192 in bf16 with a residual and MXFP8
+// in 107 us (5.7 TB/s; a large copy makes 4.9), backward with dw of 8190 rows of
+// 4096 in fp16 42 us.
 #include "lsmx_block.h"
 
 namespace lsmx {
@@ -288,7 +290,7 @@ hipError_t fwd(const NormArgs &a, hipStream_t s) {
 }
 template <int DT, int VEC, int NV, int TPR>
 hipError_t bwd(const NormBwdArgs &a, hipStream_t s) {
-    norm_bwd_kernel<DT, VEC, NV, TPR><<<(unsigned)norm_bwd_groups(a.rows, a.dim, a.dtype), TPR, 0, s>>>(a);
+    norm_bwd_kernel<DT, VEC, NV, TPR><<<(unsigned)norm_bwd_groups(a.rows), TPR, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -297,6 +299,21 @@ bool rows_of_vectors(const void *p, int64_t ld, int64_t dim, int dtype) {
     return dim % 8 == 0 && (reinterpret_cast<uintptr_t>(p) % 16) == 0 && (ld * b) % 16 == 0;
 }
 
+// Threads and vectors a row.  A row in more threads is done sooner, which counts
+// for few rows; many rows hide one another's latency, and threads of several
+// vectors have fewer barriers and sums.  us in bf16 with a residual and MXFP8:
+//   dim   rows    1024x1  512x2  512x1  256x4  256x2  256x1  64x2
+//   1024     8                                           2.5    3.3
+//          512                                           2.9    3.7
+//         8192                                          14.7   13.2
+//   4096     8                    2.7            3.5
+//          512                    4.5            5.0
+//         8192                   52.5           51.0
+//   8192     8       3.1    3.5           5.1
+//          512       7.5    7.3           8.2
+//         2048      24.8   23.8          23.0
+//         8192     107    112            121
+// and 16384: 1024x2 24.0 and 219 us (1024, 8192 rows), 1024x4 26.2 and 229.
 template <int DT>
 hipError_t fwd_of(const NormArgs &a, hipStream_t s) {
     const bool vec = rows_of_vectors(a.x, a.ldx, a.dim, DT) && (!a.r || rows_of_vectors(a.r, a.ldr, a.dim, DT)) &&
@@ -304,10 +321,12 @@ hipError_t fwd_of(const NormArgs &a, hipStream_t s) {
                      rows_of_vectors(a.h, a.dim, a.dim, DT);
     if (vec) {
         if (a.dim <= 512) return fwd<DT, 8, 1, 64>(a, s);
-        if (a.dim <= 1024) return fwd<DT, 8, 2, 64>(a, s);
+        if (a.dim <= 1024 && a.rows >= 2048) return fwd<DT, 8, 2, 64>(a, s);
         if (a.dim <= 2048) return fwd<DT, 8, 1, 256>(a, s);
-        if (a.dim <= 4096) return fwd<DT, 8, 2, 256>(a, s);
-        if (a.dim <= 8192) return fwd<DT, 8, 4, 256>(a, s);
+        if (a.dim <= 4096) return a.rows <= 512 ? fwd<DT, 8, 1, 512>(a, s) : fwd<DT, 8, 2, 256>(a, s);
+        // few rows, or more than the caches hold
+        if (a.dim <= 8192) return a.rows <= 256 || a.rows > 4096 ? fwd<DT, 8, 1, 1024>(a, s) : fwd<DT, 8, 2, 512>(a, s);
+        if (a.dim <= 16384) return fwd<DT, 8, 2, 1024>(a, s);
         if (a.dim <= 32768) return fwd<DT, 8, 4, 1024>(a, s);
         return fwd<DT, 8, 0, 1024>(a, s);
     }
@@ -317,6 +336,10 @@ hipError_t fwd_of(const NormArgs &a, hipStream_t s) {
     return fwd<DT, 1, 0, 1024>(a, s);
 }
 
+// The same for the backward pass, whose workgroups keep dw's share besides.  us
+// of 8192 rows with dh and dw in bf16: 4096 256x2 42.0, 512x1 43.2; 8192 512x2
+// 94.5, 1024x1 117, 256x4 124; 16384 1024x2 202, two passes 376; of 512 rows of
+// 32768 two passes 72, 1024x4 88.
 template <int DT>
 hipError_t bwd_of(const NormBwdArgs &a, hipStream_t s) {
     const bool vec = rows_of_vectors(a.h, a.ldh, a.dim, DT) && rows_of_vectors(a.dy, a.lddy, a.dim, DT) &&
@@ -325,7 +348,8 @@ hipError_t bwd_of(const NormBwdArgs &a, hipStream_t s) {
     if (vec) {
         if (a.dim <= 2048) return bwd<DT, 8, 1, 256>(a, s);
         if (a.dim <= 4096) return bwd<DT, 8, 2, 256>(a, s);
-        if (a.dim <= 8192) return bwd<DT, 8, 4, 256>(a, s);
+        if (a.dim <= 8192) return bwd<DT, 8, 2, 512>(a, s);
+        if (a.dim <= 16384) return bwd<DT, 8, 2, 1024>(a, s);
         return bwd<DT, 8, 0, 1024>(a, s);
     }
     if (a.dim <= 2048) return bwd<DT, 1, 8, 256>(a, s);
@@ -339,16 +363,13 @@ hipError_t launch_norm_fwd(const NormArgs &a, hipStream_t s) {
     return a.dtype == LSMX_F32 ? fwd_of<LSMX_F32>(a, s) : a.dtype == LSMX_BF16 ? fwd_of<LSMX_BF16>(a, s) : fwd_of<LSMX_F16>(a, s);
 }
 
-// Workgroups of the backward pass: rows that fill the 256 CUs, at most 1024.
-int norm_bwd_groups(int64_t rows, int64_t dim, int dtype) {
-    const int64_t most = 1024;
-    return (int)(rows < most ? rows : most);
-}
+// Workgroups of the backward pass: four a CU, each with a share of dw.
+int norm_bwd_groups(int64_t rows) { return (int)(rows < 1024 ? rows : 1024); }
 
 hipError_t launch_norm_bwd(const NormBwdArgs &a, hipStream_t s) {
     hipError_t e = a.dtype == LSMX_F32 ? bwd_of<LSMX_F32>(a, s) : a.dtype == LSMX_BF16 ? bwd_of<LSMX_BF16>(a, s) : bwd_of<LSMX_F16>(a, s);
     if (e != hipSuccess || !a.dw) return e;
-    const int groups = norm_bwd_groups(a.rows, a.dim, a.dtype);
+    const int groups = norm_bwd_groups(a.rows);
     const unsigned grid = (unsigned)((a.dim + 15) / 16);
     if (a.w_dtype == LSMX_F32)
         norm_dw_kernel<LSMX_F32><<<grid, 1024, 0, s>>>(a.part, groups, a.dim, a.dw);

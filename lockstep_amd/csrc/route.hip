@@ -7,6 +7,12 @@
 //
 // Choices are made in 64 bits: two scores may lie nearer to each other than
 // 32 bits tell apart, and the choice is a whole number.
+//
+// Few rows are a matter of latency: 64 rows of 256 experts in 8 groups, sigmoid
+// with a bias, 6.6 us.  Many are bound by the vector units, not by the logits'
+// bytes: 30001 of those rows in 28 us, of which 6 are the bytes at a copy's rate;
+// sorting a lane's 16 words, then a maximum over 16 lanes for each choice, is
+// most of it.  Backward 30001 x 64 of bf16 5.4 us.
 #include "lsmx_block.h"
 
 namespace lsmx {
@@ -524,9 +530,16 @@ void fwd16(const RouteArgs &a, unsigned grid, size_t lds, hipStream_t s) {
 }
 
 // What 16 lanes a row take: their experts in registers, the groups as whole
-// lanes.
+// lanes.  One row that 64 bits have to look at makes the call as long as the
+// other kernel and more: with a bias or groups, a few rows rarely have one, many
+// have the time; between them the other kernel is quicker (us, 256 experts,
+// sigmoid with a bias: 64 rows 6.2 against 6.3, 1024 10.2 against 6.7, 4096 10.4
+// against 9.5, 8192 12.6 against 14.5; in 8 groups 6.6 against 9.6, 12.7 against
+// 9.5, 13.0 against 13.1, 16.0 against 21.5).
 bool in16(const RouteArgs &a) {
-    return a.experts <= 256 && a.k <= 16 && (a.top_groups == a.groups || (a.experts % 16 == 0 && 16 % a.groups == 0));
+    const bool grouped = a.top_groups < a.groups;
+    return a.experts <= 256 && a.k <= 16 && (!grouped || (a.experts % 16 == 0 && 16 % a.groups == 0)) &&
+           ((!a.bias && !grouped) || a.rows <= 128 || a.rows > 4096);
 }
 
 template <int DT>
@@ -595,17 +608,6 @@ hipError_t bwd_of(const RouteArgs &a, hipStream_t s) {
 // expert find their rank from the ballots of its bits.  Ids outside the
 // experts count as expert `experts`, behind the others.
 constexpr int kDispWaves = 16, kDispPairs = 4096;
-
-// Sums of a wave's lanes up to each.
-LSMX_DEV int scan64(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // row_bcast 15, 31
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-    return v;
-}
 
 // One round of a wave: each lane's rank among the wave's pairs of its expert so
 // far, the counts brought up to date.

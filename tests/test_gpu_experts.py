@@ -285,3 +285,41 @@ def test_a_layer_as_it_is_used(dev, T):
         graph.replay()
         torch.cuda.synchronize()
         assert same(held, layer())
+
+
+@pytest.mark.parametrize("T,k,E,K,N", [(30, 1, 1, 512, 64), (60, 2, 1, 640, 130), (100, 1, 2, 1024, 192), (384, 1, 4, 512, 33), (97, 1, 1, 512, 257)])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+def test_many_rows_of_few_experts_in_few_workgroups(dev, T, k, E, K, N, out_dtype):
+    """Where the rows of an expert are many, but its rows of W few."""
+    from lockstep_amd import experts
+    h, hs = _rows(dev, (T, k, K), T + K)
+    w, ws = _weights(dev, E, N, K, N)
+    ids = _ids(dev, T, k, E, T) if k <= E else torch.zeros((T, k), dtype=torch.int32, device=dev)
+    rw = torch.randn((T, k), generator=torch.Generator(device=dev).manual_seed(1), device=dev)
+    y = experts.expert_combine(h, hs, w, ws, experts.dispatch(ids, E), rw, out_dtype=out_dtype)
+    out, mag = _products(_values8(h, hs), ids, w, ws, True)
+    c = rw.double()[..., None]
+    want, mag = (out * c).sum(1), (mag * c.abs()).sum(1)
+    assert ((y.double() - want).abs() <= want.abs() * torch.finfo(out_dtype).eps / 2 + mag * (IN_BLOCK + 2.0 ** -11)).all()
+
+
+def test_large_blocks_large_weights_and_zeros(dev):
+    """bf16 sums of many rows at the ends of fp32: a row of W that is zero gives 0
+    beside one that gives 2^120, whatever the weight; an infinite product stays one."""
+    from lockstep_amd import experts
+    T, E, K, N = 200, 1, 512, 320
+    h = torch.full((T, 1, K), 2.0, device=dev).to(torch.float8_e4m3fn)
+    hs = torch.full((T, 1, K // 32), 127, dtype=torch.uint8, device=dev)
+    hs[50:] = 127 + 100
+    w = torch.full((E, N, K // 2), 0x22, dtype=torch.uint8, device=dev)      # ones
+    w[:, ::2] = 0
+    ws = torch.full((E, N, K // 32), 127 + 10, dtype=torch.uint8, device=dev)
+    ids = torch.zeros((T, 1), dtype=torch.int32, device=dev)
+    rw = torch.full((T, 1), 2.0 ** 5, device=dev)
+    rw[100:] = 2.0 ** -100
+    rw[150:] = 2.0 ** 17        # with 2^120: infinite, and 2^17 beside the block's scale
+    y = experts.expert_combine(h, hs, w, ws, experts.dispatch(ids, E), rw)
+    want = torch.zeros((T, N), dtype=torch.float64, device=dev)
+    want[:50, 1::2], want[50:100, 1::2], want[100:150, 1::2] = 2.0 ** 25, 2.0 ** 125, 2.0 ** 20
+    want[150:, 1::2] = float("inf")
+    assert torch.equal(y.double(), want)
