@@ -19,6 +19,7 @@
 #include <ATen/TracerMode.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <ATen/autocast_mode.h>
 #include <torch/csrc/Dtype.h>
@@ -26,6 +27,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <cmath>
 
@@ -781,6 +783,36 @@ torch::autograd::variable_list once(torch::autograd::variable_list d) {
     return (*err)(std::move(in));
 }
 
+// Refuses a differentiable call that is being captured into a graph while a node
+// that its gradients would go to belongs to another stream, as a leaf's does of
+// which an eager graph is still alive: in the backward pass the engine would make
+// that stream wait for the captured one, which ends the process.  `capturing`:
+// of the current stream, or as a test has it.
+bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
+void one_stream(const Tensor &t, bool capturing) {
+    if (!capturing || !t.requires_grad()) return;
+    const auto node = t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node) return;
+    const auto there = node->stream();
+    TORCH_CHECK(!there || there->device_type() != at::kCUDA ||
+                    there->id() == c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(there->device_index()).id(),
+                "a differentiable call cannot be captured while a graph of its tensors made on another stream is alive: free that "
+                "graph's outputs first, make it on the stream of the capture, or capture the call under torch.no_grad()");
+}
+
+// captures(tensors, capturing): the same for the nodes in Python; capturing None:
+// of the current stream
+PyObject *captures(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    NONE_IF(n != 2 || !PyTuple_Check(a[0]));
+    bool c = false;
+    if (!bool_arg(a[1], c)) c = capturing();
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[0]); ++i)
+        if (const Tensor *t = plain(PyTuple_GET_ITEM(a[0], i))) one_stream(*t, c);
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
 struct NormOut {
     Tensor y, h, codes, scale;
 };
@@ -865,6 +897,11 @@ PyObject *rms_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const bool grad = at::GradMode::is_enabled() && (x->requires_grad() || w->requires_grad() || (r && r->requires_grad()));
     torch::autograd::variable_list out;
     int rc = LSMX_OK;
+    if (grad) {
+        const bool c = capturing();
+        one_stream(*x, c), one_stream(*w, c);
+        if (r) one_stream(*r, c);
+    }
     {
         NoGil released;
         try {
@@ -958,10 +995,12 @@ PyObject *route(PyObject *, PyObject *const *a, Py_ssize_t n) {
             (m && (!dense(m, at::kBool) || !m->sizes().equals(lead) || m->device() != l->device())));
     RouteOut o;
     int rc = LSMX_OK;
+    const bool grad = at::GradMode::is_enabled() && l->requires_grad();
+    if (grad) one_stream(*l, capturing());
     {
         NoGil released;
         try {
-            if (at::GradMode::is_enabled() && l->requires_grad()) {
+            if (grad) {
                 const auto v = Route::apply(*l, b ? std::optional<Tensor>(b->detach()) : std::nullopt, m ? std::optional<Tensor>(*m) : std::nullopt,
                                             k, !soft, groups, top, renorm, scale);
                 o = {v[0], v[1]};
@@ -1083,7 +1122,7 @@ PyObject *init(PyObject *, PyObject *const *a, Py_ssize_t n) {
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(init),   FAST(quantize_pack), FAST(quantize_pack2), FAST(quantize), FAST(quantize_2d), FAST(pack),
                          FAST(gemm_packed), FAST(linear), FAST(weight), FAST(gemm_fp8),
-                         FAST(attention), FAST(kv_append), FAST(kv_attend), FAST(kv_evict), FAST(rms_norm), FAST(route),
+                         FAST(attention), FAST(kv_append), FAST(kv_attend), FAST(kv_evict), FAST(rms_norm), FAST(route), FAST(captures),
                          FAST(dispatch), FAST(expert_gated), FAST(expert_combine), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -100,7 +100,8 @@ def add_rms_norm(x, weight, residual=None, *, eps=1e-6, mxfp8=False):
     [.., D // 32]), the row-major form that mxfp4_gemm_fp8 takes.
 
     Differentiable in x, residual and weight (once, in reverse mode; the
-    codes have no gradient).  The mean, the norm and every sum are fp32; y is
+    codes have no gradient).  A differentiable call is not captured into a HIP
+    graph while an eager graph of its tensors, made on another stream, is alive.  The mean, the norm and every sum are fp32; y is
     rounded once, its codes are of the unrounded y.  Deterministic."""
     if (r := C.fast.rms_norm(x, weight, residual, eps, mxfp8)) is not None:
         return r
@@ -125,6 +126,7 @@ def add_rms_norm(x, weight, residual=None, *, eps=1e-6, mxfp8=False):
     # a dual tensor too goes to the node, which refuses it
     if (torch.is_grad_enabled() and any(t.requires_grad for t in both)) or \
             any(forward_ad.unpack_dual(t).tangent is not None for t in both):
+        C.fast.captures(both, None)
         y, h, codes, scale = _AddRMSNorm.apply(x, weight, residual, eps, bool(mxfp8))
     else:
         _, y, h, codes, scale = _forward(x, weight, residual, eps, bool(mxfp8))
