@@ -197,9 +197,12 @@ __global__ __launch_bounds__(256) void route_fwd_kernel(RouteArgs a) {
 // its own once, and a choice is then a maximum over 16 heads.
 //
 // Without a bias experts rank by their logits: 16-bit logits leave room for the
-// whole index, and words never tie.  Otherwise ranks are fp32 within 2^-20 of
-// the score's size (two roundings of exp, one of the sum and the quotient), 4
-// low bits lost: together within 4e-6 (1 + |c|).  Where two neighbours of the
+// whole index, and words never tie; fp32 ones lose 4 low bits, and tie where the
+// others are equal.  With a bias ranks are fp32, and two of them may be wrong by
+// both scores' errors (a sigmoid's 2.5e-7 each: exp, the sum, the reciprocal; a
+// softmax's 2e-6 for both: the sum of up to 256 terms in 20 roundings), the
+// additions' 2^-24 each and the 4 low bits, 15 * 2^-23 |c|: 2.2e-6 |c| and 6e-7
+// or 2.2e-6.  A group's score adds two such errors.  Where two neighbours of the
 // choice, or two groups, are too near to be told apart, the wave takes that row
 // again in 64 bits.
 
@@ -318,6 +321,7 @@ __global__ __launch_bounds__(256) void route_fwd16_kernel(RouteArgs a) {
     }
     sort_down<V>(k);
     bool near = false;
+    const float off = a.sigmoid ? 6e-7f : 2.2e-6f;   // of two scores
     if (grouped) {
         // 16 / groups lanes a group: its two largest from their lanes' two
         uint32_t u = k[0], w = V > 1 ? k[1] : 0u;
@@ -331,15 +335,26 @@ __global__ __launch_bounds__(256) void route_fwd16_kernel(RouteArgs a) {
         if (per > 4) merge(__shfl_xor((int)u, 4, 64), __shfl_xor((int)w, 4, 64));
         const float fu = unordered(u & ~low), fw = unordered(w & ~low);
         const bool two = a.experts > a.groups;   // else a group's one is its score
-        const float s = scored ? fu + (two ? fw : 0.f) : score(fu) + (two ? score(fw) : 0.f);
+        // the group's score and how far it may be off
+        float s, tol;
+        if (scored) {
+            s = fu + (two ? fw : 0.f);
+            tol = 2.2e-6f * (__builtin_fabsf(fu) + __builtin_fabsf(two ? fw : 0.f)) + 2.f * off;
+        } else {
+            // a logit's lost bits change a softmax's score s by 15 * 2^-23 |l| s, a
+            // sigmoid's by less than 0.23 of 15 * 2^-23
+            const float su = score(fu), sw = two ? score(fw) : 0.f;
+            s = su + sw;
+            tol = 2.f * off + (a.sigmoid ? 1e-6f : 2e-6f * (su > 0.f ? su * __builtin_fabsf(fu) : 0.f) + 2e-6f * (sw > 0.f ? sw * __builtin_fabsf(fw) : 0.f));
+        }
+        const float lo = s - tol, hi = s + tol;
         // groups surely and perhaps ahead of this lane's
         int ahead = 0, perhaps = 0;
-        const float tol = 2e-5f * (1.f + __builtin_fabsf(s));
-        auto look = [&](float o) __attribute__((always_inline)) {
-            ahead += o > s + tol;
-            perhaps += !(o < s - tol);
+        auto look = [&](float olo, float ohi) __attribute__((always_inline)) {
+            ahead += olo > hi;
+            perhaps += !(ohi < lo);
         };
-#define LOOK(n) look(u2f(ror16<n>(f2u(s))))
+#define LOOK(n) look(u2f(ror16<n>(f2u(lo))), u2f(ror16<n>(f2u(hi))))
         LOOK(8);
         if (per <= 4) LOOK(4), LOOK(12);
         if (per <= 2) LOOK(2), LOOK(6), LOOK(10), LOOK(14);
@@ -363,7 +378,7 @@ __global__ __launch_bounds__(256) void route_fwd16_kernel(RouteArgs a) {
             near |= (wins & (wins - 1)) != 0;
             if (j > 0) {
                 const float p = unordered(last & ~low), q = unordered(best & ~low);
-                near |= scored ? !(p - q > 5e-6f * (1.f + __builtin_fabsf(p))) : (last & ~low) == (best & ~low);
+                near |= scored ? !(p - q > 2.2e-6f * __builtin_fabsf(p) + off) : (last & ~low) == (best & ~low);
             }
         }
         last = best;

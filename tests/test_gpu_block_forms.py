@@ -374,3 +374,25 @@ def test_a_capture_while_an_eager_graph_lives(dev):
         torch.cuda.synchronize()
         assert all(torch.isfinite(g).all() for g in torch.autograd.grad(eager.sum(), t))
         del eager
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("T", [100, 5000])
+def test_groups_whose_ranks_cancel_or_logits_are_large(dev, T, scoring):
+    """A group's two largest ranks of +-1000 add up to little, with the rounding of
+    1000; a softmax of logits near 3000 depends on what 32 bits hold of them."""
+    E, k, G = 128, 4, 16
+    g = torch.Generator(device=dev).manual_seed(T)
+    logits = torch.randn((T, E), generator=g, device=dev)
+    bias = torch.full((E,), -1000.0, device=dev)
+    bias[::8] = 1000.0
+    bias += (torch.randint(-4, 5, (E,), generator=g, device=dev) * 2.0 ** -13)
+    from lockstep_amd.experts import route
+    w, ids = route(logits, k, bias=bias, scoring=scoring, groups=G, top_groups=3)
+    _, at = route_tests._route64(logits, k, bias, scoring, G, 3, True, 1.0)
+    assert torch.equal(ids.long(), at)
+    big = (2990 + torch.randint(0, 40, (T, E), generator=g, device=dev) * 2.0 ** -12).float()
+    w, ids = route(big, k, scoring="softmax", groups=G, top_groups=3)
+    want, at = route_tests._route64(big, k, None, "softmax", G, 3, True, 1.0)
+    assert torch.equal(ids.long(), at) and ((w.double() - want).abs() <= want * 2.0 ** -20).all()
