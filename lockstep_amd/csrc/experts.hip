@@ -39,7 +39,6 @@ namespace lsmx {
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
-typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 
 __device__ v4f mfma_f4f8(v4i a, v8i b, v4f c, int cbsz, int blgp, int opsel_a, int scale_a, int opsel_b, int scale_b)
     __asm("llvm.amdgcn.mfma.scale.f32.16x16x128.f8f6f4.v4i32.v8i32");
@@ -54,6 +53,22 @@ LSMX_DEV v8i large_codes(v8i x) {
         x[i] &= (int)((b << 2) - (b >> 6));
     }
     return x;
+}
+
+// Maximum over the four lanes of a pair (lane, lane ^ 16, ..).
+LSMX_DEV uint32_t max4(uint32_t v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(b[0], b[1]);
+}
+// Lane g has pieces 4g .. of two tiles of 16 rows, p and q; it gets pieces 2g and
+// 2g + 1 of the 32 rows, so that its store is twice as wide and a pair's four
+// are neighbours.
+LSMX_DEV void neighbours(uint32_t &p, uint32_t &q) {
+    const auto a = __builtin_amdgcn_permlane32_swap(p, q, false, false);
+    const auto b = __builtin_amdgcn_permlane16_swap(a[0], a[1], false, false);
+    p = b[0], q = b[1];
 }
 
 // ---------------------------------------------------------------- the tiles
@@ -458,15 +473,13 @@ __global__ __launch_bounds__(64 * NW, 2) void expert_tile_kernel(ExpertArgs a) {
                     v[q] = silu_times(acc[2 * b + q / 4][j][q % 4], acc[A / 2 + 2 * b + q / 4][j][q % 4]);
                     am = max(am, f2u(v[q]) & 0x7FFFFFFFu);
                 }
-                am = max(am, (uint32_t)__shfl_xor((int)am, 16, 64));
-                am = max(am, (uint32_t)__shfl_xor((int)am, 32, 64));
-                const uint32_t byte = mx8_byte(am);
+                const uint32_t byte = mx8_byte(max4(am));
                 const float m = mx8_inverse(byte);
                 const int f = nb * 128 + wm * (A * 8) + b * 32;
+                uint32_t c0 = e4m3_x4(v[0] * m, v[1] * m, v[2] * m, v[3] * m), c1 = e4m3_x4(v[4] * m, v[5] * m, v[6] * m, v[7] * m);
+                neighbours(c0, c1);
                 if (p >= 0 && f < F) {
-                    uint8_t *h = a.h + (int64_t)p * F + f + 4 * g;
-                    *(uint32_t *)h = e4m3_x4(v[0] * m, v[1] * m, v[2] * m, v[3] * m);
-                    *(uint32_t *)(h + 16) = e4m3_x4(v[4] * m, v[5] * m, v[6] * m, v[7] * m);
+                    *(uint64_t *)(a.h + (int64_t)p * F + f + 8 * g) = (uint64_t)c1 << 32 | c0;
                     if (g == 0) a.hs[(int64_t)p * (F / 32) + f / 32] = (uint8_t)byte;
                 }
             }
@@ -484,20 +497,25 @@ __global__ __launch_bounds__(64 * NW, 2) void expert_tile_kernel(ExpertArgs a) {
                         const uint32_t u = f2u(acc[i][j][q]) & 0x7FFFFFFFu;
                         am = max(am, u < 0x7F800000u ? u : 0u);   // infinities and NaN stay what they are
                     }
-                am = max(am, (uint32_t)__shfl_xor((int)am, 16, 64));
-                am = max(am, (uint32_t)__shfl_xor((int)am, 32, 64));
-                const uint32_t e = max(am >> 23, 16u) - 14u;   // the largest below 2^15
+                const uint32_t e = max(max4(am) >> 23, 16u) - 14u;   // the largest below 2^15
                 const float m = u2f((254u - e) << 23);
                 const int n = nb * 256 + (wm * A + 4 * b) * 16;
-                if (p >= 0 && n < a.N) {
-                    _Float16 *z = (_Float16 *)a.z + (int64_t)p * a.ldz + n + 4 * g;
+                uint32_t o[4][2];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        v4h o;
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) o[q] = (_Float16)(acc[4 * b + i][j][q] * m);
-                        if (n + 16 * i + 4 * g < a.N) *(v4h *)(z + 16 * i) = o;
+                    for (int q = 0; q < 2; ++q) {
+                        typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+                        const v4f &v = acc[4 * b + i][j];
+                        o[i][q] = __builtin_bit_cast(uint32_t, v2h{(_Float16)(v[2 * q] * m), (_Float16)(v[2 * q + 1] * m)});
                     }
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) neighbours(o[i][0], o[i + 1][0]), neighbours(o[i][1], o[i + 1][1]);
+                if (p >= 0 && n < a.N) {
+                    _Float16 *z = (_Float16 *)a.z + (int64_t)p * a.ldz + n + 8 * g;   // ldz: whole eights
+#pragma unroll
+                    for (int i = 0; i < 4; i += 2)
+                        if (n + 16 * i + 8 * g < a.N) *(v4i *)(z + 16 * i) = v4i{(int)o[i][0], (int)o[i][1], (int)o[i + 1][0], (int)o[i + 1][1]};
                     if (g == 0) a.zs[(int64_t)p * ((a.N + 63) / 64) + n / 64] = u2f(e << 23);
                 }
             }
