@@ -618,11 +618,10 @@ hipError_t bwd_of(const RouteArgs &a, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------- dispatch
-// The pairs sorted by expert, stable: a counting sort.  A workgroup takes 4096
-// pairs, each of its waves 256 consecutive ones in rounds of 64; lanes of one
-// expert find their rank from the ballots of its bits.  Ids outside the
+// The pairs sorted by expert, stable: a counting sort.  A workgroup takes ROUNDS
+// times 1024 pairs, each of its waves consecutive ones in rounds of 64; lanes of
+// one expert find their rank from the ballots of its bits.  Ids outside the
 // experts count as expert `experts`, behind the others.
-constexpr int kDispWaves = 16, kDispPairs = 4096;
 
 // One round of a wave: each lane's rank among the wave's pairs of its expert so
 // far, the counts brought up to date.
@@ -641,20 +640,24 @@ LSMX_DEV int round_rank(int e, int bits, uint16_t *hist, bool live) {
     __builtin_amdgcn_wave_barrier();
     return rank;
 }
-LSMX_DEV int expert_of(const int32_t *ids, int p, int experts) {
-    const uint32_t e = (uint32_t)ids[p];
-    return e < (uint32_t)experts ? (int)e : experts;
+// of pair p, or of the last one (loads without conditions go out together)
+LSMX_DEV int expert_of(const int32_t *ids, int p, int pairs, int experts) {
+    return (int)min((uint32_t)ids[min(p, pairs - 1)], (uint32_t)experts);
 }
 
 // counts[block][expert]: the pairs of each workgroup
+template <int ROUNDS>
 __global__ __launch_bounds__(1024) void dispatch_count_kernel(const int32_t *ids, int pairs, int experts, int32_t *counts) {
     extern __shared__ int hist1[];
+    const int first = blockIdx.x * 1024 * ROUNDS + threadIdx.x;
+    int e[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) e[r] = expert_of(ids, first + 1024 * r, pairs, experts);
     for (int i = threadIdx.x; i <= experts; i += 1024) hist1[i] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < kDispPairs; i += 1024) {
-        const int p = blockIdx.x * kDispPairs + i;
-        if (p < pairs) atomicAdd(&hist1[expert_of(ids, p, experts)], 1);
-    }
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r)
+        if (first + 1024 * r < pairs) atomicAdd(&hist1[e[r]], 1);
     __syncthreads();
     for (int i = threadIdx.x; i <= experts; i += 1024) counts[(int64_t)blockIdx.x * (experts + 1) + i] = hist1[i];
 }
@@ -667,19 +670,17 @@ __global__ __launch_bounds__(1024) void dispatch_kernel(const int32_t *ids, int 
     const int threads = blockDim.x, waves = threads / 64;
     const int n = experts + 1;
     int *base = lds_i, *scan = lds_i + n;
-    uint16_t *hists = (uint16_t *)(lds_i + 2 * n);   // at most kDispPairs
+    uint16_t *hists = (uint16_t *)(lds_i + 2 * n);   // at most 1024 ROUNDS
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    for (int i = t; i < waves * n; i += threads) hists[i] = 0;
-    __syncthreads();
     uint16_t *hist = hists + wave * n;
+    const int first = blockIdx.x * 1024 * ROUNDS + wave * (64 * ROUNDS) + lane;
     int e[ROUNDS], rank[ROUNDS];
 #pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-        const int p = blockIdx.x * kDispPairs + wave * (64 * ROUNDS) + r * 64 + lane;
-        const bool live = p < pairs;
-        e[r] = live ? expert_of(ids, p, experts) : 0;
-        rank[r] = round_rank(e[r], bits, hist, live);
-    }
+    for (int r = 0; r < ROUNDS; ++r) e[r] = pairs ? expert_of(ids, first + 64 * r, pairs, experts) : 0;
+    for (int i = t; i < waves * n; i += threads) hists[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) rank[r] = round_rank(e[r], bits, hist, first + 64 * r < pairs);
     __syncthreads();
     // expert x: pairs of earlier workgroups, of all, and the waves' counts turned
     // into where each begins
@@ -693,10 +694,15 @@ __global__ __launch_bounds__(1024) void dispatch_kernel(const int32_t *ids, int 
         int before = 0, all = run;
         if (counts) {
             all = 0;
-            for (int b = 0; b < (int)gridDim.x; ++b) {
-                const int c = counts[(int64_t)b * n + x];
-                before += b < (int)blockIdx.x ? c : 0;
-                all += c;
+            for (int b = 0; b < (int)gridDim.x; b += 8) {   // eight loads at a time
+                int c[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) c[i] = counts[(int64_t)min(b + i, (int)gridDim.x - 1) * n + x];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    before += b + i < (int)blockIdx.x ? c[i] : 0;
+                    all += b + i < (int)gridDim.x ? c[i] : 0;
+                }
             }
         }
         base[x] = before;
@@ -719,7 +725,7 @@ __global__ __launch_bounds__(1024) void dispatch_kernel(const int32_t *ids, int 
         for (int x = t; x < n; x += threads) offsets[x] = scan[x];
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
-        const int p = blockIdx.x * kDispPairs + wave * (64 * ROUNDS) + r * 64 + lane;
+        const int p = first + 64 * r;
         if (p < pairs) order[scan[e[r]] + base[e[r]] + hist[e[r]] + rank[r]] = p;
     }
 }
@@ -733,28 +739,45 @@ hipError_t launch_route_bwd(const RouteArgs &a, hipStream_t s) {
     return a.dtype == LSMX_F32 ? bwd_of<LSMX_F32>(a, s) : a.dtype == LSMX_BF16 ? bwd_of<LSMX_BF16>(a, s) : bwd_of<LSMX_F16>(a, s);
 }
 
+// Rounds of a workgroup of 16 waves, 1024 pairs each.  One workgroup needs no
+// counting before it: 2000 pairs of 32 experts in two rounds 3.7 us, with it 5.2.
+// More workgroups have fewer rounds but more counts to add up: 4096 pairs in four
+// rounds 5.4, in four workgroups 5.2 (128 experts 6.7 and 5.6); 32768 in eight
+// workgroups of four rounds 8.2, in 32 of one 6.8; 65536 9.1 and 8.3; 2^21 in 512
+// workgroups 37.
+static int dispatch_rounds(int64_t pairs) { return pairs <= 1024 ? 1 : pairs <= 2048 ? 2 : pairs <= 65536 ? 1 : 4; }
+
 int64_t dispatch_workspace(int64_t pairs, int experts) {
-    const int64_t blocks = (pairs + kDispPairs - 1) / kDispPairs;
+    const int64_t each = 1024 * dispatch_rounds(pairs), blocks = (pairs + each - 1) / each;
     return blocks > 1 ? blocks * (experts + 1) * 4 : 0;
 }
-hipError_t launch_dispatch(const int32_t *ids, int pairs, int experts, int32_t *order, int32_t *offsets, int32_t *ws,
-                           hipStream_t s) {
-    const int blocks = pairs ? (pairs + kDispPairs - 1) / kDispPairs : 1;
-    int bits = 1;
-    while ((1 << bits) <= experts) ++bits;
+
+namespace {
+template <int ROUNDS>
+hipError_t dispatch(const int32_t *ids, int pairs, int experts, int32_t *order, int32_t *offsets, int32_t *ws, hipStream_t s) {
+    const int blocks = pairs ? (pairs + 1024 * ROUNDS - 1) / (1024 * ROUNDS) : 1;
     if (blocks > 1) {
-        dispatch_count_kernel<<<blocks, 1024, (experts + 1) * 4, s>>>(ids, pairs, experts, ws);
+        dispatch_count_kernel<ROUNDS><<<blocks, 1024, (experts + 1) * 4, s>>>(ids, pairs, experts, ws);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
+    int bits = 1;
+    while ((1 << bits) <= experts) ++bits;
     // up to 1024 pairs: a round for each wave, as many waves as it takes
-    const int waves = pairs <= 1024 ? (pairs + 63) / 64 + (pairs == 0) : kDispWaves;
-    const size_t lds = (size_t)(experts + 1) * (8 + 2 * waves);
-    if (pairs <= 1024)
-        dispatch_kernel<1><<<1, 64 * waves, lds, s>>>(ids, pairs, experts, bits, nullptr, order, offsets);
-    else
-        dispatch_kernel<kDispPairs / 1024><<<blocks, 1024, lds, s>>>(ids, pairs, experts, bits, blocks > 1 ? ws : nullptr, order, offsets);
+    const int waves = pairs <= 1024 ? (pairs + 63) / 64 + (pairs == 0) : 16;
+    dispatch_kernel<ROUNDS><<<blocks, 64 * waves, (size_t)(experts + 1) * (8 + 2 * waves), s>>>(ids, pairs, experts, bits, blocks > 1 ? ws : nullptr,
+                                                                                         order, offsets);
     return hipGetLastError();
+}
+}  // namespace
+
+hipError_t launch_dispatch(const int32_t *ids, int pairs, int experts, int32_t *order, int32_t *offsets, int32_t *ws,
+                           hipStream_t s) {
+    switch (dispatch_rounds(pairs)) {
+        case 1: return dispatch<1>(ids, pairs, experts, order, offsets, ws, s);
+        case 2: return dispatch<2>(ids, pairs, experts, order, offsets, ws, s);
+        default: return dispatch<4>(ids, pairs, experts, order, offsets, ws, s);
+    }
 }
 
 }  // namespace lsmx

@@ -396,3 +396,9 @@ def test_groups_whose_ranks_cancel_or_logits_are_large(dev, T, scoring):
     w, ids = route(big, k, scoring="softmax", groups=G, top_groups=3)
     want, at = route_tests._route64(big, k, None, "softmax", G, 3, True, 1.0)
     assert torch.equal(ids.long(), at) and ((w.double() - want).abs() <= want * 2.0 ** -20).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,k,E", [(1024, 1, 32), (1025, 1, 7), (1024, 2, 60), (683, 3, 1024), (8192, 8, 32), (65537, 1, 256), (262144, 8, 64)])
+def test_dispatch_forms(dev, T, k, E):
+    route_tests.test_dispatch(dev, T, k, E)
