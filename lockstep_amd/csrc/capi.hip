@@ -1149,8 +1149,12 @@ static int expert_args(const char *fn, const lsmx_experts *a, bool gated, lsmx::
     if (a->N < 1 || a->N >= (int64_t)1 << 24 || a->N * a->K / 2 >= (int64_t)1 << 31)
         return fail(LSMX_ERR_SHAPE, "%s: N=%lld: an expert's weights must stay below 2^31 bytes", fn, (long long)a->N);
     if (gated && a->N % 64) return fail(LSMX_ERR_SHAPE, "%s: N=%lld must be a multiple of 64 (F of 32)", fn, (long long)a->N);
-    // workgroups of the smallest tiles
-    if ((a->tokens * a->k / 16 + a->experts + 2) * (a->N / 64 + 1) >= (int64_t)1 << 31 || a->tokens * (a->N / 2048 + 1) >= (int64_t)1 << 31)
+    // a launch has fewer than 2^32 threads: 512 for 16 pairs and 64 rows of W, where
+    // K is at least 512 for 48 and 256 (16 or 32 pairs: of fewer than 25 an expert);
+    // the join 256 for 2048 elements
+    const int64_t pairs = a->tokens * a->k;
+    const int64_t units = a->K < 512 ? (pairs / 16 + a->experts + 2) * (a->N / 64 + 1) : (pairs / 48 + 2 * a->experts + 8) * (a->N / 256 + 1);
+    if (units >= 1 << 23 || a->tokens * (a->N / 2048 + 1) >= 1 << 24)
         return fail(LSMX_ERR_SHAPE, "%s: too many pairs times rows", fn);
     if (a->tokens && (!a->x || !a->x_scale || !a->w || !a->w_scale || !a->ids || !a->order || !a->offsets))
         return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
@@ -1171,7 +1175,7 @@ int lsmx_expert_gated(const lsmx_experts *a, uint8_t *h, uint8_t *h_scale, void 
     lsmx::ExpertArgs g;
     if (int r = expert_args(fn, a, true, &g)) return r;
     if (g.tokens && (!h || !h_scale)) return fail(LSMX_ERR_ARG, "%s: null pointer", fn);
-    if (!aligned(h, 4)) return fail(LSMX_ERR_ALIGN, "%s: h must be 4-byte aligned", fn);
+    if (!aligned(h, 8)) return fail(LSMX_ERR_ALIGN, "%s: h must be 8-byte aligned", fn);
     if (int r = device_guard()) return r;
     if (!g.tokens) return LSMX_OK;
     g.h = h, g.hs = h_scale;

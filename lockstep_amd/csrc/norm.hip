@@ -359,8 +359,19 @@ hipError_t bwd_of(const NormBwdArgs &a, hipStream_t s) {
 
 }  // namespace
 
-hipError_t launch_norm_fwd(const NormArgs &a, hipStream_t s) {
-    return a.dtype == LSMX_F32 ? fwd_of<LSMX_F32>(a, s) : a.dtype == LSMX_BF16 ? fwd_of<LSMX_BF16>(a, s) : fwd_of<LSMX_F16>(a, s);
+hipError_t launch_norm_fwd(const NormArgs &a0, hipStream_t s) {
+    NormArgs a = a0;
+    const int64_t most = 1 << 21, es = a.dtype == LSMX_F32 ? 4 : 2;   // a launch has fewer than 2^32 threads
+    for (int64_t at = 0; at < a0.rows; at += most) {
+        a.rows = a0.rows - at < most ? a0.rows - at : most;
+        auto row = [&](const void *p, int64_t bytes) { return p ? (uint8_t *)p + at * bytes : nullptr; };
+        a.x = row(a0.x, a.ldx * es), a.r = row(a0.r, a.ldr * es);
+        a.h = row(a0.h, a.dim * es), a.y = row(a0.y, a.dim * es);
+        a.codes = row(a0.codes, a.dim), a.scale = row(a0.scale, a.dim / 32);
+        const hipError_t e = a.dtype == LSMX_F32 ? fwd_of<LSMX_F32>(a, s) : a.dtype == LSMX_BF16 ? fwd_of<LSMX_BF16>(a, s) : fwd_of<LSMX_F16>(a, s);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 // Workgroups of the backward pass: four a CU, each with a share of dw.

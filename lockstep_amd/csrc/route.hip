@@ -732,11 +732,33 @@ __global__ __launch_bounds__(1024) void dispatch_kernel(const int32_t *ids, int 
 
 }  // namespace
 
-hipError_t launch_route_fwd(const RouteArgs &a, hipStream_t s) {
-    return a.dtype == LSMX_F32 ? fwd_of<LSMX_F32>(a, s) : a.dtype == LSMX_BF16 ? fwd_of<LSMX_BF16>(a, s) : fwd_of<LSMX_F16>(a, s);
+// `launch` over all rows: a launch has fewer than 2^32 threads.
+template <typename L>
+static hipError_t in_parts(const RouteArgs &a0, L launch) {
+    RouteArgs a = a0;
+    const int64_t most = 1 << 22, es = a.dtype == LSMX_F32 ? 4 : 2;
+    for (int64_t at = 0; at < a0.rows; at += most) {
+        a.rows = a0.rows - at < most ? a0.rows - at : most;
+        a.logits = (const uint8_t *)a0.logits + at * a.ld * es;
+        a.mask = a0.mask ? a0.mask + at : nullptr;
+        a.weights = a0.weights ? a0.weights + at * a.k : nullptr;
+        a.ids = a0.ids + at * a.k;
+        a.dw = a0.dw ? a0.dw + at * a.k : nullptr;
+        a.dlogits = a0.dlogits ? (uint8_t *)a0.dlogits + at * a.experts * es : nullptr;
+        const hipError_t e = launch(a);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
-hipError_t launch_route_bwd(const RouteArgs &a, hipStream_t s) {
-    return a.dtype == LSMX_F32 ? bwd_of<LSMX_F32>(a, s) : a.dtype == LSMX_BF16 ? bwd_of<LSMX_BF16>(a, s) : bwd_of<LSMX_F16>(a, s);
+hipError_t launch_route_fwd(const RouteArgs &a0, hipStream_t s) {
+    return in_parts(a0, [s](const RouteArgs &a) {
+        return a.dtype == LSMX_F32 ? fwd_of<LSMX_F32>(a, s) : a.dtype == LSMX_BF16 ? fwd_of<LSMX_BF16>(a, s) : fwd_of<LSMX_F16>(a, s);
+    });
+}
+hipError_t launch_route_bwd(const RouteArgs &a0, hipStream_t s) {
+    return in_parts(a0, [s](const RouteArgs &a) {
+        return a.dtype == LSMX_F32 ? bwd_of<LSMX_F32>(a, s) : a.dtype == LSMX_BF16 ? bwd_of<LSMX_BF16>(a, s) : bwd_of<LSMX_F16>(a, s);
+    });
 }
 
 // Rounds of a workgroup of 16 waves, 1024 pairs each.  One workgroup needs no

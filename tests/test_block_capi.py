@@ -205,3 +205,21 @@ def test_arguments_are_refused_on_the_gpu(dev):
             experts.expert_combine(**{**good, **bad})
     with pytest.raises(TypeError):
         experts.expert_combine(**good, out_dtype=torch.float64)
+
+
+@pytest.mark.parametrize("change,ok", [(dict(tokens=1 << 21, k=1, K=256, N=1 << 10), True), (dict(tokens=1 << 21, k=1, K=256, N=1 << 12), False),
+                                       (dict(tokens=1 << 21, k=1, K=512, N=1 << 13), True), (dict(tokens=1 << 21, k=1, K=512, N=1 << 16), False),
+                                       (dict(tokens=1 << 21, k=1, K=512, N=14336), False), (dict(tokens=1 << 20, k=2, K=512, N=14336), True)])
+def test_launches_past_their_limit_are_refused(change, ok):
+    """2^32 threads: the workspace's size is 0 for a refused call."""
+    a = product(**change)
+    n = rc("lsmx_expert_combine_workspace", ctypes.addressof(a))
+    assert (n > 0) == ok
+    if not ok:
+        assert rc("lsmx_expert_combine", ctypes.addressof(a), P, P, C.BF16, P, 1 << 50, None) == C.ERR_SHAPE
+        assert "too many" in C.last_error()
+
+
+def test_gated_needs_aligned_rows():
+    a = product()
+    assert rc("lsmx_expert_gated", ctypes.addressof(a), P + 4, P, None) == C.ERR_ALIGN

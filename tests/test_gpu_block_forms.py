@@ -402,3 +402,30 @@ def test_groups_whose_ranks_cancel_or_logits_are_large(dev, T, scoring):
 @pytest.mark.parametrize("T,k,E", [(1024, 1, 32), (1025, 1, 7), (1024, 2, 60), (683, 3, 1024), (8192, 8, 32), (65537, 1, 256), (262144, 8, 64)])
 def test_dispatch_forms(dev, T, k, E):
     route_tests.test_dispatch(dev, T, k, E)
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_launch_takes(dev):
+    """Past 2^21 rows of the norm and 2^22 of the router: rows near each border as when alone."""
+    from lockstep_amd.experts import route
+    from lockstep_amd.norm import add_rms_norm
+    T = 2 ** 22 + 5
+    g = torch.Generator(device=dev).manual_seed(0)
+    x, r = (torch.randn((T, 32), generator=g, device=dev).bfloat16() for _ in range(2))
+    w = torch.randn(32, generator=g, device=dev).bfloat16()
+    got = add_rms_norm(x, w, r, mxfp8=True)
+    part = [slice(a, a + 9) for a in (0, 2 ** 21 - 4, 2 ** 22 - 4)]
+    for p in part:
+        want = add_rms_norm(x[p].contiguous(), w, r[p].contiguous(), mxfp8=True)
+        assert all(torch.equal(u[p].view(torch.uint8), v.view(torch.uint8)) for u, v in zip(got, want))
+    l = torch.randn((T, 5), generator=g, device=dev)
+    mask = torch.rand(T, generator=g, device=dev) < 0.9
+    up = torch.randn((T, 2), generator=g, device=dev)
+
+    def both(p):
+        t = l[p].clone().requires_grad_(True)
+        wt, ids = route(t, 2, mask=mask[p].contiguous())
+        return wt.detach(), ids, torch.autograd.grad(wt, t, up[p].contiguous())[0]
+    got = both(slice(None))
+    for p in part:
+        assert all(torch.equal(u[p], v) for u, v in zip(got, both(p)))
