@@ -223,3 +223,10 @@ def test_launches_past_their_limit_are_refused(change, ok):
 def test_gated_needs_aligned_rows():
     a = product()
     assert rc("lsmx_expert_gated", ctypes.addressof(a), P + 4, P, None) == C.ERR_ALIGN
+
+
+@pytest.mark.parametrize("src", ["norm.hip", "route.hip", "experts.hip"])
+def test_kernels_use_no_scratch(src, tmp_path):
+    """The products count their loads in flight, which a spill would add to."""
+    from .test_kernel_resources import test_kernels_use_no_scratch as check
+    check(src, tmp_path)
