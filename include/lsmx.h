@@ -572,7 +572,8 @@ int lsmx_rms_norm_bwd(const void *h, int64_t ldh, const void *dy, int64_t lddy, 
  *   that order, ties (of groups too) to the lowest index, a NaN first
  *   weights = scale s / (renorm ? sum of the k : 1), 0 where the k sum to 0
  *
- * c is compared in 64 bits.  logits [rows, ld], LSMX_F32 | BF16 | F16; bias fp32
+ * c is compared in 64 bits; without a bias experts rank by their logits, which
+ * have the scores' order.  logits [rows, ld], LSMX_F32 | BF16 | F16; bias fp32
  * [experts] or NULL; mask [rows] bytes or NULL: a row with 0 gets ids -1 and
  * weights 0.  A row of nothing but -inf scores 0 under softmax.  experts <=
  * 1024, groups <= 64, k <= 64. */

@@ -115,7 +115,8 @@ def add_rms_norm(x, weight, residual=None, *, eps=1e-6, mxfp8=False):
     both = (x, weight) if residual is None else (x, weight, residual)
     C.require_device(*both)
     C.one_device(*both)
-    assert x.dim() >= 1 and weight.shape == x.shape[-1:], f"weight must be [{x.shape[-1] if x.dim() else 'D'}], got {list(weight.shape)}"
+    assert x.dim() >= 1 and x.shape[-1] > 0, "x must be [.., D], D at least 1"
+    assert weight.shape == x.shape[-1:], f"weight must be [{x.shape[-1]}], got {list(weight.shape)}"
     assert residual is None or residual.shape == x.shape, \
         f"x and residual must have one shape, got {list(x.shape)}, {list(residual.shape)}"
     assert not mxfp8 or x.shape[-1] % 32 == 0, f"D={x.shape[-1]} must be a multiple of 32 for MXFP8"

@@ -429,3 +429,52 @@ def test_more_rows_than_a_launch_takes(dev):
     got = both(slice(None))
     for p in part:
         assert all(torch.equal(u[p], v) for u, v in zip(got, both(p)))
+
+
+@pytest.mark.gpu
+def test_empty_rows_are_refused_and_no_rows_are_not(dev):
+    from lockstep_amd.experts import route
+    from lockstep_amd.norm import add_rms_norm
+    with pytest.raises(AssertionError, match="at least 1"):
+        add_rms_norm(torch.zeros((3, 0), device=dev), torch.zeros(0, device=dev))
+    with pytest.raises(AssertionError, match="must be"):
+        route(torch.zeros((3, 0), device=dev), 1)
+    x, w = (torch.zeros(s, device=dev, requires_grad=True) for s in ((0, 64), (64,)))
+    y, h = add_rms_norm(x, w, x)
+    gx, gw = torch.autograd.grad(y.sum() + h.sum(), (x, w))
+    assert gx.shape == (0, 64) and torch.equal(gw, torch.zeros_like(w))
+    l = torch.zeros((0, 8), device=dev, requires_grad=True)
+    wt, ids = route(l, 2)
+    assert ids.shape == (0, 2) and torch.autograd.grad(wt.sum(), l)[0].shape == (0, 8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("E,K,F,pairs", [(1, 512, 32, 3000), (3, 512, 160, 2000), (2, 1152, 96, 800), (9, 768, 128, 4000)])
+def test_uneven_experts_and_borders_of_tiles(dev, E, K, F, pairs):
+    """Experts without a pair, with one, with a tile's and one more; rows of W past a tile's end."""
+    from lockstep_amd import experts
+    g = torch.Generator(device=dev).manual_seed(pairs)
+    x, xs = experts_tests._rows(dev, (pairs, K), 1)
+    w, ws = experts_tests._weights(dev, E, 2 * F, K, 2)
+    ids = torch.full((pairs, 1), E - 1, dtype=torch.int32, device=dev)
+    if E > 1:
+        ids[:257] = 0
+    if E > 3:
+        ids[300] = 1
+        ids[400:528] = 3
+        ids[600:1112] = 5
+    ids = ids[torch.randperm(pairs, generator=g, device=dev)].contiguous()
+    d = experts.dispatch(ids, E)
+    h, hs = experts.expert_gated(x, xs, w, ws, d)
+    out, mag = experts_tests._products(experts_tests._values8(x, xs), ids, w, ws, False)
+    gate, up = out.chunk(2, -1)
+    dg, du = (mag * experts_tests.IN_BLOCK).chunk(2, -1)
+    want = gate * torch.sigmoid(gate) * up
+    err = 1.1 * dg * (up.abs() + du) + (gate * torch.sigmoid(gate)).abs() * du + want.abs() * 2.0 ** -18
+    step = torch.exp2(hs.double() - 127).repeat_interleave(32, -1) * 2.0 ** -10
+    assert ((experts_tests._values8(h, hs) - want).abs() <= err * (1 + 2.0 ** -4) + want.abs() * 2.0 ** -4 + step).all()
+    x3, xs3 = x[:, None], xs[:, None]
+    for dt in (torch.bfloat16, torch.float16):
+        y = experts.expert_combine(x3.contiguous(), xs3.contiguous(), w, ws, d, torch.ones((pairs, 1), device=dev), dt)
+        assert ((y.double() - out[:, 0]).abs() <= out[:, 0].abs() * torch.finfo(dt).eps / 2 + mag[:, 0] * (experts_tests.IN_BLOCK + 2.0 ** -11)
+                ).all()
