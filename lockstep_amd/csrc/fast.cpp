@@ -784,10 +784,11 @@ torch::autograd::variable_list once(torch::autograd::variable_list d) {
 }
 
 // Refuses a differentiable call that is being captured into a graph while a node
-// that its gradients would go to belongs to another stream, as a leaf's does of
-// which an eager graph is still alive: in the backward pass the engine would make
-// that stream wait for the captured one, which ends the process.  `capturing`:
-// of the current stream, or as a test has it.
+// that its gradients would go to belongs to the default stream, as a leaf's does
+// of which an eager graph is still alive: in the backward pass the engine would
+// make that stream wait for the captured one, which ends the process.  (Any other
+// stream becomes part of the capture, and is joined at the pass's end.)
+// `capturing`: of the current stream, or as a test has it.
 bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
 void one_stream(const Tensor &t, bool capturing) {
     if (!capturing || !t.requires_grad()) return;
@@ -795,9 +796,10 @@ void one_stream(const Tensor &t, bool capturing) {
     if (!node) return;
     const auto there = node->stream();
     TORCH_CHECK(!there || there->device_type() != at::kCUDA ||
+                    there->id() != c10::hip::getDefaultHIPStreamMasqueradingAsCUDA(there->device_index()).id() ||
                     there->id() == c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(there->device_index()).id(),
-                "a differentiable call cannot be captured while a graph of its tensors made on another stream is alive: free that "
-                "graph's outputs first, make it on the stream of the capture, or capture the call under torch.no_grad()");
+                "a differentiable call cannot be captured while a graph of its tensors made on the default stream is alive: free that "
+                "graph's outputs first, make it on another stream, or capture the call under torch.no_grad()");
 }
 
 // captures(tensors, capturing): the same for the nodes in Python; capturing None:

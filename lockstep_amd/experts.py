@@ -99,8 +99,8 @@ def route(logits, k, *, bias=None, scoring="softmax", groups=1, top_groups=1, re
     weights 0.  A NaN ranks first; a row of nothing but -inf scores 0.
     Differentiable in logits (once, in reverse mode): the choice is taken as
     given, and neither it nor bias has a gradient.  A differentiable call is not
-    captured into a HIP graph while an eager graph of the logits, made on another
-    stream, is alive."""
+    captured into a HIP graph while an eager graph of the logits, made on the
+    default stream, is alive."""
     if (r := C.fast.route(logits, k, bias, scoring, groups, top_groups, renormalize, scale, mask)) is not None:
         return r
     C.not_traced("route")

@@ -100,9 +100,10 @@ def add_rms_norm(x, weight, residual=None, *, eps=1e-6, mxfp8=False):
     [.., D // 32]), the row-major form that mxfp4_gemm_fp8 takes.
 
     Differentiable in x, residual and weight (once, in reverse mode; the
-    codes have no gradient).  A differentiable call is not captured into a HIP
-    graph while an eager graph of its tensors, made on another stream, is alive.  The mean, the norm and every sum are fp32; y is
-    rounded once, its codes are of the unrounded y.  Deterministic."""
+    codes have no gradient).  The mean, the norm and every sum are fp32; y is
+    rounded once, its codes are of the unrounded y.  Deterministic.  A
+    differentiable call is not captured into a HIP graph while an eager graph of
+    its tensors, made on the default stream, is alive."""
     if (r := C.fast.rms_norm(x, weight, residual, eps, mxfp8)) is not None:
         return r
     C.not_traced("add_rms_norm")

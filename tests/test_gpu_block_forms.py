@@ -235,6 +235,43 @@ def test_training_pass_captured_and_replayed(dev):
 
 
 @pytest.mark.gpu
+def test_capture_after_a_warm_up_on_another_stream(dev):
+    """The usual recipe: a warm-up on a side stream, whose outputs are still held, then
+    the capture on the graph's own."""
+    from lockstep_amd import experts
+    from lockstep_amd.norm import add_rms_norm
+    x, r, w = (t.requires_grad_(True) for t in norm_tests._inputs(dev, 33, 64, torch.float32, 4))
+
+    def step():
+        y, h = add_rms_norm(x, w, r)
+        wt, ids = experts.route(y, 4)
+        return (wt * torch.arange(1, 5, device=dev)).sum() + h.square().mean()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            loss = step()
+            grads = torch.autograd.grad(loss, (x, w, r))
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+        held_grads = torch.autograd.grad(held, (x, w, r))
+    del loss, grads
+    for i in range(3):
+        with torch.no_grad():
+            x.normal_(generator=torch.Generator(device=dev).manual_seed(i))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            want = torch.autograd.grad(step(), (x, w, r))
+        side.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(held_grads, want))
+
+
+@pytest.mark.gpu
 def test_threads_and_streams_at_once(dev):
     """Four threads, a stream each, one run of the operators: as when alone."""
     from lockstep_amd import experts, fp4
@@ -334,7 +371,7 @@ def test_weights_and_rows_beyond_32_bits(dev):
 @pytest.mark.gpu
 def test_leaves_of_another_streams_graph_are_told(dev):
     """The check that a captured call makes, with the capture's part played by the
-    host: only a tensor whose graph, still alive, is another stream's is refused."""
+    host: only a tensor whose graph, still alive, is the default stream's is refused."""
     x, r, w = (t.requires_grad_(True) for t in norm_tests._inputs(dev, 6, 64, torch.float32, 3))
     from lockstep_amd.norm import add_rms_norm
     side = torch.cuda.Stream()
@@ -346,13 +383,15 @@ def test_leaves_of_another_streams_graph_are_told(dev):
         for t in (x, w, eager):
             C.fast.captures((t,), False)
             C.fast.captures((t,), None)                   # nothing is captured here
-            with pytest.raises(RuntimeError, match="on another stream is alive"):
+            with pytest.raises(RuntimeError, match="on the default stream is alive"):
                 C.fast.captures((r, t), True)
         del eager, t
         C.fast.captures((x, w), True)
         y = add_rms_norm(x, w)
         C.fast.captures((x, w, y), True)
     side.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        C.fast.captures((x, w, y), True)                  # a stream that can join the capture
 
 
 @pytest.mark.gpu
